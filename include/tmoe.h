@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define TMOE_ABI_VERSION 13
+#define TMOE_ABI_VERSION 14
 
 /* error codes */
 #define TMOE_OK            0
@@ -352,6 +352,101 @@ int tmoe_latent_backward(const void* x, const void* G, const int64_t* idx, const
                          const void* dout, int64_t B, int64_t E, int64_t k, int64_t r3,
                          int64_t r2, int dtype, void* dx, void* dG, void* dp, void* workspace,
                          size_t workspace_bytes, void* stream);
+
+/* The training layer's router with its losses: sft_cot_bundle/scripts/model.py:318-332
+ * (fast_scaled_tanh, z loss, softmax, top-k, renormalised weights, balance loss), with
+ * per-expert counts and a mask of tokens. For a token's logits raw (E):
+ *   a = cap tanh(raw / cap);  P = softmax(a / temperature);  idx = the k largest raw in
+ *   descending order, the lowest index first on ties;  w_j = P[idx_j] / (sum_i P[idx_i] + 1e-6)
+ *   lb = E sum_e (counts[e] / N) (sum_b P[b,e] / N),  z = sum_b logsumexp(a_b)^2 / N
+ * over the N tokens that the mask does not leave out (mask[b] != 0, or no mask). Tokens that
+ * it leaves out have idx -1, w 0 and no gradient, whatever their logits hold; with N = 0 the
+ * losses are 0. A NaN logit ranks above every number, as in torch.topk.
+ *   raw     (B, E)  dtype, rows row_stride elements apart       idx    (B, k)  int64
+ *   mask    (B)     bytes, or null                              w      (B, k)  fp32
+ *   lb, z, tokens (one fp32 each; tokens is N)                  counts (E)     int64
+ * temperature_dev, if not null, is a device float that is read instead of temperature.
+ * dtype TMOE_BF16 or TMOE_F32, arithmetic in fp32; E <= 256, k <= min(E, 16), B <= 2^30.
+ * Backward: from dw (B, k), dlb and dz (one fp32 each; any of them null for zeros) draw
+ * (B, E) of dtype, contiguous; idx, tokens and counts as the forward wrote them. The sums
+ * over the tokens are added in a fixed order. Stream-ordered, no allocation. */
+typedef struct tmoe_router {
+  const void* raw;
+  int64_t row_stride, B, E, k;
+  int32_t dtype;
+  float cap, temperature;
+  const float* temperature_dev;
+  const uint8_t* mask;
+} tmoe_router;
+size_t tmoe_router_workspace_bytes(int64_t B, int64_t E);
+int tmoe_router_forward(const tmoe_router* router, int64_t* idx, float* w, float* lb, float* z,
+                        float* tokens, int64_t* counts, void* workspace, size_t workspace_bytes,
+                        void* stream);
+int tmoe_router_backward(const tmoe_router* router, const int64_t* idx, const float* tokens,
+                         const int64_t* counts, const float* dw, const float* dlb,
+                         const float* dz, void* draw, void* stream);
+
+/* The norms before and after a block fused with its gate and the residual's scale, with
+ * their backward: what stands around a sub-block in the reference's blocks
+ * (pure_torch_mlx/model.py:258-260, :337-341), for training. With
+ * rms(v) = sqrt(mean(v^2) + eps) over the d elements of a row:
+ *   u = y * silu(gate);  f = u / rms(u) * post_weight;  r = x + gamma * f;
+ *   h = r / rms(r) * next_weight
+ * Every operand but y may be null, and its step then falls away (post_weight null: f = u;
+ * next_weight null: no h). x, y, gate (T, d) with rows *_stride elements apart, the weights
+ * (d), all of dtype TMOE_BF16 or TMOE_F32; arithmetic in fp32, each output rounded once (h
+ * is taken from the unrounded r). r (null: not wanted) and h are (T, d), contiguous. inv,
+ * (2, T) fp32, is what the backward needs of the forward (null: no backward follows).
+ * Backward: from dr and dh ((T, d) of dtype, each may be null) the gradients that are not
+ * null: dx, dy, dgate (T, d) contiguous, dpost_weight, dgamma, dnext_weight (d), the latter
+ * three with a workspace. d <= 16384, T <= 2^30. Stream-ordered, no allocation. */
+typedef struct tmoe_block_norm {
+  const void *x, *y, *gate;
+  int64_t x_stride, y_stride, gate_stride;
+  const void *post_weight, *gamma, *next_weight;
+  int64_t T, d;
+  int32_t dtype;
+  float eps;
+} tmoe_block_norm;
+size_t tmoe_block_norm_workspace_bytes(int64_t T, int64_t d, int dtype);
+int tmoe_block_norm_forward(const tmoe_block_norm* norm, void* r, void* h, float* inv,
+                            void* stream);
+int tmoe_block_norm_backward(const tmoe_block_norm* norm, const float* inv, const void* dr,
+                             int64_t dr_stride, const void* dh, int64_t dh_stride, void* dx,
+                             void* dy, void* dgate, void* dpost_weight, void* dgamma,
+                             void* dnext_weight, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* One AdamW step over many tensors (the reference trains with torch's,
+ * pre-train/train.py:1263-1268):
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay)
+ *       - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * p and g of dtype TMOE_BF16 or TMOE_F32, n contiguous elements each, updated in fp32 and
+ * rounded to nearest. state_bits 32: m and v fp32. state_bits 8: m and r = sqrt(v) as OCP
+ * e4m3 codes, each 256 elements (the last: what is left) with one fp32 scale (m_scale,
+ * v_scale: ceil(n / 256)), the largest magnitude / 448; codes are rounded to one of the two
+ * neighbours at random, from a hash of (seed, step, tensor's number, element), so that m and
+ * v = r^2 are right in the mean, and a positive r never to zero. A block that meets a
+ * non-finite gradient has a non-finite scale from then on. step counts from 1; step_dev,
+ * if not null, is a device int64 that is read instead. Tensors may not overlap; those with
+ * n = 0 are passed over. Stream-ordered, no allocation, nothing copied to the device. */
+typedef struct tmoe_adamw_tensor {
+  void* p;
+  const void* g;
+  void *m, *v;
+  float *m_scale, *v_scale;
+  int64_t n;
+} tmoe_adamw_tensor;
+typedef struct tmoe_adamw_step_args {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;
+  const int64_t* step_dev;
+  uint32_t seed;
+  int32_t dtype, state_bits;
+} tmoe_adamw_step_args;
+int tmoe_adamw_step(const tmoe_adamw_tensor* tensors, int64_t count,
+                    const tmoe_adamw_step_args* args, void* stream);
 
 /* Per-stage timing, no counterpart in the reference (measurement support).
  * While enabled, every tmoe_forward records a HIP event before each of its

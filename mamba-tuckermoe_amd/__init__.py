@@ -13,6 +13,14 @@ Public surface:
   FusedLatentMoE               the training module's latent expert contraction with its
                                backward (latent.py; autograd.Function, reference signature)
   TuckerMoETrain               the reference's training layer (TritonTuckerMoE) on it
+  fused_router, Routing        its router with the balance and z losses, per-expert counts and
+                               their gradient in two launches (train_ops.py)
+  fused_block_norm             the norms before and after a block with its gate and residual
+                               scale, and their gradients (train_ops.py)
+  TuckerFFNTrain               TuckerFFN for training, on the two and TuckerMoETrain
+                               (block_train.py)
+  FusedAdamW, adamw_step,      one AdamW step over many tensors, moments in 32 or 8 bits
+  adamw_step_8bit              (adamw.py)
   synth                        seeded synthetic parameters and tokens
   fp8                          e4m3 weights with per-output-channel scales
   checkpoint                   the reference's .npz keys (layers, FFN, out_proj) and the
@@ -24,8 +32,13 @@ from .config import FFN_WORKLOADS, WORKLOADS, FfnWorkload, TuckerMoEConfig, Work
 from .module import RMSNorm, TuckerMoE, load_tucker
 from .block import LayerScale, TuckerFFN, TuckerOutProj
 from .latent import FusedLatentMoE, TuckerMoETrain, fused_latent_moe
+from .train_ops import Routing, fused_block_norm, fused_router
+from .block_train import TuckerFFNTrain
+from .adamw import FusedAdamW, adamw_step, adamw_step_8bit
 
 __all__ = ["TuckerMoE", "RMSNorm", "LayerScale", "TuckerFFN", "TuckerOutProj",
            "FusedLatentMoE", "TuckerMoETrain", "fused_latent_moe",
+           "fused_router", "Routing", "fused_block_norm", "TuckerFFNTrain", "FusedAdamW", "adamw_step",
+           "adamw_step_8bit",
            "TuckerMoEConfig", "Workload", "WORKLOADS", "FfnWorkload", "FFN_WORKLOADS", "load_tucker", "synth", "config", "fp8",
            "checkpoint", "_lib"]

@@ -18,7 +18,8 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(HERE, "libtmoe.so")
 
-SOURCES = ["tmoe_kernels.hip", "tmoe_static.hip", "tmoe_api.cpp"]
+SOURCES = ["tmoe_kernels.hip", "tmoe_static.hip", "tmoe_train.hip", "tmoe_api.cpp",
+           "tmoe_train_api.cpp"]
 # the measurement harness's hardware probes (include/tmoe_probe.h), a library of
 # their own so that libtmoe.so holds only the layer
 PROBE_SOURCES = ["tmoe_probe.hip"]
@@ -66,10 +67,11 @@ def native_cmd(out: str) -> list:
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     return [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
             "-Wno-unknown-pragmas", f'-DTMOE_NATIVE_TAG="{native_tag()}"',
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-D__HIP_PLATFORM_AMD__", "-I", INCLUDE, "-isystem", "/opt/rocm/include",
             "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
             "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, NATIVE_SOURCE),
-            "-o", out, "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10"]
+            "-o", out, "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]
 
 
 def build(verbose: bool = False) -> str:

@@ -22,7 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libtmoe.so")
 NATIVE_PATH = os.path.join(HERE, "_tmoe_native.so")
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 TMOE_OK, TMOE_EINVAL, TMOE_EUNSUPPORTED, TMOE_EHIP, TMOE_ESIGNAL = 0, -1, -2, -3, -4
 TMOE_F32, TMOE_BF16, TMOE_BF16_FP8W = 0, 1, 2
 TMOE_ROUTER_SOFTMAX_TOPK, TMOE_ROUTER_CAPPED = 0, 1
@@ -53,6 +53,9 @@ EXPORTED = (
     "tmoe_static_scratch_bytes", "tmoe_forward_static",
     "tmoe_latent_workspace_bytes", "tmoe_latent_form", "tmoe_latent_forward",
     "tmoe_latent_backward",
+    "tmoe_router_workspace_bytes", "tmoe_router_forward", "tmoe_router_backward",
+    "tmoe_block_norm_workspace_bytes", "tmoe_block_norm_forward", "tmoe_block_norm_backward",
+    "tmoe_adamw_step",
     "tmoe_signal_status", "tmoe_set_wait_polls", "tmoe_forward_path",
     "tmoe_forward_form",
     "tmoe_prof_enable", "tmoe_prof_read",
@@ -69,6 +72,40 @@ class TmoeShape(ctypes.Structure):
         ("router_mode", ctypes.c_int32), ("router_scale", ctypes.c_float),
         ("router_temperature", ctypes.c_float), ("flags", ctypes.c_int32),
     ]
+
+
+class TmoeRouter(ctypes.Structure):
+    """struct tmoe_router."""
+    _fields_ = [
+        ("raw", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("B", ctypes.c_int64),
+        ("E", ctypes.c_int64), ("k", ctypes.c_int64), ("dtype", ctypes.c_int32),
+        ("cap", ctypes.c_float), ("temperature", ctypes.c_float),
+        ("temperature_dev", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+    ]
+
+
+class TmoeBlockNorm(ctypes.Structure):
+    """struct tmoe_block_norm."""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64),
+        ("gate_stride", ctypes.c_int64), ("post_weight", ctypes.c_void_p),
+        ("gamma", ctypes.c_void_p), ("next_weight", ctypes.c_void_p), ("T", ctypes.c_int64),
+        ("d", ctypes.c_int64), ("dtype", ctypes.c_int32), ("eps", ctypes.c_float),
+    ]
+
+
+class TmoeAdamwTensor(ctypes.Structure):
+    """struct tmoe_adamw_tensor."""
+    _fields_ = [(f, ctypes.c_void_p) for f in ("p", "g", "m", "v", "m_scale", "v_scale")] + [
+        ("n", ctypes.c_int64)]
+
+
+class TmoeAdamwStep(ctypes.Structure):
+    """struct tmoe_adamw_step_args."""
+    _fields_ = [(f, ctypes.c_double) for f in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [
+        ("step", ctypes.c_int64), ("step_dev", ctypes.c_void_p), ("seed", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32), ("state_bits", ctypes.c_int32)]
 
 
 class TmoeError(RuntimeError):
@@ -144,6 +181,22 @@ def lib() -> ctypes.CDLL:
         L.tmoe_latent_backward.restype = ctypes.c_int
         L.tmoe_latent_backward.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64,
                                            ctypes.c_int, vp, vp, vp, vp, sz, vp]
+        L.tmoe_router_workspace_bytes.restype = sz
+        L.tmoe_router_workspace_bytes.argtypes = [i64, i64]
+        L.tmoe_router_forward.restype = ctypes.c_int
+        L.tmoe_router_forward.argtypes = [ctypes.POINTER(TmoeRouter)] + [vp] * 7 + [sz, vp]
+        L.tmoe_router_backward.restype = ctypes.c_int
+        L.tmoe_router_backward.argtypes = [ctypes.POINTER(TmoeRouter)] + [vp] * 8
+        L.tmoe_block_norm_workspace_bytes.restype = sz
+        L.tmoe_block_norm_workspace_bytes.argtypes = [i64, i64, ctypes.c_int]
+        L.tmoe_block_norm_forward.restype = ctypes.c_int
+        L.tmoe_block_norm_forward.argtypes = [ctypes.POINTER(TmoeBlockNorm), vp, vp, vp, vp]
+        L.tmoe_block_norm_backward.restype = ctypes.c_int
+        L.tmoe_block_norm_backward.argtypes = [ctypes.POINTER(TmoeBlockNorm), vp, vp, i64, vp, i64,
+                                               vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        L.tmoe_adamw_step.restype = ctypes.c_int
+        L.tmoe_adamw_step.argtypes = [ctypes.POINTER(TmoeAdamwTensor), i64,
+                                      ctypes.POINTER(TmoeAdamwStep), vp]
         L.tmoe_signal_status.restype = ctypes.c_int
         L.tmoe_signal_status.argtypes = [vp, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]
         L.tmoe_forward_path.restype = ctypes.c_int
@@ -192,7 +245,10 @@ def native():
                                    "build it again with __graft_entry__.build()")
             mod.bind(*(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in (
                 "tmoe_workspace_bytes", "tmoe_signal_status", "tmoe_forward_epi",
-                "tmoe_forward_glu", "tmoe_rmsnorm_rows")))
+                "tmoe_forward_glu", "tmoe_rmsnorm_rows", "tmoe_last_error",
+                "tmoe_router_workspace_bytes", "tmoe_router_forward", "tmoe_router_backward",
+                "tmoe_block_norm_workspace_bytes", "tmoe_block_norm_forward",
+                "tmoe_block_norm_backward", "tmoe_adamw_step")))
             _native = mod
     return _native
 

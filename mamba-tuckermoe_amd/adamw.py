@@ -1,0 +1,179 @@
+"""AdamW over many tensors at once on MI355X (gfx950), with moments in 32 or in 8 bits.
+
+The reference trains with torch's AdamW (pre-train/train.py:1263-1268):
+    m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+    p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+Here a step is one launch for up to 56 tensors (tmoe_adamw_step): bfloat16 or float32
+parameters on a HIP device with gradients of their dtype, computed in float32.
+
+8-bit states hold m and sqrt(v) as OCP e4m3 codes (torch.float8_e4m3fn) with one float32
+scale for each BLOCK elements of a tensor in its memory's order: value = code * scale.
+Codes are rounded up or down at random (from seed, step, the tensor's place in the list and
+the element's in the tensor), so that m and v are right in the mean; a moment that moves
+by a thousandth a step would otherwise never leave its code. A non-finite gradient makes the
+moments of its whole block non-finite.
+"""
+from __future__ import annotations
+
+from typing import Sequence, Union
+
+import torch
+
+from . import _lib
+
+BLOCK = 256
+E4M3_MAX = 448.0
+
+
+def _run(params, grads, m, v, ms, vs, step, lr, betas, eps, weight_decay, seed):
+    if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
+        raise ValueError(f"adamw_step: betas {betas}")
+    if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0:
+        raise ValueError(f"adamw_step: lr {lr}, eps {eps}, weight_decay {weight_decay}")
+    dev = isinstance(step, torch.Tensor)
+    _lib.native().adamw(params, grads, m, v, ms, vs, None if dev else int(step), step if dev else None,
+                        float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
+                        int(seed))
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
+               exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor], *,
+               step: Union[int, torch.Tensor], lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2) -> None:
+    """One step on lists of tensors of one dtype on one device, in place. The moments are
+    float32, laid out as their parameters. step counts from 1: a number, or an int64 tensor
+    of one value on the device, which is read when the kernels run."""
+    _run(params, grads, exp_avgs, exp_avg_sqs, None, None, step, lr, betas, eps, weight_decay, 0)
+
+
+def adamw_step_8bit(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
+                    exp_avg_codes: Sequence[torch.Tensor], exp_avg_scales: Sequence[torch.Tensor],
+                    exp_avg_sq_codes: Sequence[torch.Tensor],
+                    exp_avg_sq_scales: Sequence[torch.Tensor], *, step: Union[int, torch.Tensor],
+                    lr: float, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                    seed: int = 0) -> None:
+    """adamw_step with 8-bit moments: for a parameter of n elements n codes
+    (torch.float8_e4m3fn or its uint8 bits) and ceil(n / BLOCK) scales of each moment, the
+    second one's of sqrt(v)."""
+    _run(params, grads, exp_avg_codes, exp_avg_sq_codes, exp_avg_scales, exp_avg_sq_scales, step, lr,
+         betas, eps, weight_decay, seed)
+
+
+def dequantize_state(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The float32 values (n,) of a moment's codes and scales (of sqrt(v): square them)."""
+    if codes.dtype == torch.uint8:
+        codes = codes.view(torch.float8_e4m3fn)
+    q = codes.reshape(-1).float()
+    return q * scales.repeat_interleave(BLOCK)[:q.numel()]
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """AdamW whose step is one launch for up to 56 parameters of a group.
+
+    state_bits 32 keeps float32 moments ("exp_avg", "exp_avg_sq"), 8 keeps codes and scales
+    ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales", of
+    sqrt(v)). capturable=True holds the step count on the device, so that a captured step
+    counts on in its replays; without it a step inside a capture raises. Parameters are
+    bfloat16 or float32, dense, on HIP devices, with gradients of their dtype; bfloat16
+    ones are rounded to nearest."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, seed: int = 0,
+                 capturable: bool = False):
+        if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"FusedAdamW: lr {lr}, eps {eps}, weight_decay {weight_decay}")
+        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
+            raise ValueError(f"FusedAdamW: betas {betas}")
+        if state_bits not in (32, 8):
+            raise ValueError(f"FusedAdamW: state_bits {state_bits} is not 32 or 8")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                                      state_bits=state_bits, seed=seed, capturable=capturable))
+
+    def _init_state(self, p: torch.Tensor, group, count) -> dict:
+        st = self.state[p]
+        st["step"] = count
+        if group["state_bits"] == 32:
+            for k in ("exp_avg", "exp_avg_sq"):
+                st[k] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        else:
+            for k in ("exp_avg", "exp_avg_sq"):
+                st[k + "_codes"] = torch.zeros(p.numel(), dtype=torch.uint8,
+                                               device=p.device).view(torch.float8_e4m3fn)
+                st[k + "_scales"] = torch.zeros(-(-p.numel() // BLOCK), device=p.device)
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step over every parameter that has a gradient; closure as in torch.optim."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            on_device = group["capturable"]
+            fresh = {}      # device: the count that parameters first met in this step share
+            runs = {}       # (device, dtype, step): its parameters, one call each
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if g.is_sparse:
+                    raise RuntimeError("FusedAdamW: sparse gradients are not supported")
+                st = self.state[p]
+                if not st:
+                    if on_device and p.device not in fresh:
+                        fresh[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
+                    st = self._init_state(p, group, fresh[p.device] if on_device else 0)
+                n = st["step"]
+                key = (p.device, p.dtype, id(n) if on_device else n)
+                run = runs.get(key)
+                if run is None:
+                    run = runs[key] = (n, [], [], [])
+                run[1].append(p)
+                run[2].append(g)
+                run[3].append(st)
+            if not on_device and any(d.type == "cuda" for d, _, _ in runs) \
+                    and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("FusedAdamW: a step inside a graph capture needs "
+                                   "capturable=True (its count would stand still)")
+            counted = set()
+            for n, ps, gs, sts in runs.values():
+                if on_device and id(n) not in counted:
+                    counted.add(id(n))
+                    n.add_(1)
+                self._run(group, n if on_device else n + 1, ps, gs, sts)
+                if not on_device:
+                    for st in sts:
+                        st["step"] = n + 1
+        return loss
+
+    @staticmethod
+    def _run(group, step, ps, gs, sts):
+        def state(k):
+            return [st[k] for st in sts]
+        eight = group["state_bits"] == 8
+        m, v = ("exp_avg_codes", "exp_avg_sq_codes") if eight else ("exp_avg", "exp_avg_sq")
+        _run(ps, gs, state(m), state(v), state("exp_avg_scales") if eight else None,
+             state("exp_avg_sq_scales") if eight else None, step, group["lr"], group["betas"],
+             group["eps"], group["weight_decay"], group["seed"])
+
+    def load_state_dict(self, state_dict) -> None:
+        """As torch.optim's, but each state keeps the dtype that it was saved in (torch casts
+        them to their parameter's)."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        for mine, its in zip(self.param_groups, state_dict["param_groups"]):
+            counts = {}
+            for p, i in zip(mine["params"], its["params"]):
+                if i not in saved:
+                    continue
+                st = self.state[p] = {
+                    k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                    for k, v in saved[i].items()}
+                n = int(st["step"])
+                if mine["capturable"]:
+                    if (p.device, n) not in counts:
+                        counts[p.device, n] = torch.full((), n, dtype=torch.int64, device=p.device)
+                    st["step"] = counts[p.device, n]
+                else:
+                    st["step"] = n

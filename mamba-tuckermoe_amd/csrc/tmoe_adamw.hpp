@@ -1,0 +1,274 @@
+// One AdamW step over many tensors (the reference trains with torch's AdamW,
+// pre-train/train.py:1263-1268), with the moments in fp32 or in 8 bits:
+//   m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+// 8-bit states hold m and r = sqrt(v) as e4m3 codes, each kAdamwBlock elements with one
+// fp32 scale, the block's largest value / 448. Rounding to nearest would hold a slow
+// average where it is: at b2 = 0.999 v moves by 1/1000 a step, half a code's step is 1/16.
+// Codes are therefore rounded to the lower or the upper neighbour at random, so that the
+// expected m, and the expected v = r^2, are the unrounded ones: m goes up with the chance
+// (a - lo) / (hi - lo), r with (a^2 - lo^2) / (hi^2 - lo^2). The random bits are a hash of
+// (seed, step, tensor, element), so a step repeated gives the same bits. A positive r is
+// never coded as zero: its element's step would be m / eps.
+//
+// Bound by memory (fp32 28 bytes an element). A launch takes up to kAdamwTensors tensors,
+// their addresses in its arguments: nothing is copied to the device, and a captured step
+// holds them. A work-group takes `chunk` elements of one tensor.
+#pragma once
+
+#include "tmoe_elem.hpp"
+#include "tmoe_train.h"
+
+namespace tmoe {
+namespace dev {
+
+constexpr int kAdamwTensors = 56;     // a launch's arguments hold 4 KB at most
+constexpr int kAdamwThreads = 256;
+constexpr float kE4m3Max = 448.f;
+
+struct AdamwTable {
+  void* p[kAdamwTensors];
+  const void* g[kAdamwTensors];
+  void* m[kAdamwTensors];
+  void* v[kAdamwTensors];
+  float* ms[kAdamwTensors];
+  float* vs[kAdamwTensors];
+  int64_t n[kAdamwTensors];
+  uint32_t end[kAdamwTensors];        // work-groups of this tensor and those before it
+  const int64_t* step_dev;
+  int64_t chunk;
+  double beta1, beta2, lr;            // read where the step is on the device
+  uint32_t seed, first;               // first: number of the launch's first tensor
+  int count;
+  float b1, ob1, b2, ob2, eps, keep, rate, inv_c2;
+};
+
+__host__ __device__ __forceinline__ uint32_t mix32(uint32_t h) {
+  h = (h ^ (h >> 16)) * 0x85EBCA6Bu;
+  h = (h ^ (h >> 13)) * 0xC2B2AE35u;
+  return h ^ (h >> 16);
+}
+
+struct AdamwStep {
+  float b1, ob1, b2, ob2, eps, keep, rate, inv_c2;
+  uint32_t key;
+  int64_t base;                       // the work-group's first element
+  int t;                              // its tensor
+};
+
+// The step's numbers and the work-group's place.
+__device__ __forceinline__ AdamwStep adamw_step(const AdamwTable& a) {
+  AdamwStep s{a.b1, a.ob1, a.b2, a.ob2, a.eps, a.keep, a.rate, a.inv_c2, 0u, 0, 0};
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (blockIdx.x < a.end[mid]) hi = mid;
+    else lo = mid + 1;
+  }
+  s.t = lo;
+  s.base = (int64_t)(blockIdx.x - (lo ? a.end[lo - 1] : 0u)) * a.chunk;
+  uint32_t step = 0u;
+  if (a.step_dev) {
+    __shared__ float c[2];
+    __shared__ uint32_t st;
+    if (threadIdx.x == 0) {
+      const double n = (double)*a.step_dev;
+      c[0] = (float)(a.lr / (1.0 - pow(a.beta1, n)));
+      c[1] = 1.f / (float)sqrt(1.0 - pow(a.beta2, n));
+      st = (uint32_t)*a.step_dev;
+    }
+    __syncthreads();
+    s.rate = c[0];
+    s.inv_c2 = c[1];
+    step = st;
+    s.key = mix32(a.seed + step * 0x9E3779B1u);
+  } else {
+    s.key = a.seed;                   // mixed on the host
+  }
+  return s;
+}
+
+// The new moments and parameter of one element, each operation rounded as it is written:
+// the 8-bit codes of one step decide the next one's values.
+__device__ __forceinline__ void adamw_moments(const AdamwStep& s, float g, float& m, float& v) {
+#pragma clang fp contract(off)
+  m = m * s.b1 + g * s.ob1;
+  v = v * s.b2 + g * g * s.ob2;
+}
+__device__ __forceinline__ float adamw_param(const AdamwStep& s, float p, float m, float root) {
+#pragma clang fp contract(off)
+  return p * s.keep - (m / (root * s.inv_c2 + s.eps)) * s.rate;
+}
+
+template <class T>
+__device__ __forceinline__ void load4(const T* p, float v[4]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 q = *reinterpret_cast<const float4*>(p);
+    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+  } else {
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
+    v[0] = bf16_bits_to_f32(q.x & 0xffffu); v[1] = bf16_bits_to_f32(q.x >> 16);
+    v[2] = bf16_bits_to_f32(q.y & 0xffffu); v[3] = bf16_bits_to_f32(q.y >> 16);
+  }
+}
+template <class T>
+__device__ __forceinline__ void store4(T* p, const float v[4]) {
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+
+template <class T>
+__global__ __launch_bounds__(kAdamwThreads) void k_adamw32(const AdamwTable a) {
+  const AdamwStep s = adamw_step(a);
+  T* p = static_cast<T*>(a.p[s.t]);
+  const T* g = static_cast<const T*>(a.g[s.t]);
+  float* m = static_cast<float*>(a.m[s.t]);
+  float* v = static_cast<float*>(a.v[s.t]);
+  const int64_t end = s.base + a.chunk < a.n[s.t] ? s.base + a.chunk : a.n[s.t];
+  const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) &
+                    (4 * sizeof(T) - 1)) == 0 &&
+                   ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
+  int64_t i = s.base + 4 * threadIdx.x;
+  if (vec) {
+    for (; i + 4 <= end; i += 4 * kAdamwThreads) {
+      float pv[4], gv[4], mv[4], vv[4];
+      load4(p + i, pv);
+      load4(g + i, gv);
+      load4(m + i, mv);
+      load4(v + i, vv);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        adamw_moments(s, gv[j], mv[j], vv[j]);
+        pv[j] = adamw_param(s, pv[j], mv[j], sqrtf(vv[j]));
+      }
+      store4(p + i, pv);
+      store4(m + i, mv);
+      store4(v + i, vv);
+    }
+  }
+  for (; i < end; i += 4 * kAdamwThreads)
+    for (int64_t j = i; j < i + 4 && j < end; ++j) {
+      float mv = m[j], vv = v[j];
+      adamw_moments(s, load_as_f32(g + j), mv, vv);
+      store_from_f32(p + j, adamw_param(s, load_as_f32(p + j), mv, sqrtf(vv)));
+      m[j] = mv;
+      v[j] = vv;
+    }
+}
+
+__device__ __forceinline__ float e4m3_value(uint32_t c) {
+  // exponent and mantissa moved to fp32's places; the multiplication by 2^120 moves the
+  // exponent's bias and normalises the subnormal codes, exactly
+  const float f = __uint_as_float((c & 0x7fu) << 20) * 0x1p+120f;
+  const float s = (c & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : f;
+  return c & 0x80u ? -s : s;
+}
+
+// The code of a in [0, 448]: the largest value lo that is no larger than a, or with the
+// chance described at the top its upper neighbour; kRoot: the chance is r's.
+template <bool kRoot>
+__device__ __forceinline__ uint32_t e4m3_code(float a, float u) {
+#pragma clang fp contract(off)
+  if (a != a) return 0x7fu;
+  const int e = max((int)(__float_as_uint(a) >> 23) - 127, -6);
+  const float step = __uint_as_float((uint32_t)(e + 124) << 23);
+  const float inv_step = __uint_as_float((uint32_t)(130 - e) << 23);
+  const float q = floorf(a * inv_step), lo = q * step;
+  float chance = (a - lo) * inv_step;
+  if (kRoot) chance = chance * ((a + lo) / (lo + lo + step));
+  uint32_t c = (uint32_t)q + ((uint32_t)(e + 6) << 3) + (u < chance ? 1u : 0u);
+  if (kRoot && c == 0u && a > 0.f) c = 1u;
+  return c;
+}
+
+// A wave takes blocks of 256 elements, four neighbours a lane.
+template <class T>
+__global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
+#pragma clang fp contract(off)
+  const AdamwStep s = adamw_step(a);
+  T* p = static_cast<T*>(a.p[s.t]);
+  const T* g = static_cast<const T*>(a.g[s.t]);
+  uint8_t* mq = static_cast<uint8_t*>(a.m[s.t]);
+  uint8_t* rq = static_cast<uint8_t*>(a.v[s.t]);
+  float* ms = a.ms[s.t];
+  float* rs = a.vs[s.t];
+  const int64_t n = a.n[s.t], end = s.base + a.chunk < n ? s.base + a.chunk : n;
+  const uint32_t tkey = (a.first + (uint32_t)s.t) * 0x9E3779B9u;
+  const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) &
+                    (4 * sizeof(T) - 1)) == 0 &&
+                   ((reinterpret_cast<uintptr_t>(mq) | reinterpret_cast<uintptr_t>(rq)) & 3) == 0;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int64_t b = s.base + wave * kAdamwBlock; b < end; b += kAdamwThreads / 64 * kAdamwBlock) {
+    const int64_t i = b + 4 * lane, blk = b / kAdamwBlock;
+    const int live = (int)(n - i < 4 ? (n - i < 0 ? 0 : n - i) : 4);
+    const float sm = ms[blk], sr = rs[blk];
+    float pv[4] = {}, gv[4] = {}, m[4], v[4], r[4];
+    uint32_t mc = 0u, rc = 0u;
+    if (vec && live == 4) {
+      load4(p + i, pv);
+      load4(g + i, gv);
+      mc = *reinterpret_cast<const uint32_t*>(mq + i);
+      rc = *reinterpret_cast<const uint32_t*>(rq + i);
+    } else {
+      for (int j = 0; j < live; ++j) {
+        pv[j] = load_as_f32(p + i + j);
+        gv[j] = load_as_f32(g + i + j);
+        mc |= (uint32_t)mq[i + j] << 8 * j;
+        rc |= (uint32_t)rq[i + j] << 8 * j;
+      }
+    }
+    float am = 0.f, ar = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = e4m3_value(mc >> 8 * j & 0xffu) * sm;
+      r[j] = e4m3_value(rc >> 8 * j & 0xffu) * sr;
+      v[j] = r[j] * r[j];
+      adamw_moments(s, gv[j], m[j], v[j]);
+      r[j] = sqrtf(v[j]);
+      pv[j] = adamw_param(s, pv[j], m[j], r[j]);
+      // NaN stays: a block that holds one gets a NaN scale
+      am = fabsf(m[j]) > am || m[j] != m[j] ? fabsf(m[j]) : am;
+      ar = r[j] > ar || r[j] != r[j] ? r[j] : ar;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const float om = __shfl_xor(am, o), orr = __shfl_xor(ar, o);
+      am = om > am || om != om ? om : am;
+      ar = orr > ar || orr != orr ? orr : ar;
+    }
+    const float nsm = am * (1.f / kE4m3Max), nsr = ar * (1.f / kE4m3Max);
+    const float dm = nsm > 0.f ? nsm : 1.f, dr = nsr > 0.f ? nsr : 1.f;
+    mc = rc = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t e = (uint64_t)(i + j);
+      const uint32_t h = mix32((tkey + (uint32_t)e + (uint32_t)(e >> 32) * 0xC2B2AE35u) ^ s.key);
+      const float um = ((float)(h >> 16) + 0.5f) * 0x1p-16f;
+      const float ur = ((float)(h & 0xffffu) + 0.5f) * 0x1p-16f;
+      const uint32_t cm = e4m3_code<false>(fminf(fabsf(m[j]) / dm, kE4m3Max), um);
+      const uint32_t cr = e4m3_code<true>(fminf(r[j] / dr, kE4m3Max), ur);
+      mc |= (cm | (m[j] < 0.f ? 0x80u : 0u)) << 8 * j;
+      rc |= cr << 8 * j;
+    }
+    if (vec && live == 4) {
+      store4(p + i, pv);
+      *reinterpret_cast<uint32_t*>(mq + i) = mc;
+      *reinterpret_cast<uint32_t*>(rq + i) = rc;
+    } else {
+      for (int j = 0; j < live; ++j) {
+        store_from_f32(p + i + j, pv[j]);
+        mq[i + j] = (uint8_t)(mc >> 8 * j);
+        rq[i + j] = (uint8_t)(rc >> 8 * j);
+      }
+    }
+    if (lane == 0) {
+      ms[blk] = nsm;
+      rs[blk] = nsr;
+    }
+  }
+}
+
+}  // namespace dev
+}  // namespace tmoe

@@ -17,6 +17,7 @@
 
 #include "tmoe.h"
 #include "tmoe_internal.h"
+#include "tmoe_train.h"
 
 struct tmoe_plan {
   tmoe_shape s;
@@ -369,6 +370,11 @@ hipError_t launch_cz(const tmoe::FwdArgs& f, hipStream_t st) {
 }
 
 }  // namespace
+
+namespace tmoe {
+int fail_text(int code, const char* text) { return fail(code, "%s", text); }
+void clear_error() { g_err[0] = 0; }
+}  // namespace tmoe
 
 extern "C" {
 

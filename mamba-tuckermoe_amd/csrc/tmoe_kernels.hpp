@@ -26,12 +26,12 @@
 
 #include <type_traits>
 
+#include "tmoe_elem.hpp"
 #include "tmoe_internal.h"
 
 namespace tmoe {
 namespace dev {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -42,24 +42,6 @@ struct EltBF16 {
 struct EltF32 {
   typedef float T;
 };
-
-__device__ __forceinline__ float bf16_bits_to_f32(uint32_t h) { return __uint_as_float(h << 16); }
-__device__ __forceinline__ uint16_t f32_to_bf16_bits(float f) {
-  return __builtin_bit_cast(uint16_t, (__bf16)f);   // round to nearest even
-}
-// Two floats to two bf16 (round to nearest even) in one register; as a vector
-// conversion this is a single v_cvt_pk_bf16_f32.
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-  const f32x2_t v = {lo, hi};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
-}
-
-__device__ __forceinline__ float load_as_f32(const uint16_t* p) { return bf16_bits_to_f32(*p); }
-__device__ __forceinline__ float load_as_f32(const float* p) { return *p; }
-__device__ __forceinline__ void store_from_f32(uint16_t* p, float v) { *p = f32_to_bf16_bits(v); }
-__device__ __forceinline__ void store_from_f32(float* p, float v) { *p = v; }
 
 // One 32x32 output block += A(32 x Ks) * B(Ks x 32), where one K step is 32
 // bytes of each operand row: lane l supplies row/column (l & 31) and the 16-byte

@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdint>
 #include <vector>
 
@@ -58,14 +59,31 @@ PyObject* none() {
   return Py_None;
 }
 
+}  // namespace
+
+#include "tmoe_torch_train.hpp"
+
+namespace {
+
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (bad_args(n, 5, "bind")) return nullptr;
+  if (bad_args(n, 13, "bind")) return nullptr;
   g_lib.workspace_bytes = reinterpret_cast<decltype(g_lib.workspace_bytes)>(address(a[0]));
   g_lib.signal_status = reinterpret_cast<decltype(g_lib.signal_status)>(address(a[1]));
   g_lib.forward_epi = reinterpret_cast<decltype(g_lib.forward_epi)>(address(a[2]));
   g_lib.forward_glu = reinterpret_cast<decltype(g_lib.forward_glu)>(address(a[3]));
   g_lib.rmsnorm_rows = reinterpret_cast<decltype(g_lib.rmsnorm_rows)>(address(a[4]));
+  auto to = [&](auto& f, int i) {
+    f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(address(a[i]));
+  };
+  to(g_train.last_error, 5);
+  to(g_train.router_workspace_bytes, 6);
+  to(g_train.router_forward, 7);
+  to(g_train.router_backward, 8);
+  to(g_train.norm_workspace_bytes, 9);
+  to(g_train.norm_forward, 10);
+  to(g_train.norm_backward, 11);
+  to(g_train.adamw_step, 12);
   return none();
   END_HANDLE_TH_ERRORS
 }
@@ -228,6 +246,9 @@ PyMODINIT_FUNC PyInit__tmoe_native() {
       {"signal", (PyCFunction)(void (*)())signal_, METH_FASTCALL, nullptr},
       {"forward", (PyCFunction)(void (*)())forward, METH_FASTCALL, nullptr},
       {"glu", (PyCFunction)(void (*)())glu, METH_FASTCALL, nullptr},
+      {"router", (PyCFunction)(void (*)())router, METH_FASTCALL, nullptr},
+      {"block_norm", (PyCFunction)(void (*)())block_norm, METH_FASTCALL, nullptr},
+      {"adamw", (PyCFunction)(void (*)())adamw, METH_FASTCALL, nullptr},
       {"rmsnorm", (PyCFunction)(void (*)())rmsnorm, METH_FASTCALL, nullptr},
       {nullptr, nullptr, 0, nullptr}};
   g_gen = PyUnicode_InternFromString("_tmoe_gen");

@@ -23,6 +23,7 @@ import torch
 
 from . import _lib
 from .module import device_guard, launch_stream
+from .train_ops import fused_router
 
 
 def _ws(nbytes: int, dev) -> torch.Tensor:
@@ -123,10 +124,17 @@ class TuckerMoETrain(torch.nn.Module):
     constructor, parameters (router.weight, U_expert, U_in, U_out, core, bias,
     inner_norm.weight) and forward(x, step) -> (out, lb_loss, z_loss). The latent
     expert contraction and its backward run on FusedLatentMoE (HIP); the router,
-    projections and losses are the reference's torch expressions."""
+    projections and losses are the reference's torch expressions, or with
+    fused_router=True the router and both losses are train_ops.fused_router: in float32
+    whatever x's dtype, the lowest index first on ties, `expert_counts` (E, int64) after
+    each forward, and forward takes a mask of tokens ((...) bool, False: left out of the
+    losses and of the contraction; its row of out is the bias)."""
 
-    def __init__(self, dim_in, dim_out, num_experts=8, top_k=2, r1=4, r2=1024, r3=256):
+    def __init__(self, dim_in, dim_out, num_experts=8, top_k=2, r1=4, r2=1024, r3=256,
+                 fused_router=False):
         super().__init__()
+        self.fused_router = fused_router
+        self.expert_counts = None
         self.num_experts = num_experts
         self.top_k = min(top_k, num_experts)
         self.router = torch.nn.Linear(dim_in, num_experts, bias=False)
@@ -142,11 +150,18 @@ class TuckerMoETrain(torch.nn.Module):
         torch.nn.init.xavier_uniform_(self.U_expert)
         torch.nn.init.xavier_uniform_(self.core)
 
-    def forward(self, x, step=None):
-        orig = x.shape
-        xf = x.reshape(-1, orig[-1])
+    def _route(self, xf, step, mask):
+        """(idx, top_p, lb_loss, z_loss)."""
         temperature = router_temperature(step)
         raw = self.router(xf)
+        if self.fused_router:
+            if mask is not None:
+                mask = mask.reshape(-1)
+            idx, top_p, lb_loss, z_loss, self.expert_counts = fused_router(
+                raw, self.top_k, temperature, 10.0, mask)
+            return (idx, top_p, lb_loss, z_loss) if self.training else (idx, top_p, 0.0, 0.0)
+        if mask is not None:
+            raise RuntimeError("TuckerMoETrain: a mask needs fused_router=True")
         capped = scaled_tanh(raw, 10.0)
         z_loss = torch.mean(torch.logsumexp(capped, dim=-1) ** 2) if self.training else 0.0
         logits = capped / temperature
@@ -159,6 +174,12 @@ class TuckerMoETrain(torch.nn.Module):
             lb_loss = self.num_experts * torch.sum(mask.mean(0) * probs.float().mean(0))
         else:
             lb_loss = 0.0
+        return idx, top_p, lb_loss, z_loss
+
+    def forward(self, x, step=None, mask=None):
+        orig = x.shape
+        xf = x.reshape(-1, orig[-1])
+        idx, top_p, lb_loss, z_loss = self._route(xf, step, mask)
         xs = self.inner_norm(torch.matmul(xf, self.U_in))
         G = torch.einsum("er,rst->est", self.U_expert, self.core)
         core = FusedLatentMoE.apply(xs, G, idx, top_p).to(x.dtype)

@@ -1,0 +1,699 @@
+"""The training operators around the expert contraction on the GPU against the float64 oracle
+(oracle/train_ops_np.py).
+
+Tolerances: a float32 evaluation of n rounded steps is off by at most n 2^-24 times the sum of
+its terms' magnitudes (the oracle's *_mag), and a result stored in bfloat16 by another half
+step, 2^-8 of itself. n: a norm's value is made of under 64 operations on top of a sum over a
+row, whose longest chain is 64 elements of a thread, 6 exchanges in a wave and 16 waves; a
+column's sum adds its rows' chain (under T / 4) and 80 planes. In the router the capped logit
+is cap times a tanh that is off by under 8 steps, and enters an exponential twice over tau."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import train_ops_np as tn
+from oracle import tucker_moe_np as onp
+from test_train_ops import NORM_FORMS, norm_inputs
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+dtypes = pytest.mark.parametrize("dtype", list(DTYPES.values()), ids=list(DTYPES))
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def near(got, want, mag, n, what=""):
+    """got within n steps of float32 (and its own rounding) of want."""
+    g = f64(got)
+    tol = n * U * np.abs(mag) + 1e-37
+    if got.dtype == torch.bfloat16:
+        tol = tol * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(want) + 1e-38
+    bad = ~(np.abs(g - want) <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float(np.max(np.abs(g - want) / tol)))
+
+
+# ---- router ---------------------------------------------------------------------
+
+def _logits(B, E, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(B, E, generator=g) * 3 + torch.randn(B, 1, generator=g) * 4).to(dtype)
+
+
+def _check_router(pkg, raw, k, tau, cap, mask, seed, call=None):
+    B, E = raw.shape
+    g = torch.Generator().manual_seed(seed + 1)
+    dw, dlb, dz = torch.randn(B, k, generator=g), torch.tensor(0.7), torch.tensor(0.05)
+    leaf = raw.detach().requires_grad_()
+    r = call(leaf) if call else pkg.fused_router(leaf, k, tau, cap, mask)
+    draw, = torch.autograd.grad((r.weights, r.lb_loss, r.z_loss), leaf,
+                                (dw.to(raw.device), dlb.to(raw.device), dz.to(raw.device)))
+    assert draw.dtype == raw.dtype and r.idx.dtype == r.counts.dtype == torch.int64
+    tau = float(tau)
+    o = tn.router(f64(raw), k, tau, cap, None if mask is None else mask.cpu().numpy(), dw.numpy(), 0.7, 0.05)
+    n = 16 * cap / tau + 128
+    assert np.array_equal(r.idx.cpu().numpy(), o["idx"])
+    assert np.array_equal(r.counts.cpu().numpy(), o["counts"])
+    near(r.weights, o["w"], o["w"], n, "w")
+    near(r.lb_loss, o["lb"], o["lb"], n, "lb")
+    near(r.z_loss, o["z"], 2 * np.sqrt(o["z"]) * (8 * cap + 32) + 16 * o["z"], 1, "z")
+    near(draw, o["draw"], o["draw_mag"], 4 * n, "draw")
+
+
+@dtypes
+@pytest.mark.parametrize("B,E,k,tau,padded", [
+    (1, 1, 1, 0.5, 0), (1, 8, 2, 0.5, 0), (5, 3, 3, 2.0, 0), (257, 8, 2, 1.1, 0.3), (1000, 33, 5, 0.5, 0.5),
+    (4096, 16, 2, 2.0, 0), (333, 64, 16, 0.9, 0.1), (129, 100, 4, 1.0, 0), (70, 256, 8, 0.5, 0.2),
+    (20001, 8, 2, 0.5, 0.25), (300, 255, 16, 1.5, 0)])
+def test_router(pkg, dev, B, E, k, tau, padded, dtype):
+    mask = None
+    if padded:
+        mask = (torch.rand(B, generator=torch.Generator().manual_seed(B)) >= padded).to(dev)
+    _check_router(pkg, _logits(B, E, dtype, B + E).to(dev), k, tau, 10.0, mask, B)
+
+
+def test_router_strides_cap_and_no_grad(pkg, dev):
+    wide = _logits(77, 40, torch.float32, 3).to(dev)
+    for raw in (wide[:, 8:24], wide[:, 1:12], wide.t()[:, :30], wide[::3, :16], wide[:1].expand(9, 40)):
+        _check_router(pkg, raw, 2, 0.7, 4.0, None, 5)
+    mask = (torch.arange(154, device=dev) % 3 > 0)[::2]
+    _check_router(pkg, wide, 3, 0.7, 30.0, mask, 5)
+    with torch.no_grad():
+        a = pkg.fused_router(wide.requires_grad_(), 2, 0.5)
+    b = pkg.fused_router(wide, 2, 0.5)
+    assert not a.weights.requires_grad and b.weights.requires_grad and not b.idx.requires_grad
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+def test_router_ties_and_extremes(pkg, dev):
+    """Equal logits: the lowest index; infinities; logits far past the cap, which is flat there
+    in float32 but whose order is the logits' own; -0 is 0."""
+    inf = float("inf")
+    raw = torch.tensor([[1.0, 3, 3, 2, 3, 3, -1, 3], [0.0, -0.0, 0, 0, -0.0, 0, 0, 0],
+                        [500.0, 400, 900, 800, 1e30, 3e38, 2, 1], [-inf, -inf, 5, -inf, 4, -inf, -inf, -inf],
+                        [inf, 0, inf, 1, 2, 3, 4, 5], [-inf] * 8, [-1e30] * 7 + [-2e30]], device=dev)
+    for dt in DTYPES.values():
+        _check_router(pkg, raw.to(dt), 3, 0.5, 10.0, None, 1)
+
+
+def test_router_no_tokens(pkg, dev):
+    """No tokens, and none that the mask leaves: zero losses, counts and gradients; what the
+    left-out rows hold does not matter, and a NaN row spoils its own row alone."""
+    r = pkg.fused_router(torch.empty(0, 8, device=dev).requires_grad_(), 2, 0.5)
+    assert r.idx.shape == (0, 2) and r.lb_loss.item() == r.z_loss.item() == 0 and not r.counts.any()
+    assert torch.autograd.grad(r.lb_loss + r.z_loss + r.weights.sum(), r.weights.grad_fn.next_functions[0][0].variable)[
+        0].shape == (0, 8)
+    raw = torch.full((5, 8), float("nan"), device=dev).requires_grad_()
+    r = pkg.fused_router(raw, 2, 0.5, mask=torch.zeros(5, dtype=torch.bool, device=dev))
+    d, = torch.autograd.grad(r.lb_loss + r.z_loss + r.weights.sum(), raw)
+    assert r.lb_loss.item() == r.z_loss.item() == 0 and not r.counts.any() and not d.any()
+    assert (r.idx == -1).all() and not r.weights.any()
+    raw = _logits(300, 8, torch.float32, 2).to(dev)
+    mask = torch.ones(300, dtype=torch.bool, device=dev)
+    mask[7] = mask[250] = False
+    raw[7], raw[250, 3] = float("nan"), float("inf")
+    _check_router(pkg, raw, 2, 0.5, 10.0, mask, 3)
+    r = pkg.fused_router(raw, 2, 0.5)                       # row 7 counts now
+    assert r.idx[7].tolist() == [0, 1] and r.weights[7].isnan().all()
+    assert r.weights[torch.arange(300, device=dev) != 7].isfinite().all()
+    raw[7] = 0.0
+    raw[7, 5] = float("nan")                                # a NaN ranks first
+    assert pkg.fused_router(raw, 2, 0.5).idx[7].tolist() == [5, 0]
+
+
+def test_router_partial_gradients(pkg, dev):
+    """Each of the three alone; a temperature on the device; weights' gradient strided."""
+    raw = _logits(200, 8, torch.float32, 9).to(dev).requires_grad_()
+    tau = torch.tensor(0.8, device=dev)
+    _check_router(pkg, raw, 2, tau, 10.0, None, 4)
+    r = pkg.fused_router(raw, 2, torch.tensor(0.8))          # on the CPU: a number
+    s = pkg.fused_router(raw, 2, 0.8)
+    assert torch.equal(r.weights, s.weights)
+    dw = torch.randn(2, 200, device=dev).t()
+    for i, (out, seed) in enumerate(((r.weights, dw), (r.lb_loss, None), (r.z_loss, None))):
+        got, = torch.autograd.grad(out, raw, seed, retain_graph=True)
+        z = [np.zeros((200, 2)), 0.0, 0.0]
+        z[i] = f64(dw) if i == 0 else 1.0
+        o = tn.router(f64(raw), 2, np.float64(np.float32(0.8)), 10.0, None, *z)
+        near(got, o["draw"], o["draw_mag"], 4 * (160 / 0.8 + 128))
+
+
+# ---- block norm -----------------------------------------------------------------
+
+def _check_norm(pkg, n, dr, dh, eps=1e-5, shape=None):
+    """n: operands on the device (any strides), checked forward and backward."""
+    leaf = {k: v.detach().requires_grad_() for k, v in n.items()}
+    r, h = pkg.fused_block_norm(**leaf, eps=eps)
+    outs, seeds = [r], [dr]
+    if h is not None:
+        outs.append(h)
+        seeds.append(dh)
+    grads = torch.autograd.grad(outs, list(leaf.values()), seeds)
+    d = n["y"].shape[-1]
+
+    def flat(t):
+        return f64(t).reshape(-1, d) if t.dim() != 1 or t.shape == n["y"].shape else f64(t)
+    o = tn.block_norm(**{k: flat(v) for k, v in n.items()}, eps=eps, dr=flat(dr),
+                      dh=flat(dh) if h is not None else None)
+    T = n["y"].numel() // d
+    steps = 64 + 64 + 6 + 16
+    near(r.reshape(-1, d), o["r"], o["r_mag"], steps, "r")
+    if h is not None:
+        near(h.reshape(-1, d), o["h"], o["h_mag"], steps, "h")
+    for k, g in zip(leaf, grads):
+        assert g.dtype == n[k].dtype and g.shape == n[k].shape
+        col = n[k].dim() == 1 and n[k].shape != n["y"].shape
+        near(g if col else g.reshape(-1, d), o["d" + k], o["d" + k + "_mag"],
+             2 * steps + (T / 4 + 80 if col else 0), "d" + k)
+    with torch.no_grad():
+        r2, h2 = pkg.fused_block_norm(**leaf, eps=eps)
+    assert torch.equal(r, r2) and (h is None or torch.equal(h, h2)) and not r2.requires_grad
+
+
+@dtypes
+@pytest.mark.parametrize("form", NORM_FORMS, ids="+".join)
+def test_norm_forms(pkg, dev, form, dtype):
+    for T, d in ((1, 768), (37, 320), (19, 1001), (4, 2304)):
+        n, dr, dh = norm_inputs(form, T, d, T, dtype)
+        _check_norm(pkg, {k: v.to(dev) for k, v in n.items()}, dr.to(dev), dh.to(dev))
+
+
+@dtypes
+@pytest.mark.parametrize("T,d", [(1, 1), (2, 7), (3, 33), (5, 64), (130, 512), (67, 520), (33, 1024), (9, 1032),
+                                 (2049, 768), (4100, 72), (5, 4608), (3, 8192), (2, 8200), (2, 9999), (3, 16384)])
+def test_norm_sizes(pkg, dev, T, d, dtype):
+    n, dr, dh = norm_inputs(NORM_FORMS[-1], T, d, T + d, dtype)
+    _check_norm(pkg, {k: v.to(dev) for k, v in n.items()}, dr.to(dev), dh.to(dev))
+
+
+@dtypes
+def test_norm_strides(pkg, dev, dtype):
+    """Halves of one projection, rows at an odd stride, leading axes, a transposed operand, an
+    expanded gradient: as the contiguous ones."""
+    T, d = 24, 136
+    n, dr, dh = norm_inputs(("x", "y", "gate", "gamma", "next"), T, d, 5, dtype)
+    n = {k: v.to(dev) for k, v in n.items()}
+    dr, dh = dr.to(dev), dh.to(dev)
+    both = torch.cat([n["y"], n["gate"]], -1)
+    odd = torch.zeros(T, d + 3, dtype=dtype, device=dev)
+    odd[:, 1:d + 1] = n["x"]
+    _check_norm(pkg, {**n, "y": both[:, :d], "gate": both[:, d:]}, dr, dh)
+    _check_norm(pkg, {**n, "x": odd[:, 1:d + 1]}, dr, dh)
+    _check_norm(pkg, {**n, "x": n["x"].t().contiguous().t()}, dr[:1].expand(T, d), dh)
+    lead = {k: v.view(2, 3, 4, d) if v.dim() == 2 else v for k, v in n.items()}
+    lead["y"], lead["gate"] = both.view(2, 3, 4, 2 * d)[..., :d], both.view(2, 3, 4, 2 * d)[..., d:]
+    lead["x"] = n["x"].view(2, 3, 4, d).transpose(0, 1).contiguous().transpose(0, 1)
+    _check_norm(pkg, lead, dr.view(2, 3, 4, d), dh.view(2, 3, 4, d))
+    one = {k: v[0] if v.dim() == 2 else v for k, v in n.items()}
+    _check_norm(pkg, one, dr[0], dh[0])
+    w = torch.stack([n["gamma"], n["next_weight"]], -1)        # weights that are not contiguous
+    _check_norm(pkg, {**n, "gamma": w[:, 0], "next_weight": w[:, 1]}, dr, dh)
+
+
+def test_norm_first_block_and_partial_gradients(pkg, dev):
+    """x alone with the next norm; gradients through r alone, h alone, of some operands only."""
+    n, dr, dh = norm_inputs(("x", "y", "gamma", "next"), 50, 200, 8)
+    n = {k: v.to(dev).requires_grad_() for k, v in n.items()}
+    dr, dh = dr.to(dev), dh.to(dev)
+    x, w = n["x"], n["next_weight"]
+    r, h = pkg.fused_block_norm(x, next_weight=w)
+    assert r is x
+    dx, dw = torch.autograd.grad(h, (x, w), dh)
+    o = tn.block_norm(y=f64(x), next_weight=f64(w), dr=np.zeros((50, 200)), dh=f64(dh))
+    near(h, o["h"], o["h_mag"], 150)
+    near(dx, o["dy"], o["dy_mag"], 300)
+    near(dw, o["dnext_weight"], o["dnext_weight_mag"], 400)
+    r, h = pkg.fused_block_norm(**n)
+    zero = np.zeros((50, 200))
+    for out, seed, a, b in ((r, dr, f64(dr), None), (h, dh, zero, f64(dh))):
+        o = tn.block_norm(**{k: f64(v) for k, v in n.items()}, dr=a, dh=zero if b is None else b)
+        grads = torch.autograd.grad(out, list(n.values()), seed, retain_graph=True)
+        for k, g in zip(n, grads):
+            near(g, o["d" + k], o["d" + k + "_mag"], 400, k)
+    full = torch.autograd.grad((r, h), list(n.values()), (dr, dh), retain_graph=True)
+    for k, g in zip(n, full):           # one at a time, the same bits
+        assert torch.equal(torch.autograd.grad((r, h), n[k], (dr, dh), retain_graph=True)[0], g), k
+    y = n["y"].detach()
+    r, h = pkg.fused_block_norm(n["x"], y, gamma=n["gamma"].detach())
+    assert torch.equal(torch.autograd.grad(r, n["x"], dr)[0], dr) and h is None
+
+
+def test_norm_empty_and_extreme_rows(pkg, dev):
+    n, dr, dh = norm_inputs(NORM_FORMS[-1], 0, 64, 1)
+    leaf = {k: v.to(dev).requires_grad_() for k, v in n.items()}
+    r, h = pkg.fused_block_norm(**leaf)
+    assert r.shape == h.shape == (0, 64)
+    for k, g in zip(leaf, torch.autograd.grad((r, h), list(leaf.values()), (r.detach(), h.detach()))):
+        assert g.shape == leaf[k].shape and not g.any(), k
+    # a row of zeros (rms = sqrt(eps)), huge and tiny rows, saturated gates
+    n, dr, dh = norm_inputs(NORM_FORMS[-1], 6, 192, 2)
+    for k in ("x", "y"):
+        n[k][0] = 0
+        n[k][1] *= 1e12
+        n[k][2] *= 1e-12
+    n["gate"][3], n["gate"][4] = 60.0, -60.0
+    n["gate"][0, :5] = 0
+    _check_norm(pkg, {k: v.to(dev) for k, v in n.items()}, dr.to(dev), dh.to(dev))
+    # a row that is not finite leaves the others as they are
+    m = {k: v.to(dev) for k, v in n.items()}
+    r, h = pkg.fused_block_norm(**m)
+    m["y"] = m["y"].clone()
+    m["y"][5, 3] = float("nan")
+    r2, h2 = pkg.fused_block_norm(**m)
+    assert torch.equal(r[:5], r2[:5]) and torch.equal(h[:5], h2[:5]) and h2[5].isnan().all()
+
+
+# ---- AdamW ----------------------------------------------------------------------
+
+SHAPES = [(3,), (), (256,), (257,), (1,), (31, 33), (4, 64, 65), (1000, 130), (0, 5), (2, 255)]
+
+
+def _adamw_inputs(dev, dtype, seed, shapes=SHAPES):
+    g = torch.Generator().manual_seed(seed)
+    p = [(torch.randn(s, generator=g) * 0.05).to(dtype).to(dev) for s in shapes]
+    gr = [(torch.randn(s, generator=g) * 0.01).to(dtype).to(dev) for s in shapes]
+    m = [(torch.randn(s, generator=g) * 0.003).to(dev) for s in shapes]
+    v = [(torch.rand(s, generator=g) * 1e-4).to(dev) for s in shapes]
+    return p, gr, m, v
+
+
+HYPER = dict(lr=2e-3, betas=(0.9, 0.97), eps=1e-8, weight_decay=0.1)
+
+
+def _oracle(p, g, m, v, step, h=HYPER):
+    return tn.adamw(f64(p), f64(g), f64(m) if torch.is_tensor(m) else m, f64(v) if torch.is_tensor(v) else v, step,
+                    h["lr"], *h["betas"], h["eps"], h["weight_decay"])
+
+
+@dtypes
+@pytest.mark.parametrize("step", [1, 7, 100000])
+def test_adamw_32(pkg, dev, dtype, step):
+    p, g, m, v = _adamw_inputs(dev, dtype, step)
+    want = [_oracle(*t, step) for t in zip(p, g, m, v)]
+    vers = [t._version for t in p]
+    pkg.adamw_step(p, g, m, v, step=step, **HYPER)
+    for i, o in enumerate(want):
+        near(m[i], o["m"], o["m_mag"], 8, "m")
+        near(v[i], o["v"], o["v_mag"], 8, "v")
+        near(p[i], o["p"], o["p_mag"], 32, "p")
+        assert p[i]._version > vers[i]
+
+
+def test_adamw_layouts_and_many(pkg, dev):
+    """Transposed parameters with gradients in another order, views at odd offsets, more tensors
+    than one launch takes; a step count on the device."""
+    shapes = [(5, 9)] * 130 + [(300, 7)]
+    p, g, m, v = _adamw_inputs(dev, torch.float32, 4, shapes)
+    p[0], m[0], v[0] = (t[0].t().contiguous().t() for t in (p, m, v))
+    base = torch.zeros(200, device=dev)
+    p[1] = base[1:46].view(5, 9)
+    m[2] = torch.zeros(100, device=dev)[3:48].view(5, 9)
+    want = [_oracle(*t, 12) for t in zip(p, g, m, v)]
+    pkg.adamw_step(p, g, m, v, step=torch.tensor(12, device=dev), **HYPER)
+    for i, o in enumerate(want):
+        near(p[i], o["p"], o["p_mag"], 32, i)
+        near(m[i], o["m"], o["m_mag"], 8, i)
+    assert not base[0].any() and not base[46:].any()
+
+
+def test_adamw_zero_gradient_and_nonfinite(pkg, dev):
+    p, g, m, v = _adamw_inputs(dev, torch.float32, 5, [(700,)])
+    g[0].zero_()
+    m[0].zero_()
+    v[0].zero_()
+    q = p[0].clone()
+    pkg.adamw_step(p, g, m, v, step=1, **HYPER)             # 0 / (0 + eps)
+    assert torch.allclose(p[0], q * (1 - 2e-4), rtol=1e-6, atol=0) and not m[0].any()
+    g[0][5] = float("nan")
+    pkg.adamw_step(p, g, m, v, step=2, **HYPER)
+    ok = torch.arange(700, device=dev) != 5
+    assert p[0][5].isnan() and p[0][ok].isfinite().all()
+
+
+def _codes(t, root):
+    """float32 values as nearest codes and scales, on the CPU."""
+    n = t.numel()
+    b = torch.nn.functional.pad(t.reshape(-1).float(), (0, -n % 256)).view(-1, 256)
+    s = b.abs().amax(1) / 448.0
+    q = (b / torch.where(s > 0, s, 1.0)[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+    return q.view(torch.uint8).view(-1)[:n].clone().view(torch.float8_e4m3fn), s
+
+
+def _inputs8(dev, dtype, seed, shapes=SHAPES):
+    p, g, m, v = _adamw_inputs(dev, dtype, seed, shapes)
+    mq, ms = zip(*[_codes(t.cpu(), False) for t in m])
+    rq, rs = zip(*[_codes(t.cpu().sqrt(), True) for t in v])
+    return p, g, *[[t.to(dev) for t in l] for l in (mq, ms, rq, rs)]
+
+
+@dtypes
+@pytest.mark.parametrize("step", [1, 9])
+def test_adamw_8(pkg, dev, dtype, step):
+    """The parameters against the oracle from the decoded states; the scales; each code against
+    the oracle's with the same numbers: equal but where the chance is within rounding of the
+    number, and there one code off."""
+    p, g, mq, ms, rq, rs = _inputs8(dev, dtype, step)
+    old = [(tn.decode8(a.view(torch.uint8).cpu().numpy(), f64(b)), tn.decode8(c.view(torch.uint8).cpu().numpy(), f64(d)))
+           for a, b, c, d in zip(mq, ms, rq, rs)]
+    want = [_oracle(a, b, m.reshape(a.shape), (r * r).reshape(a.shape), step) for a, b, (m, r) in zip(p, g, old)]
+    pkg.adamw_step_8bit(p, g, mq, ms, rq, rs, step=step, seed=77, **HYPER)
+    differ = total = 0
+    for i, o in enumerate(want):
+        near(p[i], o["p"], o["p_mag"], 40, "p")
+        n = p[i].numel()
+        um, ur = tn.randoms(n, i, 77, step)
+        for q, s, t, root, u in ((mq[i], ms[i], o["m"], False, um), (rq[i], rs[i], o["v"], True, ur)):
+            c, sc = tn.encode8(t.reshape(-1), root, u)
+            near(s, sc, sc, 12, "scale")
+            got = q.view(torch.uint8).cpu().numpy().astype(int)
+            off = np.abs((got & 127) - (c.astype(int) & 127))
+            assert (off <= 1).all() and ((got & 128) == (c & 128))[off == 0].all()
+            differ += int((off > 0).sum())
+            total += n
+    # a float32 chance is off by under 64 steps of its argument's 16 places: 2^-14 of the draws at most
+    assert differ <= 2.0 ** -14 * total + 1, (differ, total)
+
+
+def test_adamw_8_is_repeatable_and_seeded(pkg, dev):
+    runs = []
+    for seed in (5, 5, 6):
+        p, g, mq, ms, rq, rs = _inputs8(dev, torch.float32, 3)
+        for step in (1, 2, 3):
+            pkg.adamw_step_8bit(p, g, mq, ms, rq, rs, step=step, seed=seed, **HYPER)
+        runs.append([t.view(torch.uint8).clone() for t in mq + rq] + [t.clone() for t in p])
+    assert all(torch.equal(a, b) for a, b in zip(runs[0], runs[1]))
+    assert not all(torch.equal(a, b) for a, b in zip(runs[0], runs[2]))
+    p, g, mq, ms, rq, rs = _inputs8(dev, torch.float32, 3)       # uint8 bits, the step on the device
+    for step in (1, 2, 3):
+        pkg.adamw_step_8bit(p, g, [t.view(torch.uint8) for t in mq], ms, [t.view(torch.uint8) for t in rq], rs,
+                            step=torch.tensor(step, device=dev), seed=5, **HYPER)
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(runs[0], mq + rq))
+
+
+def test_adamw_8_slow_average_reaches_its_value(pkg, dev):
+    """beta2 = 0.99 and one gradient for 400 steps: v must come to (1 - beta2^t) g^2 in the mean
+    (rounded to nearest it stands still at a tenth of it). The relative deviation of one
+    element's v is under the walk's, sqrt(sum of its steps' variances) < 0.5; of the mean of
+    65536 of them six deviations are 1.2%."""
+    n = 65536
+    g = [torch.full((n,), 0.01, device=dev)]
+    g[0][::256] = 0.02                                      # each block's scale is another element's
+    p, codes = [torch.zeros(n, device=dev)], lambda: [torch.zeros(n, dtype=torch.uint8, device=dev)]
+    scales = lambda: [torch.zeros(n // 256, device=dev)]
+    mq, ms, rq, rs = codes(), scales(), codes(), scales()
+    for step in range(1, 401):
+        pkg.adamw_step_8bit(p, g, mq, ms, rq, rs, step=step, lr=1e-4, betas=(0.9, 0.99), weight_decay=0.0, seed=1)
+    from mamba_tuckermoe_amd.adamw import dequantize_state
+    v = dequantize_state(rq[0], rs[0]).double() ** 2
+    m = dequantize_state(mq[0], ms[0]).double()
+    want = 1 - 0.99 ** 400
+    assert abs((v / g[0].double() ** 2).mean().item() / want - 1) < 0.012
+    assert abs((m / g[0].double()).mean().item() - 1) < 0.012
+    assert rq[0].min() > 0
+
+
+def test_adamw_8_zero_and_nonfinite_blocks(pkg, dev):
+    n = 1024
+    p, g, mq, ms, rq, rs = _inputs8(dev, torch.float32, 2, [(n,)])
+    g[0].zero_()
+    for t in mq + rq:
+        t.view(torch.uint8).zero_()
+    q = p[0].clone()
+    pkg.adamw_step_8bit(p, g, mq, ms, rq, rs, step=1, **HYPER)
+    assert torch.allclose(p[0], q * (1 - 2e-4), rtol=1e-6, atol=0)
+    assert not ms[0].any() and not rs[0].any() and not rq[0].view(torch.uint8).any()
+    g[0].fill_(0.01)
+    g[0][300] = float("inf")
+    pkg.adamw_step_8bit(p, g, mq, ms, rq, rs, step=2, **HYPER)
+    ok = torch.ones(n, dtype=torch.bool, device=dev)
+    ok[256:512] = False
+    pkg.adamw_step_8bit(p, g, mq, ms, rq, rs, step=3, **HYPER)
+    assert p[0][ok].isfinite().all() and not p[0][300].isfinite()
+    assert ms[0][[0, 2, 3]].isfinite().all() and not ms[0][1].isfinite()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_against_torch(pkg, dev, bits):
+    """FusedAdamW over steps with a parameter that gets its gradients late; 32-bit states
+    against torch's AdamW in float64, 8-bit ones against the functional call."""
+    torch.manual_seed(0)
+    ps = [torch.nn.Parameter(torch.randn(s, device=dev) * 0.05) for s in ((70, 40), (300,), (9,))]
+    ref = [torch.nn.Parameter(p.detach().double()) for p in ps]
+    opt = pkg.FusedAdamW(ps, state_bits=bits, seed=3, **HYPER)
+    topt = torch.optim.AdamW(ref, **HYPER)
+    for step in range(1, 6):
+        for i, (p, r) in enumerate(zip(ps, ref)):
+            if i == 2 and step < 3:
+                continue
+            p.grad = torch.randn(p.shape, device=dev) * 0.01
+            r.grad = p.grad.double()
+        opt.step()
+        topt.step()
+    assert opt.state[ps[0]]["step"] == 5 and opt.state[ps[2]]["step"] == 3
+    for p, r in zip(ps, ref):
+        if bits == 32:
+            # five steps of 32 roundings of p and of updates of lr
+            assert (p.double() - r).abs().max() <= 5 * 32 * U * (r.abs().max() + 10 * HYPER["lr"])
+        else:
+            # an update is at most lr |m| / sqrt(v); states off by a code, 1/8, in each
+            assert (p.double() - r).abs().max() <= 5 * HYPER["lr"] * 4
+
+
+# ---- streams, graphs, autograd ---------------------------------------------------
+
+def test_side_stream(pkg, dev):
+    raw = _logits(5000, 16, torch.float32, 1).to(dev)
+    n, dr, dh = norm_inputs(NORM_FORMS[-1], 500, 256, 1)
+    n = {k: v.to(dev) for k, v in n.items()}
+    dr, dh = dr.to(dev), dh.to(dev)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        _check_router(pkg, raw, 2, 0.5, 10.0, None, 1)
+        _check_norm(pkg, n, dr, dh)
+        p, g, m, v = _adamw_inputs(dev, torch.float32, 1)
+        want = [_oracle(*t, 3) for t in zip(p, g, m, v)]
+        pkg.adamw_step(p, g, m, v, step=3, **HYPER)
+        for i, o in enumerate(want):
+            near(p[i], o["p"], o["p_mag"], 32)
+    torch.cuda.synchronize()
+
+
+def test_graph_capture(pkg, dev):
+    """Router, norm and optimizer step captured with their backward: each replay on new inputs
+    gives what the eager calls give, the step counting on; eager work between the replays."""
+    torch.manual_seed(0)
+    T, d, E, k = 600, 192, 8, 2
+    x, y = torch.randn(T, d, device=dev), torch.randn(T, d, device=dev)
+    tau = torch.tensor(0.5, device=dev)
+
+    def params():
+        g = torch.Generator().manual_seed(4)
+        return [torch.nn.Parameter((torch.randn(s, generator=g) * 0.1 + 1).to(dev)) for s in ((d,), (d,), (d, E))]
+
+    def body(ps, opt):
+        gamma, w, router = ps
+        r, h = pkg.fused_block_norm(x, y, gamma=gamma, next_weight=w)
+        q = pkg.fused_router(h @ router, k, tau)
+        loss = (q.weights * q.weights).sum() / T + q.lb_loss + q.z_loss + (r * r).mean()
+        grads = torch.autograd.grad(loss, ps)
+        for p, g in zip(ps, grads):
+            p.grad = g
+        opt.step()
+        return q.idx, q.counts, loss.detach()
+    ps, ref = params(), params()
+    opt = pkg.FusedAdamW(ps, state_bits=8, capturable=True, lr=1e-2)
+    ropt = pkg.FusedAdamW(ref, state_bits=8, lr=1e-2)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        body(ps, opt)
+    torch.cuda.synchronize()
+    body(ref, ropt)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        out = body(ps, opt)
+    for i in range(4):
+        x.copy_(torch.randn(T, d, device=dev))
+        tau.fill_(0.5 + 0.3 * i)
+        graph.replay()
+        want = body(ref, ropt)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), i
+        for a, b in zip(ps, ref):
+            # lr / (1 - beta^t): the device's pow and the host's may differ in the last place
+            assert (a - b).abs().max() <= 1e-2 * 16 * U + 8 * U * b.abs().max(), i
+        with torch.no_grad():
+            for a, b in zip(ref, ps):
+                a.copy_(b)
+    assert opt.state[ps[0]]["step"].item() == 5 == ropt.state[ref[0]]["step"]
+
+
+def test_step_in_capture_needs_capturable(pkg, dev):
+    p = torch.nn.Parameter(torch.ones(8, device=dev))
+    p.grad = torch.ones_like(p)
+    opt = pkg.FusedAdamW([p])
+    opt.step()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="capturable"):
+        with torch.cuda.graph(g):
+            opt.step()
+    torch.cuda.synchronize()
+    assert opt.state[p]["step"] == 1
+
+
+def test_capturable_state_is_loaded_shared(pkg, dev):
+    ps = [torch.nn.Parameter(torch.ones(8, device=dev)) for _ in range(3)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt = pkg.FusedAdamW(ps, capturable=True)
+    opt.step()
+    opt.step()
+    opt2 = pkg.FusedAdamW(ps, capturable=True)
+    opt2.load_state_dict(opt.state_dict())
+    steps = [opt2.state[p]["step"] for p in ps]
+    assert all(s is steps[0] for s in steps) and steps[0].dtype == torch.int64
+    opt2.step()
+    assert steps[0].item() == 3 and opt.state[ps[0]]["step"].item() == 2
+
+
+def test_second_derivatives_are_refused(pkg, dev):
+    raw = _logits(4, 8, torch.float32, 0).to(dev).requires_grad_()
+    g, = torch.autograd.grad(pkg.fused_router(raw, 2, 0.5).z_loss, raw, create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        g.sum().backward()
+    x = torch.randn(4, 8, device=dev, requires_grad=True)
+    g, = torch.autograd.grad(pkg.fused_block_norm(y=x, post_weight=torch.ones(8, device=dev))[0].sum(), x,
+                             create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        g.sum().backward()
+
+
+def test_saved_inputs_are_guarded(pkg, dev):
+    """A tensor that the backward needs and that was written to in between is an error."""
+    raw = _logits(40, 8, torch.float32, 0).to(dev).requires_grad_()
+    r = pkg.fused_router(raw, 2, 0.5)
+    r.counts.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        r.lb_loss.backward()
+    w = torch.ones(8, device=dev, requires_grad=True)
+    x = torch.randn(4, 8, device=dev)
+    out, _ = pkg.fused_block_norm(y=x, post_weight=w)
+    p = [w]
+    pkg.adamw_step(p, [torch.ones_like(w)], [torch.zeros(8, device=dev)], [torch.zeros(8, device=dev)], step=1, lr=1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.sum().backward()
+
+
+# ---- the layers that call them ----------------------------------------------------
+
+def _latent_torch(xs, G, idx, p):
+    out = 0
+    for j in range(idx.shape[1]):
+        on = (idx[:, j:j + 1] >= 0).to(p.dtype)
+        out = out + on * p[:, j:j + 1] * torch.einsum("bs,bsq->bq", xs, G[idx[:, j].clamp(min=0)])
+    return out
+
+
+def _router64(raw, k, tau, scale, mask):
+    """train_ops.fused_router as float64 torch expressions."""
+    from test_train_ops import _router_torch
+    w, lb, z = _router_torch(raw, k, float(tau), scale, mask)
+    idx = torch.sort(raw.detach(), dim=-1, descending=True, stable=True).indices[:, :k]
+    if mask is not None:
+        idx = torch.where(mask[:, None], idx, -1)
+    return idx, w, lb, z, None
+
+
+def _norm64(x=None, y=None, gate=None, post_weight=None, gamma=None, next_weight=None, eps=1e-5):
+    from test_train_ops import _norm_torch
+    if y is None:
+        return x, _norm_torch(y=x, next_weight=next_weight, eps=eps)[1]
+    return _norm_torch(x, y, gate, post_weight, gamma, next_weight, eps)
+
+
+@pytest.mark.parametrize("padded", [False, True])
+def test_block_train_gradients(pkg, dev, monkeypatch, padded):
+    """TuckerFFNTrain: output, losses and every parameter's gradient against the same module in
+    float64 on the CPU with plain expressions in the operators' places."""
+    import mamba_tuckermoe_amd.block_train as bt
+    import mamba_tuckermoe_amd.latent as lat
+    cfg = pkg.TuckerMoEConfig(kmoe_num_experts=8, kmoe_r1=4, kmoe_r2=64, kmoe_r3=64, ffn_expand=2)
+    torch.manual_seed(0)
+    m = pkg.TuckerFFNTrain(64, cfg).train()
+    ref = pkg.TuckerFFNTrain(64, cfg).double().train()
+    with torch.no_grad():
+        for l in (m.ffn_gate, m.ffn_up, m.ffn_down):
+            l.router.weight.mul_(30)
+            l.core.mul_(6)
+    ref.load_state_dict({k: v.double() for k, v in m.state_dict().items()})
+    x = torch.randn(3, 50, 64)
+    mask = torch.rand(3, 50) > 0.3 if padded else None
+    with monkeypatch.context() as mp:
+        mp.setattr(lat.FusedLatentMoE, "apply", staticmethod(_latent_torch))
+        mp.setattr(lat, "fused_router", _router64)
+        mp.setattr(bt, "fused_block_norm", _norm64)
+        xr = x.double().requires_grad_()
+        o_ref, lb_ref, z_ref = ref(xr, step=700, mask=mask)
+        (o_ref.square().mean() + 0.1 * lb_ref + 0.01 * z_ref).backward()
+    m = m.to(dev)
+    xg = x.to(dev).requires_grad_()
+    o, lb, z = m(xg, step=700, mask=None if mask is None else mask.to(dev))
+    (o.square().mean() + 0.1 * lb + 0.01 * z).backward()
+    assert onp.rel_l2(f64(o), f64(o_ref)) <= 1e-5
+    assert abs(lb.item() - lb_ref.item()) <= 1e-4 and abs(z.item() - z_ref.item()) <= 1e-4 * z_ref.item()
+    n = 150 if mask is None else int(mask.sum())
+    assert m.ffn_gate.expert_counts.sum().item() == 2 * n
+    assert onp.rel_l2(f64(xg.grad), f64(xr.grad)) <= 1e-4
+    for (name, p), (_, q) in zip(m.named_parameters(), ref.named_parameters()):
+        assert onp.rel_l2(f64(p.grad), f64(q.grad)) <= 1e-4, name
+
+
+def test_training_layer_fused_router_is_the_plain_one(pkg, dev):
+    """fused_router=True against the torch expressions in float32: the same routing, outputs
+    and gradients to float32 rounding."""
+    torch.manual_seed(1)
+    a = pkg.TuckerMoETrain(128, 96, num_experts=8, r2=128, r3=64).to(dev).train()
+    b = pkg.TuckerMoETrain(128, 96, num_experts=8, r2=128, r3=64, fused_router=True).to(dev).train()
+    b.load_state_dict(a.state_dict())
+    x = torch.randn(300, 128, device=dev)
+    for step in (None, 700, torch.tensor(700.0, device=dev)):
+        outs = []
+        for m in (a, b):
+            m.zero_grad()
+            o, lb, z = m(x, step=step)
+            (o.square().mean() + lb + z).backward()
+            outs.append((o, lb, z))
+        for u, v in zip(*outs):
+            assert onp.rel_l2(f64(v), f64(u)) <= 1e-5
+        for (n, p), (_, q) in zip(a.named_parameters(), b.named_parameters()):
+            assert onp.rel_l2(f64(q.grad), f64(p.grad)) <= 1e-4, n
+    b.eval()
+    assert b(x)[1:] == (0.0, 0.0)
+
+
+@pytest.mark.parametrize("bits,dtype", [(32, torch.float32), (8, torch.float32), (8, torch.bfloat16)])
+def test_training_steps_run_together(pkg, dev, bits, dtype):
+    """Norms, routers, contraction and optimizer over a few steps: all finite, every parameter
+    moved, and by no more than AdamW's bound of its steps."""
+    cfg = pkg.TuckerMoEConfig(kmoe_num_experts=8, kmoe_r1=4, kmoe_r2=128, kmoe_r3=128, ffn_expand=2)
+    torch.manual_seed(0)
+    m = pkg.TuckerFFNTrain(128, cfg).to(dev, dtype).train()
+    opt = pkg.FusedAdamW(m.parameters(), lr=1e-2, betas=(0.9, 0.95), weight_decay=0.0, state_bits=bits)
+    start = [p.detach().clone() for p in m.parameters()]
+    x = torch.randn(400, 128, device=dev).to(dtype)
+    mask = torch.arange(400, device=dev) < 350
+    for step in range(3):
+        opt.zero_grad()
+        out, lb, z = m(x, step=step, mask=mask)
+        (out.float().square().mean() + 0.01 * lb + 0.001 * z).backward()
+        opt.step()
+        assert out.isfinite().all() and lb.isfinite() and z.isfinite()
+    for (n, p), q in zip(m.named_parameters(), start):
+        moved = (p.detach().float() - q.float()).abs()
+        # |m / sqrt(v)| after bias correction is at most sqrt(3 steps); a code is off by 1/8
+        assert p.isfinite().all() and moved.max() > 0, n
+        assert moved.max() <= 3 * 1e-2 * 2.5 + 2.0 ** -7 * q.float().abs().max(), n
