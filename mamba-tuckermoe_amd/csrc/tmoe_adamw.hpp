@@ -158,35 +158,61 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw32(const AdamwTable a) {
     }
 }
 
-__device__ __forceinline__ float e4m3_value(uint32_t c) {
-  // exponent and mantissa moved to fp32's places; the multiplication by 2^120 moves the
-  // exponent's bias and normalises the subnormal codes, exactly
-  const float f = __uint_as_float((c & 0x7fu) << 20) * 0x1p+120f;
-  const float s = (c & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : f;
-  return c & 0x80u ? -s : s;
+// a / b rounded as the division is, of a reciprocal y of b that is rounded so (the product's
+// error, found exactly, corrects it): the codes are the unrounded quotient's.
+__device__ __forceinline__ float quotient(float a, float b, float y) {
+  const float q = a * y;
+  return fmaf(fmaf(-q, b, a), y, q);
 }
 
-// The code of a in [0, 448]: the largest value lo that is no larger than a, or with the
-// chance described at the top its upper neighbour; kRoot: the chance is r's.
-template <bool kRoot>
-__device__ __forceinline__ uint32_t e4m3_code(float a, float u) {
+// sqrt(v) to the last place but for one value in millions
+__device__ __forceinline__ float root_of(float v) {
+  const float y = __builtin_amdgcn_rsqf(v), s = v * y;
+  const float r = fmaf(fmaf(-s, s, v), 0.5f * y, s);
+  return v == 0.f || v == INFINITY ? v : r;
+}
+
+// A magnitude a in [0, 448] as the e4m3 value below it and what is left over: `code`, and in
+// units of 2^-20 of the step between the two, `at` = the value's place counted from its
+// octave's (the subnormals': zero's) first, `rest` over it.
+struct E4m3Place {
+  uint32_t code, at, rest;
+};
+__device__ __forceinline__ E4m3Place e4m3_place(float a) {
+  // under 2^-6 values are 2^-9 apart, as they are from 2^-6 on: the sum's mantissa is both
+  const bool sub = a < 0x1p-6f;
+  const uint32_t b = __float_as_uint(sub ? a + 0x1p-6f : a);
+  const uint32_t A = (b & 0x7fffffu) | (sub ? 0u : 0x800000u);
+  return {(b >> 20) - (sub ? 968u : 960u), A & 0xf00000u, A & 0xfffffu};
+}
+// The code of a magnitude, up with the chance rest / step; u16: 16 random bits.
+__device__ __forceinline__ uint32_t e4m3_code(float a, uint32_t u16) {
+  const E4m3Place p = e4m3_place(a);
+  return p.code + ((u16 << 4 | 8u) < p.rest ? 1u : 0u);
+}
+// The code of a root r, up with the chance (r^2 - lo^2) / (hi^2 - lo^2)
+// = rest (r + lo) / (hi + lo); inv_odd: 1 / (2 q + 1) rounded, for q = 0 .. 15.
+__device__ __forceinline__ uint32_t e4m3_root_code(float r, uint32_t u16, const float* inv_odd) {
 #pragma clang fp contract(off)
-  if (a != a) return 0x7fu;
-  const int e = max((int)(__float_as_uint(a) >> 23) - 127, -6);
-  const float step = __uint_as_float((uint32_t)(e + 124) << 23);
-  const float inv_step = __uint_as_float((uint32_t)(130 - e) << 23);
-  const float q = floorf(a * inv_step), lo = q * step;
-  float chance = (a - lo) * inv_step;
-  if (kRoot) chance = chance * ((a + lo) / (lo + lo + step));
-  uint32_t c = (uint32_t)q + ((uint32_t)(e + 6) << 3) + (u < chance ? 1u : 0u);
-  if (kRoot && c == 0u && a > 0.f) c = 1u;
-  return c;
+  const E4m3Place p = e4m3_place(r);
+  const uint32_t q = p.at >> 20;
+  const float t = quotient((float)(2u * p.at + p.rest), (float)(2u * q + 1u), inv_odd[q]);
+  const float chance = (float)p.rest * t;                       // 2^40 of it
+  const float u = fmaf((float)u16, 0x1p+24f, 0x1p+23f);
+  const uint32_t c = p.code + (u < chance ? 1u : 0u);
+  return max(c, min(__float_as_uint(r), 1u));
 }
 
-// A wave takes blocks of 256 elements, four neighbours a lane.
+// A wave takes blocks of 256 elements, four neighbours a lane. What decides a code is
+// computed as the formulas round it (a step's codes are the next one's values), the rest
+// with the hardware's reciprocals: at 170 instructions an element the arithmetic, not the
+// memory, was the bound.
 template <class T>
 __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
 #pragma clang fp contract(off)
+  __shared__ float inv_odd[16];
+  if (threadIdx.x < 16) inv_odd[threadIdx.x] = 1.f / (float)(2 * threadIdx.x + 1);
+  __syncthreads();
   const AdamwStep s = adamw_step(a);
   T* p = static_cast<T*>(a.p[s.t]);
   const T* g = static_cast<const T*>(a.g[s.t]);
@@ -204,7 +230,7 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
     const int64_t i = b + 4 * lane, blk = b / kAdamwBlock;
     const int live = (int)(n - i < 4 ? (n - i < 0 ? 0 : n - i) : 4);
     const float sm = ms[blk], sr = rs[blk];
-    float pv[4] = {}, gv[4] = {}, m[4], v[4], r[4];
+    float pv[4] = {}, gv[4] = {}, m[4], r[4];
     uint32_t mc = 0u, rc = 0u;
     if (vec && live == 4) {
       load4(p + i, pv);
@@ -219,38 +245,38 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
         rc |= (uint32_t)rq[i + j] << 8 * j;
       }
     }
-    float am = 0.f, ar = 0.f;
+    const f32x2_t mc01 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, false);
+    const f32x2_t mc23 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, true);
+    const f32x2_t rc01 = __builtin_amdgcn_cvt_pk_f32_fp8(rc, false);
+    const f32x2_t rc23 = __builtin_amdgcn_cvt_pk_f32_fp8(rc, true);
+    const float mv[4] = {mc01[0], mc01[1], mc23[0], mc23[1]};
+    const float rv[4] = {rc01[0], rc01[1], rc23[0], rc23[1]};
+    // magnitudes as integers: in their order, a NaN above all
+    uint32_t am = 0u, ar = 0u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      m[j] = e4m3_value(mc >> 8 * j & 0xffu) * sm;
-      r[j] = e4m3_value(rc >> 8 * j & 0xffu) * sr;
-      v[j] = r[j] * r[j];
-      adamw_moments(s, gv[j], m[j], v[j]);
-      r[j] = sqrtf(v[j]);
-      pv[j] = adamw_param(s, pv[j], m[j], r[j]);
-      // NaN stays: a block that holds one gets a NaN scale
-      am = fabsf(m[j]) > am || m[j] != m[j] ? fabsf(m[j]) : am;
-      ar = r[j] > ar || r[j] != r[j] ? r[j] : ar;
+      m[j] = mv[j] * sm;
+      r[j] = rv[j] * sr;
+      float v = r[j] * r[j];
+      adamw_moments(s, gv[j], m[j], v);
+      r[j] = root_of(v);
+      pv[j] = fmaf(m[j] * -s.rate, __builtin_amdgcn_rcpf(fmaf(r[j], s.inv_c2, s.eps)), pv[j] * s.keep);
+      am = max(am, __float_as_uint(m[j]) & 0x7fffffffu);
+      ar = max(ar, __float_as_uint(r[j]) & 0x7fffffffu);
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      const float om = __shfl_xor(am, o), orr = __shfl_xor(ar, o);
-      am = om > am || om != om ? om : am;
-      ar = orr > ar || orr != orr ? orr : ar;
-    }
-    const float nsm = am * (1.f / kE4m3Max), nsr = ar * (1.f / kE4m3Max);
+    const float nsm = __uint_as_float(lanes_max<64>(am)) * (1.f / kE4m3Max);
+    const float nsr = __uint_as_float(lanes_max<64>(ar)) * (1.f / kE4m3Max);
     const float dm = nsm > 0.f ? nsm : 1.f, dr = nsr > 0.f ? nsr : 1.f;
+    const float im = 1.f / dm, ir = 1.f / dr;
     mc = rc = 0u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint64_t e = (uint64_t)(i + j);
       const uint32_t h = mix32((tkey + (uint32_t)e + (uint32_t)(e >> 32) * 0xC2B2AE35u) ^ s.key);
-      const float um = ((float)(h >> 16) + 0.5f) * 0x1p-16f;
-      const float ur = ((float)(h & 0xffffu) + 0.5f) * 0x1p-16f;
-      const uint32_t cm = e4m3_code<false>(fminf(fabsf(m[j]) / dm, kE4m3Max), um);
-      const uint32_t cr = e4m3_code<true>(fminf(r[j] / dr, kE4m3Max), ur);
-      mc |= (cm | (m[j] < 0.f ? 0x80u : 0u)) << 8 * j;
-      rc |= cr << 8 * j;
+      const float qm = fminf(quotient(fabsf(m[j]), dm, im), kE4m3Max);
+      const float qr = fminf(quotient(r[j], dr, ir), kE4m3Max);
+      mc |= (e4m3_code(qm, h >> 16) | (m[j] < 0.f ? 0x80u : 0u)) << 8 * j;
+      rc |= e4m3_root_code(qr, h & 0xffffu, inv_odd) << 8 * j;
     }
     if (vec && live == 4) {
       store4(p + i, pv);

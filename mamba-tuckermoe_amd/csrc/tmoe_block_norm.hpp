@@ -10,11 +10,12 @@
 // All in fp32 from the stored inputs; h is taken from the unrounded r, and the backward
 // forms r again from x and y, so that both see the same r; each output is rounded once.
 //
-// Bound by memory: every activation is read once and every output written once, a row's
-// chunks of 16 bytes lie in the registers of its lanes between the two norms. Rows of at
-// most kWaveChunks chunks a lane take one wave (no barrier), longer ones a work-group of
-// as many waves as the row has chunks for. The weights' gradients are summed in registers
-// over a work-group's rows, then in planes of `part` that k_block_norm_cols adds in order.
+// Bound by memory: every activation is read once and every output written once; a row lies
+// in the registers of its threads between its two norms, and the next row is on its way
+// meanwhile. Rows of at most 1024 elements take one wave (no barrier), four neighbours a
+// lane and step; longer ones a work-group, 16 bytes a thread and step. The weights'
+// gradients are summed in registers over a work-group's rows, then in planes of `part` that
+// k_block_norm_cols adds in a fixed order; one work-group alone has them whole.
 #pragma once
 
 #include "tmoe_elem.hpp"
@@ -23,266 +24,386 @@
 namespace tmoe {
 namespace dev {
 
-// Threads of one row and where each of its elements lies. kVec: chunks of 16 bytes, one
-// chunk a thread and step; else element by element, neighbours on neighbouring threads.
-template <class T, int NCH, bool kVec>
+// Elements a thread holds of a row: NCH steps of EPC neighbours, each one load of any
+// alignment (a row of odd width begins anywhere). kTail: d is no multiple of EPC, and one
+// thread's last step takes what is left element by element.
+template <class T, int EPC_, int NCH_, bool kTail_>
 struct RowMap {
-  static constexpr int EPC = 16 / (int)sizeof(T), N = NCH * EPC;
+  static constexpr int EPC = EPC_, NCH = NCH_, N = NCH * EPC, kWords = EPC * (int)sizeof(T) / 4;
+  static constexpr bool kTail = kTail_;
+  typedef uint32_t vec __attribute__((ext_vector_type(kWords), aligned(sizeof(T))));
   int tid, tpr;
   int64_t d;
-  __device__ int64_t col(int k, int j) const {
-    return kVec ? ((int64_t)k * tpr + tid) * EPC + j : ((int64_t)k * EPC + j) * tpr + tid;
-  }
-  __device__ bool in(int k, int j) const { return col(k, kVec ? 0 : j) < d; }
-  __device__ void load(const void* base, float v[N]) const {
-    const T* p = static_cast<const T*>(base);
+  __device__ int64_t col(int k) const { return ((int64_t)k * tpr + tid) * EPC; }
+  __device__ bool whole(int k) const { return col(k) + (kTail ? EPC : 1) <= d; }
+};
+
+// A row's elements in registers as they are stored.
+template <class M, class T>
+struct RowRegs {
+  uint32_t q[M::NCH][M::kWords];
+  __device__ void load(const M& m, const void* base, int64_t row, int64_t stride) {
+    const T* p = static_cast<const T*>(base) + row * stride;
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      if constexpr (kVec) {
-        u32x4 q = {0u, 0u, 0u, 0u};
-        if (in(k, 0)) q = *reinterpret_cast<const u32x4*>(p + col(k, 0));
-        const T* e = reinterpret_cast<const T*>(&q);
+    for (int k = 0; k < M::NCH; ++k) {
+      typename M::vec v = (uint32_t)0;
+      if (m.whole(k)) v = *reinterpret_cast<const typename M::vec*>(p + m.col(k));
+      else if constexpr (M::kTail) {
 #pragma unroll
-        for (int j = 0; j < EPC; ++j) v[k * EPC + j] = load_as_f32(e + j);
-      } else {
-#pragma unroll
-        for (int j = 0; j < EPC; ++j) v[k * EPC + j] = in(k, j) ? load_as_f32(p + col(k, j)) : 0.f;
+        for (int j = 0; j < M::EPC - 1; ++j)
+          if (m.col(k) + j < m.d) {
+            if constexpr (sizeof(T) == 2) v[j / 2] |= (uint32_t)p[m.col(k) + j] << 16 * (j & 1);
+            else v[j] = __float_as_uint(p[m.col(k) + j]);
+          }
       }
+#pragma unroll
+      for (int j = 0; j < M::kWords; ++j) q[k][j] = v[j];
     }
   }
-  __device__ void store(void* base, const float v[N]) const {
-    T* p = static_cast<T*>(base);
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      if constexpr (kVec) {
-        if (!in(k, 0)) continue;
-        u32x4 q;
-        T* e = reinterpret_cast<T*>(&q);
-#pragma unroll
-        for (int j = 0; j < EPC; ++j) store_from_f32(e + j, v[k * EPC + j]);
-        *reinterpret_cast<u32x4*>(p + col(k, 0)) = q;
-      } else {
-#pragma unroll
-        for (int j = 0; j < EPC; ++j)
-          if (in(k, j)) store_from_f32(p + col(k, j), v[k * EPC + j]);
-      }
-    }
+  __device__ float operator[](int i) const {
+    const int k = i / M::EPC, j = i % M::EPC;
+    if constexpr (sizeof(T) == 4) return __uint_as_float(q[k][j]);
+    else return __uint_as_float(j & 1 ? q[k][j / 2] & 0xffff0000u : q[k][j / 2] << 16);
   }
 };
 
-// Sum over a row's threads, the same value in all of them.
+template <class T, class M, int N>
+__device__ __forceinline__ void row_store(const M& m, void* base, int64_t row, const float (&v)[N]) {
+  T* p = static_cast<T*>(base) + row * m.d;
+#pragma unroll
+  for (int k = 0; k < M::NCH; ++k) {
+    if (m.whole(k)) {
+      typename M::vec q;
+#pragma unroll
+      for (int j = 0; j < M::kWords; ++j)
+        if constexpr (sizeof(T) == 2)
+          q[j] = pack_bf16x2(v[k * M::EPC + 2 * j], v[k * M::EPC + 2 * j + 1]);
+        else
+          q[j] = __float_as_uint(v[k * M::EPC + j]);
+      *reinterpret_cast<typename M::vec*>(p + m.col(k)) = q;
+    } else if constexpr (M::kTail) {
+#pragma unroll
+      for (int j = 0; j < M::EPC - 1; ++j)
+        if (m.col(k) + j < m.d) store_from_f32(p + m.col(k) + j, v[k * M::EPC + j]);
+    }
+  }
+}
+
+// Sum over a row's threads, the same value in all of them. lds: sixteen floats, zero past
+// the work-group's waves, that nobody else has written to since the barrier before the last
+// (one barrier a sum).
 template <bool kWave>
 __device__ __forceinline__ float row_sum(float v, float* lds) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+  v = lanes_sum<64>(v);
   if constexpr (!kWave) {
-    const int W = blockDim.x >> 6;
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = 0.f;
-    for (int w = 0; w < W; ++w) v += lds[w];
-    __syncthreads();
+    v = lanes_sum<16>(lds[threadIdx.x & 15]);
   }
   return v;
 }
-
-__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + __expf(-g)); }
-
-template <class T>
-__device__ __forceinline__ const void* row_at(const void* p, int64_t row, int64_t stride) {
-  return static_cast<const T*>(p) + row * stride;
+__device__ __forceinline__ void row_sum_clear(float (*lds)[16]) {
+  if (threadIdx.x < 64) lds[threadIdx.x >> 4][threadIdx.x & 15] = 0.f;
+  __syncthreads();
 }
-template <class T>
-__device__ __forceinline__ void* row_at(void* p, int64_t row, int64_t stride) {
-  return static_cast<T*>(p) + row * stride;
+
+// 1 / (1 + exp(-g)) to about 3 steps of fp32 (the hardware's reciprocal and exponential: an
+// exact division would be a third of the gated kernels' instructions)
+__device__ __forceinline__ float sigmoid(float g) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
 }
 
 constexpr int kNormThreads = 256;   // of a work-group whose rows take a wave each
+constexpr int kNormTeams = kNormThreads / 64;
 
-template <class T, int NCH, bool kWave, bool kVec>
-__global__ __launch_bounds__(kWave ? kNormThreads : 1024) void k_block_norm_fwd(BlockNormArgs a) {
-  using M = RowMap<T, NCH, kVec>;
+// The step of a kernel over the rows, and its threads' place in a row.
+template <class M, bool kWave>
+struct RowWalk {
+  M m;
+  int teams, team;
+  int64_t row, step;
+  __device__ explicit RowWalk(int64_t d)
+      : m{kWave ? (int)(threadIdx.x & 63) : (int)threadIdx.x, kWave ? 64 : (int)blockDim.x, d},
+        teams(kWave ? kNormTeams : 1), team(kWave ? (int)(threadIdx.x >> 6) : 0),
+        row((int64_t)blockIdx.x * teams + team), step((int64_t)gridDim.x * teams) {}
+};
+
+template <class T, int EPC, int NCH, bool kWave, bool kTail, int kThreads>
+__global__ __launch_bounds__(kThreads) void k_block_norm_fwd(BlockNormArgs a) {
+  using M = RowMap<T, EPC, NCH, kTail>;
+  using R = RowRegs<M, T>;
   constexpr int N = M::N;
-  __shared__ float lds[16];
-  const M m = {kWave ? (int)(threadIdx.x & 63) : (int)threadIdx.x, kWave ? 64 : (int)blockDim.x, a.d};
-  const int teams = kWave ? kNormThreads / 64 : 1;
-  const int64_t first = (int64_t)blockIdx.x * teams + (kWave ? threadIdx.x >> 6 : 0);
+  __shared__ float lds[4][16];
+  RowWalk<M, kWave> w(a.d);
+  const M& m = w.m;
   const float inv_d = 1.f / (float)a.d;
-  for (int64_t b = first; b < a.T; b += (int64_t)gridDim.x * teams) {
-    float f[N], x[N];
-    m.load(row_at<T>(a.y, b, a.y_rs), f);
-    if (a.x) m.load(row_at<T>(a.x, b, a.x_rs), x);
+  if (!kWave) row_sum_clear(lds);
+  R ny, nx, ng;
+  if (w.row < a.T) {
+    ny.load(m, a.y, w.row, a.y_rs);
+    if (a.x) nx.load(m, a.x, w.row, a.x_rs);
+    if (a.gate) ng.load(m, a.gate, w.row, a.gate_rs);
+  }
+  int par = 0;
+  for (int64_t b = w.row; b < a.T; b += w.step, par ^= 2) {
+    const R y = ny, x = nx, g = ng;
+    if (b + w.step < a.T) {
+      ny.load(m, a.y, b + w.step, a.y_rs);
+      if (a.x) nx.load(m, a.x, b + w.step, a.x_rs);
+      if (a.gate) ng.load(m, a.gate, b + w.step, a.gate_rs);
+    }
+    float f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = y[i];
     if (a.gate) {
-      float g[N];
-      m.load(row_at<T>(a.gate, b, a.gate_rs), g);
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] *= g[i] * sigmoid(g[i]);
     }
     if (a.post_w) {
-      float w[N], ss = 0.f;
-      m.load(a.post_w, w);
+      R pw;
+      pw.load(m, a.post_w, 0, 0);
+      float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) ss += f[i] * f[i];
-      const float inv = 1.f / sqrtf(row_sum<kWave>(ss, lds) * inv_d + a.eps);
+      const float inv = 1.f / sqrtf(row_sum<kWave>(ss, lds[par]) * inv_d + a.eps);
       if (a.inv && m.tid == 0) a.inv[b] = inv;
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] *= inv * w[i];
+      for (int i = 0; i < N; ++i) f[i] *= inv * pw[i];
     }
     if (a.gamma) {
-      float w[N];
-      m.load(a.gamma, w);
+      R gm;
+      gm.load(m, a.gamma, 0, 0);
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] *= w[i];
+      for (int i = 0; i < N; ++i) f[i] *= gm[i];
     }
     if (a.x) {
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] += x[i];
     }
-    if (a.r) m.store(row_at<T>(a.r, b, a.d), f);
+    if (a.r) row_store<T>(m, a.r, b, f);
     if (a.next_w) {
-      float w[N], ss = 0.f;
-      m.load(a.next_w, w);
+      R nw;
+      nw.load(m, a.next_w, 0, 0);
+      float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) ss += f[i] * f[i];
-      const float inv = 1.f / sqrtf(row_sum<kWave>(ss, lds) * inv_d + a.eps);
+      const float inv = 1.f / sqrtf(row_sum<kWave>(ss, lds[par + 1]) * inv_d + a.eps);
       if (a.inv && m.tid == 0) a.inv[a.T + b] = inv;
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] *= inv * w[i];
-      m.store(row_at<T>(a.h, b, a.d), f);
+      for (int i = 0; i < N; ++i) f[i] *= inv * nw[i];
+      row_store<T>(m, a.h, b, f);
     }
   }
 }
 
-template <class T, int NCH, bool kWave, bool kVec>
-__global__ __launch_bounds__(kWave ? kNormThreads : 1024) void k_block_norm_bwd(BlockNormArgs a) {
-  using M = RowMap<T, NCH, kVec>;
+// Operands of a backward as the bits of F: known when it is compiled, and with them every
+// gradient wanted and dr (and dh with kNext) there, so that a row's loads and stores have
+// their places and none waits for another; F = -1 looks at the pointers. kFull: F may hold
+// a gate or a norm after the block; without, neither's registers are held.
+constexpr int kGate = 1, kPost = 2, kRes = 4, kGamma = 8, kNext = 16;
+
+template <class T, int EPC, int NCH, bool kWave, bool kTail, int kThreads, bool kFull, int F>
+__global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
+// the same roundings whichever gradients are wanted: fused where it is written
+#pragma clang fp contract(off)
+  using M = RowMap<T, EPC, NCH, kTail>;
+  using R = RowRegs<M, T>;
   constexpr int N = M::N;
-  __shared__ float lds[16];
-  const M m = {kWave ? (int)(threadIdx.x & 63) : (int)threadIdx.x, kWave ? 64 : (int)blockDim.x, a.d};
-  const int teams = kWave ? kNormThreads / 64 : 1;
-  const int64_t first = (int64_t)blockIdx.x * teams + (kWave ? threadIdx.x >> 6 : 0);
+  constexpr bool kAny = F < 0;
+  __shared__ float lds[4][16];
+  RowWalk<M, kWave> w(a.d);
+  const M& m = w.m;
   const float inv_d = 1.f / (float)a.d;
-  float s_post[N], s_gamma[N], s_next[N];
+  if (!kWave) row_sum_clear(lds);
+  const bool gated = kFull && (kAny ? a.gate != nullptr : (F & kGate) != 0);
+  const bool post = kFull && (kAny ? a.post_w != nullptr : (F & kPost) != 0);
+  const bool res = kAny ? a.x != nullptr : (F & kRes) != 0;
+  const bool scaled = kAny ? a.gamma != nullptr : (F & kGamma) != 0;
+  const bool next = kAny ? a.dh != nullptr : (F & kNext) != 0;
+  const bool dr_in = kAny ? a.dr != nullptr : true;
+  float s_post[kFull ? N : 1], s_gamma[N], s_next[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) s_post[i] = s_gamma[i] = s_next[i] = 0.f;
-  for (int64_t b = first; b < a.T; b += (int64_t)gridDim.x * teams) {
-    // u (in f), then f
-    float y[N], f[N], D[N];
-    m.load(row_at<T>(a.y, b, a.y_rs), y);
-    if (a.dr) m.load(row_at<T>(a.dr, b, a.dr_rs), D);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      f[i] = y[i];
-      if (!a.dr) D[i] = 0.f;
+  for (int i = 0; i < N; ++i) {
+    if (kFull) s_post[i] = 0.f;
+    s_gamma[i] = s_next[i] = 0.f;
+  }
+  R pw, gm, nw;
+  if (post) pw.load(m, a.post_w, 0, 0);
+  if (scaled) gm.load(m, a.gamma, 0, 0);
+  if (next) nw.load(m, a.next_w, 0, 0);
+  R ny, nx, ng, ndr, ndh;
+  float n_u = 1.f, n_r = 0.f;
+  auto fetch = [&](int64_t b) {
+    ny.load(m, a.y, b, a.y_rs);
+    if (gated) ng.load(m, a.gate, b, a.gate_rs);
+    if (next) {
+      ndh.load(m, a.dh, b, a.dh_rs);
+      if (res) nx.load(m, a.x, b, a.x_rs);
+      n_r = a.inv[a.T + b];
     }
-    if (a.gate) {
-      float g[N];
-      m.load(row_at<T>(a.gate, b, a.gate_rs), g);
+    if (dr_in) ndr.load(m, a.dr, b, a.dr_rs);
+    if (post) n_u = a.inv[b];
+  };
+  constexpr bool kAhead = kThreads <= 512;   // past that a thread's registers hold one row only
+  if (kAhead && w.row < a.T) fetch(w.row);
+  int par = 0;
+  for (int64_t b = w.row; b < a.T; b += w.step, par ^= 2) {
+    if (!kAhead) fetch(b);
+    const R y = ny, x = nx, g = ng, dr = ndr, dh = ndh;
+    const float inv_u = n_u, inv_r = n_r;
+    if (kAhead) fetch(b + w.step < a.T ? b + w.step : b);
+    // sigmoid(gate); nu (u where no norm follows the block); D
+    float sg[kFull ? N : 1], nu[N], D[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] *= g[i] * sigmoid(g[i]);
-    }
-    float inv_u = 0.f;
-    if (a.post_w) {
-      float w[N];
-      m.load(a.post_w, w);
-      inv_u = a.inv[b];
+    for (int i = 0; i < N; ++i) nu[i] = y[i];
+    if constexpr (kFull) {
+      if (gated) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] *= inv_u * w[i];
-    }
-    float gm[N];
-    if (a.gamma) m.load(a.gamma, gm);
-    if (a.dh) {
-      float r[N], w[N], dh[N];
-      m.load(row_at<T>(a.dh, b, a.dh_rs), dh);
-      m.load(a.next_w, w);
-      if (a.x) m.load(row_at<T>(a.x, b, a.x_rs), r);
-      const float inv_r = a.inv[a.T + b];
-      float dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float v = a.gamma ? f[i] * gm[i] : f[i];
-        r[i] = (a.x ? r[i] + v : v) * inv_r;       // nr
-        s_next[i] += dh[i] * r[i];
-        dh[i] *= w[i];
-        dot += dh[i] * r[i];
+        for (int i = 0; i < N; ++i) {
+          sg[i] = sigmoid(g[i]);
+          nu[i] *= g[i] * sg[i];
+        }
       }
-      dot = row_sum<kWave>(dot, lds) * inv_d;
+      if (post) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) D[i] += (dh[i] - r[i] * dot) * inv_r;
+        for (int i = 0; i < N; ++i) nu[i] *= inv_u;
+      }
     }
-    if (a.dx) m.store(row_at<T>(a.dx, b, a.d), D);
-    if (a.gamma) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) D[i] = 0.f;
+    if (dr_in) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) D[i] = dr[i];
+    }
+    if (next) {
+      float nr[N], dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) nr[i] = nu[i];
+      if constexpr (kFull)
+        if (post) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) nr[i] *= pw[i];
+        }
+      if (scaled && res) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) nr[i] = fmaf(nr[i], gm[i], x[i]);
+      } else if (scaled) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) nr[i] *= gm[i];
+      } else if (res) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) nr[i] += x[i];
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        s_gamma[i] += D[i] * f[i];
+        nr[i] *= inv_r;
+        const float t = dh[i] * nr[i];
+        s_next[i] += t;
+        dot = fmaf(t, nw[i], dot);
+      }
+      dot = row_sum<kWave>(dot, lds[par]) * inv_d * inv_r;
+#pragma unroll
+      for (int i = 0; i < N; ++i) D[i] = fmaf(-nr[i], dot, fmaf(dh[i] * nw[i], inv_r, D[i]));
+    }
+    if (kAny ? a.dx != nullptr : res) row_store<T>(m, a.dx, b, D);
+    if (post) {
+      if constexpr (kFull) {
+        float dot = 0.f;
+        if (scaled) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            s_gamma[i] = fmaf(D[i], nu[i] * pw[i], s_gamma[i]);
+            D[i] *= gm[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float t = D[i] * nu[i];
+          s_post[i] += t;
+          dot = fmaf(t, pw[i], dot);
+        }
+        dot = row_sum<kWave>(dot, lds[par + 1]) * inv_d * inv_u;
+#pragma unroll
+        for (int i = 0; i < N; ++i) D[i] = fmaf(-nu[i], dot, D[i] * pw[i] * inv_u);
+      }
+    } else if (scaled) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        s_gamma[i] = fmaf(D[i], nu[i], s_gamma[i]);
         D[i] *= gm[i];
       }
     }
-    if (a.post_w) {
-      // nu from y and the gate again: f has the weight in it, which may be zero
-      float w[N], g[N], dot = 0.f;
-      m.load(a.post_w, w);
-      if (a.gate) m.load(row_at<T>(a.gate, b, a.gate_rs), g);
+    if constexpr (kFull)
+      if (gated) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        f[i] = (a.gate ? y[i] * (g[i] * sigmoid(g[i])) : y[i]) * inv_u;
-        s_post[i] += D[i] * f[i];
-        D[i] *= w[i];
-        dot += D[i] * f[i];
+        for (int i = 0; i < N; ++i) {
+          // silu' = s (1 + g (1 - s))
+          nu[i] = D[i] * y[i] * (sg[i] * fmaf(g[i], 1.f - sg[i], 1.f));
+          D[i] *= g[i] * sg[i];
+        }
+        if (kAny ? a.dgate != nullptr : true) row_store<T>(m, a.dgate, b, nu);
       }
-      dot = row_sum<kWave>(dot, lds) * inv_d;
-#pragma unroll
-      for (int i = 0; i < N; ++i) D[i] = (D[i] - f[i] * dot) * inv_u;
-    }
-    if (a.gate) {
-      float g[N];
-      m.load(row_at<T>(a.gate, b, a.gate_rs), g);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float s = sigmoid(g[i]);
-        y[i] *= D[i] * (s * (1.f + g[i] * (1.f - s)));
-        D[i] *= g[i] * s;
-      }
-      if (a.dgate) m.store(row_at<T>(a.dgate, b, a.d), y);
-    }
-    if (a.dy) m.store(row_at<T>(a.dy, b, a.d), D);
+    if (kAny ? a.dy != nullptr : true) row_store<T>(m, a.dy, b, D);
   }
-  // part: (3, planes, d); a plane for each row of threads
-  if (!a.part) return;
-  const int64_t planes = (int64_t)gridDim.x * teams;
+  if (!a.dpost_w && !a.dgamma && !a.dnext_w) return;
+  // a wave's rows apart: their sums over the work-group first, in the waves' order
+  if constexpr (kWave) {
+    __shared__ float s[kNormTeams][N * 64];
+    auto join = [&](float (&v)[N]) {
+      __syncthreads();
 #pragma unroll
-  for (int k = 0; k < NCH; ++k)
+      for (int i = 0; i < N; ++i) s[w.team][i * 64 + m.tid] = v[i];
+      __syncthreads();
 #pragma unroll
-    for (int j = 0; j < M::EPC; ++j) {
-      const int64_t c = m.col(k, j);
-      if (c >= a.d) continue;
-      const int i = k * M::EPC + j;
-      if (a.dpost_w) a.part[(0 * planes + first) * a.d + c] = s_post[i];
-      if (a.dgamma) a.part[(1 * planes + first) * a.d + c] = s_gamma[i];
-      if (a.dnext_w) a.part[(2 * planes + first) * a.d + c] = s_next[i];
-    }
+      for (int i = 0; i < N; ++i) {
+        v[i] = 0.f;
+#pragma unroll
+        for (int t = 0; t < kNormTeams; ++t) v[i] += s[t][i * 64 + m.tid];
+      }
+    };
+    if constexpr (kFull)
+      if (a.dpost_w) join(s_post);
+    if (a.dgamma) join(s_gamma);
+    if (a.dnext_w) join(s_next);
+    if (w.team > 0) return;
+  }
+  // part: (3, work-groups, d)
+  auto put = [&](const float (&v)[N], int which, void* out) {
+    if (!out) return;
+    if (gridDim.x == 1) return row_store<T>(m, out, 0, v);
+    float* p = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * a.d;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+      for (int j = 0; j < EPC; ++j)
+        if (m.col(k) + j < a.d) p[m.col(k) + j] = v[k * EPC + j];
+  };
+  if constexpr (kFull) put(s_post, 0, a.dpost_w);
+  put(s_gamma, 1, a.dgamma);
+  put(s_next, 2, a.dnext_w);
 }
 
-// The weights' gradients from the backward's planes: 64 columns of one weight a work-group.
+// The weights' gradients from the backward's planes: 32 columns of one weight a work-group,
+// its 32 groups of threads to the planes.
 template <class T>
 __global__ __launch_bounds__(1024) void k_block_norm_cols(BlockNormArgs a, int64_t planes) {
   T* out = static_cast<T*>(blockIdx.y == 0 ? a.dpost_w : blockIdx.y == 1 ? a.dgamma : a.dnext_w);
   if (!out) return;   // uniform over the work-group
-  __shared__ float s[16][64];
-  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  __shared__ float s[32][33];
+  const int g = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const int64_t c = (int64_t)blockIdx.x * 32 + l;
   const float* p = a.part + blockIdx.y * planes * a.d + c;
   float v = 0.f;
   if (c < a.d)
 #pragma unroll 8
-    for (int64_t i = threadIdx.x >> 6; i < planes; i += 16) v += p[i * a.d];
-  s[threadIdx.x >> 6][threadIdx.x & 63] = v;
+    for (int64_t i = g; i < planes; i += 32) v += p[i * a.d];
+  s[g][l] = v;
   __syncthreads();
-  if (threadIdx.x < 64 && c < a.d) {
-    v = 0.f;
+  v = s[l][g];          // column g's sums in the lanes of half a wave
 #pragma unroll
-    for (int g = 0; g < 16; ++g) v += s[g][threadIdx.x];
-    store_from_f32(out + c, v);
-  }
+  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+  const int64_t col = (int64_t)blockIdx.x * 32 + g;
+  if (l == 0 && col < a.d) store_from_f32(out + col, v);
 }
 
 }  // namespace dev

@@ -26,5 +26,43 @@ __device__ __forceinline__ float load_as_f32(const float* p) { return *p; }
 __device__ __forceinline__ void store_from_f32(uint16_t* p, float v) { *p = f32_to_bf16_bits(v); }
 __device__ __forceinline__ void store_from_f32(float* p, float v) { *p = v; }
 
+// f over the values of L lanes (a power of two, aligned), the same result in all of them:
+// neighbours of a quad, quads of 8, halves of 16 (mirrored: each holds one value by then),
+// then the swapped rows of 16 and halves of the wave. Lanes of other groups may be off.
+template <int L, int kStep = 1, class F>
+__device__ __forceinline__ uint32_t lanes_reduce(uint32_t v, F f) {
+  if constexpr (kStep < L) {
+    if constexpr (kStep == 1) v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true));
+    if constexpr (kStep == 2) v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true));
+    if constexpr (kStep == 4) v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true));
+    if constexpr (kStep == 8) v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true));
+    if constexpr (kStep == 16) {
+      const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+      v = f(r[0], r[1]);
+    }
+    if constexpr (kStep == 32) {
+      const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+      v = f(r[0], r[1]);
+    }
+    return lanes_reduce<L, 2 * kStep>(v, f);
+  } else {
+    return v;
+  }
+}
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+  return __uint_as_float(lanes_reduce<L>(__float_as_uint(v), [](uint32_t x, uint32_t y) {
+    return __float_as_uint(__uint_as_float(x) + __uint_as_float(y));
+  }));
+}
+template <int L>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  return lanes_reduce<L>(v, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+}
+template <int L>
+__device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
+  return lanes_reduce<L>(v, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+}
+
 }  // namespace dev
 }  // namespace tmoe

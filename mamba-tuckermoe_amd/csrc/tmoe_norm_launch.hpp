@@ -1,0 +1,137 @@
+// Launchers of the block norms (tmoe_block_norm.hpp) for one element type; a source file of
+// its own for each (tmoe_norm_bf16.hip, tmoe_norm_f32.hip), compiled side by side.
+#pragma once
+
+#include "tmoe_block_norm.hpp"
+
+namespace tmoe {
+namespace {
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct NormPlan {
+  bool wave;            // a wave to a row
+  int steps;            // of 4 elements a lane, or of 16 bytes a thread
+  unsigned threads;
+  int teams;            // rows at a time in a work-group
+};
+// full: the backward with a gate or a norm after the block, whose rows of over 512 elements
+// would need more registers than one wave's lanes have.
+NormPlan norm_plan(int64_t d, int es, bool full) {
+  if (d <= (full ? 512 : 1024))
+    return {true, (int)ceil_div(d, 256), dev::kNormThreads, dev::kNormTeams};
+  const int64_t nch = ceil_div(d * es, 16);
+  const int c = nch <= 1024 ? 1 : nch <= 2048 ? 2 : 4;
+  return {false, c, (unsigned)(ceil_div(nch, 64 * c) * 64), 1};
+}
+// Work-groups of a persistent walk over the rows: what the chip holds at once.
+int64_t norm_blocks(int64_t T, const NormPlan& p) {
+  const int64_t n = ceil_div(T, p.teams);
+  const int64_t most = p.threads <= 256 ? 2048 : p.threads <= 512 ? 1024 : 512;
+  return n < most ? n : most;
+}
+// The backward's, with a plane of each weight's gradient for each: two to a compute unit
+// (measured against 256, 768 and 1024: 119 us of T = 16384, d = 2304 with all operands
+// against 114, 123 and 127, 25.7 against 26.6, 26.2 and 26.8 of d = 768 with a residual
+// and the next norm). One for so few rows that a second launch would cost more than their
+// walk.
+constexpr int64_t kNormBwdBlocks = 512;
+int64_t norm_bwd_blocks(int64_t T, const NormPlan& p) {
+  const int64_t n = ceil_div(T, p.teams);
+  return n <= 2 ? 1 : n < kNormBwdBlocks ? n : kNormBwdBlocks;
+}
+
+using NormKernel = void (*)(BlockNormArgs);
+
+// The form of a backward that has a kernel of its own (-1: it has none): what the training
+// blocks' ends are made of, with every gradient wanted.
+int norm_form(const BlockNormArgs& a) {
+  using namespace dev;
+  const int f = (a.gate ? kGate : 0) | (a.post_w ? kPost : 0) | (a.x ? kRes : 0) |
+                (a.gamma ? kGamma : 0) | (a.next_w ? kNext : 0);
+  const bool all = a.dr && a.dy && (a.dh || !a.next_w) && (a.dx || !a.x) && (a.dgate || !a.gate);
+  const bool own = f == (kRes | kGamma | kNext) || f == (kRes | kGamma) || f == kGate ||
+                   f == (kGate | kPost) || f == (kGate | kPost | kRes | kGamma | kNext);
+  return all && own ? f : -1;
+}
+template <class T, int EPC, int NCH, bool kWave, bool kTail, int kThreads>
+NormKernel norm_bwd_kernel(int form, bool full) {
+  using namespace dev;
+#define TMOE_FORM(F)                                                                         \
+  if (form == (F))                                                                           \
+    return k_block_norm_bwd<T, EPC, NCH, kWave, kTail, kThreads, ((F) & (kGate | kPost)) != 0, (F)>;
+  if constexpr (kThreads <= 512) {
+    TMOE_FORM(kRes | kGamma | kNext)
+    TMOE_FORM(kRes | kGamma)
+    if constexpr (!kWave || NCH <= 2) {
+      TMOE_FORM(kGate)
+      TMOE_FORM(kGate | kPost)
+      TMOE_FORM(kGate | kPost | kRes | kGamma | kNext)
+    }
+  }
+#undef TMOE_FORM
+  if constexpr (!kWave || NCH <= 2)
+    if (full) return k_block_norm_bwd<T, EPC, NCH, kWave, kTail, kThreads, true, -1>;
+  return k_block_norm_bwd<T, EPC, NCH, kWave, kTail, kThreads, false, -1>;
+}
+template <class T, bool kTail>
+NormKernel norm_kernel(const BlockNormArgs& a, bool backward, const NormPlan& p) {
+  const bool full = a.gate || a.post_w;
+  const int form = backward ? norm_form(a) : -1;
+#define TMOE_NORM(EPC, C, W, THREADS)                                                        \
+  if (p.wave == W && p.steps == C && p.threads <= THREADS)                                   \
+    return backward ? norm_bwd_kernel<T, EPC, C, W, kTail, THREADS>(form, full)              \
+                    : dev::k_block_norm_fwd<T, EPC, C, W, kTail, THREADS>;
+  constexpr int E16 = 16 / (int)sizeof(T);
+  TMOE_NORM(4, 1, true, 256) TMOE_NORM(4, 2, true, 256)
+  TMOE_NORM(4, 3, true, 256) TMOE_NORM(4, 4, true, 256)
+  TMOE_NORM(E16, 1, false, 512) TMOE_NORM(E16, 1, false, 1024)
+  TMOE_NORM(E16, 2, false, 1024) TMOE_NORM(E16, 4, false, 1024)
+#undef TMOE_NORM
+  return nullptr;
+}
+template <class T>
+hipError_t norm_launch(const BlockNormArgs& a, bool backward, const NormPlan& p, int64_t blocks,
+                       hipStream_t st) {
+  const int epc = p.wave ? 4 : 16 / (int)sizeof(T);
+  const NormKernel k = a.d % epc ? norm_kernel<T, true>(a, backward, p)
+                                 : norm_kernel<T, false>(a, backward, p);
+  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(p.threads), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+template <class T>
+size_t block_norm_workspace(int64_t T_, int64_t d) {
+  int64_t blocks = 1;
+  for (bool full : {false, true}) {
+    const int64_t n = norm_bwd_blocks(T_, norm_plan(d, sizeof(T), full));
+    blocks = n > blocks ? n : blocks;
+  }
+  return blocks > 1 ? (size_t)(3 * blocks * d) * sizeof(float) : 0;
+}
+template <class T>
+hipError_t block_norm_fwd(const BlockNormArgs& a, hipStream_t st) {
+  const NormPlan p = norm_plan(a.d, sizeof(T), false);
+  return norm_launch<T>(a, false, p, norm_blocks(a.T, p), st);
+}
+template <class T>
+hipError_t block_norm_bwd(const BlockNormArgs& a, hipStream_t st) {
+  const NormPlan p = norm_plan(a.d, sizeof(T), a.gate || a.post_w);
+  const int64_t blocks = norm_bwd_blocks(a.T, p);
+  if (a.T > 0)
+    if (hipError_t e = norm_launch<T>(a, true, p, blocks, st); e != hipSuccess) return e;
+  if ((!a.dpost_w && !a.dgamma && !a.dnext_w) || (a.T > 0 && blocks == 1)) return hipSuccess;
+  // without rows the sums of no planes: zeros
+  hipLaunchKernelGGL(dev::k_block_norm_cols<T>, dim3((unsigned)ceil_div(a.d, 32), 3), dim3(1024), 0,
+                     st, a, a.T > 0 ? blocks : 0);
+  return hipGetLastError();
+}
+
+#define TMOE_NORM_TYPE(T)                                                 \
+  template size_t block_norm_workspace<T>(int64_t, int64_t);              \
+  template hipError_t block_norm_fwd<T>(const BlockNormArgs&, hipStream_t); \
+  template hipError_t block_norm_bwd<T>(const BlockNormArgs&, hipStream_t);
+
+}  // namespace tmoe

@@ -8,9 +8,18 @@
 // idx -1 (which selects nothing in the contraction), w 0 and no gradient.
 //   g_e  = dlb E n_e / N^2 + [e = idx_j] (dw_j - sum_i dw_i w_i) / s
 //   draw = (1 - tanh^2) ((P_e (g_e - sum_f P_f g_f)) / tau + dz 2 lse softmax(a)_e / N)
+// where both differences are taken from the likeliest expert's (dw_0, g_0): with its
+// P near 1 the sums are next to those, and the differences what is left of two equals.
 //
-// A token's logits lie in L lanes, four to a lane (L a power of two, 4 L >= E): everything a
-// token needs is exchanged between those lanes. The column sums over the tokens (n_e,
+// With Q = exp(-2 raw / c) and R = 1 / (1 + Q), tanh = 1 - 2 Q R, 1 - tanh^2 = 4 Q R^2 and
+//   a_e - a_m = 2 c R_m R_e (Q_m - Q_e)
+// for the largest logit m: the exponents of both softmaxes without the cancellation of two
+// capped logits near the cap. raw / c is cut at +-20, past which tanh is +-1 in fp32.
+//
+// A token's logits lie in L lanes, V to a lane (L a power of two, V L >= E; V = 8, or 4 where
+// that is all of them): what a token needs of them is exchanged by lane permutations. Eight
+// to a lane rather than four: the exchanges, and not the exponentials, are most of the
+// instructions. The column sums over the tokens (n_e,
 // sum_b P_be) stay in registers over a work-group's tokens, then in a plane of `part`, and
 // k_router_finish adds the planes in a fixed order: the losses do not depend on which
 // work-group ends first.
@@ -23,118 +32,186 @@ namespace tmoe {
 namespace dev {
 
 constexpr int kRouterThreads = 256;
+constexpr int kFinishCols = 16;       // experts of a work-group of k_router_finish
 
-template <int L>
-__device__ __forceinline__ float lanes_sum(float v) {
+// raw[e0 .. e0 + V - 1] of a row of E logits (0 past its end), at any alignment
+template <class T, int V>
+__device__ __forceinline__ void router_load(const T* row, int e0, int E, float v[V]) {
+  constexpr int W = V * (int)sizeof(T) / 4;
+  typedef uint32_t vec __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+  if (e0 + V <= E) {
+    const vec q = *reinterpret_cast<const vec*>(row + e0);
 #pragma unroll
-  for (int o = L / 2; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-
-// raw[e0 .. e0 + 3] of a row of E logits (0 past its end)
-template <class T>
-__device__ __forceinline__ void router_load(const T* row, int e0, int E, bool vec, float v[4]) {
-  if (vec && e0 + 4 <= E) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 q = *reinterpret_cast<const float4*>(row + e0);
-      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-    } else {
-      const uint2 q = *reinterpret_cast<const uint2*>(row + e0);
-      v[0] = bf16_bits_to_f32(q.x & 0xffffu); v[1] = bf16_bits_to_f32(q.x >> 16);
-      v[2] = bf16_bits_to_f32(q.y & 0xffffu); v[3] = bf16_bits_to_f32(q.y >> 16);
-    }
+    for (int j = 0; j < V; ++j)
+      if constexpr (sizeof(T) == 4) v[j] = __uint_as_float(q[j]);
+      else v[j] = __uint_as_float(j & 1 ? q[j / 2] & 0xffff0000u : q[j / 2] << 16);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = e0 + j < E ? load_as_f32(row + e0 + j) : 0.f;
+    for (int j = 0; j < V; ++j) v[j] = e0 + j < E ? load_as_f32(row + e0 + j) : 0.f;
   }
 }
 
-// An unsigned key in the order of the floats: NaN above +inf, -0 equal to 0, never 0.
+template <int V>
+__device__ __forceinline__ uint32_t max_of(const uint32_t (&k)[V]) {
+  uint32_t m = max(k[0], k[1]);
+#pragma unroll
+  for (int j = 2; j < V; j += 2) m = max(m, max(k[j], k[j + 1]));
+  return m;
+}
+
+// An unsigned key in the order of the floats: NaN above +inf, -0 equal to 0, never 0; and
+// the float of a key.
 __device__ __forceinline__ uint32_t order_key(float f) {
   f += 0.f;
   if (f != f) return 0xffffffffu;
   const uint32_t b = __float_as_uint(f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-
-struct Capped {
-  float t, sech2;   // tanh(u) and 1 - tanh^2(u) without the cancellation near +-1
-};
-__device__ __forceinline__ Capped capped(float u) {
-  const float q = __expf(-2.f * fabsf(u)), r = 1.f / (1.f + q);
-  return {copysignf((1.f - q) * r, u), 4.f * q * r * r};
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-template <class T, int L>
+struct Capped {
+  float Q, R;
+};
+// c1 = -2 log2(e) / cap; a NaN stays one
+__device__ __forceinline__ Capped capped(float raw, float c1) {
+  constexpr float kCut = 20.f * 2.8853900817779268f;
+  float u = raw * c1;
+  u = u > kCut ? kCut : u < -kCut ? -kCut : u;
+  const float Q = __builtin_amdgcn_exp2f(u);
+  return {Q, __builtin_amdgcn_rcpf(1.f + Q)};
+}
+
+// cap tanh(raw / cap) to the last places, for the logsumexp: once a token
+__device__ __forceinline__ float capped_value(float raw, float c1, float cap) {
+  const float q = __builtin_amdgcn_exp2f(-fabsf(raw * c1)), d = 1.f + q;
+  const float r = __builtin_amdgcn_rcpf(d);
+  return copysignf(cap * ((1.f - q) * fmaf(r, fmaf(-d, r, 1.f), r)), raw);
+}
+
+struct RouterScales {
+  float c1, k_z, k_p;   // exponents in base 2 of R_m R_e (Q_m - Q_e): of both softmaxes
+  __device__ RouterScales(const RouterArgs& a) {
+    const float tau = a.tau_dev ? *a.tau_dev : a.tau;
+    c1 = -2.8853900817779268f / a.cap;
+    k_z = 2.8853900817779268f * a.cap;
+    k_p = k_z / tau;
+  }
+};
+
+// counts, lb, z and N of column sums that are whole: ps, cn of expert e in the lanes of
+// this wave (nothing past E), every lane the same z and n. lb's part of these experts.
+__device__ __forceinline__ float router_finish_wave(const RouterArgs& a, int e, float ps, uint32_t cn,
+                                                    float inv_n) {
+  float t = 0.f;
+  if (e < a.E) {
+    a.counts[e] = cn;
+    t = ((float)cn * inv_n) * (ps * inv_n);
+  }
+  return lanes_sum<64>(t);
+}
+
+template <class T, int L, int V>
 __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
   constexpr int G = kRouterThreads / L;
   const T* raw = static_cast<const T*>(a.raw);
-  const int E = a.E, k = a.k, l = threadIdx.x & (L - 1), e0 = 4 * l;
-  const float cap = a.cap, inv_cap = 1.f / cap;
-  const float inv_tau = 1.f / (a.tau_dev ? *a.tau_dev : a.tau);
-  const bool vec = (reinterpret_cast<uintptr_t>(raw) & (4 * sizeof(T) - 1)) == 0 &&
-                   (a.row_stride & 3) == 0;
-  float ps[4] = {0.f, 0.f, 0.f, 0.f}, zs = 0.f;
-  uint32_t cn[4] = {0u, 0u, 0u, 0u}, n = 0u;
-  for (int64_t b = (int64_t)blockIdx.x * G + threadIdx.x / L; b < a.B;
-       b += (int64_t)gridDim.x * G) {
-    if (a.mask && !a.mask[b]) {
+  const int E = a.E, k = a.k, l = threadIdx.x & (L - 1), e0 = V * l;
+  const RouterScales sc(a);
+  const int64_t step = (int64_t)gridDim.x * G;
+  int64_t b = (int64_t)blockIdx.x * G + threadIdx.x / L;
+  float ps[V] = {}, zs = 0.f;
+  uint32_t cn[V] = {}, n = 0u;
+  float next[V];
+  bool next_on = true;
+  if (b < a.B) {
+    router_load<T, V>(raw + b * a.row_stride, e0, E, next);
+    if (a.mask) next_on = a.mask[b] != 0;
+  }
+  for (; b < a.B; b += step) {
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = next[j];
+    const bool on = next_on;
+    if (b + step < a.B) {     // the next token's row is on its way under this one's work
+      router_load<T, V>(raw + (b + step) * a.row_stride, e0, E, next);
+      if (a.mask) next_on = a.mask[b + step] != 0;
+    }
+    if (!on) {
       for (int j = l; j < k; j += L) {
         a.idx[b * k + j] = -1;
         a.w[b * k + j] = 0.f;
       }
       continue;
     }
-    float v[4];
-    router_load(raw + b * a.row_stride, e0, E, vec, v);
-    uint32_t key[4];
-    int pos[4] = {-1, -1, -1, -1};
+    uint32_t key[V], full[V], top = 0u, last = 0u;
+    int pos[V];
+    bool tied = false;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) key[j] = e0 + j < E ? order_key(v[j]) : 0u;
-    float top = 0.f;
-    for (int i = 0; i < k; ++i) {
-      uint64_t best = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint64_t c = (uint64_t)key[j] << 32 | (uint32_t)(kRouterMaxE - (e0 + j));
-        best = c > best ? c : best;
-      }
-#pragma unroll
-      for (int o = L / 2; o >= 1; o >>= 1) {
-        const uint64_t c = (uint64_t)__shfl_xor((uint32_t)(best >> 32), o) << 32 |
-                           __shfl_xor((uint32_t)best, o);
-        best = c > best ? c : best;
-      }
-      const int e = (int)kRouterMaxE - (int)(uint32_t)best;
-      if (i == 0) {
-        const uint32_t kb = (uint32_t)(best >> 32);
-        top = kb == 0xffffffffu ? __uint_as_float(0x7fc00000u)
-                                : __uint_as_float(kb & 0x80000000u ? kb & 0x7fffffffu : ~kb);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (e == e0 + j) {
-          pos[j] = i;
-          key[j] = 0u;
-        }
+    for (int j = 0; j < V; ++j) {
+      full[j] = e0 + j < E ? order_key(v[j]) : 0u;
+      key[j] = full[j] ? (full[j] & ~0xffu) | (255u - (uint32_t)(e0 + j)) : 0u;
+      pos[j] = -1;
     }
-    const float amax = cap * capped(top * inv_cap).t;
-    float ep[4], sp = 0.f, sz = 0.f, ss = 0.f;
+    // The k largest by keys with the expert in their low byte: each is one lane's, and one
+    // maximum finds it. bf16 logits' keys end before that byte; of fp32 ones two that
+    // differ in it alone, neighbours among the k + 1 largest, go to the exact search.
+    const int rounds = sizeof(T) == 4 && k < E ? k + 1 : k;
+    for (int i = 0; i < rounds; ++i) {
+      const uint32_t best = lanes_max<L>(max_of(key));
+      if (sizeof(T) == 4) tied = tied || (best ^ last) < 256u;
+      else if (i == 0) top = best & 0x80000000u ? best & 0xffff0000u : best | 0xffffu;
+      last = best;
+      if (i < k) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float d = cap * capped(v[j] * inv_cap).t - amax;
+        for (int j = 0; j < V; ++j) {
+          const bool it = key[j] == best;
+          pos[j] = it ? i : pos[j];
+          key[j] = it ? 0u : key[j];
+        }
+      }
+    }
+    if constexpr (sizeof(T) == 4) {
+      top = lanes_max<L>(max_of(full));
+      if (__any(tied)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) pos[j] = -1;
+        for (int i = 0; i < k; ++i) {
+          // the largest key left, in the lowest lane that holds it, its first
+          const uint32_t mine = max_of(full);
+          const uint32_t best = lanes_max<L>(mine);
+          if (lanes_min<L>(mine == best ? l : L) == l) {
+            bool open = true;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+              if (open && full[j] == best) {
+                open = false;
+                pos[j] = i;
+                full[j] = 0u;
+              }
+          }
+        }
+      }
+    }
+    const Capped m = capped(key_value(top), sc.c1);
+    float ep[V], sp = 0.f, sz = 0.f, ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const Capped c = capped(v[j], sc.c1);
+      const float d = (m.Q - c.Q) * (m.R * c.R);
       const bool in = e0 + j < E;
-      ep[j] = in ? __expf(d * inv_tau) : 0.f;
-      sz += in ? __expf(d) : 0.f;
+      ep[j] = in ? __builtin_amdgcn_exp2f(d * sc.k_p) : 0.f;
+      sz += in ? __builtin_amdgcn_exp2f(d * sc.k_z) : 0.f;
       sp += ep[j];
       ss += pos[j] >= 0 ? ep[j] : 0.f;
     }
     sp = lanes_sum<L>(sp);
     sz = lanes_sum<L>(sz);
     ss = lanes_sum<L>(ss);
-    const float inv_sp = 1.f / sp, inv_s = 1.f / (ss * inv_sp + 1e-6f);
+    const float inv_sp = __builtin_amdgcn_rcpf(sp);
+    const float inv_s = __builtin_amdgcn_rcpf(fmaf(ss, inv_sp, 1e-6f));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < V; ++j) {
       const float P = ep[j] * inv_sp;
       ps[j] += P;
       if (pos[j] >= 0) {
@@ -144,7 +221,7 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
       }
     }
     if (l == 0) {
-      const float lse = amax + __logf(sz);
+      const float lse = capped_value(key_value(top), sc.c1, a.cap) + __logf(sz);
       zs += lse * lse;
       ++n;
     }
@@ -153,7 +230,7 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
 #pragma unroll
   for (int o = L; o < 64; o <<= 1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < V; ++j) {
       ps[j] += __shfl_xor(ps[j], o);
       cn[j] += __shfl_xor(cn[j], o);
     }
@@ -161,12 +238,12 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
     n += __shfl_xor(n, o);
   }
   constexpr int W = kRouterThreads / 64;
-  __shared__ float s_p[W][4 * L], s_z[W];
-  __shared__ uint32_t s_c[W][4 * L], s_n[W];
+  __shared__ float s_p[W][V * L], s_z[W];
+  __shared__ uint32_t s_c[W][V * L], s_n[W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   if (lane < L) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < V; ++j) {
       s_p[wave][e0 + j] = ps[j];
       s_c[wave][e0 + j] = cn[j];
     }
@@ -176,146 +253,226 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
     }
   }
   __syncthreads();
-  // part: (2 E + 2, blocks): sums of P, counts, then z and N
-  const int64_t nb = gridDim.x;
-  for (int c = threadIdx.x; c < 2 * E + 2; c += kRouterThreads) {
-    if (c < E || c == 2 * E) {
-      float v = 0.f;
+  float z = 0.f;
+  uint32_t N = 0u;
 #pragma unroll
-      for (int w = 0; w < W; ++w) v += c < E ? s_p[w][c] : s_z[w];
-      a.part[c * nb + blockIdx.x] = v;
-    } else {
-      uint32_t v = 0u;
-#pragma unroll
-      for (int w = 0; w < W; ++w) v += c < 2 * E ? s_c[w][c - E] : s_n[w];
-      a.part[c * nb + blockIdx.x] = __uint_as_float(v);
-    }
+  for (int w = 0; w < W; ++w) {
+    z += s_z[w];
+    N += s_n[w];
   }
-}
-
-// counts, lb, z and N from the forward's planes; one work-group, a wave to a column.
-__global__ __launch_bounds__(1024) void k_router_finish(RouterArgs a) {
-  const int E = a.E, nb = a.blocks, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  __shared__ float s_p[kRouterMaxE], s_c[kRouterMaxE], s_z, s_n;
-  for (int c = wave; c < 2 * E + 2; c += 16) {
-    const float* col = a.part + (int64_t)c * nb;
-    if (c < E || c == 2 * E) {
-      float v = 0.f;
-      for (int i = lane; i < nb; i += 64) v += col[i];
-      v = lanes_sum<64>(v);
-      if (lane == 0) (c < E ? s_p[c] : s_z) = v;
-    } else {
-      uint32_t v = 0u;
-      for (int i = lane; i < nb; i += 64) v += __float_as_uint(col[i]);
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-      if (lane == 0) {
-        if (c < 2 * E) {
-          a.counts[c - E] = v;
-          s_c[c - E] = (float)v;
-        } else {
-          s_n = (float)v;
-        }
-      }
-    }
-  }
-  __syncthreads();
-  if (wave == 0) {
-    const float inv_n = s_n > 0.f ? 1.f / s_n : 0.f;
+  if (gridDim.x == 1) {       // the sums are whole
+    if (wave > 0) return;
+    const float inv_n = N ? 1.f / (float)N : 0.f;
     float lb = 0.f;
-    for (int e = lane; e < E; e += 64) lb += (s_c[e] * inv_n) * (s_p[e] * inv_n);
-    lb = lanes_sum<64>(lb);
+    for (int e = lane; e - lane < E; e += 64) {
+      float p = 0.f;
+      uint32_t c = 0u;
+      if (e < E)
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          p += s_p[w][e];
+          c += s_c[w][e];
+        }
+      lb += router_finish_wave(a, e, p, c, inv_n);
+    }
     if (lane == 0) {
       *a.lb = (float)E * lb;
-      *a.z = s_z * inv_n;
-      *a.tokens = s_n;
+      *a.z = z * inv_n;
+      *a.tokens = (float)N;
     }
+    return;
+  }
+  // part: (blocks, E) pairs of a sum of P and a count, (blocks) pairs of z and N, then
+  // k_router_finish's own words
+  float2* pairs = reinterpret_cast<float2*>(a.part);
+  for (int e = threadIdx.x; e < E; e += kRouterThreads) {
+    float p = 0.f;
+    uint32_t c = 0u;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      p += s_p[w][e];
+      c += s_c[w][e];
+    }
+    pairs[(int64_t)blockIdx.x * E + e] = make_float2(p, __uint_as_float(c));
+  }
+  if (threadIdx.x == 0) {
+    pairs[(int64_t)gridDim.x * E + blockIdx.x] = make_float2(z, __uint_as_float(N));
+    if (blockIdx.x == 0)      // k_router_finish counts its work-groups here
+      *reinterpret_cast<uint32_t*>(pairs + (int64_t)gridDim.x * (E + 1)) = 0u;
   }
 }
 
-template <class T, int L>
+// counts, lb, z and N from the forward's planes: a work-group to kFinishCols experts, its
+// 64 groups of lanes to the planes; with more than one the last to end adds lb's parts.
+__global__ __launch_bounds__(1024) void k_router_finish(RouterArgs a) {
+  const int E = a.E, nb = a.blocks;
+  const float2* pairs = reinterpret_cast<const float2*>(a.part);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int c = threadIdx.x & (kFinishCols - 1), e = blockIdx.x * kFinishCols + c;
+  __shared__ float s_p[16][kFinishCols], s_z[16];
+  __shared__ uint32_t s_c[16][kFinishCols], s_n[16];
+  float p = 0.f, z = 0.f;
+  uint32_t cn = 0u, n = 0u;
+  for (int i = threadIdx.x; i < nb; i += 1024) {
+    const float2 q = pairs[(int64_t)nb * E + i];
+    z += q.x;
+    n += __float_as_uint(q.y);
+  }
+  if (e < E)
+#pragma unroll 4
+    for (int i = threadIdx.x / kFinishCols; i < nb; i += 1024 / kFinishCols) {
+      const float2 q = pairs[(int64_t)i * E + e];
+      p += q.x;
+      cn += __float_as_uint(q.y);
+    }
+#pragma unroll
+  for (int o = 32; o >= kFinishCols; o >>= 1) {
+    p += __shfl_xor(p, o);
+    cn += __shfl_xor(cn, o);
+  }
+  z = lanes_sum<64>(z);
+  n = lanes_reduce<64>(n, [](uint32_t x, uint32_t y) { return x + y; });
+  if (lane < kFinishCols) {
+    s_p[wave][c] = p;
+    s_c[wave][c] = cn;
+  }
+  if (lane == 0) {
+    s_z[wave] = z;
+    s_n[wave] = n;
+  }
+  __syncthreads();
+  if (wave > 0) return;
+  p = z = 0.f;
+  cn = n = 0u;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    p += s_p[w][c];
+    cn += s_c[w][c];
+    z += s_z[w];
+    n += s_n[w];
+  }
+  const float inv_n = n ? 1.f / (float)n : 0.f;
+  const float lb = router_finish_wave(a, lane < kFinishCols ? e : E, p, cn, inv_n);
+  if (lane > 0) return;
+  if (blockIdx.x == 0) {
+    *a.z = z * inv_n;
+    *a.tokens = (float)n;
+  }
+  if (gridDim.x == 1) {
+    *a.lb = (float)E * lb;
+    return;
+  }
+  uint32_t* ended = reinterpret_cast<uint32_t*>(a.part + 2 * (int64_t)nb * (E + 1));
+  float* parts = reinterpret_cast<float*>(ended + 1);
+  __hip_atomic_store(parts + blockIdx.x, lb, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (__hip_atomic_fetch_add(ended, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) + 1u != gridDim.x)
+    return;
+  float sum = 0.f;
+  for (unsigned i = 0; i < gridDim.x; ++i)
+    sum += __hip_atomic_load(parts + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  *a.lb = (float)E * sum;
+}
+
+template <class T, int L, int V>
 __global__ __launch_bounds__(kRouterThreads) void k_router_bwd(RouterArgs a) {
   constexpr int G = kRouterThreads / L;
   const T* raw = static_cast<const T*>(a.raw);
   T* draw = static_cast<T*>(a.draw);
-  const int E = a.E, k = a.k, l = threadIdx.x & (L - 1), e0 = 4 * l;
-  const float cap = a.cap, inv_cap = 1.f / cap;
+  const int E = a.E, k = a.k, l = threadIdx.x & (L - 1), e0 = V * l;
+  const RouterScales sc(a);
   const float inv_tau = 1.f / (a.tau_dev ? *a.tau_dev : a.tau);
-  const bool vec = (reinterpret_cast<uintptr_t>(raw) & (4 * sizeof(T) - 1)) == 0 &&
-                   (a.row_stride & 3) == 0;
-  const bool vec_out = (E & 3) == 0 && (reinterpret_cast<uintptr_t>(draw) & (4 * sizeof(T) - 1)) == 0;
   const float N = *a.tokens, inv_n = N > 0.f ? 1.f / N : 0.f;
   const float cg = a.dlb ? *a.dlb * (float)E * inv_n * inv_n : 0.f;
   const float cz = a.dz ? *a.dz * 2.f * inv_n : 0.f;
-  float g0[4];
+  float g0[V];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) g0[j] = e0 + j < E ? cg * (float)a.counts[e0 + j] : 0.f;
+  for (int j = 0; j < V; ++j) g0[j] = e0 + j < E ? cg * (float)a.counts[e0 + j] : 0.f;
+  // a token's selected experts, handed from the lanes that read them to those that hold them
+  __shared__ float2 s_sel[G][V * L];
+  float2* sel = s_sel[threadIdx.x / L];
   for (int64_t b = (int64_t)blockIdx.x * G + threadIdx.x / L; b < a.B;
        b += (int64_t)gridDim.x * G) {
-    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    float o[V] = {};
+    // a masked token's row and indices (-1) are read too: the loads wait for no other
+    float v[V];
+    router_load<T, V>(raw + b * a.row_stride, e0, E, v);
+    int64_t e_first = -1;
+    float d_first = 0.f;
+    if (l < k) {
+      e_first = a.idx[b * k + l];
+      if (a.dw) d_first = a.dw[b * k + l];
+    }
+    const int64_t e_top = a.idx[b * k];
+    const float d_top = a.dw ? a.dw[b * k] : 0.f;
     if (!a.mask || a.mask[b]) {
-      float v[4], dw[4] = {0.f, 0.f, 0.f, 0.f};
-      bool sel[4] = {false, false, false, false};
-      router_load(raw + b * a.row_stride, e0, E, vec, v);
-      for (int i = 0; i < k; ++i) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) sel[e0 + j] = make_float2(0.f, 0.f);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      const float g_top = e_top >= 0 && e_top < E ? cg * (float)a.counts[e_top] : 0.f;
+      if (e_first >= 0 && e_first < E) sel[e_first] = make_float2(1.f, d_first - d_top);
+      for (int i = l + L; i < k; i += L) {
         const int64_t e = a.idx[b * k + i];
-        const float d = a.dw ? a.dw[b * k + i] : 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (e == e0 + j) {
-            sel[j] = true;
-            dw[j] = d;
-          }
+        if (e >= 0 && e < E) sel[e] = make_float2(1.f, (a.dw ? a.dw[b * k + i] : 0.f) - d_top);
       }
-      Capped t[4];
-      float amax = -INFINITY;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        t[j] = capped(v[j] * inv_cap);
-        if (e0 + j < E) amax = fmaxf(amax, cap * t[j].t);
-      }
+      for (int j = 0; j < V; ++j)
+        if (e0 + j < E) top = fmaxf(top, v[j]);
+      top = __uint_as_float(lanes_reduce<L>(__float_as_uint(top), [](uint32_t x, uint32_t y) {
+        return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+      }));
+      const Capped m = capped(top, sc.c1);
+      Capped t[V];
+      float ep[V], ez[V], dw[V], on[V], sp = 0.f, sz = 0.f, su = 0.f, sd = 0.f, sg = 0.f;
 #pragma unroll
-      for (int s = L / 2; s >= 1; s >>= 1) amax = fmaxf(amax, __shfl_xor(amax, s));
-      float ep[4], ez[4], sp = 0.f, sz = 0.f, ss = 0.f, sd = 0.f, sg = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float d = cap * t[j].t - amax;
+      for (int j = 0; j < V; ++j) {
+        const float2 s = sel[e0 + j];
+        on[j] = s.x;
+        dw[j] = s.y;
+        t[j] = capped(v[j], sc.c1);
+        const float d = (m.Q - t[j].Q) * (m.R * t[j].R);
         const bool in = e0 + j < E;
-        ep[j] = in ? __expf(d * inv_tau) : 0.f;
-        ez[j] = in ? __expf(d) : 0.f;
+        ep[j] = in ? __builtin_amdgcn_exp2f(d * sc.k_p) : 0.f;
+        ez[j] = in ? __builtin_amdgcn_exp2f(d * sc.k_z) : 0.f;
         sp += ep[j];
         sz += ez[j];
-        ss += sel[j] ? ep[j] : 0.f;
-        sd += sel[j] ? ep[j] * dw[j] : 0.f;
-        sg += ep[j] * g0[j];
+        su += on[j] != 0.f ? 0.f : ep[j];
+        sd += on[j] != 0.f ? ep[j] * dw[j] : 0.f;
+        sg += ep[j] * (g0[j] - g_top);
       }
       sp = lanes_sum<L>(sp);
       sz = lanes_sum<L>(sz);
-      ss = lanes_sum<L>(ss);
+      su = lanes_sum<L>(su);
       sd = lanes_sum<L>(sd);
       sg = lanes_sum<L>(sg);
-      const float inv_sp = 1.f / sp;
-      const float S = ss * inv_sp, inv_s = 1.f / (S + 1e-6f);
-      const float dot = sd * inv_sp * inv_s;                       // sum_i dw_i w_i
-      // sum_e P_e g_e: the balance loss's part and the selected ones'
-      const float pg = sg * inv_sp + (sd * inv_sp - S * dot) * inv_s;
-      const float zc = cz * (amax + __logf(sz)) / sz;
+      const float inv_sp = __builtin_amdgcn_rcpf(sp);
+      const float inv_s = __builtin_amdgcn_rcpf((sp - su) * inv_sp + 1e-6f);
+      // the top's own part of g beside the balance loss's: dw_0 - sum_i dw_i w_i, over s
+      const float gs = (d_top * 1e-6f * inv_s - sd * inv_sp * inv_s) * inv_s;
+      const float pg = (sg + sd * inv_s - su * gs) * inv_sp;       // sum_e P_e (g_e - g_0)
+      const float zc = cz * (capped_value(top, sc.c1, a.cap) + __logf(sz)) * __builtin_amdgcn_rcpf(sz);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float g = g0[j] + (sel[j] ? (dw[j] - dot) * inv_s : 0.f);
-        o[j] = (ep[j] * inv_sp * (g - pg) * inv_tau + zc * ez[j]) * t[j].sech2;
+      for (int j = 0; j < V; ++j) {
+        const float g = g0[j] - g_top + (on[j] != 0.f ? dw[j] * inv_s : -gs);
+        o[j] = (ep[j] * inv_sp * (g - pg) * inv_tau + zc * ez[j]) * (4.f * t[j].Q * t[j].R * t[j].R);
       }
     }
     T* row = draw + b * E;
-    if (vec_out && e0 + 4 <= E) {
-      if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<float4*>(row + e0) = make_float4(o[0], o[1], o[2], o[3]);
-      else
-        *reinterpret_cast<uint2*>(row + e0) =
-            make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    if (e0 + V <= E) {
+      constexpr int W = V * (int)sizeof(T) / 4;
+      typedef uint32_t vec __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+      vec q;
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        if constexpr (sizeof(T) == 4) q[j] = __float_as_uint(o[j]);
+        else q[j] = pack_bf16x2(o[2 * j], o[2 * j + 1]);
+      *reinterpret_cast<vec*>(row + e0) = q;
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < V; ++j)
         if (e0 + j < E) store_from_f32(row + e0 + j, o[j]);
     }
   }

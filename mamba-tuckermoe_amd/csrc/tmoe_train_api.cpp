@@ -104,7 +104,7 @@ int tmoe_router_forward(const tmoe_router* r, int64_t* idx, float* w, float* lb,
   if ((r->B > 0 && (!idx || !w)) || !lb || !z || !tokens || !counts || !workspace)
     return fail(TMOE_EINVAL, "%s: null pointer", who);
   if (!on(idx, 8) || !on(w, 4) || !on(lb, 4) || !on(z, 4) || !on(tokens, 4) || !on(counts, 8) ||
-      !on(workspace, 4))
+      !on(workspace, 8))
     return fail(TMOE_EINVAL, "%s: misaligned pointer", who);
   const size_t need = tmoe::router_workspace_bytes(r->B, r->E);
   if (workspace_bytes < need)

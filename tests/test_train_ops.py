@@ -206,14 +206,14 @@ def test_router_abi_refuses_pointers(pkg):
 
 def _norm(pkg, **kw):
     d = dict(x=OK, y=OK, gate=OK, x_stride=64, y_stride=64, gate_stride=64, post_weight=OK, gamma=OK,
-             next_weight=OK, T=4, d=64, dtype=0, eps=1e-5)
+             next_weight=OK, T=40, d=64, dtype=0, eps=1e-5)
     d.update(kw)
     return ctypes.byref(pkg._lib.TmoeBlockNorm(**d))
 
 
 def test_norm_abi_refuses(pkg):
     L = pkg._lib.lib()
-    ws = L.tmoe_block_norm_workspace_bytes(4, 64, 0)
+    ws = L.tmoe_block_norm_workspace_bytes(40, 64, 0)
     assert ws > 0 and L.tmoe_block_norm_workspace_bytes(4, 20000, 0) == 0
     assert L.tmoe_block_norm_workspace_bytes(4, 64, 5) == 0
 
