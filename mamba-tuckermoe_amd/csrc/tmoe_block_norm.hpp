@@ -12,8 +12,9 @@
 //
 // Bound by memory: every activation is read once and every output written once; a row lies
 // in the registers of its threads between its two norms, and the next row is on its way
-// meanwhile. Rows of at most 1024 elements take one wave (no barrier), four neighbours a
-// lane and step; longer ones a work-group, 16 bytes a thread and step. The weights'
+// meanwhile. Rows of at most 1024 elements take a wave, or a half or a quarter of one (no
+// barrier), four neighbours a lane and step; longer ones a work-group, 16 bytes a thread
+// and step. The weights'
 // gradients are summed in registers over a work-group's rows, then in planes of `part` that
 // k_block_norm_cols adds in a fixed order; one work-group alone has them whole.
 #pragma once
@@ -25,17 +26,29 @@ namespace tmoe {
 namespace dev {
 
 // Elements a thread holds of a row: NCH steps of EPC neighbours, each one load of any
-// alignment (a row of odd width begins anywhere). kTail: d is no multiple of EPC, and one
-// thread's last step takes what is left element by element.
-template <class T, int EPC_, int NCH_, bool kTail_>
+// alignment (a row of odd width begins anywhere). Where d is no multiple of EPC (kOverlap)
+// the last step's are the row's last EPC: the first `dup` of them are its neighbour's too,
+// computed and stored alike by both, and left out of the row's sums here. Rows of fewer than
+// EPC elements (kTiny) go element by element.
+enum RowEnd { kWhole, kOverlap, kTiny };
+
+template <class T, int EPC_, int NCH_, RowEnd kEnd_>
 struct RowMap {
   static constexpr int EPC = EPC_, NCH = NCH_, N = NCH * EPC, kWords = EPC * (int)sizeof(T) / 4;
-  static constexpr bool kTail = kTail_;
+  static constexpr RowEnd kEnd = kEnd_;
   typedef uint32_t vec __attribute__((ext_vector_type(kWords), aligned(sizeof(T))));
   int tid, tpr;
   int64_t d;
-  __device__ int64_t col(int k) const { return ((int64_t)k * tpr + tid) * EPC; }
-  __device__ bool whole(int k) const { return col(k) + (kTail ? EPC : 1) <= d; }
+  __device__ int64_t first(int k) const { return ((int64_t)k * tpr + tid) * EPC; }
+  __device__ bool in(int k) const { return first(k) < d; }
+  __device__ int64_t col(int k) const {
+    const int64_t c = first(k);
+    return kEnd == kOverlap && c > d - EPC ? d - EPC : c;
+  }
+  // whether element i of the thread's is this thread's to count
+  __device__ bool mine(int i) const {
+    return kEnd != kOverlap || col(i / EPC) + i % EPC >= first(i / EPC);
+  }
 };
 
 // A row's elements in registers as they are stored.
@@ -47,14 +60,14 @@ struct RowRegs {
 #pragma unroll
     for (int k = 0; k < M::NCH; ++k) {
       typename M::vec v = (uint32_t)0;
-      if (m.whole(k)) v = *reinterpret_cast<const typename M::vec*>(p + m.col(k));
-      else if constexpr (M::kTail) {
-#pragma unroll
-        for (int j = 0; j < M::EPC - 1; ++j)
-          if (m.col(k) + j < m.d) {
-            if constexpr (sizeof(T) == 2) v[j / 2] |= (uint32_t)p[m.col(k) + j] << 16 * (j & 1);
-            else v[j] = __float_as_uint(p[m.col(k) + j]);
+      if constexpr (M::kEnd == kTiny) {
+        for (int j = 0; j < M::EPC; ++j)
+          if (m.first(k) + j < m.d) {
+            if constexpr (sizeof(T) == 2) v[j / 2] |= (uint32_t)p[m.first(k) + j] << 16 * (j & 1);
+            else v[j] = __float_as_uint(p[m.first(k) + j]);
           }
+      } else if (m.in(k)) {
+        v = *reinterpret_cast<const typename M::vec*>(p + m.col(k));
       }
 #pragma unroll
       for (int j = 0; j < M::kWords; ++j) q[k][j] = v[j];
@@ -72,7 +85,10 @@ __device__ __forceinline__ void row_store(const M& m, void* base, int64_t row, c
   T* p = static_cast<T*>(base) + row * m.d;
 #pragma unroll
   for (int k = 0; k < M::NCH; ++k) {
-    if (m.whole(k)) {
+    if constexpr (M::kEnd == kTiny) {
+      for (int j = 0; j < M::EPC; ++j)
+        if (m.first(k) + j < m.d) store_from_f32(p + m.first(k) + j, v[k * M::EPC + j]);
+    } else if (m.in(k)) {
       typename M::vec q;
 #pragma unroll
       for (int j = 0; j < M::kWords; ++j)
@@ -81,21 +97,18 @@ __device__ __forceinline__ void row_store(const M& m, void* base, int64_t row, c
         else
           q[j] = __float_as_uint(v[k * M::EPC + j]);
       *reinterpret_cast<typename M::vec*>(p + m.col(k)) = q;
-    } else if constexpr (M::kTail) {
-#pragma unroll
-      for (int j = 0; j < M::EPC - 1; ++j)
-        if (m.col(k) + j < m.d) store_from_f32(p + m.col(k) + j, v[k * M::EPC + j]);
     }
   }
 }
 
-// Sum over a row's threads, the same value in all of them. lds: sixteen floats, zero past
+// Sum over a row's threads (kLanes of a wave, or 0: the work-group), the same value in all of
+// them. lds: sixteen floats, zero past
 // the work-group's waves, that nobody else has written to since the barrier before the last
 // (one barrier a sum).
-template <bool kWave>
+template <int kLanes>
 __device__ __forceinline__ float row_sum(float v, float* lds) {
-  v = lanes_sum<64>(v);
-  if constexpr (!kWave) {
+  v = lanes_sum<kLanes ? kLanes : 64>(v);
+  if constexpr (kLanes == 0) {
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     v = lanes_sum<16>(lds[threadIdx.x & 15]);
@@ -113,31 +126,32 @@ __device__ __forceinline__ float sigmoid(float g) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
 }
 
-constexpr int kNormThreads = 256;   // of a work-group whose rows take a wave each
-constexpr int kNormTeams = kNormThreads / 64;
+constexpr int kNormThreads = 256;   // of a work-group whose rows take at most a wave each
 
 // The step of a kernel over the rows, and its threads' place in a row.
-template <class M, bool kWave>
+template <class M, int kLanes>
 struct RowWalk {
+  static constexpr int kTeams = kLanes ? kNormThreads / kLanes : 1;   // rows at a time
   M m;
-  int teams, team;
+  int team;
   int64_t row, step;
   __device__ explicit RowWalk(int64_t d)
-      : m{kWave ? (int)(threadIdx.x & 63) : (int)threadIdx.x, kWave ? 64 : (int)blockDim.x, d},
-        teams(kWave ? kNormTeams : 1), team(kWave ? (int)(threadIdx.x >> 6) : 0),
-        row((int64_t)blockIdx.x * teams + team), step((int64_t)gridDim.x * teams) {}
+      : m{kLanes ? (int)(threadIdx.x & (kLanes - 1)) : (int)threadIdx.x,
+          kLanes ? kLanes : (int)blockDim.x, d},
+        team(kLanes ? (int)(threadIdx.x / (kLanes ? kLanes : 1)) : 0),
+        row((int64_t)blockIdx.x * kTeams + team), step((int64_t)gridDim.x * kTeams) {}
 };
 
-template <class T, int EPC, int NCH, bool kWave, bool kTail, int kThreads>
+template <class T, int EPC, int NCH, int kLanes, RowEnd kEnd, int kThreads>
 __global__ __launch_bounds__(kThreads) void k_block_norm_fwd(BlockNormArgs a) {
-  using M = RowMap<T, EPC, NCH, kTail>;
+  using M = RowMap<T, EPC, NCH, kEnd>;
   using R = RowRegs<M, T>;
   constexpr int N = M::N;
   __shared__ float lds[4][16];
-  RowWalk<M, kWave> w(a.d);
+  RowWalk<M, kLanes> w(a.d);
   const M& m = w.m;
   const float inv_d = 1.f / (float)a.d;
-  if (!kWave) row_sum_clear(lds);
+  if (kLanes == 0) row_sum_clear(lds);
   R ny, nx, ng;
   if (w.row < a.T) {
     ny.load(m, a.y, w.row, a.y_rs);
@@ -164,8 +178,8 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_fwd(BlockNormArgs a) {
       pw.load(m, a.post_w, 0, 0);
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) ss += f[i] * f[i];
-      const float inv = 1.f / sqrtf(row_sum<kWave>(ss, lds[par]) * inv_d + a.eps);
+      for (int i = 0; i < N; ++i) ss += m.mine(i) ? f[i] * f[i] : 0.f;
+      const float inv = 1.f / sqrtf(row_sum<kLanes>(ss, lds[par]) * inv_d + a.eps);
       if (a.inv && m.tid == 0) a.inv[b] = inv;
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] *= inv * pw[i];
@@ -186,8 +200,8 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_fwd(BlockNormArgs a) {
       nw.load(m, a.next_w, 0, 0);
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) ss += f[i] * f[i];
-      const float inv = 1.f / sqrtf(row_sum<kWave>(ss, lds[par + 1]) * inv_d + a.eps);
+      for (int i = 0; i < N; ++i) ss += m.mine(i) ? f[i] * f[i] : 0.f;
+      const float inv = 1.f / sqrtf(row_sum<kLanes>(ss, lds[par + 1]) * inv_d + a.eps);
       if (a.inv && m.tid == 0) a.inv[a.T + b] = inv;
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] *= inv * nw[i];
@@ -196,29 +210,30 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_fwd(BlockNormArgs a) {
   }
 }
 
-// Operands of a backward as the bits of F: known when it is compiled, and with them every
-// gradient wanted and dr (and dh with kNext) there, so that a row's loads and stores have
-// their places and none waits for another; F = -1 looks at the pointers. kFull: F may hold
-// a gate or a norm after the block; without, neither's registers are held.
-constexpr int kGate = 1, kPost = 2, kRes = 4, kGamma = 8, kNext = 16;
+// What a backward's rows load and store as the bits of F: known when it is compiled, with
+// dr (and dh with kNext) there and every row's gradient wanted, so that the loads and stores
+// have their places and none waits for another (a load of the next row that may or may not
+// be followed by a store is waited for with that store); F = -1 looks at the pointers.
+// kFull: with a gate or a norm after the block; without, neither's registers are held.
+constexpr int kGate = 1, kRes = 2, kNext = 4, kPost = 8;
 
-template <class T, int EPC, int NCH, bool kWave, bool kTail, int kThreads, bool kFull, int F>
+template <class T, int EPC, int NCH, int kLanes, RowEnd kEnd, int kThreads, bool kFull, int F>
 __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
 // the same roundings whichever gradients are wanted: fused where it is written
 #pragma clang fp contract(off)
-  using M = RowMap<T, EPC, NCH, kTail>;
+  using M = RowMap<T, EPC, NCH, kEnd>;
   using R = RowRegs<M, T>;
   constexpr int N = M::N;
   constexpr bool kAny = F < 0;
   __shared__ float lds[4][16];
-  RowWalk<M, kWave> w(a.d);
+  RowWalk<M, kLanes> w(a.d);
   const M& m = w.m;
   const float inv_d = 1.f / (float)a.d;
-  if (!kWave) row_sum_clear(lds);
+  if (kLanes == 0) row_sum_clear(lds);
   const bool gated = kFull && (kAny ? a.gate != nullptr : (F & kGate) != 0);
   const bool post = kFull && (kAny ? a.post_w != nullptr : (F & kPost) != 0);
   const bool res = kAny ? a.x != nullptr : (F & kRes) != 0;
-  const bool scaled = kAny ? a.gamma != nullptr : (F & kGamma) != 0;
+  const bool scaled = a.gamma != nullptr;
   const bool next = kAny ? a.dh != nullptr : (F & kNext) != 0;
   const bool dr_in = kAny ? a.dr != nullptr : true;
   float s_post[kFull ? N : 1], s_gamma[N], s_next[N];
@@ -299,9 +314,9 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
         nr[i] *= inv_r;
         const float t = dh[i] * nr[i];
         s_next[i] += t;
-        dot = fmaf(t, nw[i], dot);
+        dot = m.mine(i) ? fmaf(t, nw[i], dot) : dot;
       }
-      dot = row_sum<kWave>(dot, lds[par]) * inv_d * inv_r;
+      dot = row_sum<kLanes>(dot, lds[par]) * inv_d * inv_r;
 #pragma unroll
       for (int i = 0; i < N; ++i) D[i] = fmaf(-nr[i], dot, fmaf(dh[i] * nw[i], inv_r, D[i]));
     }
@@ -320,9 +335,9 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
         for (int i = 0; i < N; ++i) {
           const float t = D[i] * nu[i];
           s_post[i] += t;
-          dot = fmaf(t, pw[i], dot);
+          dot = m.mine(i) ? fmaf(t, pw[i], dot) : dot;
         }
-        dot = row_sum<kWave>(dot, lds[par + 1]) * inv_d * inv_u;
+        dot = row_sum<kLanes>(dot, lds[par + 1]) * inv_d * inv_u;
 #pragma unroll
         for (int i = 0; i < N; ++i) D[i] = fmaf(-nu[i], dot, D[i] * pw[i] * inv_u);
       }
@@ -346,19 +361,20 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
     if (kAny ? a.dy != nullptr : true) row_store<T>(m, a.dy, b, D);
   }
   if (!a.dpost_w && !a.dgamma && !a.dnext_w) return;
-  // a wave's rows apart: their sums over the work-group first, in the waves' order
-  if constexpr (kWave) {
-    __shared__ float s[kNormTeams][N * 64];
+  // a work-group's rows apart: their sums over it first, in the order of the teams
+  if constexpr (kLanes > 0) {
+    constexpr int kTeams = RowWalk<M, kLanes>::kTeams;
+    __shared__ float s[kTeams][N * kLanes];
     auto join = [&](float (&v)[N]) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < N; ++i) s[w.team][i * 64 + m.tid] = v[i];
+      for (int i = 0; i < N; ++i) s[w.team][i * kLanes + m.tid] = v[i];
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         v[i] = 0.f;
 #pragma unroll
-        for (int t = 0; t < kNormTeams; ++t) v[i] += s[t][i * 64 + m.tid];
+        for (int t = 0; t < kTeams; ++t) v[i] += s[t][i * kLanes + m.tid];
       }
     };
     if constexpr (kFull)
@@ -376,7 +392,7 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
     for (int k = 0; k < NCH; ++k)
 #pragma unroll
       for (int j = 0; j < EPC; ++j)
-        if (m.col(k) + j < a.d) p[m.col(k) + j] = v[k * EPC + j];
+        if (m.in(k) && m.col(k) + j < a.d) p[m.col(k) + j] = v[k * EPC + j];
   };
   if constexpr (kFull) put(s_post, 0, a.dpost_w);
   put(s_gamma, 1, a.dgamma);

@@ -10,7 +10,7 @@ namespace {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct NormPlan {
-  bool wave;            // a wave to a row
+  int lanes;            // of a row in a wave, or 0: a row takes a work-group
   int steps;            // of 4 elements a lane, or of 16 bytes a thread
   unsigned threads;
   int teams;            // rows at a time in a work-group
@@ -18,11 +18,13 @@ struct NormPlan {
 // full: the backward with a gate or a norm after the block, whose rows of over 512 elements
 // would need more registers than one wave's lanes have.
 NormPlan norm_plan(int64_t d, int es, bool full) {
-  if (d <= (full ? 512 : 1024))
-    return {true, (int)ceil_div(d, 256), dev::kNormThreads, dev::kNormTeams};
+  if (d <= (full ? 512 : 1024)) {
+    const int lanes = d <= 64 ? 16 : d <= 128 ? 32 : 64;
+    return {lanes, (int)ceil_div(d, 4 * lanes), dev::kNormThreads, dev::kNormThreads / lanes};
+  }
   const int64_t nch = ceil_div(d * es, 16);
   const int c = nch <= 1024 ? 1 : nch <= 2048 ? 2 : 4;
-  return {false, c, (unsigned)(ceil_div(nch, 64 * c) * 64), 1};
+  return {0, c, (unsigned)(ceil_div(nch, 64 * c) * 64), 1};
 }
 // Work-groups of a persistent walk over the rows: what the chip holds at once.
 int64_t norm_blocks(int64_t T, const NormPlan& p) {
@@ -35,67 +37,69 @@ int64_t norm_blocks(int64_t T, const NormPlan& p) {
 // against 114, 123 and 127, 25.7 against 26.6, 26.2 and 26.8 of d = 768 with a residual
 // and the next norm). One for so few rows that a second launch would cost more than their
 // walk.
-constexpr int64_t kNormBwdBlocks = 512;
 int64_t norm_bwd_blocks(int64_t T, const NormPlan& p) {
   const int64_t n = ceil_div(T, p.teams);
-  return n <= 2 ? 1 : n < kNormBwdBlocks ? n : kNormBwdBlocks;
+  const int64_t most = p.threads <= 512 ? 512 : 256;   // of 1024 threads a unit holds one
+  return n <= 2 ? 1 : n < most ? n : most;
 }
 
 using NormKernel = void (*)(BlockNormArgs);
 
-// The form of a backward that has a kernel of its own (-1: it has none): what the training
-// blocks' ends are made of, with every gradient wanted.
+// The form (F) of a backward whose rows' gradients are all wanted, else -1.
 int norm_form(const BlockNormArgs& a) {
   using namespace dev;
-  const int f = (a.gate ? kGate : 0) | (a.post_w ? kPost : 0) | (a.x ? kRes : 0) |
-                (a.gamma ? kGamma : 0) | (a.next_w ? kNext : 0);
   const bool all = a.dr && a.dy && (a.dh || !a.next_w) && (a.dx || !a.x) && (a.dgate || !a.gate);
-  const bool own = f == (kRes | kGamma | kNext) || f == (kRes | kGamma) || f == kGate ||
-                   f == (kGate | kPost) || f == (kGate | kPost | kRes | kGamma | kNext);
-  return all && own ? f : -1;
+  return !all ? -1
+              : (a.gate ? kGate : 0) | (a.x ? kRes : 0) | (a.next_w ? kNext : 0) | (a.post_w ? kPost : 0);
 }
-template <class T, int EPC, int NCH, bool kWave, bool kTail, int kThreads>
-NormKernel norm_bwd_kernel(int form, bool full) {
+template <class T, int EPC, int NCH, int kLanes, dev::RowEnd kEnd, int kThreads, bool kFull>
+NormKernel norm_bwd_form(int form) {
   using namespace dev;
-#define TMOE_FORM(F)                                                                         \
-  if (form == (F))                                                                           \
-    return k_block_norm_bwd<T, EPC, NCH, kWave, kTail, kThreads, ((F) & (kGate | kPost)) != 0, (F)>;
-  if constexpr (kThreads <= 512) {
-    TMOE_FORM(kRes | kGamma | kNext)
-    TMOE_FORM(kRes | kGamma)
-    if constexpr (!kWave || NCH <= 2) {
-      TMOE_FORM(kGate)
-      TMOE_FORM(kGate | kPost)
-      TMOE_FORM(kGate | kPost | kRes | kGamma | kNext)
+#define TMOE_FORM(F) \
+  case F: return k_block_norm_bwd<T, EPC, NCH, kLanes, kEnd, kThreads, kFull, (F)>;
+#define TMOE_FORMS(F) TMOE_FORM(F) TMOE_FORM(F | kRes) TMOE_FORM(F | kNext) TMOE_FORM(F | kRes | kNext)
+  if constexpr (kThreads <= 512 && kEnd != kTiny) {
+    if constexpr (kFull) switch (form) {
+      TMOE_FORMS(kGate) TMOE_FORMS(kPost) TMOE_FORMS(kGate | kPost)
+    }
+    else switch (form) {
+      TMOE_FORMS(0)
     }
   }
+#undef TMOE_FORMS
 #undef TMOE_FORM
-  if constexpr (!kWave || NCH <= 2)
-    if (full) return k_block_norm_bwd<T, EPC, NCH, kWave, kTail, kThreads, true, -1>;
-  return k_block_norm_bwd<T, EPC, NCH, kWave, kTail, kThreads, false, -1>;
+  return k_block_norm_bwd<T, EPC, NCH, kLanes, kEnd, kThreads, kFull, -1>;
 }
-template <class T, bool kTail>
+template <class T, dev::RowEnd kEnd>
 NormKernel norm_kernel(const BlockNormArgs& a, bool backward, const NormPlan& p) {
   const bool full = a.gate || a.post_w;
   const int form = backward ? norm_form(a) : -1;
-#define TMOE_NORM(EPC, C, W, THREADS)                                                        \
-  if (p.wave == W && p.steps == C && p.threads <= THREADS)                                   \
-    return backward ? norm_bwd_kernel<T, EPC, C, W, kTail, THREADS>(form, full)              \
-                    : dev::k_block_norm_fwd<T, EPC, C, W, kTail, THREADS>;
+#define TMOE_NORM(EPC, C, LANES, THREADS)                                                     \
+  if (p.lanes == LANES && p.steps == C && p.threads <= THREADS) {                             \
+    if (!backward) return dev::k_block_norm_fwd<T, EPC, C, LANES, kEnd, THREADS>;            \
+    if constexpr (LANES == 0 || C <= 2)                                                       \
+      if (full) return norm_bwd_form<T, EPC, C, LANES, kEnd, THREADS, true>(form);           \
+    return norm_bwd_form<T, EPC, C, LANES, kEnd, THREADS, false>(form);                      \
+  }
   constexpr int E16 = 16 / (int)sizeof(T);
-  TMOE_NORM(4, 1, true, 256) TMOE_NORM(4, 2, true, 256)
-  TMOE_NORM(4, 3, true, 256) TMOE_NORM(4, 4, true, 256)
-  TMOE_NORM(E16, 1, false, 512) TMOE_NORM(E16, 1, false, 1024)
-  TMOE_NORM(E16, 2, false, 1024) TMOE_NORM(E16, 4, false, 1024)
+  TMOE_NORM(4, 1, 16, 256)
+  if constexpr (kEnd != dev::kTiny) {
+    TMOE_NORM(4, 1, 32, 256)
+    TMOE_NORM(4, 1, 64, 256) TMOE_NORM(4, 2, 64, 256)
+    TMOE_NORM(4, 3, 64, 256) TMOE_NORM(4, 4, 64, 256)
+    TMOE_NORM(E16, 1, 0, 512) TMOE_NORM(E16, 1, 0, 768) TMOE_NORM(E16, 1, 0, 1024)
+    TMOE_NORM(E16, 2, 0, 768) TMOE_NORM(E16, 2, 0, 1024) TMOE_NORM(E16, 4, 0, 1024)
+  }
 #undef TMOE_NORM
   return nullptr;
 }
 template <class T>
 hipError_t norm_launch(const BlockNormArgs& a, bool backward, const NormPlan& p, int64_t blocks,
                        hipStream_t st) {
-  const int epc = p.wave ? 4 : 16 / (int)sizeof(T);
-  const NormKernel k = a.d % epc ? norm_kernel<T, true>(a, backward, p)
-                                 : norm_kernel<T, false>(a, backward, p);
+  const int epc = p.lanes ? 4 : 16 / (int)sizeof(T);
+  const NormKernel k = a.d < epc    ? norm_kernel<T, dev::kTiny>(a, backward, p)
+                       : a.d % epc ? norm_kernel<T, dev::kOverlap>(a, backward, p)
+                                   : norm_kernel<T, dev::kWhole>(a, backward, p);
   hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(p.threads), 0, st, a);
   return hipGetLastError();
 }
