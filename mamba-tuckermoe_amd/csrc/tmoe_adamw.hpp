@@ -165,74 +165,100 @@ __device__ __forceinline__ float quotient(float a, float b, float y) {
   return fmaf(fmaf(-q, b, a), y, q);
 }
 
-// sqrt(v) to the last place but for one value in millions
+// sqrt(v) to the last place but for one value in millions (and for v below 2^-126)
 __device__ __forceinline__ float root_of(float v) {
-  const float y = __builtin_amdgcn_rsqf(v), s = v * y;
-  const float r = fmaf(fmaf(-s, s, v), 0.5f * y, s);
-  return v == 0.f || v == INFINITY ? v : r;
+  const float y = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-126f)), s = v * y;
+  return v != v ? v : fmaf(fmaf(-s, s, v), 0.5f * y, s);
 }
 
 // A magnitude a in [0, 448] as the e4m3 value below it and what is left over: `code`, and in
 // units of 2^-20 of the step between the two, `at` = the value's place counted from its
-// octave's (the subnormals': zero's) first, `rest` over it.
+// octave's (the subnormals': zero's) first, `rest` over it. kSub: a may be under 2^-6, where
+// values are 2^-9 apart as they are from 2^-6 on: the sum's mantissa is both places.
 struct E4m3Place {
   uint32_t code, at, rest;
 };
+template <bool kSub>
 __device__ __forceinline__ E4m3Place e4m3_place(float a) {
-  // under 2^-6 values are 2^-9 apart, as they are from 2^-6 on: the sum's mantissa is both
-  const bool sub = a < 0x1p-6f;
+  const bool sub = kSub && a < 0x1p-6f;
   const uint32_t b = __float_as_uint(sub ? a + 0x1p-6f : a);
   const uint32_t A = (b & 0x7fffffu) | (sub ? 0u : 0x800000u);
   return {(b >> 20) - (sub ? 968u : 960u), A & 0xf00000u, A & 0xfffffu};
 }
-// The code of a magnitude, up with the chance rest / step; u16: 16 random bits.
+// The code of a magnitude, up with the chance rest / step; u16: 16 random bits. A quotient
+// that rounding put over 448 is a place or two over it: no bits are low enough to go up.
+template <bool kSub>
 __device__ __forceinline__ uint32_t e4m3_code(float a, uint32_t u16) {
-  const E4m3Place p = e4m3_place(a);
+  const E4m3Place p = e4m3_place<kSub>(a);
   return p.code + ((u16 << 4 | 8u) < p.rest ? 1u : 0u);
 }
 // The code of a root r, up with the chance (r^2 - lo^2) / (hi^2 - lo^2)
-// = rest (r + lo) / (hi + lo); inv_odd: 1 / (2 q + 1) rounded, for q = 0 .. 15.
-__device__ __forceinline__ uint32_t e4m3_root_code(float r, uint32_t u16, const float* inv_odd) {
+// = rest (r + lo) / (hi + lo); odd: (2 q + 1, its reciprocal rounded) for q = 0 .. 15.
+template <bool kSub>
+__device__ __forceinline__ uint32_t e4m3_root_code(float r, uint32_t u16, const float2* odd) {
 #pragma clang fp contract(off)
-  const E4m3Place p = e4m3_place(r);
-  const uint32_t q = p.at >> 20;
-  const float t = quotient((float)(2u * p.at + p.rest), (float)(2u * q + 1u), inv_odd[q]);
+  const E4m3Place p = e4m3_place<kSub>(r);
+  const float2 o = odd[p.at >> 20];
+  const float t = quotient((float)(2u * p.at + p.rest), o.x, o.y);
   const float chance = (float)p.rest * t;                       // 2^40 of it
   const float u = fmaf((float)u16, 0x1p+24f, 0x1p+23f);
   const uint32_t c = p.code + (u < chance ? 1u : 0u);
-  return max(c, min(__float_as_uint(r), 1u));
+  return kSub ? max(c, min(__float_as_uint(r), 1u)) : c;
+}
+// The codes of four moments (m over their scale, r over theirs).
+template <bool kSub>
+__device__ __forceinline__ uint2 e4m3_codes(const float (&m)[4], const float (&qm)[4],
+                                            const float (&qr)[4], uint32_t key, uint32_t step_key,
+                                            const float2* odd) {
+  uint2 c = {0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t h = mix32((key + (uint32_t)j) ^ step_key);
+    const uint32_t sign = __float_as_uint(m[j]) >> 24 & 0x80u;
+    c.x |= (e4m3_code<kSub>(qm[j], h >> 16) | sign) << 8 * j;
+    c.y |= e4m3_root_code<kSub>(qr[j], h & 0xffffu, odd) << 8 * j;
+  }
+  return c;
 }
 
 // A wave takes blocks of 256 elements, four neighbours a lane. What decides a code is
 // computed as the formulas round it (a step's codes are the next one's values), the rest
-// with the hardware's reciprocals: at 170 instructions an element the arithmetic, not the
-// memory, was the bound.
+// with the hardware's reciprocals: the arithmetic, not the memory, is the bound. A moment
+// whose block's scale is under 2^-110 is taken for zero (the reciprocal of less overflows).
 template <class T>
 __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
 #pragma clang fp contract(off)
-  __shared__ float inv_odd[16];
-  if (threadIdx.x < 16) inv_odd[threadIdx.x] = 1.f / (float)(2 * threadIdx.x + 1);
+  __shared__ float2 odd[16];
+  if (threadIdx.x < 16) {
+    const float o = (float)(2 * threadIdx.x + 1);
+    odd[threadIdx.x] = make_float2(o, 1.f / o);
+  }
   __syncthreads();
   const AdamwStep s = adamw_step(a);
-  T* p = static_cast<T*>(a.p[s.t]);
-  const T* g = static_cast<const T*>(a.g[s.t]);
-  uint8_t* mq = static_cast<uint8_t*>(a.m[s.t]);
-  uint8_t* rq = static_cast<uint8_t*>(a.v[s.t]);
-  float* ms = a.ms[s.t];
-  float* rs = a.vs[s.t];
-  const int64_t n = a.n[s.t], end = s.base + a.chunk < n ? s.base + a.chunk : n;
-  const uint32_t tkey = (a.first + (uint32_t)s.t) * 0x9E3779B9u;
+  const int64_t n = a.n[s.t];
+  // the wave's part of the work-group's chunk: `count` elements from `first` on, in 32 bits
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t all = (uint32_t)(a.chunk < n - s.base ? a.chunk : n - s.base);
+  const int64_t first = s.base + wave * kAdamwBlock;
+  const uint32_t count = all > wave * kAdamwBlock ? all - wave * kAdamwBlock : 0u;
+  T* p = static_cast<T*>(a.p[s.t]) + first;
+  const T* g = static_cast<const T*>(a.g[s.t]) + first;
+  uint8_t* mq = static_cast<uint8_t*>(a.m[s.t]) + first;
+  uint8_t* rq = static_cast<uint8_t*>(a.v[s.t]) + first;
+  float* ms = a.ms[s.t] + first / kAdamwBlock;
+  float* rs = a.vs[s.t] + first / kAdamwBlock;
   const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) &
                     (4 * sizeof(T) - 1)) == 0 &&
                    ((reinterpret_cast<uintptr_t>(mq) | reinterpret_cast<uintptr_t>(rq)) & 3) == 0;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int64_t b = s.base + wave * kAdamwBlock; b < end; b += kAdamwThreads / 64 * kAdamwBlock) {
-    const int64_t i = b + 4 * lane, blk = b / kAdamwBlock;
-    const int live = (int)(n - i < 4 ? (n - i < 0 ? 0 : n - i) : 4);
+  for (uint32_t b = 0, blk = 0; b < count;
+       b += kAdamwThreads / 64 * kAdamwBlock, blk += kAdamwThreads / 64) {
+    const uint32_t i = b + 4 * lane;
+    const bool whole = vec && i + 4 <= count;
+    const int live = i + 4 <= count ? 4 : i < count ? (int)(count - i) : 0;
     const float sm = ms[blk], sr = rs[blk];
     float pv[4] = {}, gv[4] = {}, m[4], r[4];
     uint32_t mc = 0u, rc = 0u;
-    if (vec && live == 4) {
+    if (whole) {
       load4(p + i, pv);
       load4(g + i, gv);
       mc = *reinterpret_cast<const uint32_t*>(mq + i);
@@ -264,29 +290,37 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
       am = max(am, __float_as_uint(m[j]) & 0x7fffffffu);
       ar = max(ar, __float_as_uint(r[j]) & 0x7fffffffu);
     }
-    const float nsm = __uint_as_float(lanes_max<64>(am)) * (1.f / kE4m3Max);
-    const float nsr = __uint_as_float(lanes_max<64>(ar)) * (1.f / kE4m3Max);
-    const float dm = nsm > 0.f ? nsm : 1.f, dr = nsr > 0.f ? nsr : 1.f;
-    const float im = 1.f / dm, ir = 1.f / dr;
-    mc = rc = 0u;
+    float nsm = __uint_as_float(lanes_max<64>(am)) * (1.f / kE4m3Max);
+    float nsr = __uint_as_float(lanes_max<64>(ar)) * (1.f / kE4m3Max);
+    nsm = nsm < 0x1p-110f ? 0.f : nsm;
+    nsr = nsr < 0x1p-110f ? 0.f : nsr;
+    const float dm = nsm == 0.f ? 1.f : nsm, dr = nsr == 0.f ? 1.f : nsr;
+    // reciprocals to half a place, for quotient()
+    float im = __builtin_amdgcn_rcpf(dm), ir = __builtin_amdgcn_rcpf(dr);
+    im = fmaf(fmaf(-dm, im, 1.f), im, im);
+    ir = fmaf(fmaf(-dr, ir, 1.f), ir, ir);
+    float qm[4], qr[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint64_t e = (uint64_t)(i + j);
-      const uint32_t h = mix32((tkey + (uint32_t)e + (uint32_t)(e >> 32) * 0xC2B2AE35u) ^ s.key);
-      const float qm = fminf(quotient(fabsf(m[j]), dm, im), kE4m3Max);
-      const float qr = fminf(quotient(r[j], dr, ir), kE4m3Max);
-      mc |= (e4m3_code(qm, h >> 16) | (m[j] < 0.f ? 0x80u : 0u)) << 8 * j;
-      rc |= e4m3_root_code(qr, h & 0xffffu, inv_odd) << 8 * j;
+      qm[j] = quotient(fabsf(m[j]), dm, im);
+      qr[j] = quotient(r[j], dr, ir);
     }
-    if (vec && live == 4) {
+    const uint64_t e = (uint64_t)(first + i);    // four neighbours share its upper half
+    const uint32_t key = (a.first + (uint32_t)s.t) * 0x9E3779B9u + (uint32_t)e +
+                         (uint32_t)(e >> 32) * 0xC2B2AE35u;
+    const float least = fminf(fminf(fminf(qm[0], qm[1]), fminf(qm[2], qm[3])),
+                              fminf(fminf(qr[0], qr[1]), fminf(qr[2], qr[3])));
+    const uint2 c = __any(!(least >= 0x1p-6f)) ? e4m3_codes<true>(m, qm, qr, key, s.key, odd)
+                                               : e4m3_codes<false>(m, qm, qr, key, s.key, odd);
+    if (whole) {
       store4(p + i, pv);
-      *reinterpret_cast<uint32_t*>(mq + i) = mc;
-      *reinterpret_cast<uint32_t*>(rq + i) = rc;
+      *reinterpret_cast<uint32_t*>(mq + i) = c.x;
+      *reinterpret_cast<uint32_t*>(rq + i) = c.y;
     } else {
       for (int j = 0; j < live; ++j) {
         store_from_f32(p + i + j, pv[j]);
-        mq[i + j] = (uint8_t)(mc >> 8 * j);
-        rq[i + j] = (uint8_t)(rc >> 8 * j);
+        mq[i + j] = (uint8_t)(c.x >> 8 * j);
+        rq[i + j] = (uint8_t)(c.y >> 8 * j);
       }
     }
     if (lane == 0) {

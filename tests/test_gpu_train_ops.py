@@ -697,3 +697,20 @@ def test_training_steps_run_together(pkg, dev, bits, dtype):
         # |m / sqrt(v)| after bias correction is at most sqrt(3 steps); a code is off by 1/8
         assert p.isfinite().all() and moved.max() > 0, n
         assert moved.max() <= 3 * 1e-2 * 2.5 + 2.0 ** -7 * q.float().abs().max(), n
+
+
+def test_adamw_8_decays_to_zero(pkg, dev):
+    """A first moment whose scale's reciprocal fp32 does not hold (decayed over hundreds of steps
+    without a gradient) becomes zero, not something else; v far below 1 keeps its codes."""
+    p, g, mq, ms, rq, rs = _inputs8(dev, torch.float32, 2, [(512,)])
+    g[0].zero_()
+    ms[0].fill_(1e-39)
+    rs[0].fill_(1e-15)
+    old = tn.decode8(rq[0].view(torch.uint8).cpu().numpy(), f64(rs[0]))
+    q = p[0].clone()
+    pkg.adamw_step_8bit(p, g, mq, ms, rq, rs, step=5, seed=1, **HYPER)
+    assert not ms[0].any() and (mq[0].view(torch.uint8) & 127 == 0).all()
+    assert torch.allclose(p[0], q * (1 - 2e-4), rtol=1e-6, atol=0)
+    new = tn.decode8(rq[0].view(torch.uint8).cpu().numpy(), f64(rs[0]))
+    # one code up or down, and sqrt(0.97) of it
+    assert np.all(np.abs(new - old * np.sqrt(0.97)) <= old / 7.9)
