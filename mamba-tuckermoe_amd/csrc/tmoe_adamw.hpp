@@ -100,24 +100,29 @@ __device__ __forceinline__ float adamw_param(const AdamwStep& s, float p, float 
   return p * s.keep - (m / (root * s.inv_c2 + s.eps)) * s.rate;
 }
 
+// Four neighbours at any alignment (a view may begin anywhere).
 template <class T>
 __device__ __forceinline__ void load4(const T* p, float v[4]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 q = *reinterpret_cast<const float4*>(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  } else {
-    const uint2 q = *reinterpret_cast<const uint2*>(p);
-    v[0] = bf16_bits_to_f32(q.x & 0xffffu); v[1] = bf16_bits_to_f32(q.x >> 16);
-    v[2] = bf16_bits_to_f32(q.y & 0xffffu); v[3] = bf16_bits_to_f32(q.y >> 16);
-  }
+  constexpr int W = (int)sizeof(T);
+  typedef uint32_t vec __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+  const vec q = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if constexpr (sizeof(T) == 4) v[j] = __uint_as_float(q[j]);
+    else v[j] = __uint_as_float(j & 1 ? q[j / 2] & 0xffff0000u : q[j / 2] << 16);
 }
 template <class T>
 __device__ __forceinline__ void store4(T* p, const float v[4]) {
-  if constexpr (sizeof(T) == 4)
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  else
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  constexpr int W = (int)sizeof(T);
+  typedef uint32_t vec __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+  vec q;
+#pragma unroll
+  for (int j = 0; j < W; ++j)
+    if constexpr (sizeof(T) == 4) q[j] = __float_as_uint(v[j]);
+    else q[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+  *reinterpret_cast<vec*>(p) = q;
 }
+typedef uint32_t codes4 __attribute__((aligned(1)));
 
 template <class T>
 __global__ __launch_bounds__(kAdamwThreads) void k_adamw32(const AdamwTable a) {
@@ -127,35 +132,29 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw32(const AdamwTable a) {
   float* m = static_cast<float*>(a.m[s.t]);
   float* v = static_cast<float*>(a.v[s.t]);
   const int64_t end = s.base + a.chunk < a.n[s.t] ? s.base + a.chunk : a.n[s.t];
-  const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) &
-                    (4 * sizeof(T) - 1)) == 0 &&
-                   ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
   int64_t i = s.base + 4 * threadIdx.x;
-  if (vec) {
-    for (; i + 4 <= end; i += 4 * kAdamwThreads) {
-      float pv[4], gv[4], mv[4], vv[4];
-      load4(p + i, pv);
-      load4(g + i, gv);
-      load4(m + i, mv);
-      load4(v + i, vv);
+  for (; i + 4 <= end; i += 4 * kAdamwThreads) {
+    float pv[4], gv[4], mv[4], vv[4];
+    load4(p + i, pv);
+    load4(g + i, gv);
+    load4(m + i, mv);
+    load4(v + i, vv);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        adamw_moments(s, gv[j], mv[j], vv[j]);
-        pv[j] = adamw_param(s, pv[j], mv[j], sqrtf(vv[j]));
-      }
-      store4(p + i, pv);
-      store4(m + i, mv);
-      store4(v + i, vv);
+    for (int j = 0; j < 4; ++j) {
+      adamw_moments(s, gv[j], mv[j], vv[j]);
+      pv[j] = adamw_param(s, pv[j], mv[j], sqrtf(vv[j]));
     }
+    store4(p + i, pv);
+    store4(m + i, mv);
+    store4(v + i, vv);
   }
-  for (; i < end; i += 4 * kAdamwThreads)
-    for (int64_t j = i; j < i + 4 && j < end; ++j) {
-      float mv = m[j], vv = v[j];
-      adamw_moments(s, load_as_f32(g + j), mv, vv);
-      store_from_f32(p + j, adamw_param(s, load_as_f32(p + j), mv, sqrtf(vv)));
-      m[j] = mv;
-      v[j] = vv;
-    }
+  for (; i < end; ++i) {      // a tensor's last one to three elements, one thread's
+    float mv = m[i], vv = v[i];
+    adamw_moments(s, load_as_f32(g + i), mv, vv);
+    store_from_f32(p + i, adamw_param(s, load_as_f32(p + i), mv, sqrtf(vv)));
+    m[i] = mv;
+    v[i] = vv;
+  }
 }
 
 // a / b rounded as the division is, of a reciprocal y of b that is rounded so (the product's
@@ -247,22 +246,19 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
   uint8_t* rq = static_cast<uint8_t*>(a.v[s.t]) + first;
   float* ms = a.ms[s.t] + first / kAdamwBlock;
   float* rs = a.vs[s.t] + first / kAdamwBlock;
-  const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) &
-                    (4 * sizeof(T) - 1)) == 0 &&
-                   ((reinterpret_cast<uintptr_t>(mq) | reinterpret_cast<uintptr_t>(rq)) & 3) == 0;
   for (uint32_t b = 0, blk = 0; b < count;
        b += kAdamwThreads / 64 * kAdamwBlock, blk += kAdamwThreads / 64) {
     const uint32_t i = b + 4 * lane;
-    const bool whole = vec && i + 4 <= count;
-    const int live = i + 4 <= count ? 4 : i < count ? (int)(count - i) : 0;
+    const bool whole = i + 4 <= count;
+    const int live = i < count ? (int)(count - i) : 0;   // where not whole
     const float sm = ms[blk], sr = rs[blk];
     float pv[4] = {}, gv[4] = {}, m[4], r[4];
     uint32_t mc = 0u, rc = 0u;
     if (whole) {
       load4(p + i, pv);
       load4(g + i, gv);
-      mc = *reinterpret_cast<const uint32_t*>(mq + i);
-      rc = *reinterpret_cast<const uint32_t*>(rq + i);
+      mc = *reinterpret_cast<const codes4*>(mq + i);
+      rc = *reinterpret_cast<const codes4*>(rq + i);
     } else {
       for (int j = 0; j < live; ++j) {
         pv[j] = load_as_f32(p + i + j);
@@ -314,8 +310,8 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
                                                : e4m3_codes<false>(m, qm, qr, key, s.key, odd);
     if (whole) {
       store4(p + i, pv);
-      *reinterpret_cast<uint32_t*>(mq + i) = c.x;
-      *reinterpret_cast<uint32_t*>(rq + i) = c.y;
+      *reinterpret_cast<codes4*>(mq + i) = c.x;
+      *reinterpret_cast<codes4*>(rq + i) = c.y;
     } else {
       for (int j = 0; j < live; ++j) {
         store_from_f32(p + i + j, pv[j]);

@@ -51,6 +51,10 @@ struct RowMap {
   }
 };
 
+// A word of ones.
+template <class T>
+constexpr uint32_t kOneWords = sizeof(T) == 2 ? 0x3f803f80u : 0x3f800000u;
+
 // A row's elements in registers as they are stored.
 template <class M, class T>
 struct RowRegs {
@@ -72,6 +76,12 @@ struct RowRegs {
 #pragma unroll
       for (int j = 0; j < M::kWords; ++j) q[k][j] = v[j];
     }
+  }
+  __device__ void fill(uint32_t word) {
+#pragma unroll
+    for (int k = 0; k < M::NCH; ++k)
+#pragma unroll
+      for (int j = 0; j < M::kWords; ++j) q[k][j] = word;
   }
   __device__ float operator[](int i) const {
     const int k = i / M::EPC, j = i % M::EPC;
@@ -144,6 +154,8 @@ struct RowWalk {
 
 template <class T, int EPC, int NCH, int kLanes, RowEnd kEnd, int kThreads>
 __global__ __launch_bounds__(kThreads) void k_block_norm_fwd(BlockNormArgs a) {
+// the same roundings for an element wherever it lies in a thread: fused where it is written
+#pragma clang fp contract(off)
   using M = RowMap<T, EPC, NCH, kEnd>;
   using R = RowRegs<M, T>;
   constexpr int N = M::N;
@@ -153,6 +165,7 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_fwd(BlockNormArgs a) {
   const float inv_d = 1.f / (float)a.d;
   if (kLanes == 0) row_sum_clear(lds);
   R ny, nx, ng;
+  nx.fill(0u);
   if (w.row < a.T) {
     ny.load(m, a.y, w.row, a.y_rs);
     if (a.x) nx.load(m, a.x, w.row, a.x_rs);
@@ -178,29 +191,24 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_fwd(BlockNormArgs a) {
       pw.load(m, a.post_w, 0, 0);
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) ss += m.mine(i) ? f[i] * f[i] : 0.f;
+      for (int i = 0; i < N; ++i) ss = m.mine(i) ? fmaf(f[i], f[i], ss) : ss;
       const float inv = 1.f / sqrtf(row_sum<kLanes>(ss, lds[par]) * inv_d + a.eps);
       if (a.inv && m.tid == 0) a.inv[b] = inv;
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] *= inv * pw[i];
     }
-    if (a.gamma) {
-      R gm;
-      gm.load(m, a.gamma, 0, 0);
+    R gm;
+    if (a.gamma) gm.load(m, a.gamma, 0, 0);
+    else gm.fill(kOneWords<T>);
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] *= gm[i];
-    }
-    if (a.x) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] += x[i];
-    }
+    for (int i = 0; i < N; ++i) f[i] = fmaf(f[i], gm[i], x[i]);
     if (a.r) row_store<T>(m, a.r, b, f);
     if (a.next_w) {
       R nw;
       nw.load(m, a.next_w, 0, 0);
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) ss += m.mine(i) ? f[i] * f[i] : 0.f;
+      for (int i = 0; i < N; ++i) ss = m.mine(i) ? fmaf(f[i], f[i], ss) : ss;
       const float inv = 1.f / sqrtf(row_sum<kLanes>(ss, lds[par + 1]) * inv_d + a.eps);
       if (a.inv && m.tid == 0) a.inv[a.T + b] = inv;
 #pragma unroll
@@ -219,7 +227,8 @@ constexpr int kGate = 1, kRes = 2, kNext = 4, kPost = 8;
 
 template <class T, int EPC, int NCH, int kLanes, RowEnd kEnd, int kThreads, bool kFull, int F>
 __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
-// the same roundings whichever gradients are wanted: fused where it is written
+// the same roundings for an element wherever it lies, and whichever gradients are wanted:
+// fused where it is written
 #pragma clang fp contract(off)
   using M = RowMap<T, EPC, NCH, kEnd>;
   using R = RowRegs<M, T>;
@@ -233,7 +242,6 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
   const bool gated = kFull && (kAny ? a.gate != nullptr : (F & kGate) != 0);
   const bool post = kFull && (kAny ? a.post_w != nullptr : (F & kPost) != 0);
   const bool res = kAny ? a.x != nullptr : (F & kRes) != 0;
-  const bool scaled = a.gamma != nullptr;
   const bool next = kAny ? a.dh != nullptr : (F & kNext) != 0;
   const bool dr_in = kAny ? a.dr != nullptr : true;
   float s_post[kFull ? N : 1], s_gamma[N], s_next[N];
@@ -244,7 +252,8 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
   }
   R pw, gm, nw;
   if (post) pw.load(m, a.post_w, 0, 0);
-  if (scaled) gm.load(m, a.gamma, 0, 0);
+  if (a.gamma) gm.load(m, a.gamma, 0, 0);
+  else gm.fill(kOneWords<T>);   // a product by one: the same bits as without it
   if (next) nw.load(m, a.next_w, 0, 0);
   R ny, nx, ng, ndr, ndh;
   float n_u = 1.f, n_r = 0.f;
@@ -299,16 +308,8 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
 #pragma unroll
           for (int i = 0; i < N; ++i) nr[i] *= pw[i];
         }
-      if (scaled && res) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) nr[i] = fmaf(nr[i], gm[i], x[i]);
-      } else if (scaled) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) nr[i] *= gm[i];
-      } else if (res) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) nr[i] += x[i];
-      }
+      for (int i = 0; i < N; ++i) nr[i] = res ? fmaf(nr[i], gm[i], x[i]) : nr[i] * gm[i];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         nr[i] *= inv_r;
@@ -324,12 +325,10 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
     if (post) {
       if constexpr (kFull) {
         float dot = 0.f;
-        if (scaled) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            s_gamma[i] = fmaf(D[i], nu[i] * pw[i], s_gamma[i]);
-            D[i] *= gm[i];
-          }
+        for (int i = 0; i < N; ++i) {
+          s_gamma[i] = fmaf(D[i], nu[i] * pw[i], s_gamma[i]);
+          D[i] *= gm[i];
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -341,7 +340,7 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
 #pragma unroll
         for (int i = 0; i < N; ++i) D[i] = fmaf(-nu[i], dot, D[i] * pw[i] * inv_u);
       }
-    } else if (scaled) {
+    } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         s_gamma[i] = fmaf(D[i], nu[i], s_gamma[i]);

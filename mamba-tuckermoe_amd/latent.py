@@ -128,7 +128,8 @@ class TuckerMoETrain(torch.nn.Module):
     fused_router=True the router and both losses are train_ops.fused_router: in float32
     whatever x's dtype, the lowest index first on ties, `expert_counts` (E, int64) after
     each forward, and forward takes a mask of tokens ((...) bool, False: left out of the
-    losses and of the contraction; its row of out is the bias)."""
+    losses and of the contraction; its row of out is the bias; its row of x has to be
+    finite all the same, a padding token's embedding say)."""
 
     def __init__(self, dim_in, dim_out, num_experts=8, top_k=2, r1=4, r2=1024, r3=256,
                  fused_router=False):

@@ -714,3 +714,83 @@ def test_adamw_8_decays_to_zero(pkg, dev):
     new = tn.decode8(rq[0].view(torch.uint8).cpu().numpy(), f64(rs[0]))
     # one code up or down, and sqrt(0.97) of it
     assert np.all(np.abs(new - old * np.sqrt(0.97)) <= old / 7.9)
+
+
+def test_adamw_8_odd_views(pkg, dev):
+    """Views that begin anywhere, of parameters and of codes: as aligned copies; what lies beside
+    them stays."""
+    for dtype in DTYPES.values():
+        n = 1031
+        p, g, mq, ms, rq, rs = _inputs8(dev, dtype, 6, [(n,)])
+        wide = {k: torch.zeros(n + 8, dtype=t.dtype, device=dev) for k, t in (("p", p[0]), ("g", g[0]))}
+        wide.update({k: torch.zeros(n + 8, dtype=torch.uint8, device=dev) for k in ("m", "r")})
+        v = {"p": wide["p"][3:n + 3], "g": wide["g"][1:n + 1], "m": wide["m"][1:n + 1], "r": wide["r"][3:n + 3]}
+        for k, t in (("p", p[0]), ("g", g[0]), ("m", mq[0].view(torch.uint8)), ("r", rq[0].view(torch.uint8))):
+            v[k].copy_(t)
+        ms2, rs2 = ms[0].clone(), rs[0].clone()
+        pkg.adamw_step_8bit(p, g, mq, ms, rq, rs, step=4, seed=9, **HYPER)
+        pkg.adamw_step_8bit([v["p"]], [v["g"]], [v["m"]], [ms2], [v["r"]], [rs2], step=4, seed=9, **HYPER)
+        assert torch.equal(v["p"], p[0]) and torch.equal(v["m"], mq[0].view(torch.uint8))
+        assert torch.equal(v["r"], rq[0].view(torch.uint8)) and torch.equal(ms2, ms[0]) and torch.equal(rs2, rs[0])
+        for k, a in (("p", 3), ("m", 1), ("r", 3)):
+            assert not wide[k][:a].any() and not wide[k][n + a:].any()
+
+
+@pytest.mark.parametrize("T,d", [(5, 2), (9, 3), (6, 4), (6, 5), (40, 129), (7, 513), (3, 1025), (3, 4097), (3, 8193)])
+def test_norm_odd_widths_leave_the_rest(pkg, dev, T, d):
+    """Rows whose width is no multiple of a load, their outputs in the middle of larger buffers
+    (through the C ABI): the elements beside them stay as they were."""
+    lib = pkg._lib
+    L = lib.lib()
+    for dtype in DTYPES.values():
+        n, dr, dh = norm_inputs(NORM_FORMS[-1], T, d, T + d, dtype)
+        n = {k: v.to(dev) for k, v in n.items()}
+        dr, dh = dr.to(dev), dh.to(dev)
+        names = ("x", "y", "gate", "post_weight", "gamma", "next_weight")
+        a = lib.TmoeBlockNorm(*[n[k].data_ptr() for k in names[:3]], d, d, d, *[n[k].data_ptr() for k in names[3:]],
+                              T, d, lib.dtype_code(dtype), 1e-5)
+        es = dr.element_size()
+
+        def out(rows):
+            return torch.full((rows * d + 16,), 7.0, dtype=dtype, device=dev)
+        r, h, dx, dy, dg = (out(T) for _ in range(5))
+        dp, dga, dn = (out(1) for _ in range(3))
+        inv = torch.zeros(2, T, device=dev)
+        nws = L.tmoe_block_norm_workspace_bytes(T, d, lib.dtype_code(dtype))
+        ws = torch.empty(max(nws, 1), dtype=torch.uint8, device=dev)
+        st = torch.cuda.current_stream().cuda_stream
+        at = lambda t: t.data_ptr() + 5 * es
+        lib.check(L.tmoe_block_norm_forward(a, at(r), at(h), inv.data_ptr(), st))
+        lib.check(L.tmoe_block_norm_backward(a, inv.data_ptr(), dr.data_ptr(), d, dh.data_ptr(), d, at(dx), at(dy),
+                                             at(dg), at(dp), at(dga), at(dn), ws.data_ptr(), nws, st))
+        o = tn.block_norm(**{k: f64(v) for k, v in n.items()}, dr=f64(dr), dh=f64(dh))
+        for k, t, rows in (("r", r, T), ("h", h, T), ("dx", dx, T), ("dy", dy, T), ("dgate", dg, T),
+                           ("dpost_weight", dp, 1), ("dgamma", dga, 1), ("dnext_weight", dn, 1)):
+            assert (t[:5] == 7).all() and (t[5 + rows * d:] == 7).all(), k
+            got = t[5:5 + rows * d]
+            near(got, o[k].reshape(-1), o[k + "_mag"].reshape(-1), 400, k)
+
+
+@pytest.mark.parametrize("shape", [(2048, 8, 2, 256, 256), (300, 8, 2, 64, 128)])
+def test_masked_tokens_select_nothing_in_the_contraction(pkg, dev, shape):
+    """The contraction of a masked routing (idx -1, weights 0) is that of the tokens that are left,
+    in both of its forms: zero rows, and the same dG to the rounding of sums in another order."""
+    B, E, k, r3, r2 = shape
+    g = torch.Generator().manual_seed(B)
+    raw = _logits(B, E, torch.float32, 1).to(dev)
+    mask = (torch.rand(B, generator=g) > 0.4).to(dev)
+    x = torch.randn(B, r3, generator=g).bfloat16().to(dev)
+    G = (torch.randn(E, r3, r2, generator=g) * r3 ** -0.5).bfloat16().to(dev)
+    dout = torch.randn(B, r2, generator=g).bfloat16().to(dev)
+
+    def run(raw, x, dout, mask):
+        leaves = [t.detach().requires_grad_() for t in (raw, x, G)]
+        q = pkg.fused_router(leaves[0], k, 0.5, mask=mask)
+        out = pkg.FusedLatentMoE.apply(leaves[1], leaves[2], q.idx, q.weights)
+        return [out.detach()] + list(torch.autograd.grad(out, leaves, dout))
+    a = run(raw, x, dout, mask)
+    b = run(raw[mask], x[mask], dout[mask], None)
+    for i in range(3):
+        assert not a[i][~mask].any()
+        assert onp.rel_l2(f64(a[i][mask]), f64(b[i])) <= 1e-2
+    assert onp.rel_l2(f64(a[3]), f64(b[3])) <= 1e-2
