@@ -9,9 +9,11 @@
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <optional>
@@ -58,6 +60,21 @@ bool wants_grad(std::initializer_list<const OptTensor*> ts) {
   for (const OptTensor* t : ts)
     if (*t && (*t)->requires_grad()) return true;
   return false;
+}
+
+// A leaf's accumulator lives as long as a graph that holds it and runs on the stream that
+// this graph was made on. Under capture a backward that meets one of another stream would
+// take that stream into the capture, which ends the process: refused here instead.
+void check_capture(std::initializer_list<const OptTensor*> ts, const char* who) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const OptTensor* t : ts) {
+    if (!*t || !(*t)->requires_grad() || (*t)->grad_fn()) continue;
+    const auto acc = torch::autograd::impl::try_get_grad_accumulator(**t);
+    if (!acc || !acc->stream()) continue;
+    TORCH_CHECK(acc->stream()->id() == c10::hip::getCurrentHIPStream((*t)->device().index()).id(), who,
+                ": a graph that was made outside this capture, on another stream, still holds one of "
+                "these leaves; delete its outputs before the capture");
+  }
 }
 
 // The rows (..., d) of t at one stride; a contiguous copy where they have none.
@@ -222,6 +239,9 @@ PyObject* router(PyObject*, PyObject* const* a, Py_ssize_t n) {
       c.raw = rows_of(raw).t;
     }
     if (at::GradMode::is_enabled() && raw.requires_grad()) {
+      const c10::DeviceGuard guard(raw.device());
+      const OptTensor leaf = raw;
+      check_capture({&leaf}, kRouter);
       o = Router::apply(raw, c);
     } else {
       o = router_forward(c);
@@ -385,6 +405,8 @@ PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release nogil;
     if (wants_grad({&x, &y, &gate, &post, &gamma, &next})) {
+      const c10::DeviceGuard guard(y->device());
+      check_capture({&x, &y, &gate, &post, &gamma, &next}, kNorm);
       const variable_list o = BlockNorm::apply(x, *y, gate, post, gamma, next, eps, want_r);
       if (want_r) r = o[0];
       if (next) h = o.back();

@@ -532,6 +532,35 @@ def test_graph_capture(pkg, dev):
     assert opt.state[ps[0]]["step"].item() == 5 == ropt.state[ref[0]]["step"]
 
 
+def test_capture_refuses_leaves_of_a_living_eager_graph(pkg, dev):
+    """A capture whose leaves an eager graph of another stream still holds is refused when the
+    operator is called; once that graph is gone it is captured and replayed."""
+    x = torch.randn(64, 32, device=dev)
+    w = torch.ones(32, device=dev, requires_grad=True)
+    raw = torch.randn(64, 8, device=dev, requires_grad=True)
+    for leaf, call in ((w, lambda: pkg.fused_block_norm(y=x, post_weight=w)[0]),
+                       (raw, lambda: pkg.fused_router(raw, 2, 0.5).z_loss)):
+        living = call()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="outside this capture"):
+            with torch.cuda.graph(g, stream=s):
+                call()
+        del living
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = call()
+            grad, = torch.autograd.grad(out, leaf, torch.ones_like(out))
+        want, = torch.autograd.grad(call().sum(), leaf)
+        for _ in range(3):
+            grad.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(grad, want)
+
+
 def test_step_in_capture_needs_capturable(pkg, dev):
     p = torch.nn.Parameter(torch.ones(8, device=dev))
     p.grad = torch.ones_like(p)
