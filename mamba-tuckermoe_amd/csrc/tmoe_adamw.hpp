@@ -11,7 +11,8 @@
 // (seed, step, tensor, element), so a step repeated gives the same bits. A positive r is
 // never coded as zero: its element's step would be m / eps.
 //
-// Bound by memory (fp32 28 bytes an element). A launch takes up to kAdamwTensors tensors,
+// fp32 is bound by memory: 28 bytes an element, 417 M of them in 2256 us, 5.2 TB/s. 8 bits
+// by instructions, ~88 an element: 19.3 M bf16 parameters in 55 us, 3.5 TB/s. A launch takes up to kAdamwTensors tensors,
 // their addresses in its arguments: nothing is copied to the device, and a captured step
 // holds them. A work-group takes `chunk` elements of one tensor.
 #pragma once

@@ -19,7 +19,9 @@
 // A token's logits lie in L lanes, V to a lane (L a power of two, V L >= E; V = 8, or 4 where
 // that is all of them): what a token needs of them is exchanged by lane permutations. Eight
 // to a lane rather than four: the exchanges, and not the exponentials, are most of the
-// instructions. The column sums over the tokens (n_e,
+// instructions (E = 64, B = 131072: forward 29 against 32 us). Bound by instructions: that
+// size's forward takes 29.8 us (1.3 TB/s of what it moves), its backward 25.0 (3.1 TB/s);
+// B = 16384, E = 8 5.8 and 5.5 us. The column sums over the tokens (n_e,
 // sum_b P_be) stay in registers over a work-group's tokens, then in a plane of `part`, and
 // k_router_finish adds the planes in a fixed order: the losses do not depend on which
 // work-group ends first.

@@ -24,8 +24,8 @@ int router_lanes(int64_t E) {
 }
 // Work-groups of the forward, a plane each for the second launch to add: at E = 64, B = 131072
 // the two take 29.8 + 4.7 us with 768, 33.9 + 3.9 with 512, 29.4 + 5.2 with 1024. The
-// backward's, whose lanes keep nothing between tokens but the counts: 22.5 us with 1024,
-// 23.8 with 2048, 27.0 with 4096.
+// backward's, whose lanes keep nothing between tokens but the counts, against 2048 and 4096:
+// 22.5, 23.8 and 27.0 us (25.0 since its differences are taken from the likeliest expert).
 constexpr int64_t kRouterBlocks = 768, kRouterBwdBlocks = 1024;
 int64_t router_blocks(int64_t B, int64_t E) {
   const int64_t n = ceil_div(B, dev::kRouterThreads / router_lanes(E));

@@ -823,3 +823,16 @@ def test_masked_tokens_select_nothing_in_the_contraction(pkg, dev, shape):
         assert not a[i][~mask].any()
         assert onp.rel_l2(f64(a[i][mask]), f64(b[i])) <= 1e-2
     assert onp.rel_l2(f64(a[3]), f64(b[3])) <= 1e-2
+
+
+def test_router_top1_weights_gradient(pkg, dev):
+    """k = 1: the weight is P / (P + 1e-6), its gradient the 1e-6 that it lacks to one. Taken as
+    the difference of two sums next to each other it would be 1e-2 off in float32; here within
+    the rounding of its own terms, as every other k's."""
+    raw = _logits(5000, 16, torch.float32, 8).to(dev).requires_grad_()
+    dw = torch.randn(5000, 1, device=dev)
+    r = pkg.fused_router(raw, 1, 0.5)
+    draw, = torch.autograd.grad(r.weights, raw, dw)
+    o = tn.router(f64(raw), 1, 0.5, 10.0, None, f64(dw))
+    # 16 cap / tau + 128 roundings of each factor, in the 2-norm
+    assert onp.rel_l2(f64(draw), o["draw"]) <= 4 * (16 * 10 / 0.5 + 128) * U
