@@ -20,7 +20,7 @@ Public surface:
   TuckerFFNTrain               TuckerFFN for training, on the two and TuckerMoETrain
                                (block_train.py)
   FusedAdamW, adamw_step,      one AdamW step over many tensors, moments in 32 or 8 bits
-  adamw_step_8bit              (adamw.py)
+  adamw_step_8bit              (adamw.py; dequantize_state: a state's values)
   synth                        seeded synthetic parameters and tokens
   fp8                          e4m3 weights with per-output-channel scales
   checkpoint                   the reference's .npz keys (layers, FFN, out_proj) and the
@@ -34,11 +34,11 @@ from .block import LayerScale, TuckerFFN, TuckerOutProj
 from .latent import FusedLatentMoE, TuckerMoETrain, fused_latent_moe
 from .train_ops import Routing, fused_block_norm, fused_router
 from .block_train import TuckerFFNTrain
-from .adamw import FusedAdamW, adamw_step, adamw_step_8bit
+from .adamw import FusedAdamW, adamw_step, adamw_step_8bit, dequantize_state
 
 __all__ = ["TuckerMoE", "RMSNorm", "LayerScale", "TuckerFFN", "TuckerOutProj",
            "FusedLatentMoE", "TuckerMoETrain", "fused_latent_moe",
            "fused_router", "Routing", "fused_block_norm", "TuckerFFNTrain", "FusedAdamW", "adamw_step",
-           "adamw_step_8bit",
+           "adamw_step_8bit", "dequantize_state",
            "TuckerMoEConfig", "Workload", "WORKLOADS", "FfnWorkload", "FFN_WORKLOADS", "load_tucker", "synth", "config", "fp8",
            "checkpoint", "_lib"]

@@ -17,14 +17,15 @@
 // capped logits near the cap. raw / c is cut at +-20, past which tanh is +-1 in fp32.
 //
 // A token's logits lie in L lanes, V to a lane (L a power of two, V L >= E; V = 8, or 4 where
-// that is all of them): what a token needs of them is exchanged by lane permutations. Eight
-// to a lane rather than four: the exchanges, and not the exponentials, are most of the
-// instructions (E = 64, B = 131072: forward 29 against 32 us). Bound by instructions: that
-// size's forward takes 29.8 us (1.3 TB/s of what it moves), its backward 25.0 (3.1 TB/s);
-// B = 16384, E = 8 5.8 and 5.5 us. The column sums over the tokens (n_e,
-// sum_b P_be) stay in registers over a work-group's tokens, then in a plane of `part`, and
-// k_router_finish adds the planes in a fixed order: the losses do not depend on which
-// work-group ends first.
+// that is all of them): what a token needs of them is exchanged by lane permutations, what
+// k lanes store or read is handed through shared memory, so that idx, w and dw are moved
+// side by side. Eight to a lane rather than four: the exchanges, and not the exponentials,
+// are most of the instructions (forward 29 against 32 us when that was measured). Bound by
+// instructions: E = 64, k = 6, B = 131072 (fp32) takes 23.0 us forward (1.7 TB/s of what it
+// moves) and 21.6 backward (3.5 TB/s); B = 16384, E = 8, k = 2 5.2 and 5.2 us. The column
+// sums over the tokens (sum_b P_be in registers, n_e in shared memory) are a work-group's
+// own until its plane of `part`, and k_router_finish adds the planes in a fixed order: the
+// losses do not depend on which work-group ends first.
 #pragma once
 
 #include "tmoe_elem.hpp"
@@ -34,9 +35,10 @@ namespace tmoe {
 namespace dev {
 
 constexpr int kRouterThreads = 256;
+constexpr int kRouterTopK = 16;       // slots of a token at most
 constexpr int kFinishCols = 16;       // experts of a work-group of k_router_finish
 
-// raw[e0 .. e0 + V - 1] of a row of E logits (0 past its end), at any alignment
+// raw[e0 .. e0 + V - 1] of a row of E logits (-inf past its end), at any alignment
 template <class T, int V>
 __device__ __forceinline__ void router_load(const T* row, int e0, int E, float v[V]) {
   constexpr int W = V * (int)sizeof(T) / 4;
@@ -49,7 +51,7 @@ __device__ __forceinline__ void router_load(const T* row, int e0, int E, float v
       else v[j] = __uint_as_float(j & 1 ? q[j / 2] & 0xffff0000u : q[j / 2] << 16);
   } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = e0 + j < E ? load_as_f32(row + e0 + j) : 0.f;
+    for (int j = 0; j < V; ++j) v[j] = e0 + j < E ? load_as_f32(row + e0 + j) : -INFINITY;
   }
 }
 
@@ -64,10 +66,8 @@ __device__ __forceinline__ uint32_t max_of(const uint32_t (&k)[V]) {
 // An unsigned key in the order of the floats: NaN above +inf, -0 equal to 0, never 0; and
 // the float of a key.
 __device__ __forceinline__ uint32_t order_key(float f) {
-  f += 0.f;
-  if (f != f) return 0xffffffffu;
-  const uint32_t b = __float_as_uint(f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const int32_t b = (int32_t)__float_as_uint(f + 0.f);
+  return f != f ? 0xffffffffu : (uint32_t)(b ^ (b >> 31 | (int32_t)0x80000000));
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
@@ -76,13 +76,19 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 struct Capped {
   float Q, R;
 };
-// c1 = -2 log2(e) / cap; a NaN stays one
-__device__ __forceinline__ Capped capped(float raw, float c1) {
-  constexpr float kCut = 20.f * 2.8853900817779268f;
-  float u = raw * c1;
-  u = u > kCut ? kCut : u < -kCut ? -kCut : u;
+// u = raw c1, c1 = -2 log2(e) / cap
+__device__ __forceinline__ Capped capped_of(float u) {
   const float Q = __builtin_amdgcn_exp2f(u);
   return {Q, __builtin_amdgcn_rcpf(1.f + Q)};
+}
+constexpr float kCut = 20.f * 2.8853900817779268f;
+// of a token's largest logit: a NaN stays one, and makes all that is taken from it NaN
+__device__ __forceinline__ Capped capped_top(float raw, float c1) {
+  const float u = raw * c1;
+  return capped_of(u > kCut ? kCut : u < -kCut ? -kCut : u);
+}
+__device__ __forceinline__ Capped capped(float raw, float c1) {
+  return capped_of(__builtin_amdgcn_fmed3f(raw * c1, -kCut, kCut));
 }
 
 // cap tanh(raw / cap) to the last places, for the logsumexp: once a token
@@ -90,6 +96,22 @@ __device__ __forceinline__ float capped_value(float raw, float c1, float cap) {
   const float q = __builtin_amdgcn_exp2f(-fabsf(raw * c1)), d = 1.f + q;
   const float r = __builtin_amdgcn_rcpf(d);
   return copysignf(cap * ((1.f - q) * fmaf(r, fmaf(-d, r, 1.f), r)), raw);
+}
+
+// Where a token's lanes keep expert e's word among them: the lanes' j-th words are
+// neighbours, and tokens lie (V + 1) L words apart, so that a wave meets every bank alike.
+template <int L, int V>
+__device__ __forceinline__ uint32_t place(uint32_t e) {
+  return e % V * L + e / V;
+}
+
+// The largest key below `best`; one exists, or a key of 0 is none.
+template <int L, int V>
+__device__ __forceinline__ uint32_t key_below(const uint32_t (&key)[V], uint32_t best) {
+  uint32_t below[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) below[j] = key[j] - best;
+  return lanes_max<L>(max_of(below)) + best;
 }
 
 struct RouterScales {
@@ -123,7 +145,17 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
   const int64_t step = (int64_t)gridDim.x * G;
   int64_t b = (int64_t)blockIdx.x * G + threadIdx.x / L;
   float ps[V] = {}, zs = 0.f;
-  uint32_t cn[V] = {}, n = 0u;
+  uint32_t low[V], n = 0u;
+#pragma unroll
+  for (int j = 0; j < V; ++j) low[j] = 255u - (uint32_t)(e0 + j);
+  // a token's selected keys, by rank, and its exponentials: handed from the lanes that
+  // hold them to those that store the routing, neighbours side by side; and the counts
+  __shared__ uint32_t s_slot[G][kRouterTopK + 1], s_c[V * L];
+  __shared__ float s_exp[G][(V + 1) * L];
+  uint32_t* slot = s_slot[threadIdx.x / L];
+  float* exps = s_exp[threadIdx.x / L];
+  for (int e = threadIdx.x; e < V * L; e += kRouterThreads) s_c[e] = 0u;
+  __syncthreads();
   float next[V];
   bool next_on = true;
   if (b < a.B) {
@@ -146,82 +178,78 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
       }
       continue;
     }
-    uint32_t key[V], full[V], top = 0u, last = 0u;
-    int pos[V];
-    bool tied = false;
+    uint32_t key[V], full[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      full[j] = e0 + j < E ? order_key(v[j]) : 0u;
-      key[j] = full[j] ? (full[j] & ~0xffu) | (255u - (uint32_t)(e0 + j)) : 0u;
-      pos[j] = -1;
+      full[j] = order_key(v[j]);
+      key[j] = (full[j] & ~0xffu) | low[j];
     }
-    // The k largest by keys with the expert in their low byte: each is one lane's, and one
-    // maximum finds it. bf16 logits' keys end before that byte; of fp32 ones two that
-    // differ in it alone, neighbours among the k + 1 largest, go to the exact search.
-    const int rounds = sizeof(T) == 4 && k < E ? k + 1 : k;
-    for (int i = 0; i < rounds; ++i) {
-      const uint32_t best = lanes_max<L>(max_of(key));
-      if (sizeof(T) == 4) tied = tied || (best ^ last) < 256u;
-      else if (i == 0) top = best & 0x80000000u ? best & 0xffff0000u : best | 0xffffu;
-      last = best;
-      if (i < k) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const bool it = key[j] == best;
-          pos[j] = it ? i : pos[j];
-          key[j] = it ? 0u : key[j];
-        }
-      }
+    // The k largest by keys with 255 - the expert in their low byte, one maximum each. The
+    // largest key below `best` is the largest of key - best, unsigned, plus best: those
+    // below wrap round to above all others. bf16 logits' keys end before that byte; of
+    // fp32 ones two that differ in it alone, neighbours among the k + 1 largest, go to the
+    // exact search.
+    uint32_t best = lanes_max<L>(max_of(key)), top, apart = ~0u;
+    if (sizeof(T) == 4) top = lanes_max<L>(max_of(full));
+    else top = best & 0x80000000u ? best & 0xffff0000u : best | 0xffffu;
+    slot[0] = best;
+    for (int i = 1; i < k; ++i) {
+      const uint32_t lower = key_below<L>(key, best);
+      apart = min(apart, best ^ lower);
+      slot[i] = best = lower;
     }
     if constexpr (sizeof(T) == 4) {
-      top = lanes_max<L>(max_of(full));
-      if (__any(tied)) {
+      if (k < E) apart = min(apart, best ^ key_below<L>(key, best));
+      if (__any(apart < 256u)) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) pos[j] = -1;
+        for (int j = 0; j < V; ++j) full[j] = order_key(v[j]);
         for (int i = 0; i < k; ++i) {
           // the largest key left, in the lowest lane that holds it, its first
           const uint32_t mine = max_of(full);
-          const uint32_t best = lanes_max<L>(mine);
-          if (lanes_min<L>(mine == best ? l : L) == l) {
+          const uint32_t most = lanes_max<L>(mine);
+          if (lanes_min<L>(mine == most ? l : L) == l) {
             bool open = true;
 #pragma unroll
             for (int j = 0; j < V; ++j)
-              if (open && full[j] == best) {
+              if (open && full[j] == most) {
                 open = false;
-                pos[j] = i;
                 full[j] = 0u;
+                slot[i] = low[j];
               }
           }
         }
       }
     }
-    const Capped m = capped(key_value(top), sc.c1);
+    const Capped m = capped_top(key_value(top), sc.c1);
+    const float k_p = m.R * sc.k_p, k_z = m.R * sc.k_z;
     float ep[V], sp = 0.f, sz = 0.f, ss = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const Capped c = capped(v[j], sc.c1);
-      const float d = (m.Q - c.Q) * (m.R * c.R);
-      const bool in = e0 + j < E;
-      ep[j] = in ? __builtin_amdgcn_exp2f(d * sc.k_p) : 0.f;
-      sz += in ? __builtin_amdgcn_exp2f(d * sc.k_z) : 0.f;
+      const float d = e0 + j < E ? (m.Q - c.Q) * c.R : -INFINITY;
+      ep[j] = __builtin_amdgcn_exp2f(d * k_p);
+      sz += __builtin_amdgcn_exp2f(d * k_z);
       sp += ep[j];
-      ss += pos[j] >= 0 ? ep[j] : 0.f;
+      exps[j * L + l] = ep[j];
     }
     sp = lanes_sum<L>(sp);
     sz = lanes_sum<L>(sz);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for (int i = l; i < k; i += L) ss += exps[place<L, V>(255u - (slot[i] & 255u))];
     ss = lanes_sum<L>(ss);
     const float inv_sp = __builtin_amdgcn_rcpf(sp);
     const float inv_s = __builtin_amdgcn_rcpf(fmaf(ss, inv_sp, 1e-6f));
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float P = ep[j] * inv_sp;
-      ps[j] += P;
-      if (pos[j] >= 0) {
-        ++cn[j];
-        a.idx[b * k + pos[j]] = e0 + j;
-        a.w[b * k + pos[j]] = P * inv_s;
-      }
+    for (int j = 0; j < V; ++j) ps[j] += ep[j] * inv_sp;
+    for (int i = l; i < k; i += L) {
+      const uint32_t e = 255u - (slot[i] & 255u);
+      a.idx[b * k + i] = e;
+      a.w[b * k + i] = exps[place<L, V>(e)] * inv_sp * inv_s;
+      atomicAdd(s_c + e, 1u);
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     if (l == 0) {
       const float lse = capped_value(key_value(top), sc.c1, a.cap) + __logf(sz);
       zs += lse * lse;
@@ -232,23 +260,17 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
 #pragma unroll
   for (int o = L; o < 64; o <<= 1) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      ps[j] += __shfl_xor(ps[j], o);
-      cn[j] += __shfl_xor(cn[j], o);
-    }
+    for (int j = 0; j < V; ++j) ps[j] += __shfl_xor(ps[j], o);
     zs += __shfl_xor(zs, o);
     n += __shfl_xor(n, o);
   }
   constexpr int W = kRouterThreads / 64;
   __shared__ float s_p[W][V * L], s_z[W];
-  __shared__ uint32_t s_c[W][V * L], s_n[W];
+  __shared__ uint32_t s_n[W];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   if (lane < L) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      s_p[wave][e0 + j] = ps[j];
-      s_c[wave][e0 + j] = cn[j];
-    }
+    for (int j = 0; j < V; ++j) s_p[wave][e0 + j] = ps[j];
     if (l == 0) {
       s_z[wave] = zs;
       s_n[wave] = n;
@@ -271,10 +293,8 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
       uint32_t c = 0u;
       if (e < E)
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          p += s_p[w][e];
-          c += s_c[w][e];
-        }
+        for (int w = 0; w < W; ++w) p += s_p[w][e];
+      if (e < E) c = s_c[e];
       lb += router_finish_wave(a, e, p, c, inv_n);
     }
     if (lane == 0) {
@@ -289,13 +309,9 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
   float2* pairs = reinterpret_cast<float2*>(a.part);
   for (int e = threadIdx.x; e < E; e += kRouterThreads) {
     float p = 0.f;
-    uint32_t c = 0u;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      p += s_p[w][e];
-      c += s_c[w][e];
-    }
-    pairs[(int64_t)blockIdx.x * E + e] = make_float2(p, __uint_as_float(c));
+    for (int w = 0; w < W; ++w) p += s_p[w][e];
+    pairs[(int64_t)blockIdx.x * E + e] = make_float2(p, __uint_as_float(s_c[e]));
   }
   if (threadIdx.x == 0) {
     pairs[(int64_t)gridDim.x * E + blockIdx.x] = make_float2(z, __uint_as_float(N));
@@ -390,8 +406,12 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_bwd(RouterArgs a) {
 #pragma unroll
   for (int j = 0; j < V; ++j) g0[j] = e0 + j < E ? cg * (float)a.counts[e0 + j] : 0.f;
   // a token's selected experts, handed from the lanes that read them to those that hold them
-  __shared__ float2 s_sel[G][V * L];
+  // (0 and dw's distance from the top's; 1 and 0 for all others)
+  __shared__ float2 s_sel[G][(V + 1) * L];
   float2* sel = s_sel[threadIdx.x / L];
+  const float2 none = make_float2(1.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < V; ++j) sel[j * L + l] = none;
   for (int64_t b = (int64_t)blockIdx.x * G + threadIdx.x / L; b < a.B;
        b += (int64_t)gridDim.x * G) {
     float o[V] = {};
@@ -407,43 +427,53 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_bwd(RouterArgs a) {
     const int64_t e_top = a.idx[b * k];
     const float d_top = a.dw ? a.dw[b * k] : 0.f;
     if (!a.mask || a.mask[b]) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) sel[e0 + j] = make_float2(0.f, 0.f);
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
       const float g_top = e_top >= 0 && e_top < E ? cg * (float)a.counts[e_top] : 0.f;
-      if (e_first >= 0 && e_first < E) sel[e_first] = make_float2(1.f, d_first - d_top);
+      const bool has = e_first >= 0 && e_first < E;
+      const uint32_t first = place<L, V>((uint32_t)e_first);
+      if (has) sel[first] = make_float2(0.f, d_first - d_top);
       for (int i = l + L; i < k; i += L) {
         const int64_t e = a.idx[b * k + i];
-        if (e >= 0 && e < E) sel[e] = make_float2(1.f, (a.dw ? a.dw[b * k + i] : 0.f) - d_top);
+        if (e >= 0 && e < E)
+          sel[place<L, V>((uint32_t)e)] = make_float2(0.f, (a.dw ? a.dw[b * k + i] : 0.f) - d_top);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (e0 + j < E) top = fmaxf(top, v[j]);
-      top = __uint_as_float(lanes_reduce<L>(__float_as_uint(top), [](uint32_t x, uint32_t y) {
-        return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
-      }));
-      const Capped m = capped(top, sc.c1);
-      Capped t[V];
-      float ep[V], ez[V], dw[V], on[V], sp = 0.f, sz = 0.f, su = 0.f, sd = 0.f, sg = 0.f;
+      float off[V], dw[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float2 s = sel[e0 + j];
-        on[j] = s.x;
+        const float2 s = sel[j * L + l];
+        off[j] = s.x;
         dw[j] = s.y;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (has) sel[first] = none;
+      for (int i = l + L; i < k; i += L) {
+        const int64_t e = a.idx[b * k + i];
+        if (e >= 0 && e < E) sel[place<L, V>((uint32_t)e)] = none;
+      }
+      float top = v[0];         // NaN if one of them is
+#pragma unroll
+      for (int j = 1; j < V; ++j) top = __builtin_elementwise_maximum(top, v[j]);
+      top = __uint_as_float(lanes_reduce<L>(__float_as_uint(top), [](uint32_t x, uint32_t y) {
+        return __float_as_uint(
+            __builtin_elementwise_maximum(__uint_as_float(x), __uint_as_float(y)));
+      }));
+      const Capped m = capped_top(top, sc.c1);
+      const float k_p = m.R * sc.k_p, k_z = m.R * sc.k_z;
+      Capped t[V];
+      float ep[V], ez[V], sp = 0.f, sz = 0.f, su = 0.f, sd = 0.f, sg = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
         t[j] = capped(v[j], sc.c1);
-        const float d = (m.Q - t[j].Q) * (m.R * t[j].R);
-        const bool in = e0 + j < E;
-        ep[j] = in ? __builtin_amdgcn_exp2f(d * sc.k_p) : 0.f;
-        ez[j] = in ? __builtin_amdgcn_exp2f(d * sc.k_z) : 0.f;
+        const float d = e0 + j < E ? (m.Q - t[j].Q) * t[j].R : -INFINITY;
+        ep[j] = __builtin_amdgcn_exp2f(d * k_p);
+        ez[j] = __builtin_amdgcn_exp2f(d * k_z);
         sp += ep[j];
         sz += ez[j];
-        su += on[j] != 0.f ? 0.f : ep[j];
-        sd += on[j] != 0.f ? ep[j] * dw[j] : 0.f;
-        sg += ep[j] * (g0[j] - g_top);
+        su = fmaf(ep[j], off[j], su);
+        sd = fmaf(ep[j], dw[j], sd);
+        sg = fmaf(ep[j], g0[j] - g_top, sg);
       }
       sp = lanes_sum<L>(sp);
       sz = lanes_sum<L>(sz);
@@ -455,11 +485,12 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_bwd(RouterArgs a) {
       // the top's own part of g beside the balance loss's: dw_0 - sum_i dw_i w_i, over s
       const float gs = (d_top * 1e-6f * inv_s - sd * inv_sp * inv_s) * inv_s;
       const float pg = (sg + sd * inv_s - su * gs) * inv_sp;       // sum_e P_e (g_e - g_0)
-      const float zc = cz * (capped_value(top, sc.c1, a.cap) + __logf(sz)) * __builtin_amdgcn_rcpf(sz);
+      const float c_p = 4.f * inv_sp * inv_tau;
+      const float c_z = 4.f * cz * (capped_value(top, sc.c1, a.cap) + __logf(sz)) * __builtin_amdgcn_rcpf(sz);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float g = g0[j] - g_top + (on[j] != 0.f ? dw[j] * inv_s : -gs);
-        o[j] = (ep[j] * inv_sp * (g - pg) * inv_tau + zc * ez[j]) * (4.f * t[j].Q * t[j].R * t[j].R);
+        const float g = fmaf(off[j], -gs, fmaf(dw[j], inv_s, g0[j] - g_top));
+        o[j] = fmaf(c_z, ez[j], ep[j] * c_p * (g - pg)) * (t[j].Q * t[j].R * t[j].R);
       }
     }
     T* row = draw + b * E;

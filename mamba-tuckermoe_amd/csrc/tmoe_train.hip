@@ -23,10 +23,11 @@ int router_lanes(int64_t E) {
   return l;
 }
 // Work-groups of the forward, a plane each for the second launch to add: at E = 64, B = 131072
-// the two take 29.8 + 4.7 us with 768, 33.9 + 3.9 with 512, 29.4 + 5.2 with 1024. The
-// backward's, whose lanes keep nothing between tokens but the counts, against 2048 and 4096:
-// 22.5, 23.8 and 27.0 us (25.0 since its differences are taken from the likeliest expert).
-constexpr int64_t kRouterBlocks = 768, kRouterBwdBlocks = 1024;
+// the two take 23.0 + 4.8 us with 768, 25.7 + 4.5 with 512, 22.8 + 5.3 with 1024, 22.6 + 5.9
+// with 1280. The backward's, which sets up more than it gains by more waves: 21.6 us with
+// 768, 22.7 with 1024, 23.2 with 1536, 25.0 with 2048; the next token's inputs read ahead,
+// as in the forward, 22.0.
+constexpr int64_t kRouterBlocks = 768, kRouterBwdBlocks = 768;
 int64_t router_blocks(int64_t B, int64_t E) {
   const int64_t n = ceil_div(B, dev::kRouterThreads / router_lanes(E));
   return n < 1 ? 1 : n < kRouterBlocks ? n : kRouterBlocks;
