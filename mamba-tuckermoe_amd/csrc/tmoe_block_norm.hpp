@@ -10,15 +10,16 @@
 // All in fp32 from the stored inputs; h is taken from the unrounded r, and the backward
 // forms r again from x and y, so that both see the same r; each output is rounded once.
 //
-// Bound by memory: every activation is read once and every output written once; a row lies
-// in the registers of its threads between its two norms, and the next row is on its way
-// meanwhile. Rows of at most 1024 elements take a wave, or a half or a quarter of one (no
-// barrier), four neighbours a lane and step; longer ones a work-group, 16 bytes a thread
-// and step. The weights' gradients are summed in registers over a work-group's rows, then in
-// planes of `part` that k_block_norm_cols adds in a fixed order; one work-group alone has
-// them whole. Measured, bf16, T = 16384: d = 768 with residual, gamma and next norm 17.1 us
-// forward and 25.6 + 4.0 backward (5.9 TB/s of what each moves), d = 2304 with every operand
-// 76.8 and 123.2 + 5.2 us (4.9 TB/s; its 981 MB don't fit the cache).
+// Bound by memory: every activation is read once (but for k_block_norm_bwd_wide's rows) and
+// every output written once; a row lies in the registers of its threads between its two
+// norms, and the next row is on its way meanwhile. Rows of at most 1024 elements take a
+// wave, or a half or a quarter of one (no barrier), four neighbours a lane and step; longer
+// ones a work-group, 16 bytes a thread and step. The weights' gradients are summed in
+// registers over a work-group's rows, then in planes of `part` that k_block_norm_cols adds
+// in a fixed order; one work-group alone has them whole. Measured, bf16, T = 16384: d = 768
+// with residual, gamma and next norm 17.1 us forward and 25.6 + 4.0 backward (5.9 TB/s of
+// what each moves), d = 2304 with every operand 76.8 and 123.2 + 5.2 us (4.9 TB/s; its
+// 981 MB don't fit the cache).
 #pragma once
 
 #include "tmoe_elem.hpp"
@@ -220,6 +221,21 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_fwd(BlockNormArgs a) {
   }
 }
 
+// A work-group's sums of one weight's gradient: its plane of part (3, work-groups, d), or
+// the gradient itself of the only work-group.
+template <class T, class M, int N>
+__device__ __forceinline__ void put_sums(const M& m, const BlockNormArgs& a, const float (&v)[N],
+                                         int which, void* out) {
+  if (!out) return;
+  if (gridDim.x == 1) return row_store<T>(m, out, 0, v);
+  float* p = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * a.d;
+#pragma unroll
+  for (int k = 0; k < M::NCH; ++k)
+#pragma unroll
+    for (int j = 0; j < M::EPC; ++j)
+      if (m.in(k) && m.col(k) + j < a.d) p[m.col(k) + j] = v[k * M::EPC + j];
+}
+
 // What a backward's rows load and store as the bits of F: known when it is compiled, with
 // dr (and dh with kNext) there and every row's gradient wanted, so that the loads and stores
 // have their places and none waits for another (a load of the next row that may or may not
@@ -384,20 +400,159 @@ __global__ __launch_bounds__(kThreads) void k_block_norm_bwd(BlockNormArgs a) {
     if (a.dnext_w) join(s_next);
     if (w.team > 0) return;
   }
-  // part: (3, work-groups, d)
-  auto put = [&](const float (&v)[N], int which, void* out) {
-    if (!out) return;
-    if (gridDim.x == 1) return row_store<T>(m, out, 0, v);
-    float* p = a.part + ((int64_t)which * gridDim.x + blockIdx.x) * a.d;
+  if constexpr (kFull) put_sums<T>(m, a, s_post, 0, a.dpost_w);
+  put_sums<T>(m, a, s_gamma, 1, a.dgamma);
+  put_sums<T>(m, a, s_next, 2, a.dnext_w);
+}
+
+// The backward of rows whose fp32 values no thread's registers hold: a row is read twice,
+// the second time from the cache, some neighbours a thread at a time; only the weights'
+// sums stay. One pass takes what both norms need of the row (D's parts by themselves, since
+// D is not known yet):
+//   s1 = sum q nr;  s2 = sum (dr + q / rms(r)) e,  s3 = sum nr e,  e = nu gamma post_w
+//   sum D e = s2 - s1 s3 / (d rms(r))
+// and the other one forms the gradients. Without a norm there is that one alone. Four
+// elements a thread and step: eight hold more than the registers left beside the sums.
+// d = 9216, bf16, T = 4096: 73 us with a gate alone (5.2 TB/s of what has to be moved), 182
+// with every operand (3.3 TB/s); d = 16384, T = 2048, residual and next norm 118 (3.4 TB/s).
+template <class T, int NCH, RowEnd kEnd, int F>
+__global__ __launch_bounds__(1024) void k_block_norm_bwd_wide(BlockNormArgs a) {
+#pragma clang fp contract(off)
+  constexpr int N = 4;
+  using M = RowMap<T, N, 1, kEnd>;
+  using R = RowRegs<M, T>;
+  constexpr bool kAny = F < 0;
+  __shared__ float lds[6][16];
+  if (threadIdx.x < 96) lds[threadIdx.x >> 4][threadIdx.x & 15] = 0.f;
+  __syncthreads();
+  const int tid = threadIdx.x, tpr = blockDim.x;
+  const float inv_d = 1.f / (float)a.d;
+  const bool gated = kAny ? a.gate != nullptr : (F & kGate) != 0;
+  const bool post = kAny ? a.post_w != nullptr : (F & kPost) != 0;
+  const bool res = kAny ? a.x != nullptr : (F & kRes) != 0;
+  const bool next = kAny ? a.dh != nullptr : (F & kNext) != 0;
+  const bool dr_in = kAny ? a.dr != nullptr : true;
+  const bool sums = a.dpost_w || a.dgamma || a.dnext_w;
+  float s_post[NCH][N] = {}, s_gamma[NCH][N] = {}, s_next[NCH][N] = {};
+  int par = 0;
+  for (int64_t b = blockIdx.x; b < a.T; b += gridDim.x, par ^= 3) {
+    const float inv_u = post ? a.inv[b] : 1.f, inv_r = next ? a.inv[a.T + b] : 0.f;
+    R y, x, g, dr, dh, pw, gm, nw;
+    x.fill(0u), dr.fill(0u), gm.fill(kOneWords<T>), pw.fill(kOneWords<T>);
+    const auto fetch = [&](const M& m) {
+      y.load(m, a.y, b, a.y_rs);
+      if (gated) g.load(m, a.gate, b, a.gate_rs);
+      if (next) {
+        dh.load(m, a.dh, b, a.dh_rs);
+        nw.load(m, a.next_w, 0, 0);
+        if (res) x.load(m, a.x, b, a.x_rs);
+      }
+      if (dr_in) dr.load(m, a.dr, b, a.dr_rs);
+      if (post) pw.load(m, a.post_w, 0, 0);
+      if (a.gamma) gm.load(m, a.gamma, 0, 0);
+    };
+    // nu and nr of the thread's elements, and D without the norm's mean
+    float sg[N], nu[N], nr[N], D[N];
+    const auto form = [&]() {
 #pragma unroll
-    for (int k = 0; k < NCH; ++k)
+      for (int i = 0; i < N; ++i) {
+        nu[i] = y[i];
+        D[i] = dr[i];
+      }
+      if (gated) {
 #pragma unroll
-      for (int j = 0; j < EPC; ++j)
-        if (m.in(k) && m.col(k) + j < a.d) p[m.col(k) + j] = v[k * EPC + j];
-  };
-  if constexpr (kFull) put(s_post, 0, a.dpost_w);
-  put(s_gamma, 1, a.dgamma);
-  put(s_next, 2, a.dnext_w);
+        for (int i = 0; i < N; ++i) {
+          sg[i] = sigmoid(g[i]);
+          nu[i] *= g[i] * sg[i];
+        }
+      }
+      if (post) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) nu[i] *= inv_u;
+      }
+      if (next) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          nr[i] = fmaf(nu[i] * pw[i], gm[i], x[i]) * inv_r;
+          D[i] = fmaf(dh[i] * nw[i], inv_r, D[i]);
+        }
+      }
+    };
+    float s1 = 0.f, s2 = 0.f, s3 = 0.f;
+    if (next || post) {
+#pragma unroll 1
+      for (int k = 0; k < NCH; ++k) {
+        const M m{tid + k * tpr, tpr, a.d};
+        fetch(m);
+        form();
+        if (next) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) s1 = m.mine(i) ? fmaf(dh[i] * nr[i], nw[i], s1) : s1;
+        }
+        if (post) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float e = nu[i] * gm[i] * pw[i];
+            s2 = m.mine(i) ? fmaf(D[i], e, s2) : s2;
+            if (next) s3 = m.mine(i) ? fmaf(nr[i], e, s3) : s3;
+          }
+        }
+      }
+      s1 = lanes_sum<64>(s1), s2 = lanes_sum<64>(s2), s3 = lanes_sum<64>(s3);
+      if ((tid & 63) == 0) {
+        lds[par][tid >> 6] = s1;
+        lds[par + 1][tid >> 6] = s2;
+        lds[par + 2][tid >> 6] = s3;
+      }
+      __syncthreads();
+      s1 = lanes_sum<16>(lds[par][tid & 15]) * inv_d * inv_r;
+      s3 = lanes_sum<16>(lds[par + 2][tid & 15]);
+      s2 = fmaf(-s1, s3, lanes_sum<16>(lds[par + 1][tid & 15])) * inv_d * inv_u;
+    }
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      const M m{tid + k * tpr, tpr, a.d};
+      fetch(m);
+      form();
+      if (next) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          s_next[k][i] += dh[i] * nr[i];
+          D[i] = fmaf(-nr[i], s1, D[i]);
+        }
+      }
+      if (kAny ? a.dx != nullptr : res) row_store<T>(m, a.dx, b, D);
+#pragma unroll
+      for (int i = 0; i < N; ++i) s_gamma[k][i] = fmaf(D[i], nu[i] * pw[i], s_gamma[k][i]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) D[i] *= gm[i];
+      if (post) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          s_post[k][i] += D[i] * nu[i];
+          D[i] = fmaf(-nu[i], s2, D[i] * pw[i] * inv_u);
+        }
+      }
+      if (gated) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          nu[i] = D[i] * y[i] * (sg[i] * fmaf(g[i], 1.f - sg[i], 1.f));
+          D[i] *= g[i] * sg[i];
+        }
+        if (kAny ? a.dgate != nullptr : true) row_store<T>(m, a.dgate, b, nu);
+      }
+      if (kAny ? a.dy != nullptr : true) row_store<T>(m, a.dy, b, D);
+      __builtin_amdgcn_sched_barrier(0);      // one step's registers at a time
+    }
+  }
+  if (!sums) return;
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) {
+    const M m{tid + k * tpr, tpr, a.d};
+    put_sums<T>(m, a, s_post[k], 0, a.dpost_w);
+    put_sums<T>(m, a, s_gamma[k], 1, a.dgamma);
+    put_sums<T>(m, a, s_next[k], 2, a.dnext_w);
+  }
 }
 
 // The weights' gradients from the backward's planes: 32 columns of one weight a work-group,

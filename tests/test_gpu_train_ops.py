@@ -190,6 +190,40 @@ def test_norm_sizes(pkg, dev, T, d, dtype):
 
 
 @dtypes
+@pytest.mark.parametrize("T,d", [(300, 6150), (5, 8192), (270, 9216), (7, 12290), (3, 16381)])
+@pytest.mark.parametrize("form", [("y", "gate"), ("x", "y", "gamma", "next"), ("y", "gate", "post"),
+                                  ("x", "y", "gate", "post", "next"), NORM_FORMS[-1]], ids="+".join)
+def test_norm_wide_rows(pkg, dev, form, T, d, dtype):
+    """Rows whose backward reads them twice, more of them than work-groups and fewer, the two
+    halves of one projection."""
+    n, dr, dh = norm_inputs(form, T, d, T + d, dtype)
+    n = {k: v.to(dev) for k, v in n.items()}
+    if "gate" in n:
+        both = torch.cat([n["y"], n["gate"]], -1)
+        n["y"], n["gate"] = both[:, :d], both[:, d:]
+    _check_norm(pkg, n, dr.to(dev), dh.to(dev))
+
+
+@dtypes
+def test_norm_wide_rows_partial_gradients(pkg, dev, dtype):
+    """One gradient at a time, and of one output alone, as all of them, bit for bit."""
+    for form in (NORM_FORMS[-1], ("x", "y", "gamma", "next")):
+        for d in (9216, 16384):
+            n, dr, dh = norm_inputs(form, 4, d, d, dtype)
+            n = {k: v.to(dev).requires_grad_() for k, v in n.items()}
+            r, h = pkg.fused_block_norm(**n)
+            dr, dh = dr.to(dev), dh.to(dev)
+            full = torch.autograd.grad((r, h), list(n.values()), (dr, dh), retain_graph=True)
+            for k, g in zip(n, full):
+                one = torch.autograd.grad((r, h), n[k], (dr, dh), retain_graph=True)[0]
+                assert torch.equal(one, g), (k, d)
+            alone = torch.autograd.grad(h, list(n.values()), dh, retain_graph=True)
+            zero = torch.autograd.grad((r, h), list(n.values()), (torch.zeros_like(r), dh))
+            for k, a, b in zip(n, alone, zero):
+                assert torch.equal(a, b), (k, d)
+
+
+@dtypes
 def test_norm_strides(pkg, dev, dtype):
     """Halves of one projection, rows at an odd stride, leading axes, a transposed operand, an
     expanded gradient: as the contiguous ones."""
