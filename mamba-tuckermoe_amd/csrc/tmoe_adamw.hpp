@@ -185,12 +185,20 @@ __device__ __forceinline__ E4m3Place e4m3_place(float a) {
   const uint32_t A = (b & 0x7fffffu) | (sub ? 0u : 0x800000u);
   return {(b >> 20) - (sub ? 968u : 960u), A & 0xf00000u, A & 0xfffffu};
 }
-// The code of a magnitude, up with the chance rest / step; u16: 16 random bits. A quotient
-// that rounding put over 448 is a place or two over it: no bits are low enough to go up.
-template <bool kSub>
-__device__ __forceinline__ uint32_t e4m3_code(float a, uint32_t u16) {
-  const E4m3Place p = e4m3_place<kSub>(a);
-  return p.code + ((u16 << 4 | 8u) < p.rest ? 1u : 0u);
+// The code of a value in byte kByte of c, up with the chance rest / step: where the upper 16
+// bits of h, 8 more below them, are under rest. The conversion adds the upper 20 bits that it
+// is given to the mantissa and cuts: with their complement it goes up just there (values
+// under 2^-6 go by their place). A quotient that rounding put over 448 is a place or two
+// over it: no bits are low enough to go up.
+template <bool kSub, int kByte>
+__device__ __forceinline__ uint32_t e4m3_code(float a, uint32_t h, uint32_t c) {
+  if constexpr (kSub) {
+    const E4m3Place p = e4m3_place<true>(fabsf(a));
+    return c | (p.code + ((h >> 16 << 4 | 8u) < p.rest ? 1u : 0u) |
+                (__float_as_uint(a) >> 24 & 0x80u)) << 8 * kByte;
+  } else {
+    return __builtin_amdgcn_cvt_sr_fp8_f32(a, (h | 0xffffu) ^ 0xffff8fffu, c, kByte);
+  }
 }
 // The code of a root r, up with the chance (r^2 - lo^2) / (hi^2 - lo^2)
 // = rest (r + lo) / (hi + lo); odd: (2 q + 1, its reciprocal rounded) for q = 0 .. 15.
@@ -207,18 +215,19 @@ __device__ __forceinline__ uint32_t e4m3_root_code(float r, uint32_t u16, const 
 }
 // The codes of four moments (m over their scale, r over theirs).
 template <bool kSub>
-__device__ __forceinline__ uint2 e4m3_codes(const float (&m)[4], const float (&qm)[4],
-                                            const float (&qr)[4], uint32_t key, uint32_t step_key,
-                                            const float2* odd) {
-  uint2 c = {0u, 0u};
+__device__ __forceinline__ uint2 e4m3_codes(const float (&qm)[4], const float (&qr)[4], uint32_t key,
+                                            uint32_t step_key, const float2* odd) {
+  uint32_t h[4], m = 0u, r = 0u;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t h = mix32((key + (uint32_t)j) ^ step_key);
-    const uint32_t sign = __float_as_uint(m[j]) >> 24 & 0x80u;
-    c.x |= (e4m3_code<kSub>(qm[j], h >> 16) | sign) << 8 * j;
-    c.y |= e4m3_root_code<kSub>(qr[j], h & 0xffffu, odd) << 8 * j;
+    h[j] = mix32((key + (uint32_t)j) ^ step_key);
+    r |= e4m3_root_code<kSub>(qr[j], h[j] & 0xffffu, odd) << 8 * j;
   }
-  return c;
+  m = e4m3_code<kSub, 0>(qm[0], h[0], m);
+  m = e4m3_code<kSub, 1>(qm[1], h[1], m);
+  m = e4m3_code<kSub, 2>(qm[2], h[2], m);
+  m = e4m3_code<kSub, 3>(qm[3], h[3], m);
+  return {m, r};
 }
 
 // A wave takes blocks of 256 elements, four neighbours a lane. What decides a code is
@@ -299,16 +308,16 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
     float qm[4], qr[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      qm[j] = quotient(fabsf(m[j]), dm, im);
+      qm[j] = quotient(m[j], dm, im);
       qr[j] = quotient(r[j], dr, ir);
     }
     const uint64_t e = (uint64_t)(first + i);    // four neighbours share its upper half
     const uint32_t key = (a.first + (uint32_t)s.t) * 0x9E3779B9u + (uint32_t)e +
                          (uint32_t)(e >> 32) * 0xC2B2AE35u;
-    const float least = fminf(fminf(fminf(qm[0], qm[1]), fminf(qm[2], qm[3])),
+    const float least = fminf(fminf(fminf(fabsf(qm[0]), fabsf(qm[1])), fminf(fabsf(qm[2]), fabsf(qm[3]))),
                               fminf(fminf(qr[0], qr[1]), fminf(qr[2], qr[3])));
-    const uint2 c = __any(!(least >= 0x1p-6f)) ? e4m3_codes<true>(m, qm, qr, key, s.key, odd)
-                                               : e4m3_codes<false>(m, qm, qr, key, s.key, odd);
+    const uint2 c = __any(!(least >= 0x1p-6f)) ? e4m3_codes<true>(qm, qr, key, s.key, odd)
+                                               : e4m3_codes<false>(qm, qr, key, s.key, odd);
     if (whole) {
       store4(p + i, pv);
       *reinterpret_cast<codes4*>(mq + i) = c.x;
