@@ -12,7 +12,7 @@
 // never coded as zero: its element's step would be m / eps.
 //
 // fp32 is bound by memory: 28 bytes an element, 417 M of them in 2256 us, 5.2 TB/s. 8 bits
-// by instructions, ~88 an element: 19.3 M bf16 parameters in 55 us, 3.5 TB/s. A launch takes up to kAdamwTensors tensors,
+// by instructions, ~71 an element: 19.3 M bf16 parameters in 48.6 us, 4.0 TB/s. A launch takes up to kAdamwTensors tensors,
 // their addresses in its arguments: nothing is copied to the device, and a captured step
 // holds them. A work-group takes `chunk` elements of one tensor.
 #pragma once
@@ -101,20 +101,20 @@ __device__ __forceinline__ float adamw_param(const AdamwStep& s, float p, float 
   return p * s.keep - (m / (root * s.inv_c2 + s.eps)) * s.rate;
 }
 
-// Four neighbours at any alignment (a view may begin anywhere).
-template <class T>
-__device__ __forceinline__ void load4(const T* p, float v[4]) {
-  constexpr int W = (int)sizeof(T);
+// N neighbours at any alignment (a view may begin anywhere).
+template <int N, class T>
+__device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
+  constexpr int W = N * (int)sizeof(T) / 4;
   typedef uint32_t vec __attribute__((ext_vector_type(W), aligned(sizeof(T))));
   const vec q = *reinterpret_cast<const vec*>(p);
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < N; ++j)
     if constexpr (sizeof(T) == 4) v[j] = __uint_as_float(q[j]);
     else v[j] = __uint_as_float(j & 1 ? q[j / 2] & 0xffff0000u : q[j / 2] << 16);
 }
-template <class T>
-__device__ __forceinline__ void store4(T* p, const float v[4]) {
-  constexpr int W = (int)sizeof(T);
+template <int N, class T>
+__device__ __forceinline__ void store_n(T* p, const float (&v)[N]) {
+  constexpr int W = N * (int)sizeof(T) / 4;
   typedef uint32_t vec __attribute__((ext_vector_type(W), aligned(sizeof(T))));
   vec q;
 #pragma unroll
@@ -123,7 +123,7 @@ __device__ __forceinline__ void store4(T* p, const float v[4]) {
     else q[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
   *reinterpret_cast<vec*>(p) = q;
 }
-typedef uint32_t codes4 __attribute__((aligned(1)));
+typedef uint32_t codes8 __attribute__((ext_vector_type(2), aligned(1)));
 
 template <class T>
 __global__ __launch_bounds__(kAdamwThreads) void k_adamw32(const AdamwTable a) {
@@ -136,18 +136,18 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw32(const AdamwTable a) {
   int64_t i = s.base + 4 * threadIdx.x;
   for (; i + 4 <= end; i += 4 * kAdamwThreads) {
     float pv[4], gv[4], mv[4], vv[4];
-    load4(p + i, pv);
-    load4(g + i, gv);
-    load4(m + i, mv);
-    load4(v + i, vv);
+    load_n<4>(p + i, pv);
+    load_n<4>(g + i, gv);
+    load_n<4>(m + i, mv);
+    load_n<4>(v + i, vv);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       adamw_moments(s, gv[j], mv[j], vv[j]);
       pv[j] = adamw_param(s, pv[j], mv[j], sqrtf(vv[j]));
     }
-    store4(p + i, pv);
-    store4(m + i, mv);
-    store4(v + i, vv);
+    store_n<4>(p + i, pv);
+    store_n<4>(m + i, mv);
+    store_n<4>(v + i, vv);
   }
   for (; i < end; ++i) {      // a tensor's last one to three elements, one thread's
     float mv = m[i], vv = v[i];
@@ -213,24 +213,30 @@ __device__ __forceinline__ uint32_t e4m3_root_code(float r, uint32_t u16, const 
   const uint32_t c = p.code + (u < chance ? 1u : 0u);
   return kSub ? max(c, min(__float_as_uint(r), 1u)) : c;
 }
-// The codes of four moments (m over their scale, r over theirs).
+// The codes of eight moments (m over their scale, r over theirs).
 template <bool kSub>
-__device__ __forceinline__ uint2 e4m3_codes(const float (&qm)[4], const float (&qr)[4], uint32_t key,
-                                            uint32_t step_key, const float2* odd) {
-  uint32_t h[4], m = 0u, r = 0u;
+__device__ __forceinline__ void e4m3_codes(const float (&qm)[8], const float (&qr)[8], uint32_t key,
+                                           uint32_t step_key, const float2* odd, codes8& m, codes8& r) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    h[j] = mix32((key + (uint32_t)j) ^ step_key);
-    r |= e4m3_root_code<kSub>(qr[j], h[j] & 0xffffu, odd) << 8 * j;
+  for (int w = 0; w < 2; ++w) {
+    uint32_t h[4], cm = 0u, cr = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h[j] = mix32((key + (uint32_t)(4 * w + j)) ^ step_key);
+      cr |= e4m3_root_code<kSub>(qr[4 * w + j], h[j] & 0xffffu, odd) << 8 * j;
+    }
+    cm = e4m3_code<kSub, 0>(qm[4 * w], h[0], cm);
+    cm = e4m3_code<kSub, 1>(qm[4 * w + 1], h[1], cm);
+    cm = e4m3_code<kSub, 2>(qm[4 * w + 2], h[2], cm);
+    cm = e4m3_code<kSub, 3>(qm[4 * w + 3], h[3], cm);
+    m[w] = cm;
+    r[w] = cr;
   }
-  m = e4m3_code<kSub, 0>(qm[0], h[0], m);
-  m = e4m3_code<kSub, 1>(qm[1], h[1], m);
-  m = e4m3_code<kSub, 2>(qm[2], h[2], m);
-  m = e4m3_code<kSub, 3>(qm[3], h[3], m);
-  return {m, r};
 }
 
-// A wave takes blocks of 256 elements, four neighbours a lane. What decides a code is
+// Half a wave takes a block of 256 elements, eight neighbours a lane (a wave with four a lane:
+// 52.9 us against 48.6 at 19.3 M; the next block read ahead gained nothing there). What
+// decides a code is
 // computed as the formulas round it (a step's codes are the next one's values), the rest
 // with the hardware's reciprocals: the arithmetic, not the memory, is the bound. A moment
 // whose block's scale is under 2^-110 is taken for zero (the reciprocal of less overflows).
@@ -245,50 +251,55 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
   __syncthreads();
   const AdamwStep s = adamw_step(a);
   const int64_t n = a.n[s.t];
-  // the wave's part of the work-group's chunk: `count` elements from `first` on, in 32 bits
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int kEach = 8, kLanes = kAdamwBlock / kEach, kTeams = kAdamwThreads / kLanes;
+  // the lanes' part of the work-group's chunk: `count` elements from `first` on, in 32 bits
+  const uint32_t lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes;
   const uint32_t all = (uint32_t)(a.chunk < n - s.base ? a.chunk : n - s.base);
-  const int64_t first = s.base + wave * kAdamwBlock;
-  const uint32_t count = all > wave * kAdamwBlock ? all - wave * kAdamwBlock : 0u;
+  const int64_t first = s.base + team * kAdamwBlock;
+  const uint32_t count = all > team * kAdamwBlock ? all - team * kAdamwBlock : 0u;
   T* p = static_cast<T*>(a.p[s.t]) + first;
   const T* g = static_cast<const T*>(a.g[s.t]) + first;
   uint8_t* mq = static_cast<uint8_t*>(a.m[s.t]) + first;
   uint8_t* rq = static_cast<uint8_t*>(a.v[s.t]) + first;
   float* ms = a.ms[s.t] + first / kAdamwBlock;
   float* rs = a.vs[s.t] + first / kAdamwBlock;
-  for (uint32_t b = 0, blk = 0; b < count;
-       b += kAdamwThreads / 64 * kAdamwBlock, blk += kAdamwThreads / 64) {
-    const uint32_t i = b + 4 * lane;
-    const bool whole = i + 4 <= count;
+  for (uint32_t b = 0, blk = 0; b < count; b += kTeams * kAdamwBlock, blk += kTeams) {
+    const uint32_t i = b + kEach * lane;
+    const bool whole = i + kEach <= count;
     const int live = i < count ? (int)(count - i) : 0;   // where not whole
     const float sm = ms[blk], sr = rs[blk];
-    float pv[4] = {}, gv[4] = {}, m[4], r[4];
-    uint32_t mc = 0u, rc = 0u;
+    float pv[kEach] = {}, gv[kEach] = {}, m[kEach], r[kEach];
+    codes8 mc = {0u, 0u}, rc = {0u, 0u};
     if (whole) {
-      load4(p + i, pv);
-      load4(g + i, gv);
-      mc = *reinterpret_cast<const codes4*>(mq + i);
-      rc = *reinterpret_cast<const codes4*>(rq + i);
+      load_n<kEach>(p + i, pv);
+      load_n<kEach>(g + i, gv);
+      mc = *reinterpret_cast<const codes8*>(mq + i);
+      rc = *reinterpret_cast<const codes8*>(rq + i);
     } else {
-      for (int j = 0; j < live; ++j) {
-        pv[j] = load_as_f32(p + i + j);
-        gv[j] = load_as_f32(g + i + j);
-        mc |= (uint32_t)mq[i + j] << 8 * j;
-        rc |= (uint32_t)rq[i + j] << 8 * j;
-      }
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (j < live) {
+          pv[j] = load_as_f32(p + i + j);
+          gv[j] = load_as_f32(g + i + j);
+          mc[j / 4] |= (uint32_t)mq[i + j] << 8 * (j % 4);
+          rc[j / 4] |= (uint32_t)rq[i + j] << 8 * (j % 4);
+        }
     }
-    const f32x2_t mc01 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, false);
-    const f32x2_t mc23 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, true);
-    const f32x2_t rc01 = __builtin_amdgcn_cvt_pk_f32_fp8(rc, false);
-    const f32x2_t rc23 = __builtin_amdgcn_cvt_pk_f32_fp8(rc, true);
-    const float mv[4] = {mc01[0], mc01[1], mc23[0], mc23[1]};
-    const float rv[4] = {rc01[0], rc01[1], rc23[0], rc23[1]};
+#pragma unroll
+    for (int j = 0; j < kEach; j += 4) {
+      const f32x2_t m01 = __builtin_amdgcn_cvt_pk_f32_fp8(mc[j / 4], false);
+      const f32x2_t m23 = __builtin_amdgcn_cvt_pk_f32_fp8(mc[j / 4], true);
+      const f32x2_t r01 = __builtin_amdgcn_cvt_pk_f32_fp8(rc[j / 4], false);
+      const f32x2_t r23 = __builtin_amdgcn_cvt_pk_f32_fp8(rc[j / 4], true);
+      m[j] = m01[0], m[j + 1] = m01[1], m[j + 2] = m23[0], m[j + 3] = m23[1];
+      r[j] = r01[0], r[j + 1] = r01[1], r[j + 2] = r23[0], r[j + 3] = r23[1];
+    }
     // magnitudes as integers: in their order, a NaN above all
     uint32_t am = 0u, ar = 0u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      m[j] = mv[j] * sm;
-      r[j] = rv[j] * sr;
+    for (int j = 0; j < kEach; ++j) {
+      m[j] *= sm;
+      r[j] *= sr;
       float v = r[j] * r[j];
       adamw_moments(s, gv[j], m[j], v);
       r[j] = root_of(v);
@@ -296,8 +307,8 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
       am = max(am, __float_as_uint(m[j]) & 0x7fffffffu);
       ar = max(ar, __float_as_uint(r[j]) & 0x7fffffffu);
     }
-    float nsm = __uint_as_float(lanes_max<64>(am)) * (1.f / kE4m3Max);
-    float nsr = __uint_as_float(lanes_max<64>(ar)) * (1.f / kE4m3Max);
+    float nsm = __uint_as_float(lanes_max<kLanes>(am)) * (1.f / kE4m3Max);
+    float nsr = __uint_as_float(lanes_max<kLanes>(ar)) * (1.f / kE4m3Max);
     nsm = nsm < 0x1p-110f ? 0.f : nsm;
     nsr = nsr < 0x1p-110f ? 0.f : nsr;
     const float dm = nsm == 0.f ? 1.f : nsm, dr = nsr == 0.f ? 1.f : nsr;
@@ -305,29 +316,30 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
     float im = __builtin_amdgcn_rcpf(dm), ir = __builtin_amdgcn_rcpf(dr);
     im = fmaf(fmaf(-dm, im, 1.f), im, im);
     ir = fmaf(fmaf(-dr, ir, 1.f), ir, ir);
-    float qm[4], qr[4];
+    float least = INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      qm[j] = quotient(m[j], dm, im);
-      qr[j] = quotient(r[j], dr, ir);
+    for (int j = 0; j < kEach; ++j) {
+      m[j] = quotient(m[j], dm, im);
+      r[j] = quotient(r[j], dr, ir);
+      least = fminf(least, fminf(fabsf(m[j]), r[j]));
     }
-    const uint64_t e = (uint64_t)(first + i);    // four neighbours share its upper half
+    const uint64_t e = (uint64_t)(first + i);    // the neighbours share its upper half
     const uint32_t key = (a.first + (uint32_t)s.t) * 0x9E3779B9u + (uint32_t)e +
                          (uint32_t)(e >> 32) * 0xC2B2AE35u;
-    const float least = fminf(fminf(fminf(fabsf(qm[0]), fabsf(qm[1])), fminf(fabsf(qm[2]), fabsf(qm[3]))),
-                              fminf(fminf(qr[0], qr[1]), fminf(qr[2], qr[3])));
-    const uint2 c = __any(!(least >= 0x1p-6f)) ? e4m3_codes<true>(qm, qr, key, s.key, odd)
-                                               : e4m3_codes<false>(qm, qr, key, s.key, odd);
+    if (__any(!(least >= 0x1p-6f))) e4m3_codes<true>(m, r, key, s.key, odd, mc, rc);
+    else e4m3_codes<false>(m, r, key, s.key, odd, mc, rc);
     if (whole) {
-      store4(p + i, pv);
-      *reinterpret_cast<codes4*>(mq + i) = c.x;
-      *reinterpret_cast<codes4*>(rq + i) = c.y;
+      store_n<kEach>(p + i, pv);
+      *reinterpret_cast<codes8*>(mq + i) = mc;
+      *reinterpret_cast<codes8*>(rq + i) = rc;
     } else {
-      for (int j = 0; j < live; ++j) {
-        store_from_f32(p + i + j, pv[j]);
-        mq[i + j] = (uint8_t)(c.x >> 8 * j);
-        rq[i + j] = (uint8_t)(c.y >> 8 * j);
-      }
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (j < live) {
+          store_from_f32(p + i + j, pv[j]);
+          mq[i + j] = (uint8_t)(mc[j / 4] >> 8 * (j % 4));
+          rq[i + j] = (uint8_t)(rc[j / 4] >> 8 * (j % 4));
+        }
     }
     if (lane == 0) {
       ms[blk] = nsm;
