@@ -236,10 +236,10 @@ __device__ __forceinline__ void e4m3_codes(const float (&qm)[8], const float (&q
 
 // Half a wave takes a block of 256 elements, eight neighbours a lane (a wave with four a lane:
 // 52.9 us against 48.6 at 19.3 M; the next block read ahead gained nothing there). What
-// decides a code is
-// computed as the formulas round it (a step's codes are the next one's values), the rest
-// with the hardware's reciprocals: the arithmetic, not the memory, is the bound. A moment
-// whose block's scale is under 2^-110 is taken for zero (the reciprocal of less overflows).
+// decides a code is computed as the formulas round it (a step's codes are the next one's
+// values), the rest with the hardware's reciprocals: the arithmetic, not the memory, is the
+// bound. A moment whose block's scale is under 2^-110 is taken for zero (the reciprocal of
+// less overflows).
 template <class T>
 __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
 #pragma clang fp contract(off)

@@ -98,11 +98,13 @@ hipError_t block_norm_backward(const BlockNormArgs& a, hipStream_t st) {
 hipError_t adamw(const tmoe_adamw_tensor* t, int64_t count, const tmoe_adamw_step_args& a,
                  hipStream_t st) {
   static_assert(sizeof(dev::AdamwTable) <= 4096, "a launch's arguments");
-  // a work-group's elements: enough work-groups for the chip where the tensors are small
+  // a work-group's elements: enough work-groups for the chip where the tensors are small, but
+  // each thread four of 32 bits or eight of 8
   int64_t total = 0;
   for (int64_t i = 0; i < count; ++i) total += t[i].n;
   int64_t chunk = 8192;
-  while (chunk > 1024 && total / chunk < 2048) chunk >>= 1;
+  const int64_t least = a.state_bits == 8 ? 2048 : 1024;
+  while (chunk > least && total / chunk < 2048) chunk >>= 1;
   dev::AdamwTable b;
   b.step_dev = a.step_dev;
   b.beta1 = a.beta1; b.beta2 = a.beta2; b.lr = a.lr;
