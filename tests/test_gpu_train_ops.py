@@ -99,6 +99,25 @@ def test_router_ties_and_extremes(pkg, dev):
         _check_router(pkg, raw.to(dt), 3, 0.5, 10.0, None, 1)
 
 
+@dtypes
+@pytest.mark.parametrize("E,k", [(4, 4), (8, 8), (11, 11), (37, 16), (64, 6), (100, 16), (256, 16)])
+def test_router_near_ties_and_padding(pkg, dev, E, k, dtype):
+    """Logits a few places apart or equal, over all lanes of a token and in tokens of one wave
+    with others that are not; rows of -inf beside widths that no lane count divides."""
+    g = torch.Generator().manual_seed(E)
+    B = 200
+    raw = _logits(B, E, torch.float32, E)
+    near_ = (torch.full((B, E), 1.0).view(torch.int32) + torch.randint(0, 400, (B, E), generator=g).int()).view(torch.float32)
+    raw[::2] = near_[::2] * torch.where(torch.rand(B, 1, generator=g) < 0.5, -1.0, 1.0)[::2]
+    raw[1::6] = torch.randint(0, 3, (B, E), generator=g).float()[1::6]
+    raw[3] = -float("inf")
+    raw[5, : E // 2] = -float("inf")
+    raw[9, E // 2:] = -float("inf")
+    mask = (torch.rand(B, generator=g) < 0.8).to(dev)
+    mask[torch.tensor([3, 5, 9])] = True
+    _check_router(pkg, raw.to(dtype).to(dev), k, 0.9, 10.0, mask, 4)
+
+
 def test_router_no_tokens(pkg, dev):
     """No tokens, and none that the mask leaves: zero losses, counts and gradients; what the
     left-out rows hold does not matter, and a NaN row spoils its own row alone."""
@@ -870,3 +889,82 @@ def test_router_top1_weights_gradient(pkg, dev):
     o = tn.router(f64(raw), 1, 0.5, 10.0, None, f64(dw))
     # 16 cap / tau + 128 roundings of each factor, in the 2-norm
     assert onp.rel_l2(f64(draw), o["draw"]) <= 4 * (16 * 10 / 0.5 + 128) * U
+
+
+def test_router_nan_row_gradient_is_its_own(pkg, dev):
+    """One NaN logit: that token's gradients are NaN, the others' what they are without it."""
+    for E in (8, 64):
+        raw = _logits(40, E, torch.float32, E).to(dev)
+        dw = torch.randn(40, 3, device=dev)
+        bad = raw.clone()
+        bad[11, E - 3] = float("nan")
+        d = [torch.autograd.grad(pkg.fused_router(t, 3, 0.5).weights, t, dw)[0]
+             for t in (raw.requires_grad_(), bad.requires_grad_())]
+        assert d[1][11].isnan().all()
+        d[1][11] = d[0][11]
+        assert torch.equal(d[0], d[1])
+
+
+def _free_gib():
+    return torch.cuda.mem_get_info()[0] / 2 ** 30
+
+
+def test_offsets_past_32_bits(pkg, dev):
+    """The last rows and elements of tensors of more than 2^31 elements, as by themselves."""
+    if _free_gib() < 80:
+        pytest.skip("needs 80 GiB of free memory")
+    T, d, last = 2 ** 17 + 3, 16384, 5
+    n, dr, dh = norm_inputs(("x", "y", "gamma", "next"), last, d, 1, torch.bfloat16)
+    n = {k: v.to(dev) for k, v in n.items()}
+    dr, dh = dr.to(dev), dh.to(dev)
+
+    def long(t):
+        z = torch.zeros(T, d, dtype=t.dtype, device=dev)
+        z[-last:] = t
+        return z
+    big = {k: (long(v) if v.dim() == 2 else v).requires_grad_() for k, v in n.items()}
+    r, h = pkg.fused_block_norm(**big)
+    gx, gy = torch.autograd.grad((r, h), (big["x"], big["y"]), (long(dr), long(dh)))
+    small = {k: v.requires_grad_() for k, v in n.items()}
+    rs, hs = pkg.fused_block_norm(**small)
+    sx, sy = torch.autograd.grad((rs, hs), (small["x"], small["y"]), (dr, dh))
+    for a, b in ((r, rs), (h, hs), (gx, sx), (gy, sy)):
+        assert torch.equal(a[-last:], b) and not a[:-last].any()
+    del r, h, gx, gy, big
+    B, E = 2 ** 23 + 3, 256
+    raw = torch.zeros(B, E, device=dev)
+    tail = _logits(last, E, torch.float32, 4).to(dev).requires_grad_()
+    raw[-last:] = tail.detach()
+    raw.requires_grad_()
+    dw = torch.randn(last, 8, device=dev)
+    a, b = pkg.fused_router(raw, 8, 0.5), pkg.fused_router(tail, 8, 0.5)
+    assert torch.equal(a.idx[-last:], b.idx) and torch.equal(a.weights[-last:], b.weights)
+    assert a.counts.sum().item() == 8 * B
+    dwl = torch.zeros(B, 8, device=dev)
+    dwl[-last:] = dw
+    assert torch.equal(torch.autograd.grad(a.weights, raw, dwl)[0][-last:], torch.autograd.grad(b.weights, tail, dw)[0])
+    del raw, a, dwl
+    N, keep = 2 ** 31 + 517, 773        # keep: from a block's begin on
+    pl, gl = (torch.zeros(N, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    p, g = ((torch.randn(keep, device=dev) * s).bfloat16() for s in (0.05, 0.01))
+    N0 = N - keep
+    assert N0 % 256 == 0
+    pl[N0:], gl[N0:] = p, g
+    for bits in (32, 8):
+        st, sl = [], []
+        for size, out in ((keep, st), (N, sl)):
+            if bits == 32:
+                out += [[torch.zeros(size, device=dev)] for _ in range(2)]
+            else:
+                for _ in range(2):
+                    out += [[torch.zeros(size, dtype=torch.uint8, device=dev)],
+                            [torch.zeros(-(-size // 256), device=dev)]]
+        step = pkg.adamw_step if bits == 32 else pkg.adamw_step_8bit
+        step([p], [g], *st, step=3, **HYPER)
+        step([pl], [gl], *sl, step=3, **HYPER)
+        assert torch.equal(pl[N0:], p) and not pl[:N0].any()
+        for a, b in zip(sl, st):
+            if a[0].dtype == torch.float32:        # (codes are rounded by the element's place)
+                assert torch.equal(a[0][-b[0].numel():], b[0])
+    del pl, gl, sl, a, b
+    torch.cuda.empty_cache()
