@@ -369,7 +369,8 @@ int tmoe_latent_backward(const void* x, const void* G, const int64_t* idx, const
  * dtype TMOE_BF16 or TMOE_F32, arithmetic in fp32; E <= 256, k <= min(E, 16), B <= 2^30.
  * Backward: from dw (B, k), dlb and dz (one fp32 each; any of them null for zeros) draw
  * (B, E) of dtype, contiguous; idx, tokens and counts as the forward wrote them. The sums
- * over the tokens are added in a fixed order. Stream-ordered, no allocation. */
+ * over the tokens are added in a fixed order. What is written overlaps nothing that is
+ * read. Stream-ordered, no allocation. */
 typedef struct tmoe_router {
   const void* raw;
   int64_t row_stride, B, E, k;
@@ -399,7 +400,8 @@ int tmoe_router_backward(const tmoe_router* router, const int64_t* idx, const fl
  * (2, T) fp32, is what the backward needs of the forward (null: no backward follows).
  * Backward: from dr and dh ((T, d) of dtype, each may be null) the gradients that are not
  * null: dx, dy, dgate (T, d) contiguous, dpost_weight, dgamma, dnext_weight (d), the latter
- * three with a workspace. d <= 16384, T <= 2^30. Stream-ordered, no allocation. */
+ * three with a workspace. What is written overlaps nothing that is read. d <= 16384,
+ * T <= 2^30. Stream-ordered, no allocation. */
 typedef struct tmoe_block_norm {
   const void *x, *y, *gate;
   int64_t x_stride, y_stride, gate_stride;
