@@ -25,6 +25,14 @@ BLOCK = 256
 E4M3_MAX = 448.0
 
 
+def _capturing(device: torch.device) -> bool:
+    """Whether the current stream of a device records a graph."""
+    if device.type != "cuda":
+        return False
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _run(params, grads, m, v, ms, vs, step, lr, betas, eps, weight_decay, seed):
     if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
         raise ValueError(f"adamw_step: betas {betas}")
@@ -73,7 +81,9 @@ class FusedAdamW(torch.optim.Optimizer):
     state_bits 32 keeps float32 moments ("exp_avg", "exp_avg_sq"), 8 keeps codes and scales
     ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales", of
     sqrt(v)). capturable=True holds the step count on the device, so that a captured step
-    counts on in its replays; without it a step inside a capture raises. Parameters are
+    counts on in its replays; without it a step inside a capture raises. Each parameter
+    counts the steps that it took: those that step together share a count until a step that only
+    some of them take, which is refused once a captured step advances that count. Parameters are
     bfloat16 or float32, dense, on HIP devices, with gradients of their dtype; bfloat16
     ones are rounded to nearest."""
 
@@ -86,8 +96,13 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError(f"FusedAdamW: betas {betas}")
         if state_bits not in (32, 8):
             raise ValueError(f"FusedAdamW: state_bits {state_bits} is not 32 or 8")
+        self._captured = {}     # by id: the device counts that captured steps advance
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       state_bits=state_bits, seed=seed, capturable=capturable))
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        self._captured = {}
 
     def _init_state(self, p: torch.Tensor, group, count) -> dict:
         st = self.state[p]
@@ -109,28 +124,32 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
+        work = [(group, [p for p in group["params"] if p.grad is not None])
+                for group in self.param_groups]
+        for group, ps in work:      # what is refused is refused before anything changes
+            self._check_step(group, ps)
+        for group, ps in work:
             on_device = group["capturable"]
             fresh = {}      # device: the count that parameters first met in this step share
             runs = {}       # (device, dtype, step): its parameters, one call each
-            for p in group["params"]:
-                g = p.grad
-                if g is None:
-                    continue
-                if g.is_sparse:
-                    raise RuntimeError("FusedAdamW: sparse gradients are not supported")
+            parted = self._shared_with_resting(group, ps) if on_device else {}
+            for p in ps:
                 st = self.state[p]
                 if not st:
                     if on_device and p.device not in fresh:
                         fresh[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
                     st = self._init_state(p, group, fresh[p.device] if on_device else 0)
                 n = st["step"]
+                if id(n) in parted:     # those that step now count by themselves from here on
+                    if parted[id(n)] is None:
+                        parted[id(n)] = n.clone()
+                    n = st["step"] = parted[id(n)]
                 key = (p.device, p.dtype, id(n) if on_device else n)
                 run = runs.get(key)
                 if run is None:
                     run = runs[key] = (n, [], [], [])
                 run[1].append(p)
-                run[2].append(g)
+                run[2].append(p.grad)
                 run[3].append(st)
             if not on_device and any(d.type == "cuda" for d, _, _ in runs) \
                     and torch.cuda.is_current_stream_capturing():
@@ -146,6 +165,38 @@ class FusedAdamW(torch.optim.Optimizer):
                     for st in sts:
                         st["step"] = n + 1
         return loss
+
+    def _shared_with_resting(self, group, ps) -> dict:
+        """{id: None} of the device counts of ps that parameters of the group without a
+        gradient hold too."""
+        if len(ps) == len(group["params"]):
+            return {}
+        mine = {id(self.state[p]["step"]) for p in ps if self.state.get(p)}
+        return {id(st["step"]): None for st in (self.state.get(p) for p in group["params"] if p.grad is None)
+                if st and id(st["step"]) in mine}
+
+    def _check_step(self, group, ps) -> None:
+        if any(p.grad.is_sparse for p in ps):
+            raise RuntimeError("FusedAdamW: sparse gradients are not supported")
+        if not group["capturable"]:
+            return
+        parted = self._shared_with_resting(group, ps)
+        capturing = {d: _capturing(d) for d in {p.device for p in ps}}
+        for p in ps:
+            st = self.state.get(p)
+            if not st:
+                continue
+            n = st["step"]
+            if id(n) not in parted:
+                if capturing[p.device]:
+                    self._captured[id(n)] = n
+            elif capturing[p.device]:
+                raise RuntimeError("FusedAdamW: a captured step of some of the parameters that have stepped "
+                                   "together so far: make one step with these gradients before the capture")
+            elif id(n) in self._captured:       # the graph counts for all of them
+                raise RuntimeError("FusedAdamW: parameters whose step was captured together step together "
+                                   "(where that graph is gone, opt.load_state_dict(opt.state_dict()) parts "
+                                   "them)")
 
     @staticmethod
     def _run(group, step, ps, gs, sts):

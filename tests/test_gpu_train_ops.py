@@ -968,3 +968,40 @@ def test_offsets_past_32_bits(pkg, dev):
                 assert torch.equal(a[0][-b[0].numel():], b[0])
     del pl, gl, sl, a, b
     torch.cuda.empty_cache()
+
+
+def test_capturable_counts_of_resting_parameters(pkg, dev):
+    """Parameters that rest for some steps: the updates of the count on the device are those of
+    the count on the host, eager and replayed."""
+    def params():
+        g = torch.Generator().manual_seed(7)
+        return [torch.nn.Parameter((torch.randn(300, generator=g) * 0.1).to(dev)) for _ in range(3)]
+    ps, ref = params(), params()
+    opt = pkg.FusedAdamW(ps, capturable=True, lr=1e-2)
+    ropt = pkg.FusedAdamW(ref, lr=1e-2)
+    grads = torch.randn(3, 300, device=dev) * 0.01
+
+    def step(o, qs, on):
+        for q, g, use in zip(qs, grads, on):
+            q.grad = g.clone() if use else None
+        o.step()
+
+    def same():
+        for a, b in zip(ps, ref):
+            # as in test_graph_capture: the device's pow against the host's, per step
+            assert (a - b).abs().max() <= 10 * (1e-2 * 16 * U + 8 * U * b.abs().max())
+        assert [opt.state[p]["step"].item() for p in ps] == [ropt.state[p]["step"] for p in ref]
+    for on in ((1, 1, 1), (0, 1, 1), (0, 1, 1), (1, 1, 1), (1, 0, 1)):
+        step(opt, ps, on)
+        step(ropt, ref, on)
+        same()
+    for q, g in zip(ps, grads):
+        q.grad = g.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+        step(ropt, ref, (1, 1, 1))
+        torch.cuda.synchronize()
+        same()

@@ -392,3 +392,68 @@ def test_training_layer_mask_needs_the_fused_router(pkg):
     m = pkg.TuckerMoETrain(64, 48, num_experts=4, r2=64, r3=64)
     with pytest.raises(RuntimeError, match="fused_router"):
         m(torch.randn(3, 64), mask=torch.ones(3, dtype=torch.bool))
+
+
+def _counting(pkg, monkeypatch):
+    """The module with a stand-in for its launch, and what that was called with: a list of
+    (parameters' ids, step)."""
+    import mamba_tuckermoe_amd.adamw as ad
+    seen = []
+    monkeypatch.setattr(ad, "_run", lambda *a: seen.append(([id(p) for p in a[0]], int(a[6]))))
+    return ad, seen
+
+
+def _step_of(opt, params, on):
+    for p, o in zip(params, on):
+        p.grad = torch.ones_like(p) if o else None
+    opt.step()
+
+
+@pytest.mark.parametrize("reload", [False, True])
+def test_optimizer_counts_follow_the_parameter(pkg, monkeypatch, reload):
+    """A parameter without a gradient rests: its count and its bias corrections stand still, on
+    the device as on the host, also where it began with others or was loaded with them."""
+    _, seen = _counting(pkg, monkeypatch)
+    pattern = [(1, 1, 0), (0, 1, 0), (1, 1, 1), (1, 0, 1), (1, 0, 0), (0, 1, 1), (1, 1, 1), (1, 1, 1)]
+    runs = []
+    for capturable in (False, True):
+        ps = [torch.nn.Parameter(torch.ones(3)) for _ in range(3)]
+        opt = pkg.FusedAdamW([{"params": ps[:2]}, {"params": ps[2:]}], capturable=capturable)
+        took, got = [0, 0, 0], []
+        for i, on in enumerate(pattern):
+            seen.clear()
+            _step_of(opt, ps, on)
+            took = [a + b for a, b in zip(took, on)]
+            steps = {q: n for ids, n in seen for q in ids}
+            assert steps == {id(p): n for p, n, o in zip(ps, took, on) if o}, (capturable, i)
+            assert [int(opt.state[p]["step"]) if p in opt.state else 0 for p in ps] == took
+            if reload:
+                opt.load_state_dict(opt.state_dict())
+        runs.append(took)
+    assert runs[0] == runs[1]
+
+
+def test_optimizer_refuses_to_part_captured_counts(pkg, monkeypatch):
+    """What a captured step counts together, a step of some of them cannot part; nor can a
+    capture of some of those that stepped together. Nothing changes where it is refused."""
+    ad, seen = _counting(pkg, monkeypatch)
+    ps = [torch.nn.Parameter(torch.ones(3)) for _ in range(2)]
+    opt = pkg.FusedAdamW(ps, capturable=True)
+    _step_of(opt, ps, (1, 1))
+    monkeypatch.setattr(ad, "_capturing", lambda d: True)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        _step_of(opt, ps, (1, 0))
+    _step_of(opt, ps, (1, 1))
+    monkeypatch.setattr(ad, "_capturing", lambda d: False)
+    with pytest.raises(RuntimeError, match="captured together"):
+        _step_of(opt, ps, (0, 1))
+    assert len(seen) == 2 and [int(opt.state[p]["step"]) for p in ps] == [2, 2]
+    _step_of(opt, ps, (1, 1))
+    opt.load_state_dict(opt.state_dict())
+    _step_of(opt, ps, (0, 1))
+    assert [int(opt.state[p]["step"]) for p in ps] == [3, 4]
+    monkeypatch.setattr(ad, "_capturing", lambda d: True)      # parted: each its own
+    _step_of(opt, ps, (0, 1))
+    monkeypatch.setattr(ad, "_capturing", lambda d: False)
+    _step_of(opt, ps, (1, 0))
+    assert [int(opt.state[p]["step"]) for p in ps] == [4, 5]
