@@ -80,12 +80,15 @@ class FusedAdamW(torch.optim.Optimizer):
 
     state_bits 32 keeps float32 moments ("exp_avg", "exp_avg_sq"), 8 keeps codes and scales
     ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales", of
-    sqrt(v)). capturable=True holds the step count on the device, so that a captured step
-    counts on in its replays; without it a step inside a capture raises. Each parameter
-    counts the steps that it took: those that step together share a count until a step that only
-    some of them take, which is refused once a captured step advances that count. Parameters are
-    bfloat16 or float32, dense, on HIP devices, with gradients of their dtype; bfloat16
-    ones are rounded to nearest."""
+    sqrt(v)). Parameters are bfloat16 or float32, dense, on HIP devices, with gradients of
+    their dtype; bfloat16 ones are rounded to nearest.
+
+    capturable=True holds the step counts on the device, so that a captured step counts on in
+    its replays; without it a step inside a capture raises, and so does a parameter's first
+    step, which makes its state. lr and the other numbers are those of the capture in each
+    replay. Each parameter counts the steps that it took: those that step together share a
+    count until a step that only some of them take, which is refused once a captured step
+    advances that count."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, seed: int = 0,
@@ -126,8 +129,9 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         work = [(group, [p for p in group["params"] if p.grad is not None])
                 for group in self.param_groups]
-        for group, ps in work:      # what is refused is refused before anything changes
-            self._check_step(group, ps)
+        # what is refused is refused before anything changes
+        captured = [n for group, ps in work for n in self._check_step(group, ps)]
+        self._captured.update((id(n), n) for n in captured)
         for group, ps in work:
             on_device = group["capturable"]
             fresh = {}      # device: the count that parameters first met in this step share
@@ -151,10 +155,6 @@ class FusedAdamW(torch.optim.Optimizer):
                 run[1].append(p)
                 run[2].append(p.grad)
                 run[3].append(st)
-            if not on_device and any(d.type == "cuda" for d, _, _ in runs) \
-                    and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("FusedAdamW: a step inside a graph capture needs "
-                                   "capturable=True (its count would stand still)")
             counted = set()
             for n, ps, gs, sts in runs.values():
                 if on_device and id(n) not in counted:
@@ -175,21 +175,29 @@ class FusedAdamW(torch.optim.Optimizer):
         return {id(st["step"]): None for st in (self.state.get(p) for p in group["params"] if p.grad is None)
                 if st and id(st["step"]) in mine}
 
-    def _check_step(self, group, ps) -> None:
+    def _check_step(self, group, ps) -> list:
+        """Refuses what a step cannot do; the device counts that it advances in a capture."""
         if any(p.grad.is_sparse for p in ps):
             raise RuntimeError("FusedAdamW: sparse gradients are not supported")
-        if not group["capturable"]:
-            return
-        parted = self._shared_with_resting(group, ps)
         capturing = {d: _capturing(d) for d in {p.device for p in ps}}
+        if not group["capturable"]:
+            if any(capturing.values()):
+                raise RuntimeError("FusedAdamW: a step inside a graph capture needs "
+                                   "capturable=True (its count would stand still)")
+            return []
+        captured = []
+        parted = self._shared_with_resting(group, ps)
         for p in ps:
             st = self.state.get(p)
             if not st:
+                if capturing[p.device]:     # each replay would clear it again
+                    raise RuntimeError("FusedAdamW: a parameter's first step inside a graph capture: make "
+                                       "one step with these gradients before the capture")
                 continue
             n = st["step"]
             if id(n) not in parted:
                 if capturing[p.device]:
-                    self._captured[id(n)] = n
+                    captured.append(n)
             elif capturing[p.device]:
                 raise RuntimeError("FusedAdamW: a captured step of some of the parameters that have stepped "
                                    "together so far: make one step with these gradients before the capture")
@@ -197,6 +205,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 raise RuntimeError("FusedAdamW: parameters whose step was captured together step together "
                                    "(where that graph is gone, opt.load_state_dict(opt.state_dict()) parts "
                                    "them)")
+        return captured
 
     @staticmethod
     def _run(group, step, ps, gs, sts):

@@ -1005,3 +1005,24 @@ def test_capturable_counts_of_resting_parameters(pkg, dev):
         step(ropt, ref, (1, 1, 1))
         torch.cuda.synchronize()
         same()
+
+
+@pytest.mark.parametrize("capturable,bits", [(True, 32), (True, 8), (False, 8)])
+def test_first_step_in_a_capture_is_refused(pkg, dev, capturable, bits):
+    """... and leaves no state; the eager steps after it are those of an optimizer that never
+    saw the capture."""
+    def make():
+        p = torch.nn.Parameter(torch.linspace(-1, 1, 700).to(dev))
+        p.grad = torch.linspace(-0.01, 0.02, 700).to(dev)
+        return p, pkg.FusedAdamW([p], state_bits=bits, capturable=capturable, lr=1e-2)
+    (p, opt), (q, ropt) = make(), make()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="first step" if capturable else "capturable"):
+        with torch.cuda.graph(g):
+            opt.step()
+    torch.cuda.synchronize()
+    assert not opt.state
+    for _ in range(3):
+        opt.step()
+        ropt.step()
+    assert torch.equal(p, q)

@@ -457,3 +457,38 @@ def test_optimizer_refuses_to_part_captured_counts(pkg, monkeypatch):
     monkeypatch.setattr(ad, "_capturing", lambda d: False)
     _step_of(opt, ps, (1, 0))
     assert [int(opt.state[p]["step"]) for p in ps] == [4, 5]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_makes_no_state_in_a_capture(pkg, monkeypatch, bits):
+    """State made inside a capture would be cleared by every replay, or, where the step is
+    refused, never: a first step there is refused and leaves nothing behind, for any group."""
+    ad, seen = _counting(pkg, monkeypatch)
+    for capturable, msg in ((True, "first step"), (False, "capturable")):
+        ps = [torch.nn.Parameter(torch.ones(300)) for _ in range(2)]
+        opt = pkg.FusedAdamW([{"params": ps[:1]}, {"params": ps[1:]}], state_bits=bits, capturable=capturable)
+        monkeypatch.setattr(ad, "_capturing", lambda d: True)
+        with pytest.raises(RuntimeError, match=msg):
+            _step_of(opt, ps, (1, 1))
+        assert not opt.state and not seen
+        monkeypatch.setattr(ad, "_capturing", lambda d: False)
+        _step_of(opt, ps, (1, 0))
+        monkeypatch.setattr(ad, "_capturing", lambda d: True)
+        seen.clear()
+        with pytest.raises(RuntimeError, match=msg):      # the second group's
+            _step_of(opt, ps, (1, 1))
+        assert list(opt.state) == [ps[0]] and not seen and int(opt.state[ps[0]]["step"]) == 1
+        monkeypatch.setattr(ad, "_capturing", lambda d: False)
+        _step_of(opt, ps, (1, 1))
+        assert [int(opt.state[p]["step"]) for p in ps] == [2, 1]
+        seen.clear()
+    # a capture that was refused for one group has captured no other's counts
+    ps = [torch.nn.Parameter(torch.ones(3)) for _ in range(3)]
+    opt = pkg.FusedAdamW([{"params": ps[:2]}, {"params": ps[2:]}], state_bits=bits, capturable=True)
+    _step_of(opt, ps, (1, 1, 0))
+    monkeypatch.setattr(ad, "_capturing", lambda d: True)
+    with pytest.raises(RuntimeError, match="first step"):
+        _step_of(opt, ps, (1, 1, 1))
+    monkeypatch.setattr(ad, "_capturing", lambda d: False)
+    _step_of(opt, ps, (0, 1, 0))
+    assert [int(opt.state[p]["step"]) for p in ps[:2]] == [1, 2]
