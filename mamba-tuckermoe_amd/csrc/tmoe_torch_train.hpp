@@ -9,6 +9,7 @@
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -75,6 +76,12 @@ void check_capture(std::initializer_list<const OptTensor*> ts, const char* who) 
                 ": a graph that was made outside this capture, on another stream, still holds one of "
                 "these leaves; delete its outputs before the capture");
   }
+}
+
+// The kernels carry no tangents: an operand that has one would lose it without a word.
+void check_tangent(const at::Tensor& t, const char* who) {
+  TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), who,
+              " has no forward-mode derivative");
 }
 
 // The rows (..., d) of t at one stride; a contiguous copy where they have none.
@@ -225,11 +232,13 @@ PyObject* router(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 ": temperature: a number, or a float32 tensor of one value that needs no gradient");
     TORCH_CHECK(t.device() == raw.device(), kRouter, ": temperature on ", t.device(), ", logits on ",
                 raw.device());
+    check_tangent(t, kRouter);
     c.tau_dev = t;
   } else {
     TORCH_CHECK(c.tau > 0 && std::isfinite((float)c.tau), kRouter, ": temperature ", c.tau);
   }
   TORCH_CHECK(c.cap > 0 && std::isfinite((float)c.cap), kRouter, ": scale ", c.cap);
+  check_tangent(raw, kRouter);
   check_hip(raw, kRouter);
   variable_list o;
   {
@@ -400,6 +409,8 @@ PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK((*t)->device() == y->device(), kNorm, ": tensors on ", (*t)->device(), " and ",
                 y->device());
   }
+  for (const OptTensor* t : std::initializer_list<const OptTensor*>{&x, &y, &gate, &post, &gamma, &next})
+    if (*t) check_tangent(**t, kNorm);
   check_hip(*y, kNorm);
   at::Tensor r, h;
   {
@@ -521,6 +532,8 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     TORCH_CHECK(q.device() == dev && g[i].device() == dev && m[i].device() == dev &&
                     v[i].device() == dev,
                 kAdamw, ": tensor ", i, ": not all on ", dev);
+    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&q, &g[i], &m[i], &v[i]})
+      check_tangent(*t, kAdamw);
     writes(q);
     writes(m[i]);
     writes(v[i]);

@@ -8,7 +8,7 @@ fused_block_norm  the norms before and after a block with the block's gate and t
 They take bfloat16 or float32 tensors on a HIP device (no fallback), compute in float32 and
 round each output once. Both run on the current stream, allocate with torch's allocator and
 wait for nothing, so that they can be captured into a HIP graph; a gradient of their
-gradients is refused.
+gradients is refused, and so is a forward-mode derivative.
 """
 from __future__ import annotations
 

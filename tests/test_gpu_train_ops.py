@@ -1026,3 +1026,21 @@ def test_first_step_in_a_capture_is_refused(pkg, dev, capturable, bits):
         opt.step()
         ropt.step()
     assert torch.equal(p, q)
+
+
+def test_forward_mode_is_refused_on_the_device(pkg, dev):
+    """With and without reverse gradients wanted; in the layer too."""
+    import torch.autograd.forward_ad as fw
+    x = torch.randn(40, 64, device=dev)
+    w = torch.ones(64, device=dev)
+    layer = pkg.TuckerMoETrain(64, 48, num_experts=8, r2=64, r3=64, fused_router=True).to(dev)
+    for grad in (False, True):
+        w.requires_grad_(grad)
+        layer.requires_grad_(grad)
+        with fw.dual_level():
+            t = fw.make_dual(x, torch.ones_like(x))
+            for call in (lambda: pkg.fused_router(t[:, :8], 2, 0.5), lambda: pkg.fused_block_norm(y=t, post_weight=w),
+                         lambda: pkg.fused_block_norm(x, t, gamma=w), lambda: layer(t)):
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call()
+        assert pkg.fused_block_norm(y=x, post_weight=w)[0].isfinite().all()

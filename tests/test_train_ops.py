@@ -492,3 +492,26 @@ def test_optimizer_makes_no_state_in_a_capture(pkg, monkeypatch, bits):
     monkeypatch.setattr(ad, "_capturing", lambda d: False)
     _step_of(opt, ps, (0, 1, 0))
     assert [int(opt.state[p]["step"]) for p in ps[:2]] == [1, 2]
+
+
+def test_forward_mode_is_refused(pkg):
+    """An operand with a tangent: the outputs would have none, a derivative of zero."""
+    import torch.autograd.forward_ad as fw
+    x, w, ones = torch.randn(4, 8), torch.ones(8), lambda: torch.ones(4, 8)
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t, torch.ones_like(t))
+        norm = dict(x=x, y=x, gate=x, post_weight=w, gamma=w, next_weight=w)
+        calls = [lambda: pkg.fused_router(dual(x), 2, 0.5), lambda: pkg.fused_block_norm(dual(x), next_weight=w),
+                 lambda: pkg.adamw_step([dual(ones())], [ones()], [ones()], [ones()], step=1, lr=1.0),
+                 lambda: pkg.adamw_step([ones()], [dual(ones())], [ones()], [ones()], step=1, lr=1.0)]
+        calls += [lambda k=k: pkg.fused_block_norm(**{**norm, k: dual(norm[k])}) for k in norm]
+        for f in calls:
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                f()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                f()
+        with torch.inference_mode(), pytest.raises(RuntimeError, match="HIP devices only"):
+            pkg.fused_router(dual(x), 2, 0.5)       # where no tangent is asked for
+    with pytest.raises(RuntimeError, match="HIP devices only"):
+        pkg.fused_router(x, 2, 0.5)
