@@ -50,7 +50,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                weight_decay: float = 1e-2) -> None:
     """One step on lists of tensors of one dtype on one device, in place. The moments are
     float32, laid out as their parameters. step counts from 1: a number, or an int64 tensor
-    of one value on the device, which is read when the kernels run."""
+    of one value on the device, which is read when the kernels run. What is written may share
+    no memory, nor may a gradient lie in what is written of another element."""
     _run(params, grads, exp_avgs, exp_avg_sqs, None, None, step, lr, betas, eps, weight_decay, 0)
 
 

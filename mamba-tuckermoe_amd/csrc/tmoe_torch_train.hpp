@@ -493,12 +493,14 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     TORCH_CHECK(s.step >= 1, kAdamw, ": step ", s.step, " (the first is 1)");
   }
   struct Span { uintptr_t at, end; };
-  std::vector<Span> written;
+  std::vector<Span> written, read;
   written.reserve(5 * n);
-  auto writes = [&](const at::Tensor& t) {
+  read.reserve(n);
+  auto span = [](const at::Tensor& t, std::vector<Span>& list) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-    if (t.numel()) written.push_back({at, at + (uintptr_t)t.numel() * t.element_size()});
+    if (t.numel()) list.push_back({at, at + (uintptr_t)t.numel() * t.element_size()});
   };
+  auto writes = [&](const at::Tensor& t) { span(t, written); };
   for (size_t i = 0; i < n; ++i) {
     const at::Tensor& q = p[i];
     TORCH_CHECK(q.scalar_type() == dt && g[i].scalar_type() == dt, kAdamw, ": tensor ", i,
@@ -541,11 +543,23 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       writes(ms[i]);
       writes(vs[i]);
     }
+    // a gradient that the kernels read where it lies (one in another order is copied first);
+    // the very elements that its own thread writes it may be
+    const auto in_place = [&](const at::Tensor& t) {
+      return t.const_data_ptr() == g[i].const_data_ptr() && t.element_size() == g[i].element_size();
+    };
+    if (g[i].strides() == q.strides() && !in_place(q) && !in_place(m[i]) && !in_place(v[i])) span(g[i], read);
   }
   std::sort(written.begin(), written.end(), [](Span x, Span y) { return x.at < y.at; });
   for (size_t i = 1; i < written.size(); ++i)
     TORCH_CHECK(written[i - 1].end <= written[i].at, kAdamw,
                 ": two of the parameters and states share memory");
+  for (const Span& r : read) {      // the last written one that begins before r ends
+    const auto w = std::lower_bound(written.begin(), written.end(), r.end,
+                                    [](const Span& x, uintptr_t end) { return x.at < end; });
+    TORCH_CHECK(w == written.begin() || (w - 1)->end <= r.at, kAdamw,
+                ": a gradient shares memory with another element's parameter or state");
+  }
   check_hip(p[0], kAdamw);
   {
     pybind11::gil_scoped_release nogil;

@@ -515,3 +515,34 @@ def test_forward_mode_is_refused(pkg):
             pkg.fused_router(dual(x), 2, 0.5)       # where no tangent is asked for
     with pytest.raises(RuntimeError, match="HIP devices only"):
         pkg.fused_router(x, 2, 0.5)
+
+
+def test_adamw_gradients_that_overlap_what_is_written(pkg):
+    """A gradient in the memory of a parameter or a state at another offset would be read after
+    it is written, or before; the very elements that are written are fine, and so is a
+    gradient in another order, which is copied first."""
+    def step(p, g, m, v, msg):
+        with pytest.raises(RuntimeError, match=msg):
+            pkg.adamw_step(p, g, m, v, step=1, lr=1e-3)
+
+    def z(n=32):
+        return torch.zeros(n)
+    a = z(128)
+    for o, bad in ((1, True), (31, True), (-1, True), (32, False), (-32, False), (0, False)):
+        g = a[48 + o:80 + o]
+        msg = "a gradient shares memory" if bad else "HIP devices only"
+        step([a[48:80]], [g], [z()], [z()], msg)
+        step([z()], [g], [a[48:80]], [z()], msg)
+        step([z()], [g], [z()], [a[48:80]], msg)
+        step([z(), a[48:80], z()], [z(), z(), g], [z(), z(), z()], [z(), z(), z()],
+             "a gradient shares memory" if bad or o == 0 else "HIP devices only")
+    sq = z(64).view(8, 8)
+    step([sq], [sq.t()], [z(64).view(8, 8)], [z(64).view(8, 8)], "HIP devices only")
+    g = z()
+    step([z(), z()], [g, g], [z(), z()], [z(), z()], "HIP devices only")     # one that two share
+    codes, sc = torch.zeros(64, dtype=torch.uint8), z(1)
+    for g in (codes.view(torch.float32)[1:9], codes.view(torch.float32)[:8]):
+        with pytest.raises(RuntimeError, match="a gradient shares memory"):
+            pkg.adamw_step_8bit([z(8)], [g], [codes[:8]], [sc], [codes[8:16]], [z(1)], step=1, lr=1e-3)
+    with pytest.raises(RuntimeError, match="a gradient shares memory"):
+        pkg.adamw_step_8bit([z(1)], [sc], [codes[:1]], [sc], [codes[8:9]], [z(1)], step=1, lr=1e-3)
