@@ -219,18 +219,32 @@ class FusedAdamW(torch.optim.Optimizer):
              group["eps"], group["weight_decay"], group["seed"])
 
     def load_state_dict(self, state_dict) -> None:
-        """As torch.optim's, but each state keeps the dtype that it was saved in (torch casts
-        them to their parameter's)."""
-        super().load_state_dict(state_dict)
-        saved = state_dict["state"]
-        for mine, its in zip(self.param_groups, state_dict["param_groups"]):
+        """As torch.optim's, but 8-bit states keep their dtypes and 32-bit moments are float32
+        in their parameter's layout (torch casts states to their parameter's dtype). A
+        torch.optim.AdamW's state is taken as 32-bit moments; what it lacks of this class's
+        options stays as it is here. States of other kinds, and amsgrad's, maximize's or an L2
+        decay's, are refused."""
+        saved, groups = state_dict["state"], state_dict["param_groups"]
+        if len(groups) == len(self.param_groups):       # (torch refuses it otherwise)
+            groups = [{**{k: mine[k] for k in self.defaults if k in mine}, **its}
+                      for mine, its in zip(self.param_groups, groups)]
+            for mine, its in zip(self.param_groups, groups):
+                self._check_load(mine, its, saved)
+        super().load_state_dict({**state_dict, "param_groups": groups})
+        for mine, its in zip(self.param_groups, groups):
             counts = {}
             for p, i in zip(mine["params"], its["params"]):
                 if i not in saved:
                     continue
-                st = self.state[p] = {
-                    k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
-                    for k, v in saved[i].items()}
+                st = self.state[p] = {}
+                for k, v in saved[i].items():
+                    if k in ("exp_avg", "exp_avg_sq"):
+                        st[k] = torch.empty_like(p, dtype=torch.float32, requires_grad=False,
+                                                 memory_format=torch.preserve_format).copy_(v.detach())
+                    elif isinstance(v, torch.Tensor):
+                        st[k] = v.detach().to(p.device, copy=True)
+                    else:
+                        st[k] = v
                 n = int(st["step"])
                 if mine["capturable"]:
                     if (p.device, n) not in counts:
@@ -238,3 +252,25 @@ class FusedAdamW(torch.optim.Optimizer):
                     st["step"] = counts[p.device, n]
                 else:
                     st["step"] = n
+
+    @staticmethod
+    def _check_load(mine, its, saved) -> None:
+        for k in ("amsgrad", "maximize"):
+            if its.get(k):
+                raise ValueError(f"FusedAdamW: a state of an optimizer with {k}")
+        if its["weight_decay"] and not its.get("decoupled_weight_decay", True):
+            raise ValueError("FusedAdamW: a state of an optimizer with an L2 decay")
+        eight = its["state_bits"] == 8
+        needed = {"step"} | {m + s for m in ("exp_avg", "exp_avg_sq")
+                             for s in (("_codes", "_scales") if eight else ("",))}
+        for p, i in zip(mine["params"], its["params"]):
+            st = saved.get(i)
+            if not st:
+                continue
+            if not needed <= set(st):
+                raise ValueError(f"FusedAdamW: a state of {sorted(st)} for state_bits {its['state_bits']}")
+            for k in needed - {"step"}:
+                want = p.shape if not eight else \
+                    (p.numel() if k.endswith("_codes") else -(-p.numel() // BLOCK),)
+                if st[k].shape != want:
+                    raise ValueError(f"FusedAdamW: {k} {tuple(st[k].shape)} for a parameter {tuple(p.shape)}")

@@ -1044,3 +1044,26 @@ def test_forward_mode_is_refused_on_the_device(pkg, dev):
                 with pytest.raises(RuntimeError, match="no forward-mode derivative"):
                     call()
         assert pkg.fused_block_norm(y=x, post_weight=w)[0].isfinite().all()
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_optimizer_goes_on_from_torchs(pkg, dev, capturable):
+    """torch's AdamW for three steps, FusedAdamW from its state for three more: as torch's for
+    six, in float64."""
+    torch.manual_seed(5)
+    ps = [torch.nn.Parameter(torch.randn(s, device=dev) * 0.05) for s in ((70, 40), (300,))]
+    ref = [torch.nn.Parameter(p.detach().double()) for p in ps]
+    topt, ropt = torch.optim.AdamW(ps, **HYPER), torch.optim.AdamW(ref, **HYPER)
+    opt = pkg.FusedAdamW(ps, capturable=capturable)
+    for step in range(6):
+        for p, r in zip(ps, ref):
+            p.grad = torch.randn(p.shape, device=dev) * 0.01
+            r.grad = p.grad.double()
+        if step == 3:
+            sd = topt.state_dict()
+            sd["param_groups"][0]["capturable"] = capturable
+            opt.load_state_dict(sd)
+        (topt if step < 3 else opt).step()
+        ropt.step()
+    for p, r in zip(ps, ref):      # six steps of 32 roundings of p and of updates of lr
+        assert (p.double() - r).abs().max() <= 6 * 32 * U * (r.abs().max() + 10 * HYPER["lr"])

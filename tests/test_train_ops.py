@@ -546,3 +546,61 @@ def test_adamw_gradients_that_overlap_what_is_written(pkg):
             pkg.adamw_step_8bit([z(8)], [g], [codes[:8]], [sc], [codes[8:16]], [z(1)], step=1, lr=1e-3)
     with pytest.raises(RuntimeError, match="a gradient shares memory"):
         pkg.adamw_step_8bit([z(1)], [sc], [codes[:1]], [sc], [codes[8:9]], [z(1)], step=1, lr=1e-3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_optimizer_takes_up_torchs_adamw(pkg, monkeypatch, capturable, dtype):
+    """A torch.optim.AdamW's state: its moments in float32 and the parameter's layout, its counts
+    and its numbers; the next step is the one after its last."""
+    _, seen = _counting(pkg, monkeypatch)
+    torch.manual_seed(2)
+    ps = [torch.nn.Parameter(torch.randn(5, 7).to(dtype)), torch.nn.Parameter(torch.randn(3).to(dtype))]
+    topt = torch.optim.AdamW([{"params": ps[:1], "lr": 0.5}, {"params": ps[1:]}], lr=2e-3, weight_decay=0.3,
+                             capturable=False)
+    for on in ((1, 1), (1, 0), (1, 1)):
+        for p, o in zip(ps, on):
+            p.grad = torch.randn_like(p) if o else None
+        topt.step()
+    qs = [torch.nn.Parameter(torch.zeros(7, 5, dtype=dtype).t()), torch.nn.Parameter(torch.zeros(3, dtype=dtype))]
+    opt = pkg.FusedAdamW([{"params": qs[:1]}, {"params": qs[1:]}], seed=9, capturable=capturable)
+    sd = topt.state_dict()
+    for g in sd["param_groups"]:
+        g["capturable"] = capturable
+    opt.load_state_dict(sd)
+    assert [(g["lr"], g["weight_decay"], g["state_bits"], g["seed"], g["capturable"]) for g in opt.param_groups] == [
+        (0.5, 0.3, 32, 9, capturable), (2e-3, 0.3, 32, 9, capturable)]
+    for p, q in zip(ps, qs):
+        for k in ("exp_avg", "exp_avg_sq"):
+            t = opt.state[q][k]
+            assert t.dtype == torch.float32 and t.stride() == q.stride() and not t.requires_grad
+            assert torch.equal(t, topt.state[p][k].float())
+        q.grad = torch.ones_like(q)
+    opt.step()
+    assert [(ids, n) for ids, n in seen] == [([id(qs[0])], 4), ([id(qs[1])], 3)]
+    assert [int(opt.state[q]["step"]) for q in qs] == [4, 3]
+
+
+def test_optimizer_refuses_other_states(pkg):
+    """... at the load, which changes nothing."""
+    def saved(cls, **kw):
+        p = torch.nn.Parameter(torch.ones(300))
+        p.grad = torch.ones_like(p)
+        opt = cls([p], **kw)
+        opt.step()
+        return opt.state_dict()
+    adamw = torch.optim.AdamW
+    short = saved(adamw)
+    short["state"][0]["exp_avg"] = torch.ones(1)
+    for bits, sd, msg in ((8, saved(adamw), "state_bits 8"), (32, saved(torch.optim.SGD, lr=0.1, momentum=0.9), "state_bits 32"),
+                          (32, saved(adamw, amsgrad=True), "amsgrad"), (32, saved(adamw, maximize=True), "maximize"),
+                          (32, short, "exp_avg"),
+                          (32, saved(torch.optim.Adam, weight_decay=0.1), "L2")):
+        p = torch.nn.Parameter(torch.ones(300))
+        opt = pkg.FusedAdamW([p], lr=0.125, state_bits=bits)
+        with pytest.raises(ValueError, match=msg):
+            opt.load_state_dict(sd)
+        assert not opt.state and opt.param_groups[0]["lr"] == 0.125 and opt.param_groups[0]["state_bits"] == bits
+    two = [torch.nn.Parameter(torch.ones(3)) for _ in range(2)]
+    with pytest.raises(ValueError):
+        pkg.FusedAdamW([{"params": two[:1]}, {"params": two[1:]}]).load_state_dict(saved(adamw))
