@@ -165,10 +165,17 @@ __device__ __forceinline__ float quotient(float a, float b, float y) {
   return fmaf(fmaf(-q, b, a), y, q);
 }
 
-// sqrt(v) to the last place but for one value in millions (and for v below 2^-126)
+// sqrt(v) to the last place but for one value in millions; v is 0 or at least 2^-126 (the
+// hardware's root takes less for 0), infinite or NaN
 __device__ __forceinline__ float root_of(float v) {
   const float y = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-126f)), s = v * y;
-  return v != v ? v : fmaf(fmaf(-s, s, v), 0.5f * y, s);
+  return v < INFINITY ? fmaf(fmaf(-s, s, v), 0.5f * y, s) : v;
+}
+__device__ __forceinline__ bool subnormal(float v) { return __builtin_amdgcn_classf(v, 0x80); }
+// of any v: a subnormal one's from 2^64 of it
+__device__ __forceinline__ float root_of_any(float v) {
+  const bool sub = subnormal(v);
+  return root_of(sub ? v * 0x1p64f : v) * (sub ? 0x1p-32f : 1.f);
 }
 
 // A magnitude a in [0, 448] as the e4m3 value below it and what is left over: `code`, and in
@@ -294,15 +301,26 @@ __global__ __launch_bounds__(kAdamwThreads) void k_adamw8(const AdamwTable a) {
       m[j] = m01[0], m[j + 1] = m01[1], m[j + 2] = m23[0], m[j + 3] = m23[1];
       r[j] = r01[0], r[j + 1] = r01[1], r[j + 2] = r23[0], r[j + 3] = r23[1];
     }
-    // magnitudes as integers: in their order, a NaN above all
-    uint32_t am = 0u, ar = 0u;
+    bool sub = false;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       m[j] *= sm;
       r[j] *= sr;
-      float v = r[j] * r[j];
-      adamw_moments(s, gv[j], m[j], v);
-      r[j] = root_of(v);
+      r[j] *= r[j];
+      adamw_moments(s, gv[j], m[j], r[j]);
+      sub |= subnormal(r[j]);
+    }
+    if (__any(sub)) {       // their roots are as large as 2^-63: with an eps of 0 they count
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) r[j] = root_of_any(r[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) r[j] = root_of(r[j]);
+    }
+    // magnitudes as integers: in their order, a NaN above all
+    uint32_t am = 0u, ar = 0u;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
       pv[j] = fmaf(m[j] * -s.rate, __builtin_amdgcn_rcpf(fmaf(r[j], s.inv_c2, s.eps)), pv[j] * s.keep);
       am = max(am, __float_as_uint(m[j]) & 0x7fffffffu);
       ar = max(ar, __float_as_uint(r[j]) & 0x7fffffffu);

@@ -1067,3 +1067,54 @@ def test_optimizer_goes_on_from_torchs(pkg, dev, capturable):
         ropt.step()
     for p, r in zip(ps, ref):      # six steps of 32 roundings of p and of updates of lr
         assert (p.double() - r).abs().max() <= 6 * 32 * U * (r.abs().max() + 10 * HYPER["lr"])
+
+
+@dtypes
+def test_adamw_8_roots_of_subnormals(pkg, dev, dtype):
+    """Gradients whose second moment is under 2^-126, with eps = 0: the step is lr in the first
+    step and the formula's in the next, and the scales are the roots'. v, in steps of 2^-149, is
+    off by half a one of each of r r (by 0.97), its product with 0.97, g g (by 0.03) and its
+    product: 1.5 (the sum is exact), and its root r by that over 2 r^2 of itself."""
+    g = torch.Generator().manual_seed(3)
+    n, hyper = 1500, dict(lr=2e-3, betas=(0.9, 0.97), eps=0.0, weight_decay=0.0)
+    mag = torch.exp(torch.empty(n).uniform_(np.log(2e-20), np.log(4e-18), generator=g))
+    mag[256:512] *= 1e3                                       # a block of ordinary ones
+    mag[700] = 1.0                                            # a block with one large element
+    grad = (mag * torch.where(torch.rand(n, generator=g) < 0.5, -1.0, 1.0)).to(dtype)
+    p = [(torch.randn(n, generator=g) * 0.05).to(dtype).to(dev)]
+    q8 = lambda: [torch.zeros(n, dtype=torch.uint8, device=dev)]
+    sc = lambda: [torch.zeros(-(-n // 256), device=dev)]
+    mq, ms, rq, rs = q8(), sc(), q8(), sc()
+    for step in (1, 2):
+        old = [tn.decode8(c[0].cpu().numpy(), f64(s[0])) for c, s in ((mq, ms), (rq, rs))]
+        o = tn.adamw(f64(p[0]), f64(grad), old[0], old[1] ** 2, step, 2e-3, 0.9, 0.97, 0.0, 0.0)
+        pkg.adamw_step_8bit(p, [grad.to(dev)], mq, ms, rq, rs, step=step, seed=4, **hyper)
+        v = o["v"]
+        off = 1.5 * 2.0 ** -149 / (2 * v)                         # of the root, relative
+        upd = np.abs(o["p_mag"]) * 40 * U + 2e-3 / (1 - 0.9 ** step) * np.abs(o["m"]) / np.sqrt(v) * off * 1.1
+        tol = upd + (2.0 ** -8 * (np.abs(o["p"]) + upd) if dtype == torch.bfloat16 else 0)
+        assert (np.abs(f64(p[0]) - o["p"]) <= tol).all(), step
+        root = np.pad(np.sqrt(v), (0, -n % 256)).reshape(-1, 256)
+        at = np.pad(off, (0, -n % 256)).reshape(-1, 256)[np.arange(root.shape[0]), root.argmax(1)]
+        want = root.max(1) / 448
+        assert (np.abs(f64(rs[0]) - want) <= want * (12 * U + 1.1 * at)).all(), step
+
+
+def test_adamw_8_square_that_overflows(pkg, dev):
+    """A finite gradient whose square is not: v is infinite and the element's step zero, as with
+    32-bit states; its block's second scale is not finite from then on."""
+    out = []
+    for bits in (32, 8):
+        p, g, mq, ms, rq, rs = _inputs8(dev, torch.float32, 2, [(700,)])
+        m, v = ([torch.zeros(700, device=dev)] for _ in range(2))
+        for t in mq + rq:
+            t.view(torch.uint8).zero_()
+        g[0][300] = 3e25
+        g[0][:256] *= 1e15
+        if bits == 32:
+            pkg.adamw_step(p, g, m, v, step=1, **HYPER)
+        else:
+            pkg.adamw_step_8bit(p, g, mq, ms, rq, rs, step=1, **HYPER)
+        out.append(p[0])
+    assert out[1].isfinite().all() and not rs[0][1].isfinite() and rs[0][[0, 2]].isfinite().all()
+    assert (out[0] - out[1]).abs().max() <= 40 * U * (out[0].abs().max() + 10 * HYPER["lr"])
