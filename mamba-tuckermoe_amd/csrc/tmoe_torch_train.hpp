@@ -13,6 +13,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 
@@ -78,10 +79,14 @@ void check_capture(std::initializer_list<const OptTensor*> ts, const char* who) 
   }
 }
 
-// The kernels carry no tangents: an operand that has one would lose it without a word.
+// The kernels carry no tangents: an operand that has one would lose it without a word. Only
+// inside a level of forward-mode derivatives does a tensor have one.
+bool tangents_live() {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+         torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
+}
 void check_tangent(const at::Tensor& t, const char* who) {
-  TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), who,
-              " has no forward-mode derivative");
+  TORCH_CHECK(!t._fw_grad(0).defined(), who, " has no forward-mode derivative");
 }
 
 // The rows (..., d) of t at one stride; a contiguous copy where they have none.
@@ -232,13 +237,15 @@ PyObject* router(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 ": temperature: a number, or a float32 tensor of one value that needs no gradient");
     TORCH_CHECK(t.device() == raw.device(), kRouter, ": temperature on ", t.device(), ", logits on ",
                 raw.device());
-    check_tangent(t, kRouter);
     c.tau_dev = t;
   } else {
     TORCH_CHECK(c.tau > 0 && std::isfinite((float)c.tau), kRouter, ": temperature ", c.tau);
   }
   TORCH_CHECK(c.cap > 0 && std::isfinite((float)c.cap), kRouter, ": scale ", c.cap);
-  check_tangent(raw, kRouter);
+  if (tangents_live()) {
+    check_tangent(raw, kRouter);
+    if (c.tau_dev) check_tangent(*c.tau_dev, kRouter);
+  }
   check_hip(raw, kRouter);
   variable_list o;
   {
@@ -409,8 +416,9 @@ PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK((*t)->device() == y->device(), kNorm, ": tensors on ", (*t)->device(), " and ",
                 y->device());
   }
-  for (const OptTensor* t : std::initializer_list<const OptTensor*>{&x, &y, &gate, &post, &gamma, &next})
-    if (*t) check_tangent(**t, kNorm);
+  if (tangents_live())
+    for (const OptTensor* t : std::initializer_list<const OptTensor*>{&x, &y, &gate, &post, &gamma, &next})
+      if (*t) check_tangent(**t, kNorm);
   check_hip(*y, kNorm);
   at::Tensor r, h;
   {
@@ -500,7 +508,7 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
     if (t.numel()) list.push_back({at, at + (uintptr_t)t.numel() * t.element_size()});
   };
-  auto writes = [&](const at::Tensor& t) { span(t, written); };
+  const bool tangents = tangents_live();
   for (size_t i = 0; i < n; ++i) {
     const at::Tensor& q = p[i];
     TORCH_CHECK(q.scalar_type() == dt && g[i].scalar_type() == dt, kAdamw, ": tensor ", i,
@@ -534,21 +542,25 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     TORCH_CHECK(q.device() == dev && g[i].device() == dev && m[i].device() == dev &&
                     v[i].device() == dev,
                 kAdamw, ": tensor ", i, ": not all on ", dev);
-    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&q, &g[i], &m[i], &v[i]})
-      check_tangent(*t, kAdamw);
-    writes(q);
-    writes(m[i]);
-    writes(v[i]);
-    if (q8) {
-      writes(ms[i]);
-      writes(vs[i]);
-    }
+    if (tangents)
+      for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&q, &g[i], &m[i], &v[i]})
+        check_tangent(*t, kAdamw);
+    const size_t first = written.size();
+    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&q, &m[i], &v[i]}) span(*t, written);
     // a gradient that the kernels read where it lies (one in another order is copied first);
     // the very elements that its own thread writes it may be
-    const auto in_place = [&](const at::Tensor& t) {
-      return t.const_data_ptr() == g[i].const_data_ptr() && t.element_size() == g[i].element_size();
-    };
-    if (g[i].strides() == q.strides() && !in_place(q) && !in_place(m[i]) && !in_place(v[i])) span(g[i], read);
+    if (g[i].strides() == q.strides()) {
+      span(g[i], read);
+      for (size_t j = first; j < written.size(); ++j)
+        if (written[j].at == read.back().at && written[j].end == read.back().end) {
+          read.pop_back();
+          break;
+        }
+    }
+    if (q8) {
+      span(ms[i], written);
+      span(vs[i], written);
+    }
   }
   std::sort(written.begin(), written.end(), [](Span x, Span y) { return x.at < y.at; });
   for (size_t i = 1; i < written.size(); ++i)
