@@ -6,10 +6,15 @@
 //   lb = E sum_e (n_e / N) (sum_b P_be / N),  z = sum_b lse(a_b)^2 / N
 // over the N tokens that no mask leaves out, n_e of which select e. A masked token has
 // idx -1 (which selects nothing in the contraction), w 0 and no gradient.
-//   g_e  = dlb E n_e / N^2 + [e = idx_j] (dw_j - sum_i dw_i w_i) / s
-//   draw = (1 - tanh^2) ((P_e (g_e - sum_f P_f g_f)) / tau + dz 2 lse softmax(a)_e / N)
-// where both differences are taken from the likeliest expert's (dw_0, g_0): with its
-// P near 1 the sums are next to those, and the differences what is left of two equals.
+//   G_e  = dlb E n_e / N^2,  A_e = [e = idx_j] (dw_j - sum_i dw_i w_i) / s
+//   draw = (1 - tanh^2) (P_e (G_e + A_e - sum_f P_f (G_f + A_f)) / tau + dz 2 lse softmax(a)_e / N)
+// where differences of G and dw are taken from the likeliest expert's (G_0, dw_0): with its P
+// near 1 the sums are next to those, and the differences what is left of two equals. The mean
+// of A is 1e-6 / s sum_i dw_i w_i, since the weights lack 1e-6 / s of one. So with
+// D = sum_i w_i (dw_i - dw_0), S and U the selected and the other P's sums, no sum is taken
+// from one that may be next to it:
+//   A_e - mean = ((dw_j - dw_0) - D + 1e-6 (dw_0 U / s - D)) / s where selected, else
+//                -1e-6 (dw_0 S / s + D) / s
 //
 // With Q = exp(-2 raw / c) and R = 1 / (1 + Q), tanh = 1 - 2 Q R, 1 - tanh^2 = 4 Q R^2 and
 //   a_e - a_m = 2 c R_m R_e (Q_m - Q_e)
@@ -462,35 +467,37 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_bwd(RouterArgs a) {
       const Capped m = capped_top(top, sc.c1);
       const float k_p = m.R * sc.k_p, k_z = m.R * sc.k_z;
       Capped t[V];
-      float ep[V], ez[V], sp = 0.f, sz = 0.f, su = 0.f, sd = 0.f, sg = 0.f;
+      float ep[V], ez[V], ss = 0.f, sz = 0.f, su = 0.f, sd = 0.f, sg = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         t[j] = capped(v[j], sc.c1);
         const float d = e0 + j < E ? (m.Q - t[j].Q) * t[j].R : -INFINITY;
         ep[j] = __builtin_amdgcn_exp2f(d * k_p);
         ez[j] = __builtin_amdgcn_exp2f(d * k_z);
-        sp += ep[j];
         sz += ez[j];
+        ss += off[j] == 0.f ? ep[j] : 0.f;
         su = fmaf(ep[j], off[j], su);
         sd = fmaf(ep[j], dw[j], sd);
         sg = fmaf(ep[j], g0[j] - g_top, sg);
       }
-      sp = lanes_sum<L>(sp);
+      // selected and not, each by itself: either may be a hundredth of the other
+      ss = lanes_sum<L>(ss);
       sz = lanes_sum<L>(sz);
       su = lanes_sum<L>(su);
       sd = lanes_sum<L>(sd);
       sg = lanes_sum<L>(sg);
-      const float inv_sp = __builtin_amdgcn_rcpf(sp);
-      const float inv_s = __builtin_amdgcn_rcpf((sp - su) * inv_sp + 1e-6f);
-      // the top's own part of g beside the balance loss's: dw_0 - sum_i dw_i w_i, over s
-      const float gs = (d_top * 1e-6f * inv_s - sd * inv_sp * inv_s) * inv_s;
-      const float pg = (sg + sd * inv_s - su * gs) * inv_sp;       // sum_e P_e (g_e - g_0)
+      const float inv_sp = __builtin_amdgcn_rcpf(ss + su);
+      const float inv_s = __builtin_amdgcn_rcpf(fmaf(ss, inv_sp, 1e-6f));
+      const float D = sd * inv_sp * inv_s;                         // sum_i w_i (dw_i - dw_0)
+      const float pg = sg * inv_sp;                                // sum_e P_e (G_e - G_0)
+      const float a_on = fmaf(1e-6f, fmaf(d_top, su * inv_sp * inv_s, -D), -D) * inv_s - pg;
+      const float a_off = -1e-6f * fmaf(d_top, ss * inv_sp * inv_s, D) * inv_s - pg;
       const float c_p = 4.f * inv_sp * inv_tau;
       const float c_z = 4.f * cz * (capped_value(top, sc.c1, a.cap) + __logf(sz)) * __builtin_amdgcn_rcpf(sz);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float g = fmaf(off[j], -gs, fmaf(dw[j], inv_s, g0[j] - g_top));
-        o[j] = fmaf(c_z, ez[j], ep[j] * c_p * (g - pg)) * (t[j].Q * t[j].R * t[j].R);
+        const float g = fmaf(dw[j], inv_s, off[j] == 0.f ? a_on : a_off) + (g0[j] - g_top);
+        o[j] = fmaf(c_z, ez[j], ep[j] * c_p * g) * (t[j].Q * t[j].R * t[j].R);
       }
     }
     T* row = draw + b * E;

@@ -1118,3 +1118,23 @@ def test_adamw_8_square_that_overflows(pkg, dev):
         out.append(p[0])
     assert out[1].isfinite().all() and not rs[0][1].isfinite() and rs[0][[0, 2]].isfinite().all()
     assert (out[0] - out[1]).abs().max() <= 40 * U * (out[0].abs().max() + 10 * HYPER["lr"])
+
+
+@pytest.mark.parametrize("E,k", [(64, 1), (200, 2), (256, 1), (256, 2), (256, 16)])
+def test_router_gradient_of_nearly_flat_logits(pkg, dev, E, k):
+    """Many experts with hardly any difference, few of them selected: the weights' gradient has
+    the selected probabilities' sum twice in its denominator, which is a hundredth of all.
+
+    Steps of 2^-24, of a term, at most: an exponential 5 (its argument 2: a difference of two
+    exponentials near 1, 3 each, times cap / (2 tau) = 1/4; itself 3). A sum of them 13 more
+    (8 in a lane, 5 exchanges); 1 / sum over all 5 + 13 + 1 + 2 = 21; 1 / s 18 + 21 + 1 + 2 = 42.
+    sum_i w_i (dw_i - dw_0): 18 + 2, the two and 2 products, 85; the term that has it times
+    1 / s 128; with its exponential 5, 1 / (sum tau) 24, Q R^2 9 and 4 more roundings 170."""
+    g = torch.Generator().manual_seed(E + k)
+    B = 400
+    raw = (torch.randn(B, E, generator=g) * 0.03).to(dev).requires_grad_()
+    dw = torch.randn(B, k, generator=g).to(dev)
+    r = pkg.fused_router(raw, k, 2.0, 1.0)
+    draw, = torch.autograd.grad(r.weights, raw, dw)
+    o = tn.router(f64(raw), k, 2.0, 1.0, None, f64(dw))
+    near(draw, o["draw"], o["draw_mag"], 170, "draw")
