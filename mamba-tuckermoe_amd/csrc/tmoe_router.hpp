@@ -19,7 +19,9 @@
 // With Q = exp(-2 raw / c) and R = 1 / (1 + Q), tanh = 1 - 2 Q R, 1 - tanh^2 = 4 Q R^2 and
 //   a_e - a_m = 2 c R_m R_e (Q_m - Q_e)
 // for the largest logit m: the exponents of both softmaxes without the cancellation of two
-// capped logits near the cap. raw / c is cut at +-20, past which tanh is +-1 in fp32.
+// capped logits near the cap. raw / c is cut at +-20, past which tanh is +-1 in fp32. A Q near
+// 1 has cap 2^-24 of a logit as its last place: for caps past 16 the capped logits' own
+// differences are taken (the backward's 1 - tanh^2 stays of Q).
 //
 // A token's logits lie in L lanes, V to a lane (L a power of two, V L >= E; V = 8, or 4 where
 // that is all of them): what a token needs of them is exchanged by lane permutations, what
@@ -102,6 +104,13 @@ __device__ __forceinline__ float capped_value(float raw, float c1, float cap) {
   const float r = __builtin_amdgcn_rcpf(d);
   return copysignf(cap * ((1.f - q) * fmaf(r, fmaf(-d, r, 1.f), r)), raw);
 }
+// The same to the last places of itself, also where the cap is far off: below a quarter of it
+// tanh's series, the terms up to x^9 (the next is under 2^-26 of the sum).
+__device__ __forceinline__ float capped_far(float raw, float c1, float cap) {
+  const float x = raw * c1 * -0.34657359028f, s = x * x;     // raw / cap and its square
+  const float p = fmaf(s, fmaf(s, fmaf(s, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f);
+  return fabsf(x) < 0.25f ? fmaf(raw * s, p, raw) : capped_value(raw, c1, cap);
+}
 
 // Where a token's lanes keep expert e's word among them: the lanes' j-th words are
 // neighbours, and tokens lie (V + 1) L words apart, so that a wave meets every bank alike.
@@ -119,13 +128,44 @@ __device__ __forceinline__ uint32_t key_below(const uint32_t (&key)[V], uint32_t
   return lanes_max<L>(max_of(below)) + best;
 }
 
+// Past this cap the differences of Q lose more places (the cap's) than those of the capped
+// logits, which are then taken themselves.
+constexpr float kFarCap = 16.f;
+
 struct RouterScales {
-  float c1, k_z, k_p;   // exponents in base 2 of R_m R_e (Q_m - Q_e): of both softmaxes
+  float c1, cap, k_z, k_p;   // exponents in base 2 of a token's distances, of both softmaxes
+  bool far;
   __device__ RouterScales(const RouterArgs& a) {
     const float tau = a.tau_dev ? *a.tau_dev : a.tau;
+    far = a.cap > kFarCap;
     c1 = -2.8853900817779268f / a.cap;
-    k_z = 2.8853900817779268f * a.cap;
+    cap = a.cap;
+    k_z = far ? 1.4426950408889634f : 2.8853900817779268f * a.cap;
     k_p = k_z / tau;
+  }
+  __device__ float value(float raw) const {
+    return far ? capped_far(raw, c1, cap) : capped_value(raw, c1, cap);
+  }
+};
+// The distances of a token's capped logits from its largest's, as they stand (far), or without
+// the factor that k_z and k_p get here: R_e (Q_m - Q_e) of 2 c R_m R_e (Q_m - Q_e).
+template <int V>
+struct RouterToken {
+  float k_z, k_p, d[V];
+  __device__ __forceinline__ RouterToken(const RouterScales& s, const float (&v)[V],
+                                         const Capped (&t)[V], float top)
+      : k_z(s.k_z), k_p(s.k_p) {
+    if (s.far) {
+      const float most = capped_far(top, s.c1, s.cap);
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] = capped_far(v[j], s.c1, s.cap) - most;
+    } else {
+      const Capped m = capped_top(top, s.c1);
+      k_z *= m.R;
+      k_p *= m.R;
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] = (m.Q - t[j].Q) * t[j].R;
+    }
   }
 };
 
@@ -225,15 +265,16 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
         }
       }
     }
-    const Capped m = capped_top(key_value(top), sc.c1);
-    const float k_p = m.R * sc.k_p, k_z = m.R * sc.k_z;
+    Capped c[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) c[j] = capped(v[j], sc.c1);
+    const RouterToken<V> tok(sc, v, c, key_value(top));
     float ep[V], sp = 0.f, sz = 0.f, ss = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const Capped c = capped(v[j], sc.c1);
-      const float d = e0 + j < E ? (m.Q - c.Q) * c.R : -INFINITY;
-      ep[j] = __builtin_amdgcn_exp2f(d * k_p);
-      sz += __builtin_amdgcn_exp2f(d * k_z);
+      const float d = e0 + j < E ? tok.d[j] : -INFINITY;
+      ep[j] = __builtin_amdgcn_exp2f(d * tok.k_p);
+      sz += __builtin_amdgcn_exp2f(d * tok.k_z);
       sp += ep[j];
       exps[j * L + l] = ep[j];
     }
@@ -256,7 +297,7 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_fwd(RouterArgs a) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (l == 0) {
-      const float lse = capped_value(key_value(top), sc.c1, a.cap) + __logf(sz);
+      const float lse = sc.value(key_value(top)) + __logf(sz);
       zs += lse * lse;
       ++n;
     }
@@ -464,16 +505,16 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_bwd(RouterArgs a) {
         return __float_as_uint(
             __builtin_elementwise_maximum(__uint_as_float(x), __uint_as_float(y)));
       }));
-      const Capped m = capped_top(top, sc.c1);
-      const float k_p = m.R * sc.k_p, k_z = m.R * sc.k_z;
       Capped t[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) t[j] = capped(v[j], sc.c1);
+      const RouterToken<V> tok(sc, v, t, top);
       float ep[V], ez[V], ss = 0.f, sz = 0.f, su = 0.f, sd = 0.f, sg = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        t[j] = capped(v[j], sc.c1);
-        const float d = e0 + j < E ? (m.Q - t[j].Q) * t[j].R : -INFINITY;
-        ep[j] = __builtin_amdgcn_exp2f(d * k_p);
-        ez[j] = __builtin_amdgcn_exp2f(d * k_z);
+        const float d = e0 + j < E ? tok.d[j] : -INFINITY;
+        ep[j] = __builtin_amdgcn_exp2f(d * tok.k_p);
+        ez[j] = __builtin_amdgcn_exp2f(d * tok.k_z);
         sz += ez[j];
         ss += off[j] == 0.f ? ep[j] : 0.f;
         su = fmaf(ep[j], off[j], su);
@@ -493,7 +534,7 @@ __global__ __launch_bounds__(kRouterThreads) void k_router_bwd(RouterArgs a) {
       const float a_on = fmaf(1e-6f, fmaf(d_top, su * inv_sp * inv_s, -D), -D) * inv_s - pg;
       const float a_off = -1e-6f * fmaf(d_top, ss * inv_sp * inv_s, D) * inv_s - pg;
       const float c_p = 4.f * inv_sp * inv_tau;
-      const float c_z = 4.f * cz * (capped_value(top, sc.c1, a.cap) + __logf(sz)) * __builtin_amdgcn_rcpf(sz);
+      const float c_z = 4.f * cz * (sc.value(top) + __logf(sz)) * __builtin_amdgcn_rcpf(sz);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float g = fmaf(dw[j], inv_s, off[j] == 0.f ? a_on : a_off) + (g0[j] - g_top);

@@ -1138,3 +1138,75 @@ def test_router_gradient_of_nearly_flat_logits(pkg, dev, E, k):
     draw, = torch.autograd.grad(r.weights, raw, dw)
     o = tn.router(f64(raw), k, 2.0, 1.0, None, f64(dw))
     near(draw, o["draw"], o["draw_mag"], 170, "draw")
+
+
+def _router_large_cap(raw, k, tau, cap, dw, dlb, dz):
+    """tn.router where exp(a - cap) is 0: the same by a's own maximum."""
+    B, E = raw.shape
+    th = np.tanh(raw / cap)
+    a = cap * th
+    top = a.max(-1, keepdims=True)
+    soft = np.exp(a - top)
+    lse = (top + np.log(soft.sum(-1, keepdims=True)))[:, 0]
+    soft /= soft.sum(-1, keepdims=True)
+    P = np.exp((a - top) / tau)
+    P /= P.sum(-1, keepdims=True)
+    idx = np.argsort(-raw, axis=-1, kind="stable")[:, :k]
+    sel = np.zeros((B, E))
+    np.put_along_axis(sel, idx, 1.0, -1)
+    pk = np.take_along_axis(P, idx, -1)
+    s = pk.sum(-1, keepdims=True) + 1e-6
+    w = pk / s
+    n = sel.sum(0)
+    G, gs, gm = dlb * E * n / B ** 2, np.zeros((B, E)), np.zeros((B, E))
+    np.put_along_axis(gs, idx, (dw - (dw * w).sum(-1, keepdims=True)) / s, -1)
+    np.put_along_axis(gm, idx, (np.abs(dw) + (np.abs(dw) * w).sum(-1, keepdims=True)) / s, -1)
+    g, gm = G + gs, np.abs(G) + gm
+    z = dz * 2 * lse[:, None] * soft / B
+    return {"idx": idx, "w": w, "lb": E * (n / B * P.mean(0)).sum(), "z": (lse ** 2).mean(),
+            "draw": (P * (g - (P * g).sum(-1, keepdims=True)) / tau + z) * (1 - th * th),
+            "draw_mag": P * (gm + (P * gm).sum(-1, keepdims=True)) / tau + np.abs(z)}
+
+
+@dtypes
+@pytest.mark.parametrize("cap,spread", [(15.9, 1.0), (16.1, 1.0), (100.0, 1.0), (100.0, 20.0), (1e3, 1.0),
+                                        (1e6, 0.01), (1e8, 1.0), (3e38, 1.0)])
+@pytest.mark.parametrize("E,k", [(4, 2), (33, 5)])
+def test_router_large_caps(pkg, dev, E, k, cap, spread, dtype):
+    """A cap that caps little or nothing, to that of a plain softmax. The bounds are those of
+    _check_router with what its capped logits reach in the cap's place: cap tanh(raw / cap) is off
+    by 8 steps of itself."""
+    g = torch.Generator().manual_seed(E)
+    raw = (_logits(500, E, torch.float32, E) * spread).to(dtype).to(dev).requires_grad_()
+    dw, dlb, dz, tau = torch.randn(500, k, generator=g), 0.7, 0.05, 1.25
+    cap = float(np.float32(cap))
+    r = pkg.fused_router(raw, k, tau, cap)
+    draw, = torch.autograd.grad((r.weights, r.lb_loss, r.z_loss), raw,
+                                (dw.to(dev), torch.tensor(dlb, device=dev), torch.tensor(dz, device=dev)))
+    o = _router_large_cap(f64(raw), k, tau, cap, f64(dw), dlb, dz)
+    if cap < 300:
+        for key, v in tn.router(f64(raw), k, tau, cap, None, f64(dw), dlb, dz).items():
+            assert key == "counts" or np.allclose(o[key], v, rtol=1e-9, atol=1e-13), key
+    most = cap * np.tanh(np.abs(f64(raw)).max() / cap)
+    n = 16 * most / tau + 128
+    assert np.array_equal(r.idx.cpu().numpy(), o["idx"])
+    near(r.weights, o["w"], o["w"], n, "w")
+    near(r.lb_loss, o["lb"], o["lb"], n, "lb")
+    near(r.z_loss, o["z"], 2 * np.sqrt(o["z"]) * (8 * most + 32) + 16 * o["z"], 1, "z")
+    near(draw, o["draw"], o["draw_mag"], 4 * n, "draw")
+
+
+@dtypes
+@pytest.mark.parametrize("cap", [0.01, 64.0])
+def test_router_extremes_of_other_caps(pkg, dev, cap, dtype):
+    """Infinities, logits far past the cap and next to zero, equal ones, with a cap far below the
+    logits and with one above most; a NaN spoils its own row."""
+    inf = float("inf")
+    raw = torch.tensor([[1.0, 3, 3, 2, 3, 3, -1, 3], [500.0, 400, 900, 800, 1e30, 3e38, 2, 1],
+                        [-inf, -inf, 5, -inf, 4, -inf, -inf, -inf], [inf, 0, inf, 1, 2, 3, 4, 5], [-inf] * 8,
+                        [1e-30, -1e-30, 1e-3, -1e-3, 0, 15.9, 16.1, -16], [-1e30] * 7 + [-2e30]]).to(dtype).to(dev)
+    _check_router(pkg, raw, 3, 0.5, cap, None, 1)
+    bad = raw.clone()
+    bad[0, 2] = float("nan")
+    r, b = pkg.fused_router(raw, 3, 0.5, cap), pkg.fused_router(bad, 3, 0.5, cap)
+    assert b.weights[0].isnan().all() and b.idx[0, 0] == 2 and torch.equal(r.weights[1:], b.weights[1:])
