@@ -1210,3 +1210,45 @@ def test_router_extremes_of_other_caps(pkg, dev, cap, dtype):
     bad[0, 2] = float("nan")
     r, b = pkg.fused_router(raw, 3, 0.5, cap), pkg.fused_router(bad, 3, 0.5, cap)
     assert b.weights[0].isnan().all() and b.idx[0, 0] == 2 and torch.equal(r.weights[1:], b.weights[1:])
+
+
+@dtypes
+@pytest.mark.parametrize("capturable", [False, True])
+def test_optimizer_8bit_is_the_functional_call(pkg, dev, capturable, dtype):
+    """FusedAdamW(state_bits=8) over steps with a parameter that gets its gradients late, a
+    transposed one and two groups, bit for bit adamw_step_8bit of the same tensors, codes, scales
+    and counts: one call for the parameters of a group that have taken as many steps."""
+    torch.manual_seed(0)
+    shapes = [(70, 40), (300,), (9,), (33, 5)]
+    ps = [torch.nn.Parameter((torch.randn(s, device=dev) * 0.05).to(dtype)) for s in shapes]
+    ps[3] = torch.nn.Parameter(ps[3].detach().t().contiguous().t())
+    groups = [[0, 1, 2], [3]]
+    opt = pkg.FusedAdamW([{"params": ps[:3]}, {"params": ps[3:], "lr": 5e-3}], state_bits=8, seed=3,
+                         capturable=capturable, **HYPER)
+    q = [p.detach().clone(memory_format=torch.preserve_format) for p in ps]
+    names = ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales")
+    st = [[torch.zeros(p.numel() if "codes" in k else -(-p.numel() // 256), device=dev,
+                       dtype=torch.uint8 if "codes" in k else torch.float32) for k in names] for p in ps]
+    count = [0] * 4
+    for step in range(1, 6):
+        for i, p in enumerate(ps):
+            p.grad = None if i == 2 and step < 3 else (torch.randn(p.shape, device=dev) * 0.01).to(dtype)
+        opt.step()
+        for g, group in enumerate(groups):
+            live = [i for i in group if ps[i].grad is not None]
+            for i in live:
+                count[i] += 1
+            for n in sorted({count[i] for i in live}, reverse=True):
+                ids = [i for i in live if count[i] == n]
+                at = torch.tensor(n, device=dev) if capturable else n
+                pkg.adamw_step_8bit([q[i] for i in ids], [ps[i].grad for i in ids],
+                                    *[[st[i][k] for i in ids] for k in range(4)], step=at, seed=3,
+                                    **{**HYPER, "lr": 5e-3 if g else HYPER["lr"]})
+        for i, p in enumerate(ps):
+            if not count[i]:
+                assert p not in opt.state
+                continue
+            assert torch.equal(p.detach(), q[i]) and int(opt.state[p]["step"]) == count[i], (step, i)
+            for k, t in zip(names, st[i]):
+                assert torch.equal(opt.state[p][k].view(t.dtype), t), (step, i, k)
+    assert count == [5, 5, 3, 5]
