@@ -158,10 +158,16 @@ class FusedAdamW(torch.optim.Optimizer):
                 run[3].append(st)
             counted = set()
             for n, ps, gs, sts in runs.values():
-                if on_device and id(n) not in counted:
+                first = on_device and id(n) not in counted
+                if first:
                     counted.add(id(n))
                     n.add_(1)
-                self._run(group, n if on_device else n + 1, ps, gs, sts)
+                try:
+                    self._run(group, n if on_device else n + 1, ps, gs, sts)
+                except Exception:
+                    if first:       # nothing was launched that this counts
+                        n.sub_(1)
+                    raise
                 if not on_device:
                     for st in sts:
                         st["step"] = n + 1

@@ -604,3 +604,30 @@ def test_optimizer_refuses_other_states(pkg):
     two = [torch.nn.Parameter(torch.ones(3)) for _ in range(2)]
     with pytest.raises(ValueError):
         pkg.FusedAdamW([{"params": two[:1]}, {"params": two[1:]}]).load_state_dict(saved(adamw))
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_optimizer_refused_step_is_not_counted(pkg, monkeypatch, capturable):
+    """A step that the call refuses leaves the counts of what it did not launch."""
+    import mamba_tuckermoe_amd.adamw as ad
+    fail, seen = [], []
+
+    def run(params, *a):
+        if any(p is q for p in params for q in fail):
+            raise RuntimeError("refused")
+        seen.append(int(a[5]))
+    monkeypatch.setattr(ad, "_run", run)
+    ps = [torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(3).bfloat16())]
+    opt = pkg.FusedAdamW([{"params": ps[:1]}, {"params": ps[1:]}], capturable=capturable)
+    _step_of(opt, ps, (1, 1))
+    fail.append(ps[1])
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="refused"):
+            _step_of(opt, ps, (0, 1))
+    assert [int(opt.state[p]["step"]) for p in ps] == [1, 1]
+    with pytest.raises(RuntimeError, match="refused"):
+        _step_of(opt, ps, (1, 1))
+    assert [int(opt.state[p]["step"]) for p in ps] == [2, 1]      # the first group's was launched
+    fail.clear()
+    _step_of(opt, ps, (0, 1))
+    assert seen == [1, 1, 2, 2] and [int(opt.state[p]["step"]) for p in ps] == [2, 2]
