@@ -94,15 +94,24 @@ class FusedAdamW(torch.optim.Optimizer):
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, seed: int = 0,
                  capturable: bool = False):
-        if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0:
-            raise ValueError(f"FusedAdamW: lr {lr}, eps {eps}, weight_decay {weight_decay}")
-        if not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
-            raise ValueError(f"FusedAdamW: betas {betas}")
-        if state_bits not in (32, 8):
-            raise ValueError(f"FusedAdamW: state_bits {state_bits} is not 32 or 8")
+        options = dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                       state_bits=state_bits, seed=seed, capturable=capturable)
+        self._check_options(options)
         self._captured = {}     # by id: the device counts that captured steps advance
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
-                                      state_bits=state_bits, seed=seed, capturable=capturable))
+        super().__init__(params, options)
+
+    @staticmethod
+    def _check_options(o) -> None:
+        if not o["lr"] >= 0.0 or not o["eps"] >= 0.0 or not o["weight_decay"] >= 0.0:
+            raise ValueError(f"FusedAdamW: lr {o['lr']}, eps {o['eps']}, weight_decay {o['weight_decay']}")
+        if not 0.0 <= o["betas"][0] < 1.0 or not 0.0 <= o["betas"][1] < 1.0:
+            raise ValueError(f"FusedAdamW: betas {o['betas']}")
+        if o["state_bits"] not in (32, 8):
+            raise ValueError(f"FusedAdamW: state_bits {o['state_bits']} is not 32 or 8")
+
+    def add_param_group(self, param_group) -> None:
+        self._check_options({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
@@ -229,7 +238,8 @@ class FusedAdamW(torch.optim.Optimizer):
         in their parameter's layout (torch casts states to their parameter's dtype). A
         torch.optim.AdamW's state is taken as 32-bit moments; what it lacks of this class's
         options stays as it is here. States of other kinds, and amsgrad's, maximize's or an L2
-        decay's, are refused."""
+        decay's, are refused. 8-bit states lie in their parameter's order in memory: they are
+        for parameters of the same strides."""
         saved, groups = state_dict["state"], state_dict["param_groups"]
         if len(groups) == len(self.param_groups):       # (torch refuses it otherwise)
             groups = [{**{k: mine[k] for k in self.defaults if k in mine}, **its}
@@ -264,6 +274,7 @@ class FusedAdamW(torch.optim.Optimizer):
         for k in ("amsgrad", "maximize"):
             if its.get(k):
                 raise ValueError(f"FusedAdamW: a state of an optimizer with {k}")
+        FusedAdamW._check_options(its)
         if its["weight_decay"] and not its.get("decoupled_weight_decay", True):
             raise ValueError("FusedAdamW: a state of an optimizer with an L2 decay")
         eight = its["state_bits"] == 8

@@ -631,3 +631,20 @@ def test_optimizer_refused_step_is_not_counted(pkg, monkeypatch, capturable):
     fail.clear()
     _step_of(opt, ps, (0, 1))
     assert seen == [1, 1, 2, 2] and [int(opt.state[p]["step"]) for p in ps] == [2, 2]
+
+
+def test_optimizer_checks_each_groups_own_values(pkg):
+    def p():
+        return [torch.nn.Parameter(torch.ones(3))]
+    for kw in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(weight_decay=-0.1),
+               dict(lr=math.nan)):
+        with pytest.raises(ValueError, match="FusedAdamW"):
+            pkg.FusedAdamW([{"params": p()}, {"params": p(), **kw}])
+        opt = pkg.FusedAdamW(p())
+        with pytest.raises(ValueError, match="FusedAdamW"):
+            opt.add_param_group({"params": p(), **kw})
+        assert len(opt.param_groups) == 1
+        with pytest.raises(ValueError, match="FusedAdamW"):      # defaults, even where no group uses them
+            pkg.FusedAdamW([{"params": p(), "state_bits": 8, "lr": 1.0, "betas": (0.9, 0.9), "eps": 1e-8,
+                             "weight_decay": 0.0}], **kw)
+    assert pkg.FusedAdamW([{"params": p(), "state_bits": 8}]).param_groups[0]["state_bits"] == 8
