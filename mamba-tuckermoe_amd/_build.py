@@ -51,6 +51,15 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found: the gfx950 library cannot be built")
 
 
+def rocm_include() -> str:
+    """HIP's headers: those beside the hipcc that builds the library, or what it links to."""
+    for path in (hipcc(), os.path.realpath(hipcc())):
+        inc = os.path.join(os.path.dirname(os.path.dirname(path)), "include")
+        if os.path.exists(os.path.join(inc, "hip", "hip_runtime.h")):
+            return inc
+    return "/opt/rocm/include"
+
+
 def native_tag() -> str:
     """What _tmoe_native.so is compiled for: the version of the C ABI's header, torch's and
     Python's (_lib.native() loads no other)."""
@@ -68,7 +77,7 @@ def native_cmd(out: str) -> list:
     return [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
             "-Wno-unknown-pragmas", f'-DTMOE_NATIVE_TAG="{native_tag()}"',
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-            "-D__HIP_PLATFORM_AMD__", "-I", INCLUDE, "-isystem", "/opt/rocm/include",
+            "-D__HIP_PLATFORM_AMD__", "-I", INCLUDE, "-isystem", rocm_include(),
             "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
             "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, NATIVE_SOURCE),
             "-o", out, "-L", lib, "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]

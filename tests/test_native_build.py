@@ -66,3 +66,24 @@ def test_build_without_native(monkeypatch, tmp_path, broken):
     assert [os.path.exists(f) for f in (b.LIB, b.PROBE_LIB, b.NATIVE_LIB)] == {
         "headers": [True, True, False], "torch": [True, True, False],
         "kernels": [False, False, True], None: [True, True, True]}[broken]
+
+
+def test_rocm_headers_follow_hipcc(tmp_path, monkeypatch):
+    """Those beside the hipcc in use, also where that is a link into its tree; a wrapper that
+    stands alone leaves the default."""
+    spec = importlib.util.spec_from_file_location(
+        "_tmoe_build_test", os.path.join(ROOT, "mamba-tuckermoe_amd", "_build.py"))
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    rocm = tmp_path / "rocm"
+    (rocm / "bin").mkdir(parents=True)
+    (rocm / "include" / "hip").mkdir(parents=True)
+    (rocm / "include" / "hip" / "hip_runtime.h").write_text("")
+    (rocm / "bin" / "hipcc").write_text("")
+    (tmp_path / "bin").mkdir()
+    (tmp_path / "bin" / "hipcc").symlink_to(rocm / "bin" / "hipcc")
+    (tmp_path / "bin" / "alone").write_text("")
+    for at, want in ((rocm / "bin" / "hipcc", rocm / "include"), (tmp_path / "bin" / "hipcc", rocm / "include"),
+                     (tmp_path / "bin" / "alone", "/opt/rocm/include")):
+        monkeypatch.setenv("HIPCC", str(at))
+        assert os.path.realpath(b.rocm_include()) == os.path.realpath(want), at
