@@ -57,6 +57,7 @@ hipError_t block_norm_forward(const BlockNormArgs& a, hipStream_t st);
 hipError_t block_norm_backward(const BlockNormArgs& a, hipStream_t st);
 
 constexpr int64_t kAdamwBlock = 256;        // elements that share a scale in 8-bit states
+constexpr int64_t kAdamwMaxN = (int64_t)1 << 36;
 
 hipError_t adamw(const tmoe_adamw_tensor* t, int64_t count, const tmoe_adamw_step_args& a,
                  hipStream_t st);

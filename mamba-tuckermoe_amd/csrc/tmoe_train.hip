@@ -24,8 +24,8 @@ int router_lanes(int64_t E) {
 }
 // Work-groups of the forward, a plane each for the second launch to add: at E = 64, B = 131072
 // the two take 23.0 + 4.8 us with 768, 25.7 + 4.5 with 512, 22.8 + 5.3 with 1024, 22.6 + 5.9
-// with 1280. The backward's, which sets up more than it gains by more waves: 21.6 us with
-// 768, 22.7 with 1024, 23.2 with 1536, 25.0 with 2048; the next token's inputs read ahead,
+// with 1280. The backward's, which sets up more than it gains by more waves (when that was
+// measured; 21.9 us now): 21.6 us with 768, 22.7 with 1024, 23.2 with 1536, 25.0 with 2048; the next token's inputs read ahead,
 // as in the forward, 22.0.
 constexpr int64_t kRouterBlocks = 768, kRouterBwdBlocks = 768;
 int64_t router_blocks(int64_t B, int64_t E) {
@@ -105,6 +105,8 @@ hipError_t adamw(const tmoe_adamw_tensor* t, int64_t count, const tmoe_adamw_ste
   int64_t chunk = 8192;
   const int64_t least = a.state_bits == 8 ? 2048 : 1024;
   while (chunk > least && total / chunk < 2048) chunk >>= 1;
+  // a tensor of the largest size is less than a launch
+  static_assert(kAdamwMaxN / 8192 <= kAdamwGroups, "");
   dev::AdamwTable b;
   b.step_dev = a.step_dev;
   b.beta1 = a.beta1; b.beta2 = a.beta2; b.lr = a.lr;
@@ -129,7 +131,6 @@ hipError_t adamw(const tmoe_adamw_tensor* t, int64_t count, const tmoe_adamw_ste
       b.p[c] = q.p; b.g[c] = q.g; b.m[c] = q.m; b.v[c] = q.v;
       b.ms[c] = q.m_scale; b.vs[c] = q.v_scale; b.n[c] = q.n; b.end[c] = groups;
     }
-    if (b.count == 0) return hipErrorInvalidValue;
     if (groups == 0) continue;
     const dim3 grid(groups), block(dev::kAdamwThreads);
     if (a.state_bits == 32) {

@@ -210,7 +210,7 @@ int tmoe_adamw_step(const tmoe_adamw_tensor* t, int64_t count, const tmoe_adamw_
     const tmoe_adamw_tensor& q = t[i];
     if (q.n < 0) return fail(TMOE_EINVAL, "%s: tensor %lld: n=%lld", who, (long long)i, (long long)q.n);
     if (q.n == 0) continue;
-    if (q.n > (int64_t)1 << 36)
+    if (q.n > tmoe::kAdamwMaxN)
       return fail(TMOE_EUNSUPPORTED, "%s: tensor %lld: n=%lld", who, (long long)i, (long long)q.n);
     if (!q.p || !q.g || !q.m || !q.v || (a->state_bits == 8 && (!q.m_scale || !q.v_scale)))
       return fail(TMOE_EINVAL, "%s: tensor %lld: null pointer", who, (long long)i);
