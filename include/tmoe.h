@@ -430,7 +430,8 @@ int tmoe_block_norm_backward(const tmoe_block_norm* norm, const float* inv, cons
  * v_scale: ceil(n / 256)), the largest magnitude / 448; codes are rounded to one of the two
  * neighbours at random, from a hash of (seed, step, tensor's number, element), so that m and
  * v = r^2 are right in the mean, and a positive r never to zero. A block that meets a
- * non-finite gradient has a non-finite scale from then on. step counts from 1; step_dev,
+ * gradient that is not finite, or whose square is not in fp32, has a non-finite scale from
+ * then on. step counts from 1; step_dev,
  * if not null, is a device int64 that is read instead. Tensors may not overlap; those with
  * n = 0 are passed over. Stream-ordered, no allocation, nothing copied to the device. */
 typedef struct tmoe_adamw_tensor {

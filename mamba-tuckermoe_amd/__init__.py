@@ -14,7 +14,7 @@ Public surface:
                                backward (latent.py; autograd.Function, reference signature)
   TuckerMoETrain               the reference's training layer (TritonTuckerMoE) on it
   fused_router, Routing        its router with the balance and z losses, per-expert counts and
-                               their gradient in two launches (train_ops.py)
+                               their gradient: one or two launches and one (train_ops.py)
   fused_block_norm             the norms before and after a block with its gate and residual
                                scale, and their gradients (train_ops.py)
   TuckerFFNTrain               TuckerFFN for training, on the two and TuckerMoETrain

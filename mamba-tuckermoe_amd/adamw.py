@@ -10,8 +10,9 @@ parameters on a HIP device with gradients of their dtype, computed in float32.
 scale for each BLOCK elements of a tensor in its memory's order: value = code * scale.
 Codes are rounded up or down at random (from seed, step, the tensor's place in the list and
 the element's in the tensor), so that m and v are right in the mean; a moment that moves
-by a thousandth a step would otherwise never leave its code. A non-finite gradient makes the
-moments of its whole block non-finite.
+by a thousandth a step would otherwise never leave its code. A gradient that is not finite, or
+whose square is not in float32 (from 1.8e19 on), makes the moments of its whole block
+non-finite.
 """
 from __future__ import annotations
 

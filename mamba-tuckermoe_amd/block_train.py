@@ -21,7 +21,8 @@ from .train_ops import fused_block_norm
 class TuckerFFNTrain(nn.Module):
     """forward(x_res, step=None, mask=None) -> (out, lb_loss, z_loss), the losses summed over
     the three layers. d and cfg as TuckerFFN's; mask (...) bool leaves tokens out (a
-    left-out token's layers are their biases)."""
+    left-out token's layers are their biases). norm_ffn and ls_ffn hold their parameters and
+    are not called: hooks on them do not run."""
 
     def __init__(self, d: int, cfg):
         super().__init__()

@@ -11,10 +11,11 @@
 // (seed, step, tensor, element), so a step repeated gives the same bits. A positive r is
 // never coded as zero: its element's step would be m / eps.
 //
-// fp32 is bound by memory: 28 bytes an element, 417 M of them in 2256 us, 5.2 TB/s. 8 bits
-// by instructions, ~71 an element: 19.3 M bf16 parameters in 48.6 us, 4.0 TB/s. A launch takes up to kAdamwTensors tensors,
-// their addresses in its arguments: nothing is copied to the device, and a captured step
-// holds them. A work-group takes `chunk` elements of one tensor.
+// fp32 is bound by memory: 28 bytes an element, 417 M of them in 2265 us, 5.2 TB/s. 8 bits
+// by instructions, 77 an element (the vector units work 94% of the time): 19.3 M bf16
+// parameters in 49.3 us, 3.9 TB/s. A launch takes up to kAdamwTensors tensors, their addresses
+// in its arguments: nothing is copied to the device, and a captured step holds them. A
+// work-group takes `chunk` elements of one tensor.
 #pragma once
 
 #include "tmoe_elem.hpp"
@@ -242,7 +243,7 @@ __device__ __forceinline__ void e4m3_codes(const float (&qm)[8], const float (&q
 }
 
 // Half a wave takes a block of 256 elements, eight neighbours a lane (a wave with four a lane:
-// 52.9 us against 48.6 at 19.3 M; the next block read ahead gained nothing there). What
+// 52.9 us against 48.6 at 19.3 M when that was measured; the next block read ahead gained nothing there). What
 // decides a code is computed as the formulas round it (a step's codes are the next one's
 // values), the rest with the hardware's reciprocals: the arithmetic, not the memory, is the
 // bound. A moment whose block's scale is under 2^-110 is taken for zero (the reciprocal of

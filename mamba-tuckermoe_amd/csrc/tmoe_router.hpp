@@ -28,8 +28,9 @@
 // k lanes store or read is handed through shared memory, so that idx, w and dw are moved
 // side by side. Eight to a lane rather than four: the exchanges, and not the exponentials,
 // are most of the instructions (forward 29 against 32 us when that was measured). Bound by
-// instructions: E = 64, k = 6, B = 131072 (fp32) takes 22.6 us forward (1.9 TB/s of what it
-// moves) and 21.6 backward (3.5 TB/s); B = 16384, E = 8, k = 2 5.2 and 5.2 us. The column
+// instructions (the vector units work 74% and 72% of the time): E = 64, k = 6, B = 131072
+// (fp32) takes 22.3 us forward (1.9 TB/s of what it moves) and 21.9 backward (3.5 TB/s);
+// B = 16384, E = 8, k = 2 5.3 and 5.4 us. The column
 // sums over the tokens (sum_b P_be in registers, n_e in shared memory) are a work-group's
 // own until its plane of `part`, and k_router_finish adds the planes in a fixed order: the
 // losses do not depend on which work-group ends first.
