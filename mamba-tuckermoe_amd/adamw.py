@@ -30,6 +30,8 @@ def _capturing(device: torch.device) -> bool:
     """Whether the current stream of a device records a graph."""
     if device.type != "cuda":
         return False
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(device):
         return torch.cuda.is_current_stream_capturing()
 
@@ -138,33 +140,40 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = [(group, [p for p in group["params"] if p.grad is not None])
-                for group in self.param_groups]
         # what is refused is refused before anything changes
-        captured = [n for group, ps in work for n in self._check_step(group, ps)]
-        self._captured.update((id(n), n) for n in captured)
-        for group, ps in work:
+        work, captured = [], {}
+        for group in self.param_groups:
+            live, resting = [], []      # (parameter, gradient, device, state or None); parameters
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    resting.append(p)
+                    continue
+                if g.is_sparse:
+                    raise RuntimeError("FusedAdamW: sparse gradients are not supported")
+                live.append((p, g, p.device, self.state.get(p)))
+            work.append((group, live, self._check_step(group, live, resting, captured)))
+        self._captured.update(captured)
+        for group, live, parted in work:
             on_device = group["capturable"]
             fresh = {}      # device: the count that parameters first met in this step share
             runs = {}       # (device, dtype, step): its parameters, one call each
-            parted = self._shared_with_resting(group, ps) if on_device else {}
-            for p in ps:
-                st = self.state[p]
+            for p, g, dev, st in live:
                 if not st:
-                    if on_device and p.device not in fresh:
-                        fresh[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
-                    st = self._init_state(p, group, fresh[p.device] if on_device else 0)
+                    if on_device and dev not in fresh:
+                        fresh[dev] = torch.zeros((), dtype=torch.int64, device=dev)
+                    st = self._init_state(p, group, fresh[dev] if on_device else 0)
                 n = st["step"]
-                if id(n) in parted:     # those that step now count by themselves from here on
+                if parted and id(n) in parted:      # those that step now count by themselves from here on
                     if parted[id(n)] is None:
                         parted[id(n)] = n.clone()
                     n = st["step"] = parted[id(n)]
-                key = (p.device, p.dtype, id(n) if on_device else n)
+                key = (dev, p.dtype, id(n) if on_device else n)
                 run = runs.get(key)
                 if run is None:
                     run = runs[key] = (n, [], [], [])
                 run[1].append(p)
-                run[2].append(p.grad)
+                run[2].append(g)
                 run[3].append(st)
             counted = set()
             for n, ps, gs, sts in runs.values():
@@ -183,46 +192,41 @@ class FusedAdamW(torch.optim.Optimizer):
                         st["step"] = n + 1
         return loss
 
-    def _shared_with_resting(self, group, ps) -> dict:
-        """{id: None} of the device counts of ps that parameters of the group without a
-        gradient hold too."""
-        if len(ps) == len(group["params"]):
-            return {}
-        mine = {id(self.state[p]["step"]) for p in ps if self.state.get(p)}
-        return {id(st["step"]): None for st in (self.state.get(p) for p in group["params"] if p.grad is None)
-                if st and id(st["step"]) in mine}
-
-    def _check_step(self, group, ps) -> list:
-        """Refuses what a step cannot do; the device counts that it advances in a capture."""
-        if any(p.grad.is_sparse for p in ps):
-            raise RuntimeError("FusedAdamW: sparse gradients are not supported")
-        capturing = {d: _capturing(d) for d in {p.device for p in ps}}
+    def _check_step(self, group, live, resting, captured) -> dict:
+        """Refuses what a step of a group cannot do; adds the device counts that it advances in a
+        capture to `captured`, by id. {id: None} of the device counts of live parameters that
+        resting ones hold too."""
+        capturing = {d: _capturing(d) for d in {d for _, _, d, _ in live}}
         if not group["capturable"]:
-            if any(capturing.values()):
+            if True in capturing.values():
                 raise RuntimeError("FusedAdamW: a step inside a graph capture needs "
                                    "capturable=True (its count would stand still)")
-            return []
-        captured = []
-        parted = self._shared_with_resting(group, ps)
-        for p in ps:
-            st = self.state.get(p)
+            return {}
+        parted = {}
+        if resting:
+            mine = {id(st["step"]) for _, _, _, st in live if st}
+            parted = {id(st["step"]): None for st in map(self.state.get, resting)
+                      if st and id(st["step"]) in mine}
+        if not parted and True not in capturing.values():
+            return parted
+        for p, _, dev, st in live:
             if not st:
-                if capturing[p.device]:     # each replay would clear it again
+                if capturing[dev]:      # each replay would clear it again
                     raise RuntimeError("FusedAdamW: a parameter's first step inside a graph capture: make "
                                        "one step with these gradients before the capture")
                 continue
             n = st["step"]
             if id(n) not in parted:
-                if capturing[p.device]:
-                    captured.append(n)
-            elif capturing[p.device]:
+                if capturing[dev]:
+                    captured[id(n)] = n
+            elif capturing[dev]:
                 raise RuntimeError("FusedAdamW: a captured step of some of the parameters that have stepped "
                                    "together so far: make one step with these gradients before the capture")
             elif id(n) in self._captured:       # the graph counts for all of them
                 raise RuntimeError("FusedAdamW: parameters whose step was captured together step together "
                                    "(where that graph is gone, opt.load_state_dict(opt.state_dict()) parts "
                                    "them)")
-        return captured
+        return parted
 
     @staticmethod
     def _run(group, step, ps, gs, sts):
