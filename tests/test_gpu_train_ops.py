@@ -1252,3 +1252,15 @@ def test_optimizer_8bit_is_the_functional_call(pkg, dev, capturable, dtype):
             for k, t in zip(names, st[i]):
                 assert torch.equal(opt.state[p][k].view(t.dtype), t), (step, i, k)
     assert count == [5, 5, 3, 5]
+
+
+@pytest.mark.parametrize("E,k,tau", [(64, 2, 2.0), (256, 2, 2.0), (256, 2, 0.3), (256, 16, 2.0)])
+def test_router_gradient_of_saturated_logits(pkg, dev, E, k, tau):
+    """Most logits past the cap, so that many experts' probabilities are next to equal: the
+    gradient of the weights in the 2-norm, by the bound of test_router_top1_weights_gradient."""
+    g = torch.Generator().manual_seed(E * 7 + k)
+    raw = (torch.randn(300, E, generator=g) * 30).to(dev).requires_grad_()
+    dw = torch.randn(300, k, generator=g).to(dev)
+    draw, = torch.autograd.grad(pkg.fused_router(raw, k, tau).weights, raw, dw)
+    o = tn.router(f64(raw), k, tau, 10.0, None, f64(dw))
+    assert onp.rel_l2(f64(draw), o["draw"]) <= 4 * (16 * 10 / tau + 128) * U
