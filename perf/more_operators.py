@@ -106,10 +106,11 @@ def draw(rng):
         groups = rng.choice([1, 1, 2, 4, 8, rng.randint(3, 16)])
         E = groups * _log_int(rng, 2, 256 // groups)
         top = rng.randint(1, groups)
-        return _route(_log_int(rng, 1, min(262144, 2 ** 23 // E)), E,
-                      rng.randint(1, min(top * (E // groups), 8)), rng.choice(["softmax", "sigmoid"]),
+        k = rng.randint(1, min(top * (E // groups), 8))
+        # (one renormalised weight is a constant: nobody trains that)
+        return _route(_log_int(rng, 1, min(262144, 2 ** 23 // E)), E, k, rng.choice(["softmax", "sigmoid"]),
                       rng.random() < 0.6, groups, top, rng.choice(["fp32", "bf16"]),
-                      rng.choice([0.0, 0.0, rng.uniform(0.0, 0.9)]), rng.random() < 0.7)
+                      rng.choice([0.0, 0.0, rng.uniform(0.0, 0.9)]), k > 1 and rng.random() < 0.7)
     if kind == "muon":
         return _muon(rng.choice(["c1", "c3", "ffn", "odd"]), rng.randint(1, 12), rng.choice(["fp32", "bf16"]))
     M = _log_int(rng, 1, 16384)
