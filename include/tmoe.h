@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define TMOE_ABI_VERSION 14
+#define TMOE_ABI_VERSION 15
 
 /* error codes */
 #define TMOE_OK            0
@@ -450,6 +450,42 @@ typedef struct tmoe_adamw_step_args {
 } tmoe_adamw_step_args;
 int tmoe_adamw_step(const tmoe_adamw_tensor* tensors, int64_t count,
                     const tmoe_adamw_step_args* args, void* stream);
+
+/* Routing to experts by softmax or sigmoid scores (no counterpart in the reference, whose
+ * routers are tmoe_router's and the layer's own). For a token's logits raw (E):
+ *   s = softmax(raw) (TMOE_SCORE_SOFTMAX) or 1 / (1 + exp(-raw)) (TMOE_SCORE_SIGMOID)
+ *   b = s + bias;  the experts lie in `groups` groups of E / groups neighbours each; a group's
+ *   worth is its two largest b added (its one b where it has one), and the top_groups
+ *   worthiest are open;  idx = the k largest b of the open groups, in descending order
+ *   w_j = scale s[idx_j] / (sum_i s[idx_i] + 1e-20) (renormalize), or scale s[idx_j]
+ * b and worths are compared as in float64, the lowest index first on ties, a NaN above every
+ * number; with groups 1 and no bias the logits themselves are compared. counts[e] is how many
+ * tokens selected e. Tokens that the mask leaves out (mask[b] == 0) have idx -1, w 0 and no
+ * gradient, and are not counted, whatever their logits hold.
+ *   raw   (B, E)  dtype TMOE_BF16 or TMOE_F32, rows row_stride elements apart
+ *   bias  (E)     fp32, or null          idx    (B, k)  int64
+ *   mask  (B)     bytes, or null         w      (B, k)  fp32
+ *                                        counts (E)     int64
+ * E <= 256, k <= 16, groups divides E, k <= top_groups E / groups, B <= 2^30. Past 64 groups of
+ * which some stay closed every token is ranked in float64 (slower). Backward: from dw (B, k)
+ * draw (B, E) of dtype, contiguous, idx and w as the forward wrote them; the bias gets no
+ * gradient. What is written overlaps nothing that is read. Stream-ordered, no allocation. */
+#define TMOE_SCORE_SOFTMAX 0
+#define TMOE_SCORE_SIGMOID 1
+typedef struct tmoe_expert_router {
+  const void* raw;
+  int64_t row_stride, B, E, k, groups, top_groups;
+  const float* bias;
+  const uint8_t* mask;
+  int32_t dtype, score, renormalize;
+  float scale;
+} tmoe_expert_router;
+size_t tmoe_expert_router_workspace_bytes(int64_t B, int64_t E);
+int tmoe_expert_router_forward(const tmoe_expert_router* router, int64_t* idx, float* w,
+                               int64_t* counts, void* workspace, size_t workspace_bytes,
+                               void* stream);
+int tmoe_expert_router_backward(const tmoe_expert_router* router, const int64_t* idx,
+                                const float* w, const float* dw, void* draw, void* stream);
 
 /* Per-stage timing, no counterpart in the reference (measurement support).
  * While enabled, every tmoe_forward records a HIP event before each of its

@@ -15,6 +15,8 @@ Public surface:
   TuckerMoETrain               the reference's training layer (TritonTuckerMoE) on it
   fused_router, Routing        its router with the balance and z losses, per-expert counts and
                                their gradient: one or two launches and one (train_ops.py)
+  fused_expert_router,         routing by softmax or sigmoid scores, a bias for balance and groups
+  ExpertRouting                of experts, and its gradient (train_ops.py)
   fused_block_norm             the norms before and after a block with its gate and residual
                                scale, and their gradients (train_ops.py)
   TuckerFFNTrain               TuckerFFN for training, on the two and TuckerMoETrain
@@ -32,13 +34,13 @@ from .config import FFN_WORKLOADS, WORKLOADS, FfnWorkload, TuckerMoEConfig, Work
 from .module import RMSNorm, TuckerMoE, load_tucker
 from .block import LayerScale, TuckerFFN, TuckerOutProj
 from .latent import FusedLatentMoE, TuckerMoETrain, fused_latent_moe
-from .train_ops import Routing, fused_block_norm, fused_router
+from .train_ops import ExpertRouting, Routing, fused_block_norm, fused_expert_router, fused_router
 from .block_train import TuckerFFNTrain
 from .adamw import FusedAdamW, adamw_step, adamw_step_8bit, dequantize_state
 
 __all__ = ["TuckerMoE", "RMSNorm", "LayerScale", "TuckerFFN", "TuckerOutProj",
            "FusedLatentMoE", "TuckerMoETrain", "fused_latent_moe",
-           "fused_router", "Routing", "fused_block_norm", "TuckerFFNTrain", "FusedAdamW", "adamw_step",
+           "fused_router", "Routing", "fused_expert_router", "ExpertRouting", "fused_block_norm", "TuckerFFNTrain", "FusedAdamW", "adamw_step",
            "adamw_step_8bit", "dequantize_state",
            "TuckerMoEConfig", "Workload", "WORKLOADS", "FfnWorkload", "FFN_WORKLOADS", "load_tucker", "synth", "config", "fp8",
            "checkpoint", "_lib"]

@@ -22,7 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libtmoe.so")
 NATIVE_PATH = os.path.join(HERE, "_tmoe_native.so")
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 TMOE_OK, TMOE_EINVAL, TMOE_EUNSUPPORTED, TMOE_EHIP, TMOE_ESIGNAL = 0, -1, -2, -3, -4
 TMOE_F32, TMOE_BF16, TMOE_BF16_FP8W = 0, 1, 2
 TMOE_ROUTER_SOFTMAX_TOPK, TMOE_ROUTER_CAPPED = 0, 1
@@ -56,6 +56,8 @@ EXPORTED = (
     "tmoe_router_workspace_bytes", "tmoe_router_forward", "tmoe_router_backward",
     "tmoe_block_norm_workspace_bytes", "tmoe_block_norm_forward", "tmoe_block_norm_backward",
     "tmoe_adamw_step",
+    "tmoe_expert_router_workspace_bytes", "tmoe_expert_router_forward",
+    "tmoe_expert_router_backward",
     "tmoe_signal_status", "tmoe_set_wait_polls", "tmoe_forward_path",
     "tmoe_forward_form",
     "tmoe_prof_enable", "tmoe_prof_read",
@@ -106,6 +108,14 @@ class TmoeAdamwStep(ctypes.Structure):
     _fields_ = [(f, ctypes.c_double) for f in ("lr", "beta1", "beta2", "eps", "weight_decay")] + [
         ("step", ctypes.c_int64), ("step_dev", ctypes.c_void_p), ("seed", ctypes.c_uint32),
         ("dtype", ctypes.c_int32), ("state_bits", ctypes.c_int32)]
+
+
+class TmoeExpertRouter(ctypes.Structure):
+    """struct tmoe_expert_router."""
+    _fields_ = [("raw", ctypes.c_void_p)] + [
+        (f, ctypes.c_int64) for f in ("row_stride", "B", "E", "k", "groups", "top_groups")] + [
+        ("bias", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+        ("score", ctypes.c_int32), ("renormalize", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
 class TmoeError(RuntimeError):
@@ -197,6 +207,12 @@ def lib() -> ctypes.CDLL:
         L.tmoe_adamw_step.restype = ctypes.c_int
         L.tmoe_adamw_step.argtypes = [ctypes.POINTER(TmoeAdamwTensor), i64,
                                       ctypes.POINTER(TmoeAdamwStep), vp]
+        L.tmoe_expert_router_workspace_bytes.restype = sz
+        L.tmoe_expert_router_workspace_bytes.argtypes = [i64, i64]
+        L.tmoe_expert_router_forward.restype = ctypes.c_int
+        L.tmoe_expert_router_forward.argtypes = [ctypes.POINTER(TmoeExpertRouter)] + [vp] * 4 + [sz, vp]
+        L.tmoe_expert_router_backward.restype = ctypes.c_int
+        L.tmoe_expert_router_backward.argtypes = [ctypes.POINTER(TmoeExpertRouter)] + [vp] * 5
         L.tmoe_signal_status.restype = ctypes.c_int
         L.tmoe_signal_status.argtypes = [vp, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]
         L.tmoe_forward_path.restype = ctypes.c_int
@@ -248,7 +264,9 @@ def native():
                 "tmoe_forward_glu", "tmoe_rmsnorm_rows", "tmoe_last_error",
                 "tmoe_router_workspace_bytes", "tmoe_router_forward", "tmoe_router_backward",
                 "tmoe_block_norm_workspace_bytes", "tmoe_block_norm_forward",
-                "tmoe_block_norm_backward", "tmoe_adamw_step")))
+                "tmoe_block_norm_backward", "tmoe_adamw_step",
+                "tmoe_expert_router_workspace_bytes", "tmoe_expert_router_forward",
+                "tmoe_expert_router_backward")))
             _native = mod
     return _native
 

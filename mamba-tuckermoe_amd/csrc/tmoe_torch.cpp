@@ -62,12 +62,13 @@ PyObject* none() {
 }  // namespace
 
 #include "tmoe_torch_train.hpp"
+#include "tmoe_torch_step.hpp"
 
 namespace {
 
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (bad_args(n, 13, "bind")) return nullptr;
+  if (bad_args(n, 16, "bind")) return nullptr;
   g_lib.workspace_bytes = reinterpret_cast<decltype(g_lib.workspace_bytes)>(address(a[0]));
   g_lib.signal_status = reinterpret_cast<decltype(g_lib.signal_status)>(address(a[1]));
   g_lib.forward_epi = reinterpret_cast<decltype(g_lib.forward_epi)>(address(a[2]));
@@ -84,6 +85,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   to(g_train.norm_forward, 10);
   to(g_train.norm_backward, 11);
   to(g_train.adamw_step, 12);
+  to(g_step.expert_router_workspace_bytes, 13);
+  to(g_step.expert_router_forward, 14);
+  to(g_step.expert_router_backward, 15);
   return none();
   END_HANDLE_TH_ERRORS
 }
@@ -249,6 +253,7 @@ PyMODINIT_FUNC PyInit__tmoe_native() {
       {"router", (PyCFunction)(void (*)())router, METH_FASTCALL, nullptr},
       {"block_norm", (PyCFunction)(void (*)())block_norm, METH_FASTCALL, nullptr},
       {"adamw", (PyCFunction)(void (*)())adamw, METH_FASTCALL, nullptr},
+      {"expert_router", (PyCFunction)(void (*)())expert_router, METH_FASTCALL, nullptr},
       {"rmsnorm", (PyCFunction)(void (*)())rmsnorm, METH_FASTCALL, nullptr},
       {nullptr, nullptr, 0, nullptr}};
   g_gen = PyUnicode_InternFromString("_tmoe_gen");

@@ -2,6 +2,8 @@
 
 fused_router      the training layer's router with its balance and z losses and per-expert
                   counts (sft_cot_bundle/scripts/model.py:318-332), and its gradient
+fused_expert_router  routing by softmax or sigmoid scores with a bias for balance, groups of
+                  experts and renormalised weights, and its gradient
 fused_block_norm  the norms before and after a block with the block's gate and the residual's
                   scale (pure_torch_mlx/model.py:258-260, :337-341), and their gradients
 
@@ -52,6 +54,37 @@ def fused_router(raw: torch.Tensor, top_k: int, temperature: Union[float, torch.
             temperature = float(temperature)
     return Routing(*_lib.native().router(raw, top_k, None if tau is not None else float(temperature),
                                          tau, float(scale), mask))
+
+
+class ExpertRouting(NamedTuple):
+    """What fused_expert_router returns."""
+    idx: torch.Tensor       # (B, k) int64, by descending biased score; -1 for masked tokens
+    weights: torch.Tensor   # (B, k) float32
+    counts: torch.Tensor    # (E) int64: how many tokens selected each expert
+
+
+def fused_expert_router(raw: torch.Tensor, top_k: int, score: str = "softmax",
+                        bias: Optional[torch.Tensor] = None, groups: int = 1,
+                        top_groups: Optional[int] = None, renormalize: bool = True, scale: float = 1.0,
+                        mask: Optional[torch.Tensor] = None) -> ExpertRouting:
+    """Routes tokens by their raw logits (B, E), E <= 256 and top_k <= 16:
+
+        s = softmax(raw), or sigmoid(raw) with score "sigmoid";  b = s + bias
+        a group's worth = its two largest b added (its one, in groups of one)
+        idx = the top_k largest b of the experts in the top_groups worthiest groups
+        weights = scale s[idx] / (sum s[idx] + 1e-20), or scale s[idx] without renormalize
+
+    bias (E, float32) moves the selection and not the weights; it gets no gradient. The groups
+    are `groups` runs of E / groups neighbours, of which top_groups (None: all) are open. b and
+    worths are compared as in float64, the lowest index first on ties; with neither bias nor
+    groups the logits are. A token that mask (B, bool) leaves out selects nothing: idx -1,
+    which FusedLatentMoE skips, weights 0 and no gradient, whatever its logits hold. Gradients
+    flow from weights to raw."""
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f'fused_expert_router: score {score!r} is not "softmax" or "sigmoid"')
+    return ExpertRouting(*_lib.native().expert_router(
+        raw, top_k, score == "sigmoid", bias, groups, groups if top_groups is None else top_groups,
+        bool(renormalize), float(scale), mask))
 
 
 def fused_block_norm(x: Optional[torch.Tensor] = None, y: Optional[torch.Tensor] = None,
