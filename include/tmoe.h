@@ -487,6 +487,41 @@ int tmoe_expert_router_forward(const tmoe_expert_router* router, int64_t* idx, f
 int tmoe_expert_router_backward(const tmoe_expert_router* router, const int64_t* idx,
                                 const float* w, const float* dw, void* draw, void* stream);
 
+/* Products in 8-bit floating point with one fp32 scale for each block of 128 elements along the
+ * summed axis (no counterpart in the reference). An operand is (rows, K): OCP e4m3 codes, rows
+ * of K padded with zeros to a multiple of 128, row_bytes apart (a multiple of 16, codes 16-byte
+ * aligned), and fp32 scales, block b of row r at scales[r * scale_row + b * scale_block]; with
+ * tiles != 0 a scale is for 128 rows too, that of row r at [(r / 128) * scale_row + ...].
+ *
+ * tmoe_fp8_quantize makes operands of x (R, C) of dtype TMOE_BF16 or TMOE_F32 with rows
+ * row_stride elements apart. `rows` (or null) gets x itself, `cols` (or null) its transpose:
+ * C rows of R; their rows must be R and C. Over a block's elements, with top = max |x|,
+ *   scale = top / 448,  code = e4m3(x (448 / top)) to nearest, even on ties
+ * in fp32; where top <= 2^-100 scale and codes are 0. A block with a value that is not finite
+ * stands for values that are not. With tiles in either, both have it and the same scales, the
+ * steps exchanged. What is written overlaps nothing else.
+ *
+ * tmoe_fp8_gemm: out (M, N) of dtype, contiguous, from a (M, K) and b (N, K):
+ *   out[m, n] = sum_b sa[m, b] sb[n, b] sum_{k in b} a[m, k] b[n, k]
+ * in fp32. tmoe_fp8_gemm_values: the same with a the operand that quantising x (M, K) by rows
+ * would make. The order of its sums depends on the sizes alone. K, N and the rows of an operand
+ * <= 2^23, M of out <= 2^23. Workspaces of at least tmoe_fp8_gemm_workspace_bytes(M, N, K,
+ * values) bytes (0: none), 16-byte aligned. M == 0 is a no-op. Stream-ordered, no allocation. */
+typedef struct tmoe_fp8_operand {
+  void* codes;
+  float* scales;
+  int64_t rows, row_bytes, scale_row, scale_block;
+  int32_t tiles;
+} tmoe_fp8_operand;
+int tmoe_fp8_quantize(const void* x, int64_t R, int64_t C, int64_t row_stride, int dtype,
+                      const tmoe_fp8_operand* rows, const tmoe_fp8_operand* cols, void* stream);
+size_t tmoe_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int values);
+int tmoe_fp8_gemm(const tmoe_fp8_operand* a, const tmoe_fp8_operand* b, int64_t K, int dtype,
+                  void* out, void* workspace, size_t workspace_bytes, void* stream);
+int tmoe_fp8_gemm_values(const void* x, int64_t M, int64_t row_stride, int x_dtype,
+                         const tmoe_fp8_operand* b, int64_t K, int dtype, void* out,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
 /* Per-stage timing, no counterpart in the reference (measurement support).
  * While enabled, every tmoe_forward records a HIP event before each of its
  * kernels and one after the last, on the forward's stream. tmoe_prof_read waits

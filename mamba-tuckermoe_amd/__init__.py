@@ -19,6 +19,9 @@ Public surface:
   ExpertRouting                of experts, and its gradient (train_ops.py)
   fused_block_norm             the norms before and after a block with its gate and residual
                                scale, and their gradients (train_ops.py)
+  fp8_matmul, fp8_quantize,    products in 8-bit floating point with a scale for each block of
+  fp8_block_matmul, BlockFp8,  128, with gradients, and on operands held in 8 bits
+  fp8_dequantize               (block_fp8.py)
   TuckerFFNTrain               TuckerFFN for training, on the two and TuckerMoETrain
                                (block_train.py)
   FusedAdamW, adamw_step,      one AdamW step over many tensors, moments in 32 or 8 bits
@@ -35,12 +38,14 @@ from .module import RMSNorm, TuckerMoE, load_tucker
 from .block import LayerScale, TuckerFFN, TuckerOutProj
 from .latent import FusedLatentMoE, TuckerMoETrain, fused_latent_moe
 from .train_ops import ExpertRouting, Routing, fused_block_norm, fused_expert_router, fused_router
+from .block_fp8 import BlockFp8, fp8_block_matmul, fp8_dequantize, fp8_matmul, fp8_quantize
 from .block_train import TuckerFFNTrain
 from .adamw import FusedAdamW, adamw_step, adamw_step_8bit, dequantize_state
 
 __all__ = ["TuckerMoE", "RMSNorm", "LayerScale", "TuckerFFN", "TuckerOutProj",
            "FusedLatentMoE", "TuckerMoETrain", "fused_latent_moe",
-           "fused_router", "Routing", "fused_expert_router", "ExpertRouting", "fused_block_norm", "TuckerFFNTrain", "FusedAdamW", "adamw_step",
+           "fused_router", "Routing", "fused_expert_router", "ExpertRouting", "fused_block_norm",
+           "BlockFp8", "fp8_quantize", "fp8_dequantize", "fp8_block_matmul", "fp8_matmul", "TuckerFFNTrain", "FusedAdamW", "adamw_step",
            "adamw_step_8bit", "dequantize_state",
            "TuckerMoEConfig", "Workload", "WORKLOADS", "FfnWorkload", "FFN_WORKLOADS", "load_tucker", "synth", "config", "fp8",
            "checkpoint", "_lib"]

@@ -58,6 +58,7 @@ EXPORTED = (
     "tmoe_adamw_step",
     "tmoe_expert_router_workspace_bytes", "tmoe_expert_router_forward",
     "tmoe_expert_router_backward",
+    "tmoe_fp8_quantize", "tmoe_fp8_gemm_workspace_bytes", "tmoe_fp8_gemm", "tmoe_fp8_gemm_values",
     "tmoe_signal_status", "tmoe_set_wait_polls", "tmoe_forward_path",
     "tmoe_forward_form",
     "tmoe_prof_enable", "tmoe_prof_read",
@@ -116,6 +117,13 @@ class TmoeExpertRouter(ctypes.Structure):
         (f, ctypes.c_int64) for f in ("row_stride", "B", "E", "k", "groups", "top_groups")] + [
         ("bias", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("dtype", ctypes.c_int32),
         ("score", ctypes.c_int32), ("renormalize", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
+class TmoeFp8Operand(ctypes.Structure):
+    """struct tmoe_fp8_operand."""
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)] + [
+        (f, ctypes.c_int64) for f in ("rows", "row_bytes", "scale_row", "scale_block")] + [
+        ("tiles", ctypes.c_int32)]
 
 
 class TmoeError(RuntimeError):
@@ -213,6 +221,16 @@ def lib() -> ctypes.CDLL:
         L.tmoe_expert_router_forward.argtypes = [ctypes.POINTER(TmoeExpertRouter)] + [vp] * 4 + [sz, vp]
         L.tmoe_expert_router_backward.restype = ctypes.c_int
         L.tmoe_expert_router_backward.argtypes = [ctypes.POINTER(TmoeExpertRouter)] + [vp] * 5
+        operand = ctypes.POINTER(TmoeFp8Operand)
+        L.tmoe_fp8_quantize.restype = ctypes.c_int
+        L.tmoe_fp8_quantize.argtypes = [vp, i64, i64, i64, ctypes.c_int, operand, operand, vp]
+        L.tmoe_fp8_gemm_workspace_bytes.restype = sz
+        L.tmoe_fp8_gemm_workspace_bytes.argtypes = [i64, i64, i64, ctypes.c_int]
+        L.tmoe_fp8_gemm.restype = ctypes.c_int
+        L.tmoe_fp8_gemm.argtypes = [operand, operand, i64, ctypes.c_int, vp, vp, sz, vp]
+        L.tmoe_fp8_gemm_values.restype = ctypes.c_int
+        L.tmoe_fp8_gemm_values.argtypes = [vp, i64, i64, ctypes.c_int, operand, i64, ctypes.c_int, vp,
+                                           vp, sz, vp]
         L.tmoe_signal_status.restype = ctypes.c_int
         L.tmoe_signal_status.argtypes = [vp, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]
         L.tmoe_forward_path.restype = ctypes.c_int
@@ -266,7 +284,8 @@ def native():
                 "tmoe_block_norm_workspace_bytes", "tmoe_block_norm_forward",
                 "tmoe_block_norm_backward", "tmoe_adamw_step",
                 "tmoe_expert_router_workspace_bytes", "tmoe_expert_router_forward",
-                "tmoe_expert_router_backward")))
+                "tmoe_expert_router_backward", "tmoe_fp8_quantize",
+                "tmoe_fp8_gemm_workspace_bytes", "tmoe_fp8_gemm", "tmoe_fp8_gemm_values")))
             _native = mod
     return _native
 

@@ -1,0 +1,77 @@
+"""Products in 8-bit floating point (OCP e4m3) with a scale for each block of 128, on MI355X
+(gfx950).
+
+The reference has no quantised path. Where fp8.py holds a layer's weights with one scale for an
+output channel and multiplies in bfloat16, here both operands are 8 bits wide when they are
+multiplied, and each 128 elements along the summed axis have a float32 scale of their own:
+
+    fp8_matmul(x, w)             x w of a training step, and its gradients
+    fp8_quantize(x)              codes and scales, to be held
+    fp8_block_matmul(a, b)       a b^T of what was quantised (or of values a by b's codes)
+
+A block's scale is max |x| / 448 and its codes are x (448 / max |x|) to the nearest e4m3 value,
+even ones on ties, in float32; blocks of no magnitude past 2^-100 are zeros, and a block with a
+value that is not finite stands for values that are not. Sums are float32. bfloat16 and float32
+tensors on a HIP device; no fallback. All calls run on the current stream and wait for nothing.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Union
+
+import torch
+
+from . import _lib
+
+BLOCK = 128
+
+
+class BlockFp8(NamedTuple):
+    """A (rows, cols) matrix in 8 bits. scales has a row for each row of codes, or for each 128."""
+    codes: torch.Tensor     # (rows, cols padded with zeros to a multiple of 128) float8_e4m3fn
+    scales: torch.Tensor    # (rows or ceil(rows / 128), ceil(cols / 128)) float32
+    cols: int
+
+
+def fp8_quantize(x: torch.Tensor, tiles: bool = False, transpose: bool = False) -> BlockFp8:
+    """x (R, C) in blocks of 1 x 128 along its rows, or of 128 x 128 (`tiles`, for weights);
+    with `transpose` x^T instead, of C rows."""
+    codes, scales = _lib.native().fp8_quantize(x, bool(transpose), bool(tiles))
+    return BlockFp8(codes, scales, x.shape[0 if transpose else 1])
+
+
+def fp8_dequantize(q: BlockFp8) -> torch.Tensor:
+    """The float32 values (rows, cols) that codes and scales stand for."""
+    codes = q.codes.view(torch.float8_e4m3fn) if q.codes.dtype == torch.uint8 else q.codes
+    s = q.scales
+    if s.shape[0] != codes.shape[0]:
+        s = s.repeat_interleave(BLOCK, 0)[:codes.shape[0]]
+    return (codes.float() * s.repeat_interleave(BLOCK, 1))[:, :q.cols]
+
+
+def fp8_block_matmul(a: Union[BlockFp8, torch.Tensor], b: BlockFp8,
+                     dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """a (M, K) times the transpose of b (N, K): out (M, N) of dtype (None: a's, bfloat16 for
+    codes). a may be values (..., K), which are quantised by rows on the way (up to 32 rows
+    within the product's own launch). No gradient."""
+    codes = isinstance(a, tuple)
+    if not isinstance(b, tuple):
+        raise TypeError("fp8_block_matmul: b is a BlockFp8")
+    if codes and a[2] != b[2]:
+        raise ValueError(f"fp8_block_matmul: rows of {a[2]} and of {b[2]}")
+    if dtype is None:
+        dtype = torch.bfloat16 if codes else a.dtype
+    bf16 = _lib.dtype_code(dtype) == _lib.TMOE_BF16
+    return _lib.native().fp8_block_matmul(a[0] if codes else a, a[1] if codes else None, int(b[2]), b[0],
+                                          b[1], bf16)
+
+
+def fp8_matmul(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    """x (..., K) times w (K, N), both of one dtype, in 8-bit block products, forward and
+    backward:
+
+        y  = q(x) q(w),    blocks of 1 x 128 of x along K, of 128 x 128 of w
+        dx = q(dy) q(w)^T,  blocks of 1 x 128 of dy along N, the same codes of w
+        dw = q(x)^T q(dy),  blocks of 128 tokens of each column of x and dy
+
+    For the backward it keeps codes of x and w (a byte an element), not x and w."""
+    return _lib.native().fp8_matmul(x, w)

@@ -30,4 +30,38 @@ size_t expert_router_workspace_bytes(int64_t B, int64_t E);
 hipError_t expert_router_forward(ExpertRouterArgs a, hipStream_t st);
 hipError_t expert_router_backward(const ExpertRouterArgs& a, hipStream_t st);
 
+constexpr int64_t kFp8MaxDim = (int64_t)1 << 23;   // rows' bytes within a tile are counted in 32 bits
+
+// x (R, C) to codes in blocks of 1 x 128 along its rows (row_codes), along its columns
+// (col_codes, transposed: C rows of R padded to 128), or of 128 x 128 (tiles: both the same codes)
+struct Fp8QuantizeArgs {
+  const void* x;
+  int64_t R, C, row_stride;
+  int dtype, tiles;
+  void* row_codes;
+  float* row_scales;
+  int64_t row_bytes, row_rs, row_ks;   // codes' rows; the scales' steps for a row and a block
+  void* col_codes;
+  float* col_scales;
+  int64_t col_bytes, col_rs, col_ks;
+};
+hipError_t fp8_quantize(const Fp8QuantizeArgs& a, hipStream_t st);
+
+struct Fp8GemmArgs {
+  const void *a, *b;       // codes; a: with a_dtype values of M rows of K elements, a_bytes apart
+  int64_t a_bytes, b_bytes;
+  const float *sa, *sb;
+  int64_t sa_rs, sa_ks, sb_rs, sb_ks;
+  int a_tiles, b_tiles;    // scales of 128 rows each
+  int a_dtype;             // -1: codes
+  int64_t M, N, K;
+  int blocks, slice_blocks, slices;
+  int dtype;
+  void* out;
+  float* planes;           // workspace: (slices, M, N), null for one slice
+};
+int64_t fp8_gemm_skinny_rows();      // up to so many rows of a may be values
+size_t fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t blocks);
+hipError_t fp8_gemm(Fp8GemmArgs a, hipStream_t st);
+
 }  // namespace tmoe

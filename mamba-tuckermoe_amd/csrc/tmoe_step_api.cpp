@@ -67,6 +67,61 @@ tmoe::ExpertRouterArgs er_args(const tmoe_expert_router* r) {
   return a;
 }
 
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// an operand of `rows` rows of K elements
+int fp8_check(const char* who, const char* what, const tmoe_fp8_operand* o, int64_t rows, int64_t K) {
+  if (!o) return fail(TMOE_EINVAL, "%s: null %s", who, what);
+  if (rows < 0 || o->rows != rows || K < 1)
+    return fail(TMOE_EINVAL, "%s: %s of %lld rows of %lld", who, what, (long long)o->rows, (long long)K);
+  if (rows > tmoe::kFp8MaxDim || K > tmoe::kFp8MaxDim)
+    return fail(TMOE_EUNSUPPORTED, "%s: %s of %lld rows of %lld (at most 2^23)", who, what,
+                (long long)rows, (long long)K);
+  if (rows == 0) return TMOE_OK;
+  if (!o->codes || !o->scales) return fail(TMOE_EINVAL, "%s: null pointer in %s", who, what);
+  if (!on(o->codes, 16) || !on(o->scales, 4))
+    return fail(TMOE_EINVAL, "%s: misaligned pointer in %s", who, what);
+  if (o->row_bytes % 16 || o->row_bytes < blocks_of(K) * 128 || o->row_bytes > 2 * tmoe::kFp8MaxDim)
+    return fail(TMOE_EINVAL, "%s: %s of rows %lld bytes apart", who, what, (long long)o->row_bytes);
+  if (o->scale_row < 0 || o->scale_block < 0)
+    return fail(TMOE_EINVAL, "%s: negative steps of scales in %s", who, what);
+  return TMOE_OK;
+}
+struct Fp8Workspace {
+  size_t planes, codes, scales, total;
+};
+Fp8Workspace fp8_workspace(int64_t M, int64_t N, int64_t K, bool values) {
+  Fp8Workspace w{};
+  w.planes = (size_t)up16((int64_t)tmoe::fp8_gemm_workspace_bytes(M, N, blocks_of(K)));
+  if (values && M > tmoe::fp8_gemm_skinny_rows()) {
+    w.codes = (size_t)(M * blocks_of(K) * 128);
+    w.scales = (size_t)up16(M * blocks_of(K) * 4);
+  }
+  w.total = w.planes + w.codes + w.scales;
+  return w;
+}
+bool fp8_sizes_ok(int64_t M, int64_t N, int64_t K) {
+  return M >= 0 && N >= 1 && K >= 1 && M <= tmoe::kFp8MaxDim && N <= tmoe::kFp8MaxDim &&
+         K <= tmoe::kFp8MaxDim;
+}
+int fp8_gemm_check(const char* who, int64_t M, const tmoe_fp8_operand* b, int64_t K, int dtype,
+                   const void* out, const void* ws, size_t bytes, size_t need) {
+  if (!dtype_ok(dtype))
+    return fail(TMOE_EINVAL, "%s: dtype %d is not TMOE_BF16 or TMOE_F32", who, dtype);
+  if (b->rows < 1) return fail(TMOE_EINVAL, "%s: b of no rows", who);
+  if (M > 0 && !out) return fail(TMOE_EINVAL, "%s: null out", who);
+  if (!on(out, 16) || !on(ws, 16)) return fail(TMOE_EINVAL, "%s: misaligned out or workspace", who);
+  if (need && (!ws || bytes < need))
+    return fail(TMOE_EINVAL, "%s: workspace of %zu bytes, %zu needed", who, bytes, need);
+  return TMOE_OK;
+}
+void fp8_b(tmoe::Fp8GemmArgs& g, const tmoe_fp8_operand* b, int64_t K, int dtype, void* out) {
+  g.b = b->codes; g.b_bytes = b->row_bytes; g.sb = b->scales;
+  g.sb_rs = b->scale_row; g.sb_ks = b->scale_block; g.b_tiles = b->tiles != 0;
+  g.N = b->rows; g.K = K; g.blocks = (int)blocks_of(K); g.dtype = dtype; g.out = out;
+}
+
 }  // namespace
 
 extern "C" {
@@ -105,6 +160,108 @@ int tmoe_expert_router_backward(const tmoe_expert_router* r, const int64_t* idx,
   tmoe::ExpertRouterArgs a = er_args(r);
   a.idx = const_cast<int64_t*>(idx); a.w = const_cast<float*>(w); a.dw = dw; a.draw = draw;
   return done(tmoe::expert_router_backward(a, static_cast<hipStream_t>(stream)), who);
+}
+
+int tmoe_fp8_quantize(const void* x, int64_t R, int64_t C, int64_t row_stride, int dtype,
+                      const tmoe_fp8_operand* rows, const tmoe_fp8_operand* cols, void* stream) {
+  const char* who = "tmoe_fp8_quantize";
+  tmoe::clear_error();
+  if (!dtype_ok(dtype))
+    return fail(TMOE_EINVAL, "%s: dtype %d is not TMOE_BF16 or TMOE_F32", who, dtype);
+  if (!rows && !cols) return fail(TMOE_EINVAL, "%s: nothing is wanted", who);
+  if (R < 0 || C < 1) return fail(TMOE_EINVAL, "%s: R=%lld C=%lld", who, (long long)R, (long long)C);
+  if (R == 0) return TMOE_OK;
+  if (rows)
+    if (int rc = fp8_check(who, "rows", rows, R, C)) return rc;
+  if (cols)
+    if (int rc = fp8_check(who, "cols", cols, C, R)) return rc;
+  if (blocks_of(R) * blocks_of(C) >= (int64_t)1 << 31)
+    return fail(TMOE_EUNSUPPORTED, "%s: R=%lld C=%lld", who, (long long)R, (long long)C);
+  const bool tiles = (rows ? rows : cols)->tiles != 0;
+  if (rows && cols) {
+    if ((cols->tiles != 0) != tiles)
+      return fail(TMOE_EINVAL, "%s: tiles in one of rows and cols", who);
+    if (tiles && (rows->scales != cols->scales || rows->scale_row != cols->scale_block ||
+                  rows->scale_block != cols->scale_row))
+      return fail(TMOE_EINVAL, "%s: tiles have one set of scales", who);
+  }
+  if (!x) return fail(TMOE_EINVAL, "%s: null x", who);
+  if (!on(x, size_of(dtype))) return fail(TMOE_EINVAL, "%s: misaligned x", who);
+  if (row_stride < (R > 1 ? C : 0)) return fail(TMOE_EINVAL, "%s: rows that overlap", who);
+  tmoe::Fp8QuantizeArgs a{};
+  a.x = x; a.R = R; a.C = C; a.row_stride = row_stride; a.dtype = dtype; a.tiles = tiles;
+  if (rows) {
+    a.row_codes = rows->codes; a.row_scales = rows->scales; a.row_bytes = rows->row_bytes;
+    a.row_rs = rows->scale_row; a.row_ks = rows->scale_block;
+  }
+  if (cols) {
+    a.col_codes = cols->codes; a.col_scales = cols->scales; a.col_bytes = cols->row_bytes;
+    a.col_rs = cols->scale_row; a.col_ks = cols->scale_block;
+    if (!rows && tiles) {      // the kernel writes a tile's scale by its place in x
+      a.row_scales = cols->scales; a.row_rs = cols->scale_block; a.row_ks = cols->scale_row;
+    }
+  }
+  return done(tmoe::fp8_quantize(a, static_cast<hipStream_t>(stream)), who);
+}
+
+size_t tmoe_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int values) {
+  if (!fp8_sizes_ok(M, N, K)) return 0;
+  return fp8_workspace(M, N, K, values != 0).total;
+}
+
+int tmoe_fp8_gemm(const tmoe_fp8_operand* a, const tmoe_fp8_operand* b, int64_t K, int dtype, void* out,
+                  void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "tmoe_fp8_gemm";
+  tmoe::clear_error();
+  if (int rc = fp8_check(who, "a", a, a ? a->rows : 0, K)) return rc;
+  if (int rc = fp8_check(who, "b", b, b ? b->rows : 0, K)) return rc;
+  const int64_t M = a->rows;
+  const size_t need = tmoe_fp8_gemm_workspace_bytes(M, b->rows, K, 0);
+  if (int rc = fp8_gemm_check(who, M, b, K, dtype, out, workspace, workspace_bytes, need)) return rc;
+  tmoe::Fp8GemmArgs g{};
+  fp8_b(g, b, K, dtype, out);
+  g.a = a->codes; g.a_bytes = a->row_bytes; g.sa = a->scales; g.sa_rs = a->scale_row;
+  g.sa_ks = a->scale_block; g.a_tiles = a->tiles != 0; g.a_dtype = -1; g.M = M;
+  g.planes = static_cast<float*>(workspace);
+  return done(tmoe::fp8_gemm(g, static_cast<hipStream_t>(stream)), who);
+}
+
+int tmoe_fp8_gemm_values(const void* x, int64_t M, int64_t row_stride, int x_dtype,
+                         const tmoe_fp8_operand* b, int64_t K, int dtype, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  const char* who = "tmoe_fp8_gemm_values";
+  tmoe::clear_error();
+  if (!dtype_ok(x_dtype))
+    return fail(TMOE_EINVAL, "%s: dtype %d of x is not TMOE_BF16 or TMOE_F32", who, x_dtype);
+  if (int rc = fp8_check(who, "b", b, b ? b->rows : 0, K)) return rc;
+  if (M < 0) return fail(TMOE_EINVAL, "%s: M=%lld", who, (long long)M);
+  if (M > tmoe::kFp8MaxDim)
+    return fail(TMOE_EUNSUPPORTED, "%s: M=%lld (at most 2^23)", who, (long long)M);
+  const Fp8Workspace w = fp8_workspace(M, b->rows < 1 ? 1 : b->rows, K, true);
+  if (int rc = fp8_gemm_check(who, M, b, K, dtype, out, workspace, workspace_bytes, w.total)) return rc;
+  if (M == 0) return TMOE_OK;
+  if (!x) return fail(TMOE_EINVAL, "%s: null x", who);
+  if (!on(x, size_of(x_dtype))) return fail(TMOE_EINVAL, "%s: misaligned x", who);
+  if (row_stride < (M > 1 ? K : 0)) return fail(TMOE_EINVAL, "%s: rows that overlap", who);
+  tmoe::Fp8GemmArgs g{};
+  fp8_b(g, b, K, dtype, out);
+  g.M = M;
+  g.planes = static_cast<float*>(workspace);
+  if (!w.codes) {
+    g.a = x; g.a_bytes = row_stride; g.a_dtype = x_dtype;
+    return done(tmoe::fp8_gemm(g, static_cast<hipStream_t>(stream)), who);
+  }
+  const int64_t kb = blocks_of(K);
+  tmoe::Fp8QuantizeArgs q{};
+  q.x = x; q.R = M; q.C = K; q.row_stride = row_stride; q.dtype = x_dtype;
+  q.row_codes = static_cast<char*>(workspace) + w.planes;
+  q.row_scales = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.planes + w.codes);
+  q.row_bytes = kb * 128; q.row_rs = 1; q.row_ks = M;
+  if (hipError_t e = tmoe::fp8_quantize(q, static_cast<hipStream_t>(stream)); e != hipSuccess)
+    return done(e, who);
+  g.a = q.row_codes; g.a_bytes = q.row_bytes; g.sa = q.row_scales; g.sa_rs = 1; g.sa_ks = M;
+  g.a_dtype = -1;
+  return done(tmoe::fp8_gemm(g, static_cast<hipStream_t>(stream)), who);
 }
 
 }  // extern "C"

@@ -68,7 +68,7 @@ namespace {
 
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (bad_args(n, 16, "bind")) return nullptr;
+  if (bad_args(n, 20, "bind")) return nullptr;
   g_lib.workspace_bytes = reinterpret_cast<decltype(g_lib.workspace_bytes)>(address(a[0]));
   g_lib.signal_status = reinterpret_cast<decltype(g_lib.signal_status)>(address(a[1]));
   g_lib.forward_epi = reinterpret_cast<decltype(g_lib.forward_epi)>(address(a[2]));
@@ -88,6 +88,10 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   to(g_step.expert_router_workspace_bytes, 13);
   to(g_step.expert_router_forward, 14);
   to(g_step.expert_router_backward, 15);
+  to(g_step.fp8_quantize, 16);
+  to(g_step.fp8_workspace_bytes, 17);
+  to(g_step.fp8_gemm, 18);
+  to(g_step.fp8_gemm_values, 19);
   return none();
   END_HANDLE_TH_ERRORS
 }
@@ -254,6 +258,9 @@ PyMODINIT_FUNC PyInit__tmoe_native() {
       {"block_norm", (PyCFunction)(void (*)())block_norm, METH_FASTCALL, nullptr},
       {"adamw", (PyCFunction)(void (*)())adamw, METH_FASTCALL, nullptr},
       {"expert_router", (PyCFunction)(void (*)())expert_router, METH_FASTCALL, nullptr},
+      {"fp8_quantize", (PyCFunction)(void (*)())fp8_quantize, METH_FASTCALL, nullptr},
+      {"fp8_block_matmul", (PyCFunction)(void (*)())fp8_block_matmul, METH_FASTCALL, nullptr},
+      {"fp8_matmul", (PyCFunction)(void (*)())fp8_matmul, METH_FASTCALL, nullptr},
       {"rmsnorm", (PyCFunction)(void (*)())rmsnorm, METH_FASTCALL, nullptr},
       {nullptr, nullptr, 0, nullptr}};
   g_gen = PyUnicode_InternFromString("_tmoe_gen");

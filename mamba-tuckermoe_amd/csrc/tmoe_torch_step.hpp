@@ -11,6 +11,10 @@ struct StepEntry {
   decltype(&tmoe_expert_router_workspace_bytes) expert_router_workspace_bytes;
   decltype(&tmoe_expert_router_forward) expert_router_forward;
   decltype(&tmoe_expert_router_backward) expert_router_backward;
+  decltype(&tmoe_fp8_quantize) fp8_quantize;
+  decltype(&tmoe_fp8_gemm_workspace_bytes) fp8_workspace_bytes;
+  decltype(&tmoe_fp8_gemm) fp8_gemm;
+  decltype(&tmoe_fp8_gemm_values) fp8_gemm_values;
 } g_step{};
 
 // ---- expert router ---------------------------------------------------------------
@@ -156,6 +160,288 @@ PyObject* expert_router(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!r) return nullptr;
   for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(o[i]));
   return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- 8-bit block products ----------------------------------------------------------
+
+constexpr int64_t kFp8Most = (int64_t)1 << 23;
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+// codes (rows, K padded to 128) and scales (rows, or 128 of them, blocks)
+struct Fp8 {
+  at::Tensor codes, scales;
+  bool tiles = false;
+  tmoe_fp8_operand args() const {
+    tmoe_fp8_operand o{};
+    o.codes = codes.data_ptr();
+    o.scales = scales.data_ptr<float>();
+    o.rows = codes.size(0);
+    o.row_bytes = codes.size(0) > 1 ? codes.stride(0) : codes.size(1);
+    o.scale_row = scales.stride(0);
+    o.scale_block = scales.stride(1);
+    o.tiles = tiles;
+    return o;
+  }
+};
+// The operand of `rows` rows of K; scales of single rows lie row by row within a block, so that
+// the rows of a tile read them side by side.
+Fp8 fp8_empty(const at::Tensor& like, int64_t rows, int64_t K, bool tiles) {
+  const auto o = like.options().requires_grad(false);
+  Fp8 q;
+  q.tiles = tiles;
+  q.codes = at::empty({rows, 128 * blocks_of(K)}, o.dtype(at::kFloat8_e4m3fn));
+  q.scales = tiles ? at::empty({blocks_of(rows), blocks_of(K)}, o.dtype(at::kFloat))
+                   : at::empty({blocks_of(K), rows}, o.dtype(at::kFloat)).t();
+  return q;
+}
+// x (its rows (R, C) at one stride) along its rows, its columns, or both
+void fp8_make(const Rows& x, int64_t R, int64_t C, bool tiles, Fp8* rows, Fp8* cols) {
+  if (rows) *rows = fp8_empty(x.t, R, C, tiles);
+  if (cols) {
+    *cols = fp8_empty(x.t, C, R, tiles);
+    if (rows && tiles) cols->scales = rows->scales.t();
+  }
+  if (R == 0) return;
+  const tmoe_fp8_operand r = rows ? rows->args() : tmoe_fp8_operand{},
+                         c = cols ? cols->args() : tmoe_fp8_operand{};
+  check_rc(g_step.fp8_quantize(x.t.const_data_ptr(), R, C, x.stride,
+                               x.t.scalar_type() == at::kBFloat16 ? TMOE_BF16 : TMOE_F32,
+                               rows ? &r : nullptr, cols ? &c : nullptr, current_stream(x.t)));
+}
+int32_t code_of(at::ScalarType t) { return t == at::kBFloat16 ? TMOE_BF16 : TMOE_F32; }
+at::Tensor fp8_product(const Fp8& a, const Fp8& b, int64_t K, at::ScalarType dt) {
+  const int64_t M = a.codes.size(0), N = b.codes.size(0);
+  at::Tensor out = at::empty({M, N}, a.codes.options().dtype(dt));
+  if (M == 0) return out;
+  const size_t nws = g_step.fp8_workspace_bytes(M, N, K, 0);
+  at::Tensor ws;
+  if (nws) ws = bytes_like(out, nws);
+  const tmoe_fp8_operand x = a.args(), y = b.args();
+  check_rc(g_step.fp8_gemm(&x, &y, K, code_of(dt), out.data_ptr(), out_ptr(ws), nws, current_stream(out)));
+  return out;
+}
+at::Tensor fp8_product(const Rows& a, int64_t M, const Fp8& b, int64_t K, at::ScalarType dt) {
+  const int64_t N = b.codes.size(0);
+  at::Tensor out = at::empty({M, N}, a.t.options().dtype(dt).requires_grad(false));
+  if (M == 0) return out;
+  const size_t nws = g_step.fp8_workspace_bytes(M, N, K, 1);
+  at::Tensor ws;
+  if (nws) ws = bytes_like(out, nws);
+  const tmoe_fp8_operand y = b.args();
+  check_rc(g_step.fp8_gemm_values(a.t.const_data_ptr(), M, a.stride, code_of(a.t.scalar_type()), &y, K,
+                                  code_of(dt), out.data_ptr(), out_ptr(ws), nws, current_stream(out)));
+  return out;
+}
+
+PyObject* fp8_pair(const Fp8& q) {
+  PyObject* t = PyTuple_New(2);
+  if (!t) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(q.codes));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(q.scales));
+  return t;
+}
+
+// fp8_quantize(x, transpose, tiles): (codes, scales)
+PyObject* fp8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  constexpr const char* kWho = "fp8_quantize";
+  HANDLE_TH_ERRORS
+  if (bad_args(n, 3, "fp8_quantize")) return nullptr;
+  const at::Tensor& x = tensor(a[0]);
+  const bool transpose = PyObject_IsTrue(a[1]), tiles = PyObject_IsTrue(a[2]);
+  dtype_of(x, kWho);
+  TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1, kWho, ": (R, C) expected, got ", x.sizes());
+  TORCH_CHECK(x.size(0) <= kFp8Most && x.size(1) <= kFp8Most, kWho, ": at most 2^23 rows and columns, got ",
+              x.sizes());
+  TORCH_CHECK(!transpose || x.size(0) >= 1, kWho, ": no rows to lie along");
+  if (tangents_live()) check_tangent(x, kWho);
+  TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), kWho,
+              " has no gradient: give it detached, or call fp8_matmul");
+  check_hip(x, kWho);
+  Fp8 q;
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::DeviceGuard guard(x.device());
+    const at::NoGradGuard no_grad;
+    fp8_make(rows_of(x), x.size(0), x.size(1), tiles, transpose ? nullptr : &q, transpose ? &q : nullptr);
+  }
+  return fp8_pair(q);
+  END_HANDLE_TH_ERRORS
+}
+
+Fp8 fp8_operand(PyObject* codes, PyObject* scales, int64_t K, const char* who) {
+  Fp8 q;
+  q.codes = tensor(codes);
+  q.scales = tensor(scales);
+  const at::Tensor &c = q.codes, &s = q.scales;
+  TORCH_CHECK((c.scalar_type() == at::kFloat8_e4m3fn || c.scalar_type() == at::kByte) && c.dim() == 2 &&
+                  K >= 1 && c.size(1) == 128 * blocks_of(K),
+              who, ": codes (rows, ", K, " padded to a multiple of 128) of float8_e4m3fn (or uint8) expected, got ",
+              c.sizes(), " of ", c.scalar_type());
+  const int64_t rows = c.size(0);
+  TORCH_CHECK(rows <= kFp8Most && K <= kFp8Most, who, ": at most 2^23 rows and columns, got ", c.sizes());
+  TORCH_CHECK(s.scalar_type() == at::kFloat && s.dim() == 2 && s.size(1) == blocks_of(K) &&
+                  (s.size(0) == rows || s.size(0) == blocks_of(rows)),
+              who, ": scales of float32 for each row or each 128 of ", rows, " and each of ", blocks_of(K),
+              " blocks expected, got ", s.sizes(), " of ", s.scalar_type());
+  TORCH_CHECK(c.device() == s.device(), who, ": codes on ", c.device(), ", scales on ", s.device());
+  TORCH_CHECK(!s.requires_grad(), who, ": scales get no gradient: give them detached");
+  q.tiles = s.size(0) != rows;
+  return q;
+}
+void fp8_align(Fp8& q) {     // rows that direct loads of 16 bytes can read
+  const at::Tensor& c = q.codes;
+  if (c.size(0) == 0) return;
+  const bool ok = c.stride(1) == 1 && reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0 &&
+                  (c.size(0) == 1 || (c.stride(0) % 16 == 0 && c.stride(0) >= c.size(1) &&
+                                      c.stride(0) <= 2 * kFp8Most));
+  if (!ok) q.codes = c.clone(at::MemoryFormat::Contiguous);
+}
+
+// fp8_block_matmul(a codes or values, a scales or None, K, b codes, b scales, out dtype is bf16):
+// out (..., N)
+PyObject* fp8_block_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  constexpr const char* kWho = "fp8_block_matmul";
+  HANDLE_TH_ERRORS
+  if (bad_args(n, 6, "fp8_block_matmul")) return nullptr;
+  const int64_t K = integer(a[2]);
+  const at::ScalarType dt = PyObject_IsTrue(a[5]) ? at::kBFloat16 : at::kFloat;
+  Fp8 b = fp8_operand(a[3], a[4], K, kWho);
+  TORCH_CHECK(b.codes.size(0) >= 1, kWho, ": b of no rows");
+  const at::Tensor& x = tensor(a[0]);
+  TORCH_CHECK(x.device() == b.codes.device(), kWho, ": operands on ", x.device(), " and ", b.codes.device());
+  at::Tensor out;
+  if (a[1] != Py_None) {
+    Fp8 q = fp8_operand(a[0], a[1], K, kWho);
+    check_hip(x, kWho);
+    pybind11::gil_scoped_release nogil;
+    const c10::DeviceGuard guard(x.device());
+    fp8_align(q);
+    fp8_align(b);
+    out = fp8_product(q, b, K, dt);
+  } else {
+    dtype_of(x, kWho);
+    TORCH_CHECK(x.dim() >= 1 && x.size(x.dim() - 1) == K, kWho, ": rows of ", K, " expected, got ", x.sizes());
+    const int64_t M = x.numel() / K;
+    TORCH_CHECK(M <= kFp8Most, kWho, ": at most 2^23 rows, got ", M);
+    if (tangents_live()) check_tangent(x, kWho);
+    TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), kWho,
+                " has no gradient: give it detached, or call fp8_matmul");
+    check_hip(x, kWho);
+    pybind11::gil_scoped_release nogil;
+    const c10::DeviceGuard guard(x.device());
+    const at::NoGradGuard no_grad;
+    fp8_align(b);
+    out = fp8_product(rows_of(x), M, b, K, dt);
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = b.codes.size(0);
+    out = out.view(shape);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+constexpr const char* kFp8Matmul = "fp8_matmul";
+
+struct Fp8Call {
+  at::Tensor x, w;
+  bool want_x = false, want_w = false;
+};
+struct Fp8Kept {
+  Fp8 x, w;      // x^T (K, M) by rows; w (K, N) by tiles
+};
+at::Tensor fp8_matmul_forward(const Fp8Call& c, Fp8Kept& kept) {
+  const c10::DeviceGuard guard(c.x.device());
+  const int64_t K = c.w.size(0), N = c.w.size(1), M = c.x.numel() / K;
+  const Rows x = rows_of(c.x);
+  Fp8 xr, wt;
+  fp8_make(rows_of(c.w), K, N, true, c.want_x ? &kept.w : nullptr, &wt);
+  at::Tensor out;
+  if (c.want_w && M > 0) {
+    fp8_make(x, M, K, false, &xr, &kept.x);
+    out = fp8_product(xr, wt, K, c.x.scalar_type());
+  } else {
+    out = fp8_product(x, M, wt, K, c.x.scalar_type());
+  }
+  std::vector<int64_t> shape = c.x.sizes().vec();
+  shape.back() = N;
+  return out.view(shape);
+}
+
+struct Fp8Matmul : torch::autograd::Function<Fp8Matmul> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, Fp8Call c) {
+    c.want_x = x.requires_grad();
+    c.want_w = w.requires_grad();
+    Fp8Kept k;
+    const at::Tensor out = fp8_matmul_forward(c, k);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({k.x.codes, k.x.scales, k.w.codes, k.w.scales});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["N"] = w.size(1);
+    return {out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    if (!g[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
+    const variable_list s = ctx->get_saved_variables();
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    const int64_t N = ctx->saved_data["N"].toInt(), K = shape.back();
+    const at::Tensor& dy = g[0];
+    const at::ScalarType dt = dy.scalar_type();
+    const int64_t M = dy.numel() / N;
+    const c10::DeviceGuard guard(dy.device());
+    const Rows d = rows_of(dy);
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+    at::Tensor dx, dw;
+    Fp8 dr, dc;
+    const Fp8 w{s[2], s[3], true}, x{s[0], s[1], false};
+    if (want_w && M > 0) {
+      fp8_make(d, M, N, false, want_x ? &dr : nullptr, &dc);
+      dw = fp8_product(x, dc, M, dt);
+      if (want_x) dx = fp8_product(dr, w, N, dt);
+    } else {
+      if (want_w) dw = at::zeros({K, N}, dy.options());
+      if (want_x) dx = fp8_product(d, M, w, N, dt);
+    }
+    if (want_x) dx = dx.view(shape);
+    return once({dx, dw, at::Tensor()}, kFp8Matmul);
+  }
+};
+
+// fp8_matmul(x, w): x w in 8-bit block products, with their gradients
+PyObject* fp8_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (bad_args(n, 2, "fp8_matmul")) return nullptr;
+  const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]);
+  dtype_of(x, kFp8Matmul);
+  TORCH_CHECK(w.scalar_type() == x.scalar_type(), kFp8Matmul, ": dtypes ", x.scalar_type(), " and ",
+              w.scalar_type());
+  TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && w.size(0) >= 1 && w.size(1) >= 1 &&
+                  x.size(x.dim() - 1) == w.size(0),
+              kFp8Matmul, ": (..., K) and (K, N) expected, got ", x.sizes(), " and ", w.sizes());
+  TORCH_CHECK(x.numel() / w.size(0) <= kFp8Most && w.size(0) <= kFp8Most && w.size(1) <= kFp8Most, kFp8Matmul,
+              ": at most 2^23 of each, got ", x.sizes(), " and ", w.sizes());
+  TORCH_CHECK(x.device() == w.device(), kFp8Matmul, ": tensors on ", x.device(), " and ", w.device());
+  if (tangents_live()) {
+    check_tangent(x, kFp8Matmul);
+    check_tangent(w, kFp8Matmul);
+  }
+  check_hip(x, kFp8Matmul);
+  at::Tensor out;
+  {
+    pybind11::gil_scoped_release nogil;
+    Fp8Call c{x, w};
+    const OptTensor xo = x, wo = w;
+    if (wants_grad({&xo, &wo})) {
+      const c10::DeviceGuard guard(x.device());
+      check_capture({&xo, &wo}, kFp8Matmul);
+      out = Fp8Matmul::apply(x, w, c)[0];
+    } else {
+      const at::NoGradGuard no_grad;
+      Fp8Kept k;
+      out = fp8_matmul_forward(c, k);
+    }
+  }
+  return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
 
