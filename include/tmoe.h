@@ -522,6 +522,36 @@ int tmoe_fp8_gemm_values(const void* x, int64_t M, int64_t row_stride, int x_dty
                          const tmoe_fp8_operand* b, int64_t K, int dtype, void* out,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* One Muon step over many tensors (no counterpart in the reference, which trains with AdamW). Each
+ * tensor is `batch` matrices (rows, cols), contiguous, one after another, and for each matrix
+ *   m = momentum m + g;  u = g + momentum m (nesterov) or m
+ *   X = u / (|u| + eps), |u| the root of the sum of its squares, transposed where rows > cols
+ *   `steps` times X = a X + (b A + c A A) X, A = X X^T, with coefficients (a, b, c)
+ *   p = p (1 - lr weight_decay) - lr update_rms sqrt(max(rows, cols)) X
+ * p and g of dtype TMOE_BF16 or TMOE_F32, m fp32; X is held in 22 bits, sums in fp32, p is rounded
+ * once. With m null in a tensor u = g. With write_only p is X instead, and need not hold
+ * anything. A matrix whose u is not finite, or the sum of whose squares is not in fp32, gets no
+ * finite p. The coefficients have to keep x in [-2, 2] and b x^2 + c x^4 in [-16, 16] over the
+ * steps from [0, 1] on (what X, A and B are stored in has no room for more). steps 1 to 16;
+ * rows, cols <= 2^22, the smaller of them <= 2^16, a tensor's elements <= 2^36; tensors without
+ * elements are passed over. Workspace of at least tmoe_muon_workspace_bytes(tensors, count) bytes,
+ * 256-byte aligned (only the sizes are read; 0: too large or wrong). What is written overlaps
+ * nothing else. Stream-ordered, no allocation, nothing copied to the device. */
+typedef struct tmoe_muon_tensor {
+  void* p;
+  const void* g;
+  float* m;
+  int64_t batch, rows, cols;
+} tmoe_muon_tensor;
+typedef struct tmoe_muon_step_args {
+  double lr, momentum, weight_decay, update_rms, eps;
+  double coefficients[3];
+  int32_t steps, nesterov, dtype, write_only;
+} tmoe_muon_step_args;
+size_t tmoe_muon_workspace_bytes(const tmoe_muon_tensor* tensors, int64_t count);
+int tmoe_muon_step(const tmoe_muon_tensor* tensors, int64_t count, const tmoe_muon_step_args* args,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* Per-stage timing, no counterpart in the reference (measurement support).
  * While enabled, every tmoe_forward records a HIP event before each of its
  * kernels and one after the last, on the forward's stream. tmoe_prof_read waits

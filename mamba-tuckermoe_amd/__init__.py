@@ -26,6 +26,8 @@ Public surface:
                                (block_train.py)
   FusedAdamW, adamw_step,      one AdamW step over many tensors, moments in 32 or 8 bits
   adamw_step_8bit              (adamw.py; dequantize_state: a state's values)
+  FusedMuon, muon_step,        one Muon step over many matrices: momentum orthogonalised by
+  orthogonalize                Newton-Schulz products (muon.py)
   synth                        seeded synthetic parameters and tokens
   fp8                          e4m3 weights with per-output-channel scales
   checkpoint                   the reference's .npz keys (layers, FFN, out_proj) and the
@@ -41,11 +43,12 @@ from .train_ops import ExpertRouting, Routing, fused_block_norm, fused_expert_ro
 from .block_fp8 import BlockFp8, fp8_block_matmul, fp8_dequantize, fp8_matmul, fp8_quantize
 from .block_train import TuckerFFNTrain
 from .adamw import FusedAdamW, adamw_step, adamw_step_8bit, dequantize_state
+from .muon import FusedMuon, muon_step, orthogonalize
 
 __all__ = ["TuckerMoE", "RMSNorm", "LayerScale", "TuckerFFN", "TuckerOutProj",
            "FusedLatentMoE", "TuckerMoETrain", "fused_latent_moe",
            "fused_router", "Routing", "fused_expert_router", "ExpertRouting", "fused_block_norm",
            "BlockFp8", "fp8_quantize", "fp8_dequantize", "fp8_block_matmul", "fp8_matmul", "TuckerFFNTrain", "FusedAdamW", "adamw_step",
-           "adamw_step_8bit", "dequantize_state",
+           "adamw_step_8bit", "dequantize_state", "FusedMuon", "muon_step", "orthogonalize",
            "TuckerMoEConfig", "Workload", "WORKLOADS", "FfnWorkload", "FFN_WORKLOADS", "load_tucker", "synth", "config", "fp8",
            "checkpoint", "_lib"]

@@ -19,8 +19,8 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(HERE, "libtmoe.so")
 
 SOURCES = ["tmoe_kernels.hip", "tmoe_static.hip", "tmoe_train.hip", "tmoe_norm_bf16.hip",
-           "tmoe_norm_f32.hip", "tmoe_expert_router.hip", "tmoe_fp8_block.hip", "tmoe_api.cpp",
-           "tmoe_train_api.cpp", "tmoe_step_api.cpp"]
+           "tmoe_norm_f32.hip", "tmoe_expert_router.hip", "tmoe_fp8_block.hip", "tmoe_muon.hip",
+           "tmoe_api.cpp", "tmoe_train_api.cpp", "tmoe_step_api.cpp"]
 # the measurement harness's hardware probes (include/tmoe_probe.h), a library of
 # their own so that libtmoe.so holds only the layer
 PROBE_SOURCES = ["tmoe_probe.hip"]

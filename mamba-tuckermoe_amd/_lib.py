@@ -59,6 +59,7 @@ EXPORTED = (
     "tmoe_expert_router_workspace_bytes", "tmoe_expert_router_forward",
     "tmoe_expert_router_backward",
     "tmoe_fp8_quantize", "tmoe_fp8_gemm_workspace_bytes", "tmoe_fp8_gemm", "tmoe_fp8_gemm_values",
+    "tmoe_muon_workspace_bytes", "tmoe_muon_step",
     "tmoe_signal_status", "tmoe_set_wait_polls", "tmoe_forward_path",
     "tmoe_forward_form",
     "tmoe_prof_enable", "tmoe_prof_read",
@@ -124,6 +125,19 @@ class TmoeFp8Operand(ctypes.Structure):
     _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)] + [
         (f, ctypes.c_int64) for f in ("rows", "row_bytes", "scale_row", "scale_block")] + [
         ("tiles", ctypes.c_int32)]
+
+
+class TmoeMuonTensor(ctypes.Structure):
+    """struct tmoe_muon_tensor."""
+    _fields_ = [(f, ctypes.c_void_p) for f in ("p", "g", "m")] + [
+        (f, ctypes.c_int64) for f in ("batch", "rows", "cols")]
+
+
+class TmoeMuonStep(ctypes.Structure):
+    """struct tmoe_muon_step_args."""
+    _fields_ = [(f, ctypes.c_double) for f in ("lr", "momentum", "weight_decay", "update_rms", "eps")] + [
+        ("coefficients", ctypes.c_double * 3)] + [
+        (f, ctypes.c_int32) for f in ("steps", "nesterov", "dtype", "write_only")]
 
 
 class TmoeError(RuntimeError):
@@ -231,6 +245,11 @@ def lib() -> ctypes.CDLL:
         L.tmoe_fp8_gemm_values.restype = ctypes.c_int
         L.tmoe_fp8_gemm_values.argtypes = [vp, i64, i64, ctypes.c_int, operand, i64, ctypes.c_int, vp,
                                            vp, sz, vp]
+        L.tmoe_muon_workspace_bytes.restype = sz
+        L.tmoe_muon_workspace_bytes.argtypes = [ctypes.POINTER(TmoeMuonTensor), i64]
+        L.tmoe_muon_step.restype = ctypes.c_int
+        L.tmoe_muon_step.argtypes = [ctypes.POINTER(TmoeMuonTensor), i64, ctypes.POINTER(TmoeMuonStep), vp,
+                                     sz, vp]
         L.tmoe_signal_status.restype = ctypes.c_int
         L.tmoe_signal_status.argtypes = [vp, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]
         L.tmoe_forward_path.restype = ctypes.c_int
@@ -285,7 +304,8 @@ def native():
                 "tmoe_block_norm_backward", "tmoe_adamw_step",
                 "tmoe_expert_router_workspace_bytes", "tmoe_expert_router_forward",
                 "tmoe_expert_router_backward", "tmoe_fp8_quantize",
-                "tmoe_fp8_gemm_workspace_bytes", "tmoe_fp8_gemm", "tmoe_fp8_gemm_values")))
+                "tmoe_fp8_gemm_workspace_bytes", "tmoe_fp8_gemm", "tmoe_fp8_gemm_values",
+                "tmoe_muon_workspace_bytes", "tmoe_muon_step")))
             _native = mod
     return _native
 

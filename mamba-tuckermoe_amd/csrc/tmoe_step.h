@@ -64,4 +64,37 @@ int64_t fp8_gemm_skinny_rows();      // up to so many rows of a may be values
 size_t fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t blocks);
 hipError_t fp8_gemm(Fp8GemmArgs a, hipStream_t st);
 
+constexpr int64_t kMuonMaxSide = (int64_t)1 << 22, kMuonMaxShort = (int64_t)1 << 16;
+
+// A tensor of `batch` matrices (rows, cols): X is (m, n), m <= n, padded to 64 each way
+struct MuonDesc {
+  void* p;
+  const void* g;
+  float* m;                // null: u = g
+  uint16_t *x[2], *xt[2];  // planes of high parts, then of low ones, a pair for each matrix
+  uint16_t *a, *b;
+  int rows, cols, mp, np;
+  uint32_t chunk0, chunks; // the first of its chunks among all tensors', and those of a matrix
+  uint32_t tile0, sym0, app0;   // the first of its tiles of each kind
+  float rate;
+};
+constexpr int kMuonTensors = 28;     // of a launch's arguments
+struct MuonChunkArgs {
+  MuonDesc* table;
+  float* sums;
+  int first, count;        // of the tensors below among all
+  float mu;
+  int nesterov;
+  MuonDesc t[kMuonTensors];
+};
+struct MuonArgs {
+  const MuonDesc* table;
+  const float* sums;
+  int count, cur, nesterov;
+  float mu, eps, a, b, c, keep;   // keep 0: p is written, not updated
+};
+size_t muon_workspace_bytes(const tmoe_muon_tensor* t, int64_t count);
+hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_args& a, void* ws,
+                hipStream_t st);
+
 }  // namespace tmoe

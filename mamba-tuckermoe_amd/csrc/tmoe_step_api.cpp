@@ -122,6 +122,31 @@ void fp8_b(tmoe::Fp8GemmArgs& g, const tmoe_fp8_operand* b, int64_t K, int dtype
   g.N = b->rows; g.K = K; g.blocks = (int)blocks_of(K); g.dtype = dtype; g.out = out;
 }
 
+bool muon_size_ok(const tmoe_muon_tensor& t) {
+  if (t.batch < 0 || t.rows < 0 || t.cols < 0 || t.rows > tmoe::kMuonMaxSide || t.cols > tmoe::kMuonMaxSide)
+    return false;
+  const int64_t lo = t.rows < t.cols ? t.rows : t.cols;
+  if (lo > tmoe::kMuonMaxShort) return false;
+  const int64_t n = t.rows * t.cols;
+  return n == 0 || t.batch <= ((int64_t)1 << 36) / n;
+}
+// Whether the polynomial keeps what the kernels store within its range, from [0, 1] on
+bool muon_stays(const double k[3], int steps) {
+  double most = 1.0;
+  for (int i = 0; i < steps; ++i) {
+    double next = 0.0;
+    constexpr int n = 512;       // (the polynomial moves little between two of so many places)
+    for (int j = 0; j <= n; ++j) {
+      const double x = most * j / n, s = x * x;
+      const double q = s * (k[1] + k[2] * s), y = fabs(x * (k[0] + q));
+      if (!(y <= 2.0) || !(fabs(q) <= 16.0) || !(fabs(k[1]) * s + fabs(k[2]) * s * s <= 64.0)) return false;
+      if (y > next) next = y;
+    }
+    most = next;
+  }
+  return true;
+}
+
 }  // namespace
 
 extern "C" {
@@ -262,6 +287,52 @@ int tmoe_fp8_gemm_values(const void* x, int64_t M, int64_t row_stride, int x_dty
   g.a = q.row_codes; g.a_bytes = q.row_bytes; g.sa = q.row_scales; g.sa_rs = 1; g.sa_ks = M;
   g.a_dtype = -1;
   return done(tmoe::fp8_gemm(g, static_cast<hipStream_t>(stream)), who);
+}
+
+size_t tmoe_muon_workspace_bytes(const tmoe_muon_tensor* t, int64_t count) {
+  if (count <= 0 || !t) return 0;
+  for (int64_t i = 0; i < count; ++i)
+    if (!muon_size_ok(t[i])) return 0;
+  return tmoe::muon_workspace_bytes(t, count);
+}
+
+int tmoe_muon_step(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_args* a, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  const char* who = "tmoe_muon_step";
+  tmoe::clear_error();
+  if (!a || count < 0 || (count > 0 && !t)) return fail(TMOE_EINVAL, "%s: null or count", who);
+  if (!dtype_ok(a->dtype))
+    return fail(TMOE_EINVAL, "%s: dtype %d is not TMOE_BF16 or TMOE_F32", who, (int)a->dtype);
+  if (a->steps < 1 || a->steps > 16) return fail(TMOE_EINVAL, "%s: steps %d (1 to 16)", who, (int)a->steps);
+  if (!(a->momentum >= 0.0 && a->momentum < 1.0))
+    return fail(TMOE_EINVAL, "%s: momentum must be in [0, 1)", who);
+  for (double v : {a->lr, a->weight_decay, a->update_rms})
+    if (!(v >= 0.0) || !isfinite((float)v))
+      return fail(TMOE_EINVAL, "%s: lr, weight_decay and update_rms must be finite and >= 0", who);
+  if (!((float)a->eps > 0.f) || !isfinite((float)a->eps))
+    return fail(TMOE_EINVAL, "%s: eps must be positive and finite", who);
+  if (!muon_stays(a->coefficients, a->steps))
+    return fail(TMOE_EINVAL, "%s: coefficients %g, %g, %g do not stay in range", who, a->coefficients[0],
+                a->coefficients[1], a->coefficients[2]);
+  const size_t es = size_of(a->dtype);
+  for (int64_t i = 0; i < count; ++i) {
+    const tmoe_muon_tensor& q = t[i];
+    if (q.batch < 0 || q.rows < 0 || q.cols < 0)
+      return fail(TMOE_EINVAL, "%s: tensor %lld: %lld of (%lld, %lld)", who, (long long)i,
+                  (long long)q.batch, (long long)q.rows, (long long)q.cols);
+    if (!muon_size_ok(q))
+      return fail(TMOE_EUNSUPPORTED, "%s: tensor %lld: %lld of (%lld, %lld)", who, (long long)i,
+                  (long long)q.batch, (long long)q.rows, (long long)q.cols);
+    if (q.batch == 0 || q.rows == 0 || q.cols == 0) continue;
+    if (!q.p || !q.g) return fail(TMOE_EINVAL, "%s: tensor %lld: null pointer", who, (long long)i);
+    if (!on(q.p, es) || !on(q.g, es) || !on(q.m, 4))
+      return fail(TMOE_EINVAL, "%s: tensor %lld: misaligned pointer", who, (long long)i);
+  }
+  const size_t need = tmoe_muon_workspace_bytes(t, count);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(TMOE_EINVAL, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
+  if (!on(workspace, 256)) return fail(TMOE_EINVAL, "%s: misaligned workspace", who);
+  return done(tmoe::muon(t, count, *a, workspace, static_cast<hipStream_t>(stream)), who);
 }
 
 }  // extern "C"

@@ -68,7 +68,7 @@ namespace {
 
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (bad_args(n, 20, "bind")) return nullptr;
+  if (bad_args(n, 22, "bind")) return nullptr;
   g_lib.workspace_bytes = reinterpret_cast<decltype(g_lib.workspace_bytes)>(address(a[0]));
   g_lib.signal_status = reinterpret_cast<decltype(g_lib.signal_status)>(address(a[1]));
   g_lib.forward_epi = reinterpret_cast<decltype(g_lib.forward_epi)>(address(a[2]));
@@ -92,6 +92,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   to(g_step.fp8_workspace_bytes, 17);
   to(g_step.fp8_gemm, 18);
   to(g_step.fp8_gemm_values, 19);
+  to(g_step.muon_workspace_bytes, 20);
+  to(g_step.muon_step, 21);
   return none();
   END_HANDLE_TH_ERRORS
 }
@@ -261,6 +263,7 @@ PyMODINIT_FUNC PyInit__tmoe_native() {
       {"fp8_quantize", (PyCFunction)(void (*)())fp8_quantize, METH_FASTCALL, nullptr},
       {"fp8_block_matmul", (PyCFunction)(void (*)())fp8_block_matmul, METH_FASTCALL, nullptr},
       {"fp8_matmul", (PyCFunction)(void (*)())fp8_matmul, METH_FASTCALL, nullptr},
+      {"muon", (PyCFunction)(void (*)())muon, METH_FASTCALL, nullptr},
       {"rmsnorm", (PyCFunction)(void (*)())rmsnorm, METH_FASTCALL, nullptr},
       {nullptr, nullptr, 0, nullptr}};
   g_gen = PyUnicode_InternFromString("_tmoe_gen");

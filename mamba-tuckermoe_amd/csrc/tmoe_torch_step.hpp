@@ -15,6 +15,8 @@ struct StepEntry {
   decltype(&tmoe_fp8_gemm_workspace_bytes) fp8_workspace_bytes;
   decltype(&tmoe_fp8_gemm) fp8_gemm;
   decltype(&tmoe_fp8_gemm_values) fp8_gemm_values;
+  decltype(&tmoe_muon_workspace_bytes) muon_workspace_bytes;
+  decltype(&tmoe_muon_step) muon_step;
 } g_step{};
 
 // ---- expert router ---------------------------------------------------------------
@@ -442,6 +444,130 @@ PyObject* fp8_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
   }
   return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- Muon ----------------------------------------------------------------------
+
+// muon(params, grads, momenta or None, lr, momentum, weight_decay, update_rms, eps, coefficients (a,
+// b, c), steps, nesterov, write only): params None: a list of new tensors like grads
+PyObject* muon(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (bad_args(nargs, 12, "muon")) return nullptr;
+  const bool write_only = a[0] == Py_None;
+  const char* const who = write_only ? "orthogonalize" : "muon_step";
+  auto list = [&](PyObject* o, const char* what, size_t want) {
+    if (!PyList_Check(o) && !PyTuple_Check(o))
+      throw torch::TypeError(std::string(who) + ": a list of tensors expected for " + what);
+    const Py_ssize_t k = PySequence_Fast_GET_SIZE(o);
+    TORCH_CHECK(want == (size_t)-1 || (size_t)k == want, who, ": ", k, " ", what, " for ", want, " gradients");
+    std::vector<at::Tensor> v;
+    v.reserve(k);
+    for (Py_ssize_t i = 0; i < k; ++i) v.push_back(tensor(PySequence_Fast_GET_ITEM(o, i)));
+    return v;
+  };
+  std::vector<at::Tensor> g = list(a[1], "gradients", (size_t)-1);
+  const size_t n = g.size();
+  std::vector<at::Tensor> p, m;
+  if (!write_only) {
+    p = list(a[0], "parameters", n);
+    m = list(a[2], "momenta", n);
+  }
+  tmoe_muon_step_args s{};
+  double num[5];
+  for (int i = 0; i < 5; ++i) num[i] = PyFloat_AsDouble(a[3 + i]);
+  if (PyErr_Occurred()) return nullptr;
+  s.lr = num[0]; s.momentum = num[1]; s.weight_decay = num[2]; s.update_rms = num[3]; s.eps = num[4];
+  if (!PyTuple_Check(a[8]) || PyTuple_GET_SIZE(a[8]) != 3)
+    throw torch::TypeError(std::string(who) + ": three coefficients expected");
+  for (int i = 0; i < 3; ++i) s.coefficients[i] = PyFloat_AsDouble(PyTuple_GET_ITEM(a[8], i));
+  if (PyErr_Occurred()) return nullptr;
+  const int64_t steps = integer(a[9]);
+  TORCH_CHECK(steps >= 1 && steps <= 16, who, ": steps ", steps, " (1 to 16)");
+  s.steps = (int32_t)steps;
+  s.nesterov = PyObject_IsTrue(a[10]);
+  s.write_only = write_only;
+  if (n == 0) return PyList_New(0);
+  const at::Device dev = g[0].device();
+  const auto dt = g[0].scalar_type();
+  s.dtype = dtype_of(g[0], who);
+  struct Span { uintptr_t at, end; };
+  std::vector<Span> written, read;
+  auto span = [](const at::Tensor& t, std::vector<Span>& to) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    if (t.numel()) to.push_back({at, at + (uintptr_t)t.numel() * t.element_size()});
+  };
+  const bool tangents = tangents_live();
+  std::vector<tmoe_muon_tensor> t(n);
+  for (size_t i = 0; i < n; ++i) {
+    TORCH_CHECK(g[i].layout() == at::kStrided, who, ": tensor ", i, ": sparse gradients are refused");
+    TORCH_CHECK(g[i].scalar_type() == dt, who, ": tensor ", i, " of ", g[i].scalar_type(), ", the first of ", dt);
+    TORCH_CHECK(g[i].dim() >= 2, who, ": tensor ", i, ": matrices (..., rows, cols) expected, got ", g[i].sizes());
+    TORCH_CHECK(g[i].device() == dev, who, ": tensor ", i, ": not all on ", dev);
+    const int64_t rows = g[i].size(-2), cols = g[i].size(-1);
+    TORCH_CHECK(std::max(rows, cols) <= (int64_t)1 << 22 && std::min(rows, cols) <= 65536, who, ": tensor ", i,
+                ": matrices of ", rows, " x ", cols, " (at most 2^22, the smaller side 65536)");
+    t[i].rows = rows;
+    t[i].cols = cols;
+    t[i].batch = rows && cols ? g[i].numel() / (rows * cols) : 0;
+    if (tangents) check_tangent(g[i], who);
+    if (write_only) continue;
+    const at::Tensor& q = p[i];
+    TORCH_CHECK(q.scalar_type() == dt && q.sizes() == g[i].sizes(), who, ": tensor ", i, ": parameter ", q.sizes(),
+                " of ", q.scalar_type(), ", gradient ", g[i].sizes(), " of ", dt);
+    TORCH_CHECK(m[i].scalar_type() == at::kFloat && m[i].sizes() == q.sizes(), who, ": tensor ", i,
+                ": momentum of float32 in the parameter's shape expected, got ", m[i].sizes(), " of ",
+                m[i].scalar_type());
+    TORCH_CHECK(q.is_contiguous() && m[i].is_contiguous(), who, ": tensor ", i,
+                ": contiguous parameters and momenta expected");
+    TORCH_CHECK(q.device() == dev && m[i].device() == dev, who, ": tensor ", i, ": not all on ", dev);
+    if (tangents) {
+      check_tangent(q, who);
+      check_tangent(m[i], who);
+    }
+    span(q, written);
+    span(m[i], written);
+    if (g[i].is_contiguous()) span(g[i], read);
+  }
+  std::sort(written.begin(), written.end(), [](Span x, Span y) { return x.at < y.at; });
+  for (size_t i = 1; i < written.size(); ++i)
+    TORCH_CHECK(written[i - 1].end <= written[i].at, who, ": two of the parameters and momenta share memory");
+  for (const Span& r : read) {      // the last written one that begins before r ends
+    const auto w = std::lower_bound(written.begin(), written.end(), r.end,
+                                    [](const Span& x, uintptr_t end) { return x.at < end; });
+    TORCH_CHECK(w == written.begin() || (w - 1)->end <= r.at, who,
+                ": a gradient shares memory with a parameter or momentum");
+  }
+  TORCH_CHECK(!(write_only && at::GradMode::is_enabled() &&
+                std::any_of(g.begin(), g.end(), [](const at::Tensor& x) { return x.requires_grad(); })),
+              who, " has no gradient: give the matrices detached");
+  check_hip(g[0], who);
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::DeviceGuard guard(dev);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    for (size_t i = 0; i < n; ++i) {
+      g[i] = g[i].contiguous();
+      if (write_only) p.push_back(at::empty(g[i].sizes(), g[i].options().requires_grad(false)));
+      t[i].p = p[i].data_ptr();
+      t[i].g = g[i].const_data_ptr();
+      t[i].m = write_only ? nullptr : m[i].data_ptr<float>();
+    }
+    const size_t nws = g_step.muon_workspace_bytes(t.data(), (int64_t)n);
+    at::Tensor ws;
+    if (nws) ws = bytes_like(g[0], nws);
+    check_rc(g_step.muon_step(t.data(), (int64_t)n, &s, out_ptr(ws), nws, current_stream(g[0])));
+    // what a graph saved of a parameter before this step is not its value any more
+    if (!write_only)
+      for (const auto* each : {&p, &m})
+        for (const at::Tensor& q : *each)
+          if (!q.is_inference()) q.unsafeGetTensorImpl()->bump_version();
+  }
+  if (!write_only) return none();
+  PyObject* out = PyList_New((Py_ssize_t)n);
+  if (!out) return nullptr;
+  for (size_t i = 0; i < n; ++i) PyList_SET_ITEM(out, (Py_ssize_t)i, THPVariable_Wrap(p[i]));
+  return out;
   END_HANDLE_TH_ERRORS
 }
 
