@@ -2,7 +2,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <vector>
 
 #include "tmoe_muon.hpp"
 
@@ -12,127 +11,167 @@ namespace {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t up(int64_t n, int64_t to) { return ceil_div(n, to) * to; }
 
-struct Shape {
-  int64_t batch, mp, np, chunks;
-};
-Shape shape_of(const tmoe_muon_tensor& t) {
-  const int64_t lo = std::min(t.rows, t.cols), hi = std::max(t.rows, t.cols);
-  return {t.batch, up(lo, 64), up(hi, 64), ceil_div(t.rows * t.cols, dev::kMuonChunk)};
-}
 bool empty(const tmoe_muon_tensor& t) { return t.batch == 0 || t.rows == 0 || t.cols == 0; }
 
-// The workspace: the table, the chunks' sums, then for each tensor X and X^T twice, A and B
-struct Layout {
-  int64_t count = 0, chunks = 0, sums, planes, total;
+struct Shape {
+  int64_t rp, cp, m, chunks, halves;   // of a matrix
 };
-Layout layout_of(const tmoe_muon_tensor* t, int64_t count) {
-  Layout l;
-  int64_t halves = 0;
-  for (int64_t i = 0; i < count; ++i) {
-    if (empty(t[i])) continue;
-    const Shape s = shape_of(t[i]);
-    ++l.count;
-    l.chunks += s.batch * s.chunks;
-    halves += s.batch * (8 * s.mp * s.np + 4 * s.mp * s.mp);
-  }
-  l.sums = up(l.count * (int64_t)sizeof(MuonDesc), 256);
-  l.planes = up(l.sums + l.chunks * 4, 256);
-  l.total = l.planes + 2 * halves;
-  return l;
+Shape shape_of(const tmoe_muon_tensor& t) {
+  Shape s;
+  s.rp = up(t.rows, 64);
+  s.cp = up(t.cols, 64);
+  s.m = t.rows > t.cols ? s.cp : s.rp;
+  s.chunks = ceil_div(t.rows * t.cols, dev::kMuonChunk);
+  s.halves = 4 * s.rp * s.cp + 4 * s.m * s.m;
+  return s;
 }
 
-template <int BT, class T>
-void gemm(int phase, const MuonArgs& a, unsigned groups, hipStream_t st) {
-  const dim3 grid(groups), block(dev::kMuonThreads);
-  switch (phase) {
-    case dev::kMuonGram: hipLaunchKernelGGL((dev::k_muon_gemm<BT, dev::kMuonGram, uint16_t>), grid, block, 0, st, a); break;
-    case dev::kMuonPoly: hipLaunchKernelGGL((dev::k_muon_gemm<BT, dev::kMuonPoly, uint16_t>), grid, block, 0, st, a); break;
-    case dev::kMuonApply: hipLaunchKernelGGL((dev::k_muon_gemm<BT, dev::kMuonApply, uint16_t>), grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL((dev::k_muon_gemm<BT, dev::kMuonLast, T>), grid, block, 0, st, a); break;
+// Tensors are stepped in groups, one after another in one workspace; a tensor that is larger is a
+// group of its own. Planes that the memory-side cache holds (256 MB) gain nothing: the 66 layers of
+// the reference model took 22.1 ms in groups of 160 MB, 18.6 of 320, 17.0 of 640, 15.8 of 1280 and
+// without a limit (48 tensors each), since each launch has a start and an end.
+constexpr int64_t kGroupBytes = (int64_t)1280 << 20;
+constexpr int64_t kTableBytes = (kMuonTensors * (int64_t)sizeof(MuonDesc) + 255) / 256 * 256;
+// the tensors from i on that are a group: their end, and what they need
+struct Group {
+  int64_t end, chunks, halves;
+  int64_t planes_at() const { return up(kTableBytes + chunks * 4, 256); }
+  int64_t bytes() const { return planes_at() + 2 * halves; }
+};
+Group group_from(const tmoe_muon_tensor* t, int64_t i, int64_t count) {
+  Group g{i, 0, 0};
+  for (int n = 0; g.end < count && n < kMuonTensors; ++g.end) {
+    if (empty(t[g.end])) continue;
+    const Shape s = shape_of(t[g.end]);
+    const int64_t halves = t[g.end].batch * s.halves;
+    if (n && 2 * (g.halves + halves) > kGroupBytes) break;
+    g.halves += halves;
+    g.chunks += t[g.end].batch * s.chunks;
+    ++n;
   }
+  return g;
+}
+
+using Small = dev::MuonTile<64, 64, 2, 2, 3>;         // 16 KB stages, three work-groups a compute unit
+using Square = dev::MuonTile<128, 128, 4, 2, 4>;      // 32 KB stages
+using Wide = dev::MuonTile<256, 128, 4, 2, 3>;        // 48 KB stages
+
+template <class TL, int PHASE, class T = uint16_t>
+void launch(const MuonArgs& a, unsigned groups, hipStream_t st) {
+  hipLaunchKernelGGL((dev::k_muon_gemm<TL, PHASE, T>), dim3(groups), dim3(TL::kThreads), 0, st, a);
+}
+template <class TL>
+void launch_symmetric(int phase, const MuonArgs& a, unsigned groups, unsigned sums, hipStream_t st) {
+  if (phase == dev::kMuonPoly) return launch<TL, dev::kMuonPoly>(a, groups, st);
+  launch<TL, dev::kMuonGram>(a, groups, st);
+  if (sums) hipLaunchKernelGGL((dev::k_muon_sum<TL>), dim3(sums), dim3(64), 0, st, a);
+}
+template <class TL>
+void launch_apply(bool last, bool bf16, const MuonArgs& a, unsigned groups, hipStream_t st) {
+  if (!last) launch<TL, dev::kMuonApply>(a, groups, st);
+  else if (bf16) launch<TL, dev::kMuonLast, uint16_t>(a, groups, st);
+  else launch<TL, dev::kMuonLast, float>(a, groups, st);
 }
 
 }  // namespace
 
 size_t muon_workspace_bytes(const tmoe_muon_tensor* t, int64_t count) {
-  const Layout l = layout_of(t, count);
-  return l.count ? (size_t)l.total : 0;
+  int64_t most = 0;
+  for (int64_t i = 0; i < count;) {
+    const Group g = group_from(t, i, count);
+    if (g.halves) most = std::max(most, g.bytes());
+    i = g.end;
+  }
+  return (size_t)most;
 }
 
 hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_args& s, void* ws, hipStream_t st) {
-  const Layout l = layout_of(t, count);
-  if (!l.count) return hipSuccess;
+  static_assert(sizeof(MuonFirstArgs) <= 4096, "a launch's arguments");
   const bool bf16 = s.dtype == TMOE_BF16;
-  // tiles of 128 where they fill the chip
-  int64_t wide = 0;
-  for (int64_t i = 0; i < count; ++i) {
-    if (empty(t[i])) continue;
-    const Shape q = shape_of(t[i]);
-    wide += q.batch * ceil_div(q.mp, 128) * ceil_div(q.np, 128);
-  }
-  const int64_t bt = wide >= 512 ? 128 : 64;
-  char* base = static_cast<char*>(ws);
-  MuonChunkArgs c{};
-  c.table = reinterpret_cast<MuonDesc*>(base);
-  c.sums = reinterpret_cast<float*>(base + l.sums);
-  c.mu = (float)s.momentum;
-  c.nesterov = s.nesterov;
-  uint16_t* plane = reinterpret_cast<uint16_t*>(base + l.planes);
-  uint32_t chunk0 = 0, tile0 = 0, sym0 = 0, app0 = 0, done = 0;
-  auto flush = [&]() {
-    if (!c.count) return hipSuccess;
-    c.first = (int)done;
-    const dim3 grid(chunk0 - c.t[0].chunk0), block(dev::kMuonThreads);
-    if (bf16) hipLaunchKernelGGL(dev::k_muon_momentum<uint16_t>, grid, block, 0, st, c);
-    else hipLaunchKernelGGL(dev::k_muon_momentum<float>, grid, block, 0, st, c);
-    done += c.count;
-    c.count = 0;
-    return hipGetLastError();
-  };
-  static_assert(sizeof(MuonChunkArgs) <= 4096, "a launch's arguments");
-  for (int64_t i = 0; i < count; ++i) {
-    if (empty(t[i])) continue;
-    const Shape q = shape_of(t[i]);
-    MuonDesc& d = c.t[c.count++];
-    d.p = t[i].p; d.g = t[i].g; d.m = t[i].m;
-    const int64_t xs = 2 * q.batch * q.mp * q.np, as = 2 * q.batch * q.mp * q.mp;
-    for (int k = 0; k < 2; ++k) {
-      d.x[k] = plane; plane += xs;
-      d.xt[k] = plane; plane += xs;
-    }
-    d.a = plane; plane += as;
-    d.b = plane; plane += as;
-    d.rows = (int)t[i].rows; d.cols = (int)t[i].cols; d.mp = (int)q.mp; d.np = (int)q.np;
-    d.chunk0 = chunk0; d.chunks = (uint32_t)q.chunks;
-    d.tile0 = tile0; d.sym0 = sym0; d.app0 = app0;
-    d.rate = s.write_only ? -1.f
-                          : (float)(s.lr * s.update_rms * sqrt((double)std::max(t[i].rows, t[i].cols)));
-    chunk0 += (uint32_t)(q.batch * q.chunks);
-    tile0 += (uint32_t)(q.batch * (q.mp / 64) * (q.np / 64));
-    const int64_t tm = ceil_div(q.mp, bt), tn = ceil_div(q.np, bt);
-    sym0 += (uint32_t)(q.batch * tm * (tm + 1) / 2);
-    app0 += (uint32_t)(q.batch * tm * tn);
-    if (c.count == kMuonTensors)
-      if (hipError_t e = flush(); e != hipSuccess) return e;
-  }
-  if (hipError_t e = flush(); e != hipSuccess) return e;
-  MuonArgs a{};
-  a.table = c.table; a.sums = c.sums; a.count = (int)l.count; a.nesterov = s.nesterov;
-  a.mu = c.mu; a.eps = (float)s.eps;
+  const dim3 block(dev::kMuonThreads);
+  MuonFirstArgs first{};
+  MuonArgs& a = first.a;
+  a.t = static_cast<MuonDesc*>(ws);
+  a.sums = reinterpret_cast<float*>(static_cast<char*>(ws) + kTableBytes);
+  a.mu = (float)s.momentum; a.eps = (float)s.eps; a.nesterov = s.nesterov; a.write_only = s.write_only;
   a.a = (float)s.coefficients[0]; a.b = (float)s.coefficients[1]; a.c = (float)s.coefficients[2];
-  a.keep = s.write_only ? 0.f : (float)(1.0 - s.lr * s.weight_decay);
-  if (bf16) hipLaunchKernelGGL(dev::k_muon_start<uint16_t>, dim3(tile0), dim3(dev::kMuonThreads), 0, st, a);
-  else hipLaunchKernelGGL(dev::k_muon_start<float>, dim3(tile0), dim3(dev::kMuonThreads), 0, st, a);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  for (int i = 0; i < s.steps; ++i) {
-    for (int phase = 0; phase < 3; ++phase) {
-      const int k = phase == dev::kMuonApply && i + 1 == s.steps ? dev::kMuonLast : phase;
-      const unsigned groups = phase < dev::kMuonApply ? sym0 : app0;
-      if (bt == 128) bf16 ? gemm<128, uint16_t>(k, a, groups, st) : gemm<128, float>(k, a, groups, st);
-      else bf16 ? gemm<64, uint16_t>(k, a, groups, st) : gemm<64, float>(k, a, groups, st);
-      if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  a.keep = (float)(1.0 - s.lr * s.weight_decay);
+  for (int64_t i = 0; i < count;) {
+    const Group g = group_from(t, i, count);
+    uint16_t* plane = reinterpret_cast<uint16_t*>(static_cast<char*>(ws) + g.planes_at());
+    // The symmetric products' tiles: 128 x 128 where those fill the chip (one of 2048 x 2048, 136
+    // of them: 801 us a step against 938 with 64 x 64; 64 of 256 x 512, 192: 359 against 341). The
+    // third product's: 256 x 128 where those fill it and are as full, for what they read less (48
+    // tensors of the reference model, 3050 of them: 16.5 ms with 128 x 128, 15.8).
+    int64_t pairs128 = 0, square = 0, wide = 0;
+    for (int64_t k = i; k < g.end; ++k) {
+      const Shape q = shape_of(t[k]);
+      if (empty(t[k])) continue;
+      const int64_t side = ceil_div(q.m, 128);
+      pairs128 += t[k].batch * side * (side + 1) / 2;
+      square += t[k].batch * ceil_div(q.rp, 128) * ceil_div(q.cp, 128);
+      wide += t[k].batch * ceil_div(q.rp, 256) * ceil_div(q.cp, 128);
     }
-    a.cur ^= 1;
+    const int64_t bt = pairs128 >= 128 && square >= 256 ? 128 : 64;
+    const int64_t bm = bt == 128 ? (20 * wide <= 11 * square ? 256 : 128) : 64, bn = bm == 64 ? 64 : 128;
+    // the Gram products' summed axes are cut into slices of about what each work-group that the
+    // chip holds has to do in the mean: a long one alone would keep the rest waiting
+    int64_t work = 0;
+    for (int64_t k = i; k < g.end; ++k) {
+      if (empty(t[k])) continue;
+      const Shape q = shape_of(t[k]);
+      const int64_t side = ceil_div(q.m, bt);
+      work += t[k].batch * side * (side + 1) / 2 * (std::max(q.rp, q.cp) / dev::kMuonK);
+    }
+    const int64_t mean = std::max(ceil_div(work, bt == 128 ? 256 : 512), bt == 128 ? (int64_t)16 : (int64_t)8);
+    uint32_t chunk0 = 0, tile0 = 0, gram0 = 0, sum0 = 0, sym0 = 0, app0 = 0;
+    a.count = a.cur = 0;
+    for (; i < g.end; ++i) {
+      if (empty(t[i])) continue;
+      const Shape q = shape_of(t[i]);
+      MuonDesc& d = first.t[a.count++];
+      d.p = t[i].p; d.g = t[i].g; d.m = t[i].m;
+      d.planes = plane;
+      plane += t[i].batch * q.halves;
+      d.rows = (int)t[i].rows; d.cols = (int)t[i].cols;
+      d.chunk0 = chunk0; d.chunks = (uint32_t)q.chunks;
+      d.tile0 = tile0; d.gram0 = gram0; d.sum0 = sum0; d.sym0 = sym0; d.app0 = app0;
+      d.rate = s.write_only ? -1.f
+                            : (float)(s.lr * s.update_rms * sqrt((double)std::max(t[i].rows, t[i].cols)));
+      const int64_t side = ceil_div(q.m, bt), pairs = side * (side + 1) / 2;
+      const int64_t all = std::max(q.rp, q.cp) / dev::kMuonK;
+      // (the slices' sums have to find room in X')
+      const int64_t n = std::max(std::min(ceil_div(all, mean), q.rp * q.cp / (pairs * bt * bt)), (int64_t)1);
+      d.slice_tiles = (int)ceil_div(all, n);
+      d.slices = (int)ceil_div(all, d.slice_tiles);
+      gram0 += (uint32_t)(t[i].batch * pairs * d.slices);
+      if (d.slices > 1) sum0 += (uint32_t)(t[i].batch * pairs * (bt / 32) * (bt / 32));
+      chunk0 += (uint32_t)(t[i].batch * q.chunks);
+      tile0 += (uint32_t)(t[i].batch * ceil_div(q.rp * q.cp, dev::kMuonChunk));
+      sym0 += (uint32_t)(t[i].batch * pairs);
+      app0 += (uint32_t)(t[i].batch * ceil_div(q.rp, bm) * ceil_div(q.cp, bn));
+    }
+    if (!a.count) continue;
+    if (bf16) {
+      hipLaunchKernelGGL(dev::k_muon_momentum<uint16_t>, dim3(chunk0), block, 0, st, first);
+      hipLaunchKernelGGL(dev::k_muon_start<uint16_t>, dim3(tile0), block, 0, st, a);
+    } else {
+      hipLaunchKernelGGL(dev::k_muon_momentum<float>, dim3(chunk0), block, 0, st, first);
+      hipLaunchKernelGGL(dev::k_muon_start<float>, dim3(tile0), block, 0, st, a);
+    }
+    for (int k = 0; k < s.steps; ++k) {
+      for (int phase : {dev::kMuonGram, dev::kMuonPoly}) {
+        const unsigned groups = phase == dev::kMuonGram ? gram0 : sym0;
+        if (bt == 128) launch_symmetric<Square>(phase, a, groups, sum0, st);
+        else launch_symmetric<Small>(phase, a, groups, sum0, st);
+      }
+      const bool last = k + 1 == s.steps;
+      if (bm == 256) launch_apply<Wide>(last, bf16, a, app0, st);
+      else if (bm == 128) launch_apply<Square>(last, bf16, a, app0, st);
+      else launch_apply<Small>(last, bf16, a, app0, st);
+      a.cur ^= 1;
+    }
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   return hipSuccess;
 }

@@ -66,32 +66,28 @@ hipError_t fp8_gemm(Fp8GemmArgs a, hipStream_t st);
 
 constexpr int64_t kMuonMaxSide = (int64_t)1 << 22, kMuonMaxShort = (int64_t)1 << 16;
 
-// A tensor of `batch` matrices (rows, cols): X is (m, n), m <= n, padded to 64 each way
+// A tensor of matrices (rows, cols). planes: each matrix's X, X', A and B (MuonPlanes)
 struct MuonDesc {
   void* p;
   const void* g;
   float* m;                // null: u = g
-  uint16_t *x[2], *xt[2];  // planes of high parts, then of low ones, a pair for each matrix
-  uint16_t *a, *b;
-  int rows, cols, mp, np;
-  uint32_t chunk0, chunks; // the first of its chunks among all tensors', and those of a matrix
-  uint32_t tile0, sym0, app0;   // the first of its tiles of each kind
+  uint16_t* planes;
+  int rows, cols;
+  uint32_t chunk0, chunks; // the first of its chunks among the group's, and those of a matrix
+  uint32_t tile0, gram0, sum0, sym0, app0;   // the first of its work-groups of each kind
+  int slices, slice_tiles; // the Gram product's of its summed axis
   float rate;
 };
-constexpr int kMuonTensors = 28;     // of a launch's arguments
-struct MuonChunkArgs {
-  MuonDesc* table;
-  float* sums;
-  int first, count;        // of the tensors below among all
-  float mu;
-  int nesterov;
-  MuonDesc t[kMuonTensors];
-};
+constexpr int kMuonTensors = 48;     // of a group
 struct MuonArgs {
-  const MuonDesc* table;
-  const float* sums;
-  int count, cur, nesterov;
-  float mu, eps, a, b, c, keep;   // keep 0: p is written, not updated
+  MuonDesc* t;             // the group's tensors, in the workspace
+  float* sums;
+  int count, cur, nesterov, write_only;
+  float mu, eps, a, b, c, keep;
+};
+struct MuonFirstArgs {     // the first launch's, which writes them there
+  MuonArgs a;
+  MuonDesc t[kMuonTensors];
 };
 size_t muon_workspace_bytes(const tmoe_muon_tensor* t, int64_t count);
 hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_args& a, void* ws,
