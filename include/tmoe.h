@@ -506,7 +506,7 @@ int tmoe_expert_router_backward(const tmoe_expert_router* router, const int64_t*
  * in fp32. tmoe_fp8_gemm_values: the same with a the operand that quantising x (M, K) by rows
  * would make. The order of its sums depends on the sizes alone. K, N and the rows of an operand
  * <= 2^23, M of out <= 2^23. Workspaces of at least tmoe_fp8_gemm_workspace_bytes(M, N, K,
- * values) bytes (0: none), 16-byte aligned. M == 0 is a no-op. Stream-ordered, no allocation. */
+ * dtype, values) bytes (0: none), 16-byte aligned. M == 0 is a no-op. Stream-ordered, no allocation. */
 typedef struct tmoe_fp8_operand {
   void* codes;
   float* scales;
@@ -515,7 +515,7 @@ typedef struct tmoe_fp8_operand {
 } tmoe_fp8_operand;
 int tmoe_fp8_quantize(const void* x, int64_t R, int64_t C, int64_t row_stride, int dtype,
                       const tmoe_fp8_operand* rows, const tmoe_fp8_operand* cols, void* stream);
-size_t tmoe_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int values);
+size_t tmoe_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int values);
 int tmoe_fp8_gemm(const tmoe_fp8_operand* a, const tmoe_fp8_operand* b, int64_t K, int dtype,
                   void* out, void* workspace, size_t workspace_bytes, void* stream);
 int tmoe_fp8_gemm_values(const void* x, int64_t M, int64_t row_stride, int x_dtype,

@@ -239,7 +239,7 @@ def lib() -> ctypes.CDLL:
         L.tmoe_fp8_quantize.restype = ctypes.c_int
         L.tmoe_fp8_quantize.argtypes = [vp, i64, i64, i64, ctypes.c_int, operand, operand, vp]
         L.tmoe_fp8_gemm_workspace_bytes.restype = sz
-        L.tmoe_fp8_gemm_workspace_bytes.argtypes = [i64, i64, i64, ctypes.c_int]
+        L.tmoe_fp8_gemm_workspace_bytes.argtypes = [i64, i64, i64, ctypes.c_int, ctypes.c_int]
         L.tmoe_fp8_gemm.restype = ctypes.c_int
         L.tmoe_fp8_gemm.argtypes = [operand, operand, i64, ctypes.c_int, vp, vp, sz, vp]
         L.tmoe_fp8_gemm_values.restype = ctypes.c_int

@@ -335,8 +335,24 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_gemm(Fp8GemmArgs a) {
         const int r = BM + wn * FN * 32 + j * 32 + (lane & 31);
         bf[j][k] = join8(s[lds_slot(r, 4 * k + (lane >> 5))], s[lds_slot(r, 4 * k + 2 + (lane >> 5))]);
       }
+    // B's scales: one, or those of the columns that the lane's elements lie in. These are read by
+    // assembly with its wait: the compiler takes them for what the loads in flight write and waits
+    // for those (M = 768, N = 4608, K = 16384: 120 us so, 103 as it is).
     float sb1 = 0.f;
-    if constexpr (!kBRows) sb1 = sc[BM + wn * FN * 32 / 128];
+    u32x4 sb[kBRows ? FN : 1][4];
+    if constexpr (kBRows) {
+      static_assert(FN == 2, "the reads below");
+      const uint32_t at = (uint32_t)(size_t)(lds_vptr)(smem + st * TL::kStageBytes + (BM + BN) * 128) +
+                          (BM + wn * FN * 32) * 4 + (lane >> 5) * 16;
+      asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:32\n\tds_read_b128 %2, %8 offset:64\n\t"
+                   "ds_read_b128 %3, %8 offset:96\n\tds_read_b128 %4, %8 offset:128\n\tds_read_b128 %5, %8 offset:160\n\t"
+                   "ds_read_b128 %6, %8 offset:192\n\tds_read_b128 %7, %8 offset:224\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(sb[0][0]), "=&v"(sb[0][1]), "=&v"(sb[0][2]), "=&v"(sb[0][3]), "=&v"(sb[1][0]),
+                     "=&v"(sb[1][1]), "=&v"(sb[1][2]), "=&v"(sb[1][3])
+                   : "v"(at) : "memory");
+    } else {
+      sb1 = sc[BM + wn * FN * 32 / 128];
+    }
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       i32x8 af[2];
@@ -351,14 +367,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_gemm(Fp8GemmArgs a) {
         t = mma_fp8<kExact>(bf[j][1], af[1], t);
         if constexpr (kBRows) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float4 sb4 = *reinterpret_cast<const float4*>(sc + BM + wn * FN * 32 + j * 32 + 8 * q +
-                                                                4 * (lane >> 5));
-            acc[i][j][4 * q] = fmaf(t[4 * q], sa1 * sb4.x, acc[i][j][4 * q]);
-            acc[i][j][4 * q + 1] = fmaf(t[4 * q + 1], sa1 * sb4.y, acc[i][j][4 * q + 1]);
-            acc[i][j][4 * q + 2] = fmaf(t[4 * q + 2], sa1 * sb4.z, acc[i][j][4 * q + 2]);
-            acc[i][j][4 * q + 3] = fmaf(t[4 * q + 3], sa1 * sb4.w, acc[i][j][4 * q + 3]);
-          }
+          for (int e = 0; e < 16; ++e)
+            acc[i][j][e] = fmaf(t[e], sa1 * __uint_as_float(sb[j][e / 4][e % 4]), acc[i][j][e]);
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(t[e], sa1, acc[i][j][e]);

@@ -91,9 +91,9 @@ int fp8_check(const char* who, const char* what, const tmoe_fp8_operand* o, int6
 struct Fp8Workspace {
   size_t planes, codes, scales, total;
 };
-Fp8Workspace fp8_workspace(int64_t M, int64_t N, int64_t K, bool values) {
+Fp8Workspace fp8_workspace(int64_t M, int64_t N, int64_t K, bool values, int dtype) {
   Fp8Workspace w{};
-  w.planes = (size_t)up16((int64_t)tmoe::fp8_gemm_workspace_bytes(M, N, blocks_of(K)));
+  w.planes = (size_t)up16((int64_t)tmoe::fp8_gemm_workspace_bytes(M, N, blocks_of(K), dtype));
   if (values && M > tmoe::fp8_gemm_skinny_rows()) {
     w.codes = (size_t)(M * blocks_of(K) * 128);
     w.scales = (size_t)up16(M * blocks_of(K) * 4);
@@ -229,9 +229,9 @@ int tmoe_fp8_quantize(const void* x, int64_t R, int64_t C, int64_t row_stride, i
   return done(tmoe::fp8_quantize(a, static_cast<hipStream_t>(stream)), who);
 }
 
-size_t tmoe_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int values) {
-  if (!fp8_sizes_ok(M, N, K)) return 0;
-  return fp8_workspace(M, N, K, values != 0).total;
+size_t tmoe_fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int values) {
+  if (!fp8_sizes_ok(M, N, K) || !dtype_ok(dtype)) return 0;
+  return fp8_workspace(M, N, K, values != 0, dtype).total;
 }
 
 int tmoe_fp8_gemm(const tmoe_fp8_operand* a, const tmoe_fp8_operand* b, int64_t K, int dtype, void* out,
@@ -241,7 +241,7 @@ int tmoe_fp8_gemm(const tmoe_fp8_operand* a, const tmoe_fp8_operand* b, int64_t 
   if (int rc = fp8_check(who, "a", a, a ? a->rows : 0, K)) return rc;
   if (int rc = fp8_check(who, "b", b, b ? b->rows : 0, K)) return rc;
   const int64_t M = a->rows;
-  const size_t need = tmoe_fp8_gemm_workspace_bytes(M, b->rows, K, 0);
+  const size_t need = tmoe_fp8_gemm_workspace_bytes(M, b->rows, K, dtype, 0);
   if (int rc = fp8_gemm_check(who, M, b, K, dtype, out, workspace, workspace_bytes, need)) return rc;
   tmoe::Fp8GemmArgs g{};
   fp8_b(g, b, K, dtype, out);
@@ -262,7 +262,7 @@ int tmoe_fp8_gemm_values(const void* x, int64_t M, int64_t row_stride, int x_dty
   if (M < 0) return fail(TMOE_EINVAL, "%s: M=%lld", who, (long long)M);
   if (M > tmoe::kFp8MaxDim)
     return fail(TMOE_EUNSUPPORTED, "%s: M=%lld (at most 2^23)", who, (long long)M);
-  const Fp8Workspace w = fp8_workspace(M, b->rows < 1 ? 1 : b->rows, K, true);
+  const Fp8Workspace w = fp8_workspace(M, b->rows < 1 ? 1 : b->rows, K, true, dtype);
   if (int rc = fp8_gemm_check(who, M, b, K, dtype, out, workspace, workspace_bytes, w.total)) return rc;
   if (M == 0) return TMOE_OK;
   if (!x) return fail(TMOE_EINVAL, "%s: null x", who);

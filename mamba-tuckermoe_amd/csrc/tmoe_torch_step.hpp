@@ -216,7 +216,7 @@ at::Tensor fp8_product(const Fp8& a, const Fp8& b, int64_t K, at::ScalarType dt)
   const int64_t M = a.codes.size(0), N = b.codes.size(0);
   at::Tensor out = at::empty({M, N}, a.codes.options().dtype(dt));
   if (M == 0) return out;
-  const size_t nws = g_step.fp8_workspace_bytes(M, N, K, 0);
+  const size_t nws = g_step.fp8_workspace_bytes(M, N, K, code_of(dt), 0);
   at::Tensor ws;
   if (nws) ws = bytes_like(out, nws);
   const tmoe_fp8_operand x = a.args(), y = b.args();
@@ -227,7 +227,7 @@ at::Tensor fp8_product(const Rows& a, int64_t M, const Fp8& b, int64_t K, at::Sc
   const int64_t N = b.codes.size(0);
   at::Tensor out = at::empty({M, N}, a.t.options().dtype(dt).requires_grad(false));
   if (M == 0) return out;
-  const size_t nws = g_step.fp8_workspace_bytes(M, N, K, 1);
+  const size_t nws = g_step.fp8_workspace_bytes(M, N, K, code_of(dt), 1);
   at::Tensor ws;
   if (nws) ws = bytes_like(out, nws);
   const tmoe_fp8_operand y = b.args();

@@ -74,8 +74,9 @@ def test_abi_refusals(pkg):
     L = pkg._lib.lib()
     r, a = ctypes.byref, _op(pkg)
     need = L.tmoe_fp8_gemm_workspace_bytes
-    assert need(-1, 64, 64, 0) == need(4, 0, 64, 0) == need(4, 64, 0, 0) == need(2 ** 23 + 1, 1, 1, 1) == 0
-    assert need(16, 64, 300, 1) == 0 and need(100, 64, 300, 1) >= 100 * 384 + 100 * 12
+    assert need(-1, 64, 64, 0, 0) == need(4, 0, 64, 0, 0) == need(4, 64, 0, 0, 0) == need(2 ** 23 + 1, 1, 1, 0, 1) == 0
+    assert need(64, 64, 64, 2, 1) == 0
+    assert need(16, 64, 300, 0, 1) == 0 and need(100, 64, 300, 0, 1) >= 100 * 384 + 100 * 12
     assert L.tmoe_fp8_gemm(None, r(a), 200, 0, 64, 64, 1 << 40, None) == -1
     assert L.tmoe_fp8_gemm(r(a), None, 200, 0, 64, 64, 1 << 40, None) == -1
     for K, dt, out, ws, n, code in ((0, 0, 64, 64, 1 << 40, -1), (2 ** 23 + 1, 0, 64, 64, 1 << 40, -2),
@@ -83,11 +84,11 @@ def test_abi_refusals(pkg):
                                     (200, 0, 72, 64, 1 << 40, -1), (200, 0, 64, 72, 1 << 40, -1)):
         assert L.tmoe_fp8_gemm(r(a), r(a), K, dt, out, ws, n, None) == code
         assert L.tmoe_fp8_gemm_values(64, 64, max(K, 200), 0, r(a), K, dt, out, ws, n, None) == code
-    n = need(64, 64, 200, 1)
+    n = need(64, 64, 200, 0, 1)
     assert n > 0 and L.tmoe_fp8_gemm_values(64, 64, 200, 0, r(a), 200, 0, 64, 64, n - 1, None) == -1
     assert L.tmoe_fp8_gemm_values(64, 64, 200, 0, r(a), 200, 0, 64, 0, n, None) == -1
     big = _op(pkg, rows=64, row_bytes=4096)
-    split = need(64, 64, 4096, 0)
+    split = need(64, 64, 4096, 0, 0)
     assert split == 0 or L.tmoe_fp8_gemm(r(big), r(big), 4096, 0, 64, 64, split - 1, None) == -1
     for x, M, rs, dt, code in ((0, 64, 200, 0, -1), (65, 64, 200, 0, -1), (64, 64, 199, 0, -1), (64, 64, 200, 2, -1),
                                (64, -1, 200, 0, -1), (64, 2 ** 23 + 1, 200, 0, -2)):
