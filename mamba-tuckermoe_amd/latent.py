@@ -19,11 +19,14 @@ Indices get no gradient (as in the reference).
 """
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 
 from . import _lib
+from .block_fp8 import fp8_matmul
 from .module import device_guard, launch_stream
-from .train_ops import fused_router
+from .train_ops import fused_expert_router, fused_router
 
 
 def _ws(nbytes: int, dev) -> torch.Tensor:
@@ -129,12 +132,25 @@ class TuckerMoETrain(torch.nn.Module):
     whatever x's dtype, the lowest index first on ties, `expert_counts` (E, int64) after
     each forward, and forward takes a mask of tokens ((...) bool, False: left out of the
     losses and of the contraction; its row of out is the bias; its row of x has to be
-    finite all the same, a padding token's embedding say)."""
+    finite all the same, a padding token's embedding say).
+
+    Two options are beyond the reference. `routing`, a dict of train_ops.fused_expert_router's
+    score, groups, top_groups, renormalize and scale (empty: their defaults), routes by that
+    instead, without a temperature and without losses (0.0 each): what keeps the experts even is
+    `balance_bias` (E; a buffer, float32 whatever the module is cast to), which update_balance()
+    moves after a step. `fp8_products` makes the products with U_in and U_out, forward and
+    backward, in 8-bit blocks (block_fp8.fp8_matmul)."""
+
+    _ROUTING = ("score", "groups", "top_groups", "renormalize", "scale")
 
     def __init__(self, dim_in, dim_out, num_experts=8, top_k=2, r1=4, r2=1024, r3=256,
-                 fused_router=False):
+                 fused_router=False, routing: Optional[dict] = None, fp8_products=False):
         super().__init__()
+        if routing is not None and not set(routing) <= set(self._ROUTING):
+            raise ValueError(f"TuckerMoETrain: routing {routing}: options are {', '.join(self._ROUTING)}")
         self.fused_router = fused_router
+        self.routing = None if routing is None else dict(routing)
+        self.fp8_products = fp8_products
         self.expert_counts = None
         self.num_experts = num_experts
         self.top_k = min(top_k, num_experts)
@@ -150,19 +166,46 @@ class TuckerMoETrain(torch.nn.Module):
         torch.nn.init.orthogonal_(self.U_out)
         torch.nn.init.xavier_uniform_(self.U_expert)
         torch.nn.init.xavier_uniform_(self.core)
+        if routing is not None:
+            self.register_buffer("balance_bias", torch.zeros(num_experts))
+
+    def _apply(self, fn, recurse=True):
+        # a cast to bfloat16 would lose the bias's steps, of 1e-3 beside a bias near one
+        bias = getattr(self, "balance_bias", None)
+        super()._apply(fn, recurse)
+        if bias is not None and self.balance_bias.dtype != torch.float32:
+            self.balance_bias = bias.to(self.balance_bias.device, torch.float32)
+        return self
+
+    @torch.no_grad()
+    def update_balance(self, rate: float = 1e-3) -> None:
+        """balance_bias += rate sign(mean count - count) by the last forward's expert_counts (of
+        all ranks, if they have been summed into it): experts with more tokens than the mean come
+        to be selected less. Nothing but the selection sees the bias."""
+        if self.routing is None or self.expert_counts is None:
+            raise RuntimeError("TuckerMoETrain: update_balance() follows a forward of a layer with routing=")
+        c = self.expert_counts.float()
+        self.balance_bias.add_(torch.sign(c.mean() - c), alpha=rate)
+
+    def _product(self, x, u):
+        return fp8_matmul(x, u) if self.fp8_products else torch.matmul(x, u)
 
     def _route(self, xf, step, mask):
         """(idx, top_p, lb_loss, z_loss)."""
-        temperature = router_temperature(step)
         raw = self.router(xf)
+        if mask is not None:
+            mask = mask.reshape(-1)
+        if self.routing is not None:
+            idx, top_p, self.expert_counts = fused_expert_router(
+                raw, self.top_k, bias=self.balance_bias, mask=mask, **self.routing)
+            return idx, top_p, 0.0, 0.0
+        temperature = router_temperature(step)
         if self.fused_router:
-            if mask is not None:
-                mask = mask.reshape(-1)
             idx, top_p, lb_loss, z_loss, self.expert_counts = fused_router(
                 raw, self.top_k, temperature, 10.0, mask)
             return (idx, top_p, lb_loss, z_loss) if self.training else (idx, top_p, 0.0, 0.0)
         if mask is not None:
-            raise RuntimeError("TuckerMoETrain: a mask needs fused_router=True")
+            raise RuntimeError("TuckerMoETrain: a mask needs fused_router=True or routing=")
         capped = scaled_tanh(raw, 10.0)
         z_loss = torch.mean(torch.logsumexp(capped, dim=-1) ** 2) if self.training else 0.0
         logits = capped / temperature
@@ -181,8 +224,8 @@ class TuckerMoETrain(torch.nn.Module):
         orig = x.shape
         xf = x.reshape(-1, orig[-1])
         idx, top_p, lb_loss, z_loss = self._route(xf, step, mask)
-        xs = self.inner_norm(torch.matmul(xf, self.U_in))
+        xs = self.inner_norm(self._product(xf, self.U_in))
         G = torch.einsum("er,rst->est", self.U_expert, self.core)
         core = FusedLatentMoE.apply(xs, G, idx, top_p).to(x.dtype)
-        out = torch.matmul(core, self.U_out).reshape(*orig[:-1], -1)
+        out = self._product(core, self.U_out).reshape(*orig[:-1], -1)
         return out + self.bias, lb_loss, z_loss

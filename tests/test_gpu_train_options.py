@@ -1,0 +1,195 @@
+"""TuckerMoETrain and TuckerFFNTrain with fused_expert_router and fp8_matmul, and training steps of
+them with FusedMuon beside FusedAdamW."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import tucker_moe_np as onp
+from test_gpu_train_ops import _latent_torch, _norm64, dtypes, f64
+
+pytestmark = pytest.mark.gpu
+
+
+def _expert_router64(raw, top_k, score="softmax", bias=None, groups=1, top_groups=None, renormalize=True,
+                     scale=1.0, mask=None):
+    B, E = raw.shape
+    s = torch.sigmoid(raw) if score == "sigmoid" else torch.softmax(raw, -1)
+    b = s.detach() + bias.double()
+    per = E // groups
+    worth = b.view(B, groups, per).topk(min(2, per), -1).values.sum(-1)
+    keep = torch.zeros_like(worth).scatter_(1, worth.topk(top_groups or groups, -1).indices, 1.0)
+    idx = b.masked_fill(keep.repeat_interleave(per, 1) == 0, -np.inf).topk(top_k, -1).indices
+    w = s.gather(-1, idx)
+    if renormalize:
+        w = w / (w.sum(-1, keepdim=True) + 1e-20)
+    w = scale * w
+    counts = torch.zeros(E, dtype=torch.int64)
+    if mask is not None:
+        w = w * mask[:, None]
+    counts.index_add_(0, (idx if mask is None else idx[mask]).reshape(-1), torch.ones((), dtype=torch.int64).expand(
+        idx.numel() if mask is None else idx[mask].numel()))
+    return idx, w, counts
+
+
+ROUTINGS = [{}, {"score": "sigmoid", "groups": 4, "top_groups": 2, "scale": 2.5},
+            {"score": "sigmoid", "renormalize": False, "scale": 0.5}]
+
+
+@pytest.mark.parametrize("padded", [False, True])
+@pytest.mark.parametrize("routing", ROUTINGS, ids=["softmax", "groups", "plain"])
+def test_routing_gradients(pkg, dev, monkeypatch, routing, padded):
+    """TuckerFFNTrain with a routing: output, counts and every gradient against the same module in
+    float64 on the CPU with plain expressions in the operators' places."""
+    import mamba_tuckermoe_amd.block_train as bt
+    import mamba_tuckermoe_amd.latent as lat
+    cfg = pkg.TuckerMoEConfig(kmoe_num_experts=8, kmoe_r1=4, kmoe_r2=64, kmoe_r3=64, ffn_expand=2)
+    torch.manual_seed(0)
+    m = pkg.TuckerFFNTrain(64, cfg, routing=routing).train()
+    ref = pkg.TuckerFFNTrain(64, cfg, routing=routing).double().train()
+    with torch.no_grad():
+        for l in (m.ffn_gate, m.ffn_up, m.ffn_down):
+            l.router.weight.mul_(30)
+            l.core.mul_(6)
+            l.balance_bias.copy_(0.1 * torch.randn(8))
+    ref.load_state_dict(m.state_dict())
+    x = torch.randn(3, 50, 64)
+    mask = torch.rand(3, 50) > 0.3 if padded else None
+    with monkeypatch.context() as mp:
+        mp.setattr(lat.FusedLatentMoE, "apply", staticmethod(_latent_torch))
+        mp.setattr(lat, "fused_expert_router", _expert_router64)
+        mp.setattr(bt, "fused_block_norm", _norm64)
+        xr = x.double().requires_grad_()
+        o_ref, lb, z = ref(xr, mask=mask)
+        assert (lb, z) == (0.0, 0.0)
+        o_ref.square().mean().backward()
+    m = m.to(dev)
+    xg = x.to(dev).requires_grad_()
+    o, lb, z = m(xg, mask=None if mask is None else mask.to(dev))
+    assert (lb, z) == (0.0, 0.0)
+    o.square().mean().backward()
+    assert onp.rel_l2(f64(o), f64(o_ref)) <= 1e-5
+    for n in ("ffn_gate", "ffn_up", "ffn_down"):
+        assert torch.equal(getattr(m, n).expert_counts.cpu(), getattr(ref, n).expert_counts), n
+    assert onp.rel_l2(f64(xg.grad), f64(xr.grad)) <= 1e-4
+    for (name, p), (_, q) in zip(m.named_parameters(), ref.named_parameters()):
+        assert onp.rel_l2(f64(p.grad), f64(q.grad)) <= 1e-4, name
+
+
+@dtypes
+def test_fp8_products_are_fp8_matmul(pkg, dev, dtype):
+    """The layer with fp8_products is the same expressions with fp8_matmul for its two products, bit
+    for bit, at odd sizes."""
+    torch.manual_seed(3)
+    m = pkg.TuckerMoETrain(100, 77, num_experts=8, r2=64, r3=64, fp8_products=True, routing={}).to(dev, dtype)
+    x = torch.randn(3, 67, 100, device=dev).to(dtype).requires_grad_()
+    g = torch.randn(3, 67, 77, device=dev).to(dtype)
+    out, _, _ = m(x)
+    got = torch.autograd.grad(out, [x, *m.parameters()], g)
+    xf = x.reshape(-1, 100)
+    r = pkg.fused_expert_router(m.router(xf), 2, bias=m.balance_bias)
+    xs = m.inner_norm(pkg.fp8_matmul(xf, m.U_in))
+    core = pkg.FusedLatentMoE.apply(xs, torch.einsum("er,rst->est", m.U_expert, m.core), r.idx, r.weights)
+    want_out = pkg.fp8_matmul(core, m.U_out).reshape(3, 67, 77) + m.bias
+    assert torch.equal(out, want_out)
+    for u, v in zip(got, torch.autograd.grad(want_out, [x, *m.parameters()], g)):
+        assert torch.equal(u, v)
+    full = pkg.TuckerMoETrain(100, 77, num_experts=8, r2=64, r3=64, routing={}).to(dev, dtype)
+    full.load_state_dict(m.state_dict())
+    assert not torch.equal(full(x)[0], out)
+
+
+def _split(m):
+    """Matrices of the layers for Muon, the rest for AdamW."""
+    muon, rest = [], []
+    for n, p in m.named_parameters():
+        (muon if n.split(".")[-1] in ("U_in", "U_out", "core") else rest).append(p)
+    return muon, rest
+
+
+@dtypes
+def test_training_steps_run_together(pkg, dev, dtype):
+    """Routing by biased scores, 8-bit products, the contraction, Muon and AdamW over a few steps:
+    all finite, every parameter moved by no more than its optimizer's bound, each bias a multiple of
+    the rate. Muon's polynomial takes a singular value of [0, 1.21] to 1.21 at most (1.2024 at 0.555,
+    its only maximum there, and 0.98 at 1.21), so that a step is of Frobenius norm
+    lr 0.2 sqrt(max) 1.25 sqrt(min) at most, its products' roundings with it; a bfloat16
+    parameter's rounding adds 2^-8 of it a step."""
+    cfg = pkg.TuckerMoEConfig(kmoe_num_experts=8, kmoe_r1=4, kmoe_r2=128, kmoe_r3=128, ffn_expand=2)
+    torch.manual_seed(0)
+    m = pkg.TuckerFFNTrain(128, cfg, routing={"score": "sigmoid", "groups": 4, "top_groups": 2},
+                           fp8_products=True).to(dev, dtype).train()
+    muon, rest = _split(m)
+    assert len(muon) == 9
+    opts = [pkg.FusedMuon(muon, lr=1e-2, weight_decay=0.0),
+            pkg.FusedAdamW(rest, lr=1e-2, betas=(0.9, 0.95), weight_decay=0.0)]
+    start = {n: p.detach().clone() for n, p in m.named_parameters()}
+    x = torch.randn(400, 128, device=dev).to(dtype)
+    mask = torch.arange(400, device=dev) < 350
+    n_steps = 3
+    for step in range(n_steps):
+        for o in opts:
+            o.zero_grad()
+        out, lb, z = m(x, mask=mask)
+        assert (lb, z) == (0.0, 0.0)
+        out.float().square().mean().backward()
+        for o in opts:
+            o.step()
+        m.update_balance(2.0 ** -10)
+        assert out.isfinite().all()
+        for l in (m.ffn_gate, m.ffn_up, m.ffn_down):
+            assert l.expert_counts.sum().item() == 2 * 350
+    for n, p in m.named_parameters():
+        q = start[n]
+        moved = p.detach().double() - q.double()
+        assert p.isfinite().all() and moved.abs().max() > 0, n
+        if n.split(".")[-1] in ("U_in", "U_out", "core"):
+            a, b = sorted(p.shape[-2:])
+            bound = n_steps * 1e-2 * 0.2 * b ** 0.5 * 1.25 * a ** 0.5
+            size = moved.flatten(-2).norm(dim=-1)
+            room = n_steps * 2.0 ** -8 * (q.double().flatten(-2).norm(dim=-1) + bound)
+            assert (size <= bound + room).all(), n
+        else:
+            assert moved.abs().max() <= n_steps * 1e-2 * 2.5 + 2.0 ** -7 * q.double().abs().max(), n
+    for l in (m.ffn_gate, m.ffn_up, m.ffn_down):
+        u = l.balance_bias * 2.0 ** 10
+        assert torch.equal(u, u.round()) and 0 < u.abs().max() <= n_steps and u.dtype == torch.float32
+
+
+def test_a_captured_step(pkg, dev):
+    """Routing, 8-bit products, contraction, their backward and a Muon step as one graph, replayed with
+    new tokens and eager work between: the bits of the eager steps."""
+    torch.manual_seed(5)
+    x = torch.randn(192, 128, device=dev)
+    g = torch.randn(192, 96, device=dev)
+    wr = torch.randn(128, 8, device=dev)
+    bias = 0.1 * torch.randn(8, device=dev)
+
+    def parts():
+        torch.manual_seed(6)
+        ps = [torch.nn.Parameter(torch.randn(s, device=dev) * 0.1) for s in ((128, 64), (8, 64, 64), (64, 96))]
+        return ps, pkg.FusedMuon(ps, lr=0.01)
+
+    def step(ps, opt, x):
+        with torch.no_grad():
+            raw = x @ wr
+        r = pkg.fused_expert_router(raw, 2, "sigmoid", bias, groups=4, top_groups=2)
+        y = pkg.fp8_matmul(pkg.FusedLatentMoE.apply(pkg.fp8_matmul(x, ps[0]), ps[1], r.idx, r.weights), ps[2])
+        for p, d in zip(ps, torch.autograd.grad(y, ps, g)):
+            p.grad = d
+        opt.step()
+    (pe, oe), (pc, oc) = parts(), parts()
+    batches = [torch.randn(192, 128, device=dev) for _ in range(4)]
+    for ps, o in ((pe, oe), (pc, oc)):
+        step(ps, o, batches[0])
+    x.copy_(batches[1])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(pc, oc, x)
+    for b in batches[1:]:
+        x.copy_(b)
+        graph.replay()
+        step(pe, oe, b)
+        torch.cuda.synchronize()
+        for u, v in zip(pe, pc):
+            assert torch.equal(u, v)
