@@ -51,8 +51,8 @@ def fp8_dequantize(q: BlockFp8) -> torch.Tensor:
 def fp8_block_matmul(a: Union[BlockFp8, torch.Tensor], b: BlockFp8,
                      dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """a (M, K) times the transpose of b (N, K): out (M, N) of dtype (None: a's, bfloat16 for
-    codes). a may be values (..., K), which are quantised by rows on the way (up to 32 rows
-    within the product's own launch). No gradient."""
+    codes). a may be values (..., K), which are quantised by rows on the way (a
+    few, 512 blocks of up to 32 rows, within the product's own launch). No gradient."""
     codes = isinstance(a, tuple)
     if not isinstance(b, tuple):
         raise TypeError("fp8_block_matmul: b is a BlockFp8")

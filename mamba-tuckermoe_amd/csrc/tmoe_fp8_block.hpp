@@ -25,6 +25,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t kFp8Tiny = 0x0d800000u;       // 2^-100
 constexpr int kFp8Block = 128;
+constexpr int kFp8Held = 512;                    // blocks of a few rows' values that one launch quantises itself
 
 __device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float d) {
   const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
@@ -420,93 +421,106 @@ __global__ __launch_bounds__(256) void k_fp8_sum(const float* __restrict__ plane
 }
 
 // Up to 32 rows against all of B, read once straight into registers: a work-group takes 32
-// columns, its waves the K tiles in turn. A's rows are codes, or (T) bf16 or fp32 values that
-// are quantised here: a row's block lies in two lanes.
+// columns, its waves a K tile each, the next one's codes on their way. A's rows are codes, or (T)
+// bf16 or fp32 values of kFp8Held blocks at most, which the work-group first quantises into LDS (by
+// each wave for itself, from its rows' lanes, that took 3.2 us a K tile; W tiles at a time between
+// the products it waited for B's codes too). Bound by latency: M = 1, K = 1536, N = 6144 takes 5.3 us, of
+// which the launch is 2 and reading 9.4 MB 1.8.
 template <class T, int W, bool kExact>
 __global__ __launch_bounds__(64 * W) void k_fp8_skinny(Fp8GemmArgs a) {
   constexpr bool kCodes = sizeof(T) == 1;
-  __shared__ float s_part[W > 1 ? W - 1 : 1][32][33];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+  __shared__ u32x4 s_codes[kCodes ? 1 : kFp8Held * 8 + 32];
+  __shared__ float s_scales[kCodes ? 1 : kFp8Held];
+  __shared__ float s_part[W][32][33];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, h = lane >> 5;
+  const int M = (int)a.M, blocks = a.blocks;
   const int64_t n0 = (int64_t)blockIdx.x * 32;
   const int64_t n = n0 + r < a.N ? n0 + r : a.N - 1;
-  const bool live = r < a.M;
+  const bool live = r < M;
+  // the codes of a row's K tile that the lane holds
+  auto codes = [&](const void* row, int64_t at, i32x8 (&f)[2]) __attribute__((always_inline)) {
+    const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const char*>(row) + at);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) f[k] = join8(p[4 * k + h], p[4 * k + 2 + h]);
+  };
   const char* bp = static_cast<const char*>(a.b) + n * a.b_bytes;
-  f32x16 acc = zero16();
-  for (int kt = wave; kt < a.blocks; kt += W) {
-    i32x8 bf[2], af[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const u32x4* p = reinterpret_cast<const u32x4*>(bp + (int64_t)kt * 128);
-      bf[k] = join8(p[4 * k + h], p[4 * k + 2 + h]);
-    }
-    float sa = 0.f;
-    if constexpr (kCodes) {
-      if (live) {
-        const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const char*>(a.a) + r * a.a_bytes +
-                                                        (int64_t)kt * 128);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) af[k] = join8(p[4 * k + h], p[4 * k + 2 + h]);
-        sa = a.sa[(a.a_tiles ? 0 : r) * a.sa_rs + kt * a.sa_ks];
-      } else {
-        af[0] = af[1] = i32x8{};
-      }
-    } else {
-      float v[4][16];
+  i32x8 next[2] = {};
+  if (wave < blocks) codes(bp, (int64_t)wave * 128, next);
+  const int row_bytes = blocks * 128 + 16;       // of LDS (rows in other banks)
+  if constexpr (!kCodes) {                       // 16 lanes to a block, the blocks of a K tile neighbours
+    const int c = 8 * (tid & 15);
+    int blk = (tid >> 4) / M, row = (tid >> 4) - blk * M;
+#pragma unroll 1
+    while (blk < blocks) {
+      float v[8];
+      fp8_load8(static_cast<const T*>(a.a) + row * a.a_bytes, (int64_t)blk * 128 + c, a.K, v);
       uint32_t top = 0u;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int j = 0; j < 8; ++j) top = umax(top, __float_as_uint(v[j]) & 0x7fffffffu);
+      const Fp8Scale s(lanes_max<16>(top));
+      *reinterpret_cast<uint2*>(reinterpret_cast<char*>(s_codes) + row * row_bytes + blk * 128 + c) =
+          uint2{pack_fp8x4(v[0] * s.inv, v[1] * s.inv, v[2] * s.inv, v[3] * s.inv),
+                pack_fp8x4(v[4] * s.inv, v[5] * s.inv, v[6] * s.inv, v[7] * s.inv)};
+      if (c == 0) s_scales[blk * M + row] = s.scale;
+      row += 4 * W % M;
+      blk += 4 * W / M;
+      if (row >= M) {
+        row -= M;
+        ++blk;
+      }
+    }
+    wait_vm_lds<63>();                           // (LDS alone: B's codes stay on their way)
+    lds_barrier();
+  }
+  f32x16 acc = zero16();
+#pragma unroll 1
+  for (int kt = wave; kt < blocks; kt += W) {
+    const i32x8 bf[2] = {next[0], next[1]};
+    if (kt + W < blocks) codes(bp, (int64_t)(kt + W) * 128, next);
+    float sb[16];
+    if (a.b_tiles) {
+      sb[0] = a.sb[n0 / kFp8Block * a.sb_rs + kt * a.sb_ks];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float u[8] = {};
-          if (live)
-            fp8_load8(static_cast<const T*>(a.a) + r * a.a_bytes, (int64_t)kt * 128 + 32 * q + 16 * h + 8 * e,
-                      a.K, u);
+      for (int e = 1; e < 16; ++e) sb[e] = sb[0];
+    } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[q][8 * e + j] = u[j];
-            top = umax(top, __float_as_uint(u[j]) & 0x7fffffffu);
-          }
-        }
-      top = umax(top, __shfl_xor(top, 32));
-      const Fp8Scale s(top);
-      sa = s.scale;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          af[q / 2][4 * (q & 1) + j] = (int)pack_fp8x4(v[q][4 * j] * s.inv, v[q][4 * j + 1] * s.inv,
-                                                       v[q][4 * j + 2] * s.inv, v[q][4 * j + 3] * s.inv);
+      for (int e = 0; e < 16; ++e) {
+        const int64_t col = n0 + 8 * (e >> 2) + 4 * h + (e & 3);
+        sb[e] = a.sb[(col < a.N ? col : a.N - 1) * a.sb_rs + kt * a.sb_ks];
+      }
+    }
+    i32x8 af[2] = {};
+    float sa = 0.f;
+    if (live) {
+      if constexpr (kCodes) {
+        codes(a.a, r * a.a_bytes + (int64_t)kt * 128, af);
+        sa = a.sa[(a.a_tiles ? 0 : r) * a.sa_rs + kt * a.sa_ks];
+      } else {
+        codes(s_codes, r * row_bytes + kt * 128, af);
+        sa = s_scales[kt * M + r];
+      }
     }
     f32x16 t = mma_fp8<kExact>(bf[0], af[0], zero16());
     t = mma_fp8<kExact>(bf[1], af[1], t);
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t col = n0 + 8 * q + 4 * h + e;
-        const int64_t cv = col < a.N ? col : a.N - 1;
-        const float sb = a.sb[(a.b_tiles ? cv / kFp8Block : cv) * a.sb_rs + kt * a.sb_ks];
-        acc[4 * q + e] = fmaf(t[4 * q + e], sa * sb, acc[4 * q + e]);
-      }
+    for (int e = 0; e < 16; ++e) acc[e] = fmaf(t[e], sa * sb[e], acc[e]);
   }
-  if (wave > 0)
+  if (live)
 #pragma unroll
     for (int q = 0; q < 4; ++q)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s_part[wave - 1][r][8 * q + 4 * h + e] = acc[4 * q + e];
+      for (int e = 0; e < 4; ++e) s_part[wave][r][8 * q + 4 * h + e] = acc[4 * q + e];
   __syncthreads();
-  if (wave > 0 || !live) return;
+  // an output of 32 columns a thread, the waves' sums in their order
+  for (int i = threadIdx.x; i < a.M * 32; i += 64 * W) {
+    const int row = i >> 5, col = i & 31;
+    if (n0 + col >= a.N) continue;
+    float t = s_part[0][row][col];
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t col = n0 + 8 * q + 4 * h + e;
-      float t = acc[4 * q + e];
-      for (int w = 1; w < W; ++w) t += s_part[w - 1][r][8 * q + 4 * h + e];
-      if (col >= a.N) continue;
-      if (a.dtype == TMOE_BF16) store_from_f32(static_cast<uint16_t*>(a.out) + r * a.N + col, t);
-      else store_from_f32(static_cast<float*>(a.out) + r * a.N + col, t);
-    }
+    for (int w = 1; w < W; ++w) t += s_part[w][row][col];
+    if (a.dtype == TMOE_BF16) store_from_f32(static_cast<uint16_t*>(a.out) + row * a.N + n0 + col, t);
+    else store_from_f32(static_cast<float*>(a.out) + row * a.N + n0 + col, t);
+  }
 }
 
 }  // namespace dev

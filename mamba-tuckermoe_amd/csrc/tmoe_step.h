@@ -60,7 +60,7 @@ struct Fp8GemmArgs {
   void* out;
   float* planes;           // workspace: (slices, M, N), null for one slice
 };
-int64_t fp8_gemm_skinny_rows();      // up to so many rows of a may be values
+bool fp8_gemm_takes_values(int64_t M, int64_t blocks);   // whether a may be values
 size_t fp8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t blocks, int dtype);
 hipError_t fp8_gemm(Fp8GemmArgs a, hipStream_t st);
 

@@ -94,7 +94,7 @@ struct Fp8Workspace {
 Fp8Workspace fp8_workspace(int64_t M, int64_t N, int64_t K, bool values, int dtype) {
   Fp8Workspace w{};
   w.planes = (size_t)up16((int64_t)tmoe::fp8_gemm_workspace_bytes(M, N, blocks_of(K), dtype));
-  if (values && M > tmoe::fp8_gemm_skinny_rows()) {
+  if (values && !tmoe::fp8_gemm_takes_values(M, blocks_of(K))) {
     w.codes = (size_t)(M * blocks_of(K) * 128);
     w.scales = (size_t)up16(M * blocks_of(K) * 4);
   }

@@ -114,6 +114,36 @@ def test_block_matmul(pkg, dev, M, K, N, dtype):
                 near(pkg.fp8_block_matmul(x, b, torch.float32), want, mag, steps(K), "values, fp32")
 
 
+@dtypes
+@pytest.mark.parametrize("M,K,N", [(1, 65536, 40), (1, 65537, 3), (7, 4608, 130), (16, 4096, 65), (17, 4000, 64),
+                                   (32, 2048, 31), (32, 2049, 31), (3, 1537, 1000)])
+def test_few_rows_of_values(pkg, dev, M, K, N, dtype):
+    """Values on both sides of what a launch quantises itself (512 blocks): the products of their
+    codes, whose order of sums is the same, bit for bit; rows apart and at any element."""
+    x, w = values((M, K), dtype, M + K, 1.0).to(dev), values((N, K), dtype, N, 1.0).to(dev)
+    wide = torch.zeros(M, K + 9, dtype=dtype, device=dev)
+    wide[:, 3:K + 3] = x
+    for tiles in (False, True):
+        b = pkg.fp8_quantize(w, tiles)
+        for out in DTYPES.values():
+            want = pkg.fp8_block_matmul(pkg.fp8_quantize(x), b, out)
+            assert torch.equal(pkg.fp8_block_matmul(x, b, out), want)
+            assert torch.equal(pkg.fp8_block_matmul(wide[:, 3:K + 3], b, out), want)
+    v, u = bf.rounded(f64(x)), f64(pkg.fp8_dequantize(b))
+    near(want, v @ u.T, np.abs(v) @ np.abs(u).T, steps(K, want.dtype))
+
+
+@pytest.mark.parametrize("M,K,N,slices", [(2040, 1100, 8100, 1), (130, 9000, 140, 15), (400, 2050, 700, 6)])
+def test_forms(pkg, dev, M, K, N, slices):
+    """Tiles of 256 x 256 with ragged edges, and sliced sums, against float64."""
+    x, w = values((M, K), torch.bfloat16, 1, 1.0).to(dev), values((N, K), torch.bfloat16, 2, 1.0).to(dev)
+    a, b = pkg.fp8_quantize(x), pkg.fp8_quantize(w, True)
+    need = pkg._lib.lib().tmoe_fp8_gemm_workspace_bytes(M, N, K, pkg._lib.TMOE_BF16, 0)
+    assert (need == 0) == (slices == 1) and need >= 4 * M * N * (slices if slices > 1 else 0)
+    v, u = pkg.fp8_dequantize(a).double(), pkg.fp8_dequantize(b).double()
+    near(pkg.fp8_block_matmul(a, b), f64(v @ u.t()), f64(v.abs() @ u.abs().t()), steps(K, torch.bfloat16) + 16)
+
+
 def test_operands_as_they_lie(pkg, dev):
     """Rows of codes apart, unaligned or every other; scales in any order, one for all; uint8."""
     M, N, K = 70, 90, 300
