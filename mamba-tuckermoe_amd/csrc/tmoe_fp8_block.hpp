@@ -402,9 +402,15 @@ __global__ __launch_bounds__(256) void k_fp8_sum(const float* __restrict__ plane
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < count; i += step) {
     if (i + 4 <= count && count % 4 == 0) {
       float4 t = *reinterpret_cast<const float4*>(planes + i);
-      for (int p = 1; p < n; ++p) {
-        const float4 u = *reinterpret_cast<const float4*>(planes + p * count + i);
-        t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
+      for (int p = 1; p < n; p += 5) {           // five loads at once
+        float4 u[5];
+#pragma unroll
+        for (int k = 0; k < 5; ++k)
+          u[k] = p + k < n ? *reinterpret_cast<const float4*>(planes + (p + k) * count + i) : float4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 5; ++k) {
+          t.x += u[k].x; t.y += u[k].y; t.z += u[k].z; t.w += u[k].w;
+        }
       }
       if constexpr (sizeof(T) == 2)
         *reinterpret_cast<uint2*>(out + i) = uint2{pack_bf16x2(t.x, t.y), pack_bf16x2(t.z, t.w)};
