@@ -11,7 +11,7 @@ int er_lanes(int64_t E) {
   while (dev::kErV * l < E) l <<= 1;
   return l;
 }
-constexpr int64_t kErBlocks = 768;
+constexpr int64_t kErBlocks = 768;      // three to a compute unit, which their registers allow
 int64_t er_blocks(int64_t B, int64_t E) {
   const int64_t n = ceil_div(B, dev::kErThreads / er_lanes(E));
   return n < 1 ? 1 : n < kErBlocks ? n : kErBlocks;

@@ -58,14 +58,11 @@ __device__ __forceinline__ double key_value64(uint64_t k) {
   return k == ~0ull ? (double)NAN
                     : __longlong_as_double((int64_t)(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
 }
+// the largest of L lanes' words, by halves
 template <int L>
 __device__ __forceinline__ uint64_t lanes_max64(uint64_t v) {
-#pragma unroll
-  for (int o = 1; o < L; o <<= 1) {
-    const uint64_t u = __shfl_xor(v, o);
-    v = u > v ? u : v;
-  }
-  return v;
+  const uint32_t hi = lanes_max<L>((uint32_t)(v >> 32));
+  return (uint64_t)hi << 32 | lanes_max<L>((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
 }
 template <int L>
 __device__ __forceinline__ double lanes_sum64(double v) {
@@ -91,7 +88,7 @@ __device__ __forceinline__ void er_order() {   // LDS of one wave: what was writ
 // registers eight exponentials side by side took as many as the rest of the kernel together.
 template <int L>
 __device__ __forceinline__ void route_exact(const ExpertRouterArgs& a, const float (&v)[kErV], int l,
-                                            bool by_logit, double* d, uint32_t* slot) {
+                                            bool by_logit, const float* bias, double* d, uint32_t* slot) {
   constexpr int V = kErV;
   const int E = a.E, e0 = V * l, mine = E - e0 < V ? E - e0 : V;    // (no expert: below 1)
   uint64_t* keys = reinterpret_cast<uint64_t*>(d);
@@ -119,7 +116,7 @@ __device__ __forceinline__ void route_exact(const ExpertRouterArgs& a, const flo
 #pragma unroll 1
   for (int j = 0; j < V; ++j) {
     const bool is = j < mine;
-    const double x = d[e0 + j] / unit + (a.bias && is ? (double)a.bias[e0 + j] : 0.0);
+    const double x = d[e0 + j] / unit + (double)bias[e0 + j];
     keys[e0 + j] = is ? order_key64(x) : 0ull;
   }
   er_order();
@@ -133,7 +130,7 @@ __device__ __forceinline__ void route_exact(const ExpertRouterArgs& a, const flo
       const int g = l + L * i;
       if (g < a.groups) {
         uint64_t top = 0ull, second = 0ull;
-#pragma unroll 1
+#pragma unroll 4
         for (int c = 0; c < per; ++c) {
           const uint64_t x = keys[g * per + c];
           second = x > top ? top : x > second ? x : second;
@@ -165,23 +162,32 @@ __device__ __forceinline__ void route_exact(const ExpertRouterArgs& a, const flo
     }
     er_order();
   }
+  uint64_t own[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) own[j] = keys[e0 + j];
   for (int i = 0; i < a.k; ++i) {
-    uint64_t best = 0ull;
-    uint32_t at = 255u;
-    for (int j = 0; j < mine; ++j) {
-      const uint64_t x = keys[e0 + j];
-      if (x > best) {
-        best = x;
-        at = e0 + j;
-      }
-    }
+    uint64_t best = own[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) best = own[j] > best ? own[j] : best;
     const uint64_t most = lanes_max64<L>(best);
-    const uint32_t e = lanes_min<L>(best == most ? at : 255u);
-    if (e == at) keys[e] = 0ull;
+    uint32_t at = 255u;
+#pragma unroll
+    for (int j = V - 1; j >= 0; --j)
+      if (own[j] == most && most) at = e0 + j;
+    const uint32_t e = lanes_min<L>(at);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (e == (uint32_t)(e0 + j)) own[j] = 0ull;
     slot[i] = 255u - e;
   }
 }
 
+// One pass over the logits, a token to L lanes: nothing but idx, w and the counts is written, and the
+// next token's row is loaded under this one's work. Bound by the chain of a token's maxima, not by
+// bytes: of (B, E) = (4096, 256), k = 8 in 4 of 8 groups, 8.8 us, and (16384, 64), k = 6 in 3 of 8, 7.0 us,
+// where no token is ranked again, 16.9 and 13.2 us with random logits, of which some thousandth is
+// (24.1 and 19.1 with the biases read from memory there and maxima of 64 bits by shuffles);
+// (131072, 64), k = 6, a third of it masked, 24.5 us, 1.1 TB/s.
 template <class T, int L>
 __global__ __launch_bounds__(kErThreads) void k_expert_router_fwd(ExpertRouterArgs a) {
   constexpr int V = kErV, G = kErThreads / L;
@@ -191,21 +197,25 @@ __global__ __launch_bounds__(kErThreads) void k_expert_router_fwd(ExpertRouterAr
   const bool grouped = a.groups > 1 && a.top_groups < a.groups;
   const int per = E / a.groups;
   __shared__ uint32_t s_slot[G][kRouterTopK + 1], s_c[V * L];
+  __shared__ float s_bias[V * L];
   __shared__ double s_wide[G][V * L];            // keys, worths and scores of a token
   uint32_t* slot = s_slot[threadIdx.x / L];
   double* wide = s_wide[threadIdx.x / L];
   uint32_t* words = reinterpret_cast<uint32_t*>(wide);          // V L keys or scores
   uint32_t* worths = words + V * L;
-  for (int e = threadIdx.x; e < V * L; e += kErThreads) s_c[e] = 0u;
+  for (int e = threadIdx.x; e < V * L; e += kErThreads) {
+    s_c[e] = 0u;
+    s_bias[e] = a.bias && e < E ? a.bias[e] : 0.f;
+  }
+  __syncthreads();
   float bias[V], bm = 0.f;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    bias[j] = a.bias && e0 + j < E ? a.bias[e0 + j] : 0.f;
+    bias[j] = s_bias[e0 + j];
     bm = __builtin_elementwise_maximum(bm, fabsf(bias[j]));
   }
   bm = lanes_top<L>(bm);
   const bool wild = !(bm < 1e30f);               // biases that leave no range
-  __syncthreads();
   const int64_t step = (int64_t)gridDim.x * G;
   int64_t b = (int64_t)blockIdx.x * G + threadIdx.x / L;
   float next[V];
@@ -307,7 +317,7 @@ __global__ __launch_bounds__(kErThreads) void k_expert_router_fwd(ExpertRouterAr
     if (k < E) apart = min(apart, best - key_below<L>(key, best));
     if (__any(near || apart < least)) {
       er_order();
-      route_exact<L>(a, v, l, by_logit, wide, slot);
+      route_exact<L>(a, v, l, by_logit, s_bias, wide, slot);
     }
     er_order();
 #pragma unroll
@@ -333,7 +343,8 @@ __global__ __launch_bounds__(kErThreads) void k_expert_router_fwd(ExpertRouterAr
   }
 }
 
-// counts from the forward's planes: 16 experts a work-group
+// counts from the forward's planes, in place of atomics on counts that a launch would have to clear:
+// 16 experts a work-group; 4 us, a launch's
 __global__ __launch_bounds__(1024) void k_expert_router_counts(ExpertRouterArgs a) {
   __shared__ uint32_t s[64][16];
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4, e = blockIdx.x * 16 + c;
@@ -350,6 +361,10 @@ __global__ __launch_bounds__(1024) void k_expert_router_counts(ExpertRouterArgs 
   a.counts[e] = n;
 }
 
+// The gradient of a token from its k selected experts alone (but a softmax that is not
+// renormalised, whose every expert has one): the row is put together in LDS and stored whole.
+// Bound by those bytes where there are many tokens: (131072, 64) in float32 17 us, 2.3 TB/s with what it
+// reads; (4096, 256) 4.6 us.
 template <class T, int L>
 __global__ __launch_bounds__(kErThreads) void k_expert_router_bwd(ExpertRouterArgs a) {
   constexpr int V = kErV, G = kErThreads / L;
