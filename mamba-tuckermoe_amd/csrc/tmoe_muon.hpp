@@ -41,8 +41,12 @@ __device__ __forceinline__ void split8(const float (&v)[8], u32x4& hi, u32x4& lo
   f16x8 h, l;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    h[j] = (_Float16)v[j];
-    l[j] = (_Float16)(v[j] - (float)h[j]);
+    // Both parts of one rounded value. Where it is a product, the compiler otherwise makes the high
+    // part of the unrounded one too, and beside a tie the two lie on different sides.
+    float x = v[j];
+    asm volatile("" : "+v"(x));
+    h[j] = (_Float16)x;
+    l[j] = (_Float16)(x - (float)h[j]);
   }
   hi = __builtin_bit_cast(u32x4, h);
   lo = __builtin_bit_cast(u32x4, l);

@@ -149,6 +149,31 @@ def test_captured_streams_and_repeats(pkg, dev):
             assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("shape", [(256, 512), (512, 128), (3, 300, 200), (64, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_single_elements_of_a_step(pkg, dev, shape):
+    """One step, element by element: a few elements' parts of 11 bits that do not belong together hide
+    in a norm (each is off by 2^-11 of itself). The result is a polynomial of fifth degree in X, of
+    magnitude a |X| + |b| |X||X|^T|X| + |c| (|X||X|^T)^2 |X|. X, A (three times) and B are held to 2^-23 of
+    themselves, five factors X in a term; products of two low parts, 2^-24 of the whole, are left out of
+    four products, and each adds as many terms as its axis is long: with Gram products over the long axis L
+    (twice) and two over the short one S, at most (2 L + 2 S + 2 (5 + 3 + 1) + 4) 2^-24, here + 40. What
+    is smaller than fp16's smallest numbers, 2^-25 / 2048 of X's elements, is below 1e-9."""
+    a, b, c = 3.4445, -4.7750, 2.0315
+    for seed in range(4):
+        u = matrices(shape, seed).to(dev)
+        x = u.double()
+        x = x / (x.flatten(-2).norm(dim=-1)[..., None, None] + 1e-7)
+        t = x if shape[-2] <= shape[-1] else x.transpose(-1, -2)
+        m = t.abs()
+        A, M = t @ t.transpose(-1, -2), m @ m.transpose(-1, -2)
+        want, mag = a * t + (b * A + c * (A @ A)) @ t, a * m + (abs(b) * M + c * (M @ M)) @ m
+        if t is not x:
+            want, mag = want.transpose(-1, -2), mag.transpose(-1, -2)
+        off = (pkg.orthogonalize(u, steps=1).double() - want).abs()
+        n = 2 * max(shape[-2:]) + 2 * min(shape[-2:]) + 40
+        assert (off <= n * 2.0 ** -24 * mag + 1e-9).all(), (seed, float((off / mag).max()))
+
+
 def test_optimizer(pkg, dev):
     """FusedMuon's steps are the functional call's, through its state dict and in a capture."""
     shapes = [(40, 70), (3, 65, 33), (128, 64)]
