@@ -116,18 +116,19 @@ __device__ __forceinline__ void muon_store8(T* p, int64_t n, const float (&v)[8]
 struct MuonPlanes {
   int rp, cp, m;           // X's rows and columns, padded to 64, and the smaller of them
   int64_t xs, as;          // elements of a plane of X, of A
-  uint16_t *x[2], *a, *b;
+  uint16_t *x0, *a, *b;
   __device__ __forceinline__ MuonPlanes(const MuonDesc& d, int64_t mat) {
     rp = (d.rows + 63) & ~63;
     cp = (d.cols + 63) & ~63;
     m = d.rows > d.cols ? cp : rp;
     xs = (int64_t)rp * cp;
     as = (int64_t)m * m;
-    x[0] = d.planes + mat * (4 * xs + 4 * as);
-    x[1] = x[0] + 2 * xs;
-    a = x[1] + 2 * xs;
+    x0 = d.planes + mat * (4 * xs + 4 * as);
+    a = x0 + 4 * xs;
     b = a + 2 * as;
   }
+  // X or X' (an array of both would lie in memory, 2.7 us a launch)
+  __device__ __forceinline__ uint16_t* x(int which) const { return x0 + which * 2 * xs; }
 };
 
 // m = mu m + g, and each chunk's sum of u^2; the first work-group leaves the tensors' table
@@ -208,8 +209,8 @@ __global__ __launch_bounds__(kMuonThreads) void k_muon_start(MuonArgs a) {
     for (int j = 0; j < 8; ++j) v[j] *= f;
     u32x4 hi, lo;
     split8(v, hi, lo);
-    *reinterpret_cast<u32x4*>(w.x[0] + q * 8) = hi;
-    *reinterpret_cast<u32x4*>(w.x[0] + w.xs + q * 8) = lo;
+    *reinterpret_cast<u32x4*>(w.x0 + q * 8) = hi;
+    *reinterpret_cast<u32x4*>(w.x0 + w.xs + q * 8) = lo;
   }
 }
 
@@ -659,7 +660,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_muon_gemm(MuonArgs a) {
     }
   }
   const MuonPlanes w(d, mat);
-  const uint16_t* x = w.x[a.cur];
+  const uint16_t* x = w.x(a.cur);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
   f32x16 acc[FM][FN];
 #pragma unroll
@@ -680,7 +681,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_muon_gemm(MuonArgs a) {
                                      nkt, smem);
     }
     if (d.slices > 1) {                          // k_muon_sum adds them
-      float* part = muon_part<BM>(w.x[a.cur ^ 1], slice, d.slices, tm * (tm + 1) / 2 + tn);
+      float* part = muon_part<BM>(w.x(a.cur ^ 1), slice, d.slices, tm * (tm + 1) / 2 + tn);
       const float f = 1.f / kMuonOne;
 #pragma unroll
       for (int i = 0; i < FM; ++i)
@@ -740,7 +741,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_muon_gemm(MuonArgs a) {
       if constexpr (PHASE != kMuonLast) {
         u32x4 hi, lo;
         split8(v, hi, lo);
-        uint16_t* o = (PHASE == kMuonGram ? w.a : PHASE == kMuonPoly ? w.b : w.x[a.cur ^ 1]) + row * ld + col;
+        uint16_t* o = (PHASE == kMuonGram ? w.a : PHASE == kMuonPoly ? w.b : w.x(a.cur ^ 1)) + row * ld + col;
         *reinterpret_cast<u32x4*>(o) = hi;
         *reinterpret_cast<u32x4*>(o + (kSymmetric ? w.as : w.xs)) = lo;
       } else if (row < d.rows && col < d.cols) {
@@ -803,7 +804,7 @@ __global__ __launch_bounds__(64) void k_muon_sum(MuonArgs a) {
   if (r0 >= m || c0 >= m) return;
   float v[16] = {};
   for (int s = 0; s < d.slices; ++s) {
-    const float* p = muon_part<BT>(w.x[a.cur ^ 1], s, d.slices, tile) + blk * 1024 + lane * 4;
+    const float* p = muon_part<BT>(w.x(a.cur ^ 1), s, d.slices, tile) + blk * 1024 + lane * 4;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float4 u = *reinterpret_cast<const float4*>(p + q * 256);
