@@ -52,9 +52,15 @@ Group group_from(const tmoe_muon_tensor* t, int64_t i, int64_t count) {
   return g;
 }
 
-using Small = dev::MuonTile<64, 64, 2, 2, 3>;         // 16 KB stages, three work-groups a compute unit
+// 64 x 64: 16 KB stages, two work-groups of four waves to a compute unit. Three stages, and three
+// work-groups, took 129 us a step against 124 (three small matrices of 128 to 256) and 406 against 389 (34 of 256 x 1024 and wider).
+using Small = dev::MuonTile<64, 64, 2, 2, 4>;
+// 128 x 128, for the symmetric products eight waves in two groups, for the third product two
+// work-groups of four waves, one of which has its products while the other starts or stores: of 96 of
+// 256 x 512 beside six wide ones 745 us a step against 782 with 256 x 128 of eight waves (4.63 ms against
+// 4.48 for one of 4096 x 4096), and 762 with such work-groups for all three.
 using Square = dev::MuonTile<128, 128, 4, 2, 4>;      // 32 KB stages
-using Wide = dev::MuonTile<256, 128, 4, 2, 3>;        // 48 KB stages
+using Pair = dev::MuonTile<128, 128, 2, 2, 2>;        // 32 KB stages
 
 template <class TL, int PHASE, class T = uint16_t>
 void launch(const MuonArgs& a, unsigned groups, hipStream_t st) {
@@ -99,21 +105,17 @@ hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_a
   for (int64_t i = 0; i < count;) {
     const Group g = group_from(t, i, count);
     uint16_t* plane = reinterpret_cast<uint16_t*>(static_cast<char*>(ws) + g.planes_at());
-    // The symmetric products' tiles: 128 x 128 where those fill the chip (one of 2048 x 2048, 136
-    // of them: 801 us a step against 938 with 64 x 64; 64 of 256 x 512, 192: 359 against 341). The
-    // third product's: 256 x 128 where those fill it and are as full, for what they read less (48
-    // tensors of the reference model, 3050 of them: 16.5 ms with 128 x 128, 15.8).
-    int64_t pairs128 = 0, square = 0, wide = 0;
+    // Tiles of 128 x 128 where those fill the chip: one of 2048 x 2048, 136 of them in half of A: 773 us a
+    // step against 938 with 64 x 64; 64 of 256 x 512, 192: 283 against 341
+    int64_t pairs128 = 0, square = 0;
     for (int64_t k = i; k < g.end; ++k) {
       const Shape q = shape_of(t[k]);
       if (empty(t[k])) continue;
       const int64_t side = ceil_div(q.m, 128);
       pairs128 += t[k].batch * side * (side + 1) / 2;
       square += t[k].batch * ceil_div(q.rp, 128) * ceil_div(q.cp, 128);
-      wide += t[k].batch * ceil_div(q.rp, 256) * ceil_div(q.cp, 128);
     }
     const int64_t bt = pairs128 >= 128 && square >= 256 ? 128 : 64;
-    const int64_t bm = bt == 128 ? (20 * wide <= 11 * square ? 256 : 128) : 64, bn = bm == 64 ? 64 : 128;
     // the Gram products' summed axes are cut into slices of about what each work-group that the
     // chip holds has to do in the mean: a long one alone would keep the rest waiting
     int64_t work = 0;
@@ -149,7 +151,7 @@ hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_a
       chunk0 += (uint32_t)(t[i].batch * q.chunks);
       tile0 += (uint32_t)(t[i].batch * ceil_div(q.rp * q.cp, dev::kMuonChunk));
       sym0 += (uint32_t)(t[i].batch * pairs);
-      app0 += (uint32_t)(t[i].batch * ceil_div(q.rp, bm) * ceil_div(q.cp, bn));
+      app0 += (uint32_t)(t[i].batch * ceil_div(q.rp, bt) * ceil_div(q.cp, bt));
     }
     if (!a.count) continue;
     if (bf16) {
@@ -166,8 +168,7 @@ hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_a
         else launch_symmetric<Small>(phase, a, groups, sum0, st);
       }
       const bool last = k + 1 == s.steps;
-      if (bm == 256) launch_apply<Wide>(last, bf16, a, app0, st);
-      else if (bm == 128) launch_apply<Square>(last, bf16, a, app0, st);
+      if (bt == 128) launch_apply<Pair>(last, bf16, a, app0, st);
       else launch_apply<Small>(last, bf16, a, app0, st);
       a.cur ^= 1;
     }

@@ -9,15 +9,17 @@
 // and B are held as two fp16 numbers each (22 bits; all of them times 2^11, which keeps the
 // second one out of fp16's smallest numbers), and a product is three matrix instructions: high
 // high, high low and low high, fp32 sums. One bf16 number instead puts the update 1e-2 off.
-// Bound by the matrix units: three times the products' work, of which A and B, symmetric, are
-// computed by half and stored twice.
-//
 // A launch takes all matrices of a group of tensors: a work-group finds its tile's tensor in the
-// launch's arguments. X lies as its parameter does, its symmetric products along either axis: what
-// is summed over rows (a tall matrix's X^T X, a wide one's B X) is read transposed from LDS. B
-// holds a on its diagonal as well, so that X' = B X and nothing else is read. Groups are as large
-// as the memory-side cache holds their X: a step over 417 M elements moves 60 bytes an element
-// between its products and 20 before them, of which the 60 come from that cache.
+// launch's arguments. A and B, symmetric, are computed by half and stored twice. X lies as its
+// parameter does, its symmetric products along either axis: what is summed over rows (a tall
+// matrix's X^T X, a wide one's B X) is read transposed from LDS. B holds a on its diagonal as well,
+// so that X' = B X and nothing else is read.
+//
+// Small groups are bound by launches: a step of three matrices of up to 256 x 1024 is 22 of them, of
+// 4 to 6 us. Large ones by memory and matrix units together: 66 layers (2112 matrices of 256 x 512
+// and 139 M elements of wider ones, in float32) take 14.7 ms, of it the third products 6.5 (the bytes
+// of X and X' alone 3.9 at a copy's rate, three fp16 products at the library's rate 3.1), the Gram
+// products 4.0, B 2.3, and the two passes before them 1.8.
 #pragma once
 
 #include "tmoe_mma.hpp"
@@ -416,33 +418,6 @@ __device__ __forceinline__ void muon_read(MuonFrags<FM, LK>& l, MuonFrags<FN, RK
                  [R11x] "n"(1 * BN * 64 + 1 * 16 * BN * 2 + 0 * 4 * BN * 2),
                  [R11y] "n"(1 * BN * 64 + 1 * 16 * BN * 2 + 1 * 4 * BN * 2)
                  : "memory");
-  else if constexpr (!LK && RK && FM == 1 && FN == 2)
-    asm volatile(TMOE_MR(l000, lp, L00) TMOE_MR(l001, lp, L01) TMOE_MR(l010, lq, L00) TMOE_MR(l011, lq, L01)
-                 TMOE_MT(r000x, rp, R00x) TMOE_MT(r000y, rp, R00y) TMOE_MT(r001x, rp, R01x)
-                 TMOE_MT(r001y, rp, R01y) TMOE_MT(r010x, rp, R10x) TMOE_MT(r010y, rp, R10y)
-                 TMOE_MT(r011x, rp, R11x) TMOE_MT(r011y, rp, R11y) TMOE_MT(r100x, rq, R00x)
-                 TMOE_MT(r100y, rq, R00y) TMOE_MT(r101x, rq, R01x) TMOE_MT(r101y, rq, R01y)
-                 TMOE_MT(r110x, rq, R10x) TMOE_MT(r110y, rq, R10y) TMOE_MT(r111x, rq, R11x)
-                 TMOE_MT(r111y, rq, R11y) "s_waitcnt lgkmcnt(0)"
-                 : [l000] "=&v"(l.f[0][0][0]), [l001] "=&v"(l.f[0][0][1]), [l010] "=&v"(l.f[0][1][0]),
-                 [l011] "=&v"(l.f[0][1][1]),
-                   [r000x] "=&v"(rw[0][0][0][0]), [r000y] "=&v"(rw[0][0][0][1]), [r001x] "=&v"(rw[0][0][1][0]),
-                 [r001y] "=&v"(rw[0][0][1][1]), [r010x] "=&v"(rw[0][1][0][0]), [r010y] "=&v"(rw[0][1][0][1]),
-                 [r011x] "=&v"(rw[0][1][1][0]), [r011y] "=&v"(rw[0][1][1][1]), [r100x] "=&v"(rw[1][0][0][0]),
-                 [r100y] "=&v"(rw[1][0][0][1]), [r101x] "=&v"(rw[1][0][1][0]), [r101y] "=&v"(rw[1][0][1][1]),
-                 [r110x] "=&v"(rw[1][1][0][0]), [r110y] "=&v"(rw[1][1][0][1]), [r111x] "=&v"(rw[1][1][1][0]),
-                 [r111y] "=&v"(rw[1][1][1][1])
-                 : [lp] "v"(l0), [lq] "v"(l1), [rp] "v"(r0), [rq] "v"(r1), [L00] "n"(0 * 2048 + 0 * BM * 64),
-                 [L01] "n"(0 * 2048 + 1 * BM * 64),
-                   [R00x] "n"(0 * BN * 64 + 0 * 16 * BN * 2 + 0 * 4 * BN * 2),
-                 [R00y] "n"(0 * BN * 64 + 0 * 16 * BN * 2 + 1 * 4 * BN * 2),
-                 [R01x] "n"(1 * BN * 64 + 0 * 16 * BN * 2 + 0 * 4 * BN * 2),
-                 [R01y] "n"(1 * BN * 64 + 0 * 16 * BN * 2 + 1 * 4 * BN * 2),
-                 [R10x] "n"(0 * BN * 64 + 1 * 16 * BN * 2 + 0 * 4 * BN * 2),
-                 [R10y] "n"(0 * BN * 64 + 1 * 16 * BN * 2 + 1 * 4 * BN * 2),
-                 [R11x] "n"(1 * BN * 64 + 1 * 16 * BN * 2 + 0 * 4 * BN * 2),
-                 [R11y] "n"(1 * BN * 64 + 1 * 16 * BN * 2 + 1 * 4 * BN * 2)
-                 : "memory");
   else if constexpr (!LK && RK && FM == 2 && FN == 2)
     asm volatile(TMOE_MR(l000, lp, L00) TMOE_MR(l001, lp, L01) TMOE_MR(l010, lq, L00) TMOE_MR(l011, lq, L01)
                  TMOE_MR(l100, lp, L10) TMOE_MR(l101, lp, L11) TMOE_MR(l110, lq, L10) TMOE_MR(l111, lq, L11)
@@ -504,7 +479,7 @@ struct MuonTile {
 //
 // Eight waves work in two groups, one of each on every SIMD, the second a barrier behind the first:
 // while one reads its fragments the other has its matrix instructions, and its loads between those
-// (ahead of the reads they kept them waiting for the vector memory queue: 2760 instead of 1700
+// (ahead of the reads they kept them waiting for the vector memory queue: 2760 instead of 1980
 // cycles a K tile of 256 x 128). With phases between barriers, group 0 reads tile kt in phase 2 kt
 // and computes in 2 kt + 1, group 1 in 2 kt + 1 and 2 kt + 2. Tile kt's stage is read last in phase
 // 2 kt + 1: in its computing phase of tile kt group 0 loads tile kt + NS - 1, into the stage of tile
