@@ -9,6 +9,7 @@
 // and B are held as two fp16 numbers each (22 bits; all of them times 2^11, which keeps the
 // second one out of fp16's smallest numbers), and a product is three matrix instructions: high
 // high, high low and low high, fp32 sums. One bf16 number instead puts the update 1e-2 off.
+//
 // A launch takes all matrices of a group of tensors: a work-group finds its tile's tensor in the
 // launch's arguments. A and B, symmetric, are computed by half and stored twice. X lies as its
 // parameter does, its symmetric products along either axis: what is summed over rows (a tall
@@ -18,7 +19,7 @@
 // Small groups are bound by launches: a step of three matrices of up to 256 x 1024 is 22 of them, of
 // 4 to 6 us. Large ones by memory and matrix units together: 66 layers (2112 matrices of 256 x 512
 // and 139 M elements of wider ones, in float32) take 14.7 ms, of it the third products 6.5 (the bytes
-// of X and X' alone 3.9 at a copy's rate, three fp16 products at the library's rate 3.1), the Gram
+// of X, X' and the parameters alone 3.5 at a copy's rate, three fp16 products at the library's rate 3.2), the Gram
 // products 4.0, B 2.3, and the two passes before them 1.8.
 #pragma once
 
@@ -735,21 +736,21 @@ __global__ __launch_bounds__(TL::kThreads) void k_muon_gemm(MuonArgs a) {
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (kSymmetric && tm != tn) {                // the other half: a lane's column is a row of it
-      const int c = lane % (32 * FN), r1 = lane / (32 * FN) * 8;
-      if (c0 + c - n0 < nv)
+    if (kSymmetric && tm != tn) {                // the other half: four lanes take a column, a row of it
+      const int r = lane % 4 * 8;
 #pragma unroll
-        for (int r = r1; r < 32; r += 64 / (32 * FN) * 8) {
-          if (r0 + r - m0 >= mv) continue;
-          float v[8];
+      for (int it = 0; it < 2 * FN; ++it) {
+        const int c = it * 16 + lane / 4;
+        if (c0 + c - n0 >= nv || r0 + r - m0 >= mv) continue;
+        float v[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = res[(r + j) * kRow + c];
-          u32x4 hi, lo;
-          split8(v, hi, lo);
-          uint16_t* o = (PHASE == kMuonGram ? w.a : w.b) + (c0 + c) * ld + r0 + r;
-          *reinterpret_cast<u32x4*>(o) = hi;
-          *reinterpret_cast<u32x4*>(o + w.as) = lo;
-        }
+        for (int j = 0; j < 8; ++j) v[j] = res[(r + j) * kRow + c];
+        u32x4 hi, lo;
+        split8(v, hi, lo);
+        uint16_t* o = (PHASE == kMuonGram ? w.a : w.b) + (c0 + c) * ld + r0 + r;
+        *reinterpret_cast<u32x4*>(o) = hi;
+        *reinterpret_cast<u32x4*>(o + w.as) = lo;
+      }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
