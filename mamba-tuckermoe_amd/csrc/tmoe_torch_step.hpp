@@ -197,42 +197,30 @@ Fp8 fp8_empty(const at::Tensor& like, int64_t rows, int64_t K, bool tiles) {
                    : at::empty({blocks_of(K), rows}, o.dtype(at::kFloat)).t();
   return q;
 }
-// x (its rows (R, C) at one stride) along its rows, its columns, or both
-void fp8_make(const Rows& x, int64_t R, int64_t C, bool tiles, Fp8* rows, Fp8* cols) {
-  if (rows) *rows = fp8_empty(x.t, R, C, tiles);
-  if (cols) {
-    *cols = fp8_empty(x.t, C, R, tiles);
-    if (rows && tiles) cols->scales = rows->scales.t();
-  }
-  if (R == 0) return;
-  const tmoe_fp8_operand r = rows ? rows->args() : tmoe_fp8_operand{},
-                         c = cols ? cols->args() : tmoe_fp8_operand{};
-  check_rc(g_step.fp8_quantize(x.t.const_data_ptr(), R, C, x.stride,
-                               x.t.scalar_type() == at::kBFloat16 ? TMOE_BF16 : TMOE_F32,
-                               rows ? &r : nullptr, cols ? &c : nullptr, current_stream(x.t)));
-}
 int32_t code_of(at::ScalarType t) { return t == at::kBFloat16 ? TMOE_BF16 : TMOE_F32; }
-at::Tensor fp8_product(const Fp8& a, const Fp8& b, int64_t K, at::ScalarType dt) {
-  const int64_t M = a.codes.size(0), N = b.codes.size(0);
-  at::Tensor out = at::empty({M, N}, a.codes.options().dtype(dt));
-  if (M == 0) return out;
-  const size_t nws = g_step.fp8_workspace_bytes(M, N, K, code_of(dt), 0);
-  at::Tensor ws;
-  if (nws) ws = bytes_like(out, nws);
-  const tmoe_fp8_operand x = a.args(), y = b.args();
-  check_rc(g_step.fp8_gemm(&x, &y, K, code_of(dt), out.data_ptr(), out_ptr(ws), nws, current_stream(out)));
-  return out;
+// x (its rows (R, C) at one stride) along its rows, its columns, or both
+void fp8_quantize_into(const Rows& x, int64_t R, int64_t C, const tmoe_fp8_operand* rows,
+                       const tmoe_fp8_operand* cols) {
+  check_rc(g_step.fp8_quantize(x.t.const_data_ptr(), R, C, x.stride, code_of(x.t.scalar_type()), rows, cols,
+                               current_stream(x.t)));
 }
-at::Tensor fp8_product(const Rows& a, int64_t M, const Fp8& b, int64_t K, at::ScalarType dt) {
+// out (M, N) = a b^T, of codes, or of the rows of values x
+void fp8_gemm_into(const tmoe_fp8_operand* a, const Rows* x, int64_t M, const tmoe_fp8_operand& b, int64_t K,
+                   const at::Tensor& out, void* ws, size_t nws) {
+  const int dt = code_of(out.scalar_type());
+  if (a) check_rc(g_step.fp8_gemm(a, &b, K, dt, out.data_ptr(), ws, nws, current_stream(out)));
+  else check_rc(g_step.fp8_gemm_values(x->t.const_data_ptr(), M, x->stride, code_of(x->t.scalar_type()), &b, K, dt,
+                                       out.data_ptr(), ws, nws, current_stream(out)));
+}
+at::Tensor fp8_product(const Fp8* a, const Rows* x, int64_t M, const Fp8& b, int64_t K, at::ScalarType dt) {
   const int64_t N = b.codes.size(0);
-  at::Tensor out = at::empty({M, N}, a.t.options().dtype(dt).requires_grad(false));
+  at::Tensor out = at::empty({M, N}, b.codes.options().dtype(dt));
   if (M == 0) return out;
-  const size_t nws = g_step.fp8_workspace_bytes(M, N, K, code_of(dt), 1);
+  const size_t nws = g_step.fp8_workspace_bytes(M, N, K, code_of(dt), !a);
   at::Tensor ws;
   if (nws) ws = bytes_like(out, nws);
-  const tmoe_fp8_operand y = b.args();
-  check_rc(g_step.fp8_gemm_values(a.t.const_data_ptr(), M, a.stride, code_of(a.t.scalar_type()), &y, K,
-                                  code_of(dt), out.data_ptr(), out_ptr(ws), nws, current_stream(out)));
+  const tmoe_fp8_operand l = a ? a->args() : tmoe_fp8_operand{};
+  fp8_gemm_into(a ? &l : nullptr, x, M, b.args(), K, out, out_ptr(ws), nws);
   return out;
 }
 
@@ -265,7 +253,12 @@ PyObject* fp8_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     pybind11::gil_scoped_release nogil;
     const c10::DeviceGuard guard(x.device());
     const at::NoGradGuard no_grad;
-    fp8_make(rows_of(x), x.size(0), x.size(1), tiles, transpose ? nullptr : &q, transpose ? &q : nullptr);
+    const int64_t R = x.size(0), C = x.size(1);
+    q = transpose ? fp8_empty(x, C, R, tiles) : fp8_empty(x, R, C, tiles);
+    if (R) {
+      const tmoe_fp8_operand o = q.args();
+      fp8_quantize_into(rows_of(x), R, C, transpose ? nullptr : &o, transpose ? &o : nullptr);
+    }
   }
   return fp8_pair(q);
   END_HANDLE_TH_ERRORS
@@ -320,7 +313,7 @@ PyObject* fp8_block_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::DeviceGuard guard(x.device());
     fp8_align(q);
     fp8_align(b);
-    out = fp8_product(q, b, K, dt);
+    out = fp8_product(&q, nullptr, q.codes.size(0), b, K, dt);
   } else {
     dtype_of(x, kWho);
     TORCH_CHECK(x.dim() >= 1 && x.size(x.dim() - 1) == K, kWho, ": rows of ", K, " expected, got ", x.sizes());
@@ -334,7 +327,8 @@ PyObject* fp8_block_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::DeviceGuard guard(x.device());
     const at::NoGradGuard no_grad;
     fp8_align(b);
-    out = fp8_product(rows_of(x), M, b, K, dt);
+    const Rows rows = rows_of(x);
+    out = fp8_product(nullptr, &rows, M, b, K, dt);
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = b.codes.size(0);
     out = out.view(shape);
@@ -345,66 +339,124 @@ PyObject* fp8_block_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 constexpr const char* kFp8Matmul = "fp8_matmul";
 
+// Operands that no caller sees lie in one byte tensor, codes and then scales: an allocation each,
+// with views, took a fifth of a small layer's step on the host.
+int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+struct Fp8Place {
+  int64_t rows = 0, K = 0, at = 0, scales_at = 0;
+  bool tiles = false;
+  // behind the `end` bytes that are taken
+  Fp8Place(int64_t rows, int64_t K, bool tiles, int64_t& end) : rows(rows), K(K), at(end), tiles(tiles) {
+    scales_at = at + up256(rows * 128 * blocks_of(K));
+    end = scales_at + up256((tiles ? blocks_of(rows) : rows) * blocks_of(K) * 4);
+  }
+  tmoe_fp8_operand in(const at::Tensor& buf) const {
+    char* p = static_cast<char*>(buf.data_ptr());
+    tmoe_fp8_operand o{};
+    o.codes = p + at;
+    o.scales = reinterpret_cast<float*>(p + scales_at);
+    o.rows = rows;
+    o.row_bytes = 128 * blocks_of(K);
+    o.scale_row = tiles ? blocks_of(K) : 1;
+    o.scale_block = tiles ? 1 : rows;
+    o.tiles = tiles;
+    return o;
+  }
+};
 struct Fp8Call {
   at::Tensor x, w;
   bool want_x = false, want_w = false;
 };
+// What the backward keeps: x^T (K, M) by rows for dw, w (K, N) by tiles for dx
 struct Fp8Kept {
-  Fp8 x, w;      // x^T (K, M) by rows; w (K, N) by tiles
+  int64_t end = 0;
+  Fp8Place x, w;
+  Fp8Kept(int64_t M, int64_t K, int64_t N, bool want_x, bool want_w)
+      : x(want_w ? K : 0, M, false, end), w(want_x ? K : 0, N, true, end) {}
 };
-at::Tensor fp8_matmul_forward(const Fp8Call& c, Fp8Kept& kept) {
+at::Tensor fp8_matmul_forward(const Fp8Call& c, at::Tensor* kept) {
   const c10::DeviceGuard guard(c.x.device());
   const int64_t K = c.w.size(0), N = c.w.size(1), M = c.x.numel() / K;
   const Rows x = rows_of(c.x);
-  Fp8 xr, wt;
-  fp8_make(rows_of(c.w), K, N, true, c.want_x ? &kept.w : nullptr, &wt);
-  at::Tensor out;
-  if (c.want_w && M > 0) {
-    fp8_make(x, M, K, false, &xr, &kept.x);
-    out = fp8_product(xr, wt, K, c.x.scalar_type());
-  } else {
-    out = fp8_product(x, M, wt, K, c.x.scalar_type());
-  }
   std::vector<int64_t> shape = c.x.sizes().vec();
   shape.back() = N;
-  return out.view(shape);
+  at::Tensor out = at::empty(shape, c.x.options().requires_grad(false));
+  const Fp8Kept k(M, K, N, c.want_x, c.want_w);
+  if (k.end) *kept = bytes_like(out, (size_t)k.end);
+  const bool both = c.want_w && M > 0;            // x is quantised along both axes at once
+  int64_t end = 0;
+  const Fp8Place wt(N, K, true, end), xr(both ? M : 0, K, false, end);
+  const size_t nws = M ? g_step.fp8_workspace_bytes(M, N, K, code_of(out.scalar_type()), !both) : 0;
+  const at::Tensor tmp = bytes_like(out, (size_t)end + nws);
+  tmoe_fp8_operand b = wt.in(tmp), w{};
+  if (c.want_x) {
+    w = k.w.in(*kept);
+    b.scales = w.scales;
+    b.scale_row = w.scale_block;
+    b.scale_block = w.scale_row;
+  }
+  if (c.want_x || M > 0) fp8_quantize_into(rows_of(c.w), K, N, c.want_x ? &w : nullptr, &b);
+  if (M == 0) return out;
+  void* ws = nws ? static_cast<char*>(tmp.data_ptr()) + end : nullptr;
+  if (both) {
+    const tmoe_fp8_operand r = xr.in(tmp), t = k.x.in(*kept);
+    fp8_quantize_into(x, M, K, &r, &t);
+    fp8_gemm_into(&r, nullptr, M, b, K, out, ws, nws);
+  } else {
+    fp8_gemm_into(nullptr, &x, M, b, K, out, ws, nws);
+  }
+  return out;
 }
 
 struct Fp8Matmul : torch::autograd::Function<Fp8Matmul> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, Fp8Call c) {
     c.want_x = x.requires_grad();
     c.want_w = w.requires_grad();
-    Fp8Kept k;
-    const at::Tensor out = fp8_matmul_forward(c, k);
+    at::Tensor kept;
+    const at::Tensor out = fp8_matmul_forward(c, &kept);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({k.x.codes, k.x.scales, k.w.codes, k.w.scales});
-    ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["N"] = w.size(1);
+    ctx->save_for_backward({kept});
+    // (K and what was kept, in one number)
+    ctx->saved_data["kept"] = w.size(0) * 4 + (c.want_x ? 2 : 0) + (c.want_w ? 1 : 0);
     return {out};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     if (!g[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
     const variable_list s = ctx->get_saved_variables();
-    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
-    const int64_t N = ctx->saved_data["N"].toInt(), K = shape.back();
+    const int64_t kept = ctx->saved_data["kept"].toInt(), K = kept >> 2;
     const at::Tensor& dy = g[0];
-    const at::ScalarType dt = dy.scalar_type();
-    const int64_t M = dy.numel() / N;
+    const int64_t N = dy.size(-1), M = dy.numel() / N;
+    const Fp8Kept k(M, K, N, kept & 2, kept & 1);
     const c10::DeviceGuard guard(dy.device());
     const Rows d = rows_of(dy);
-    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), both = want_w && M > 0;
+    const int dt = code_of(dy.scalar_type());
     at::Tensor dx, dw;
-    Fp8 dr, dc;
-    const Fp8 w{s[2], s[3], true}, x{s[0], s[1], false};
-    if (want_w && M > 0) {
-      fp8_make(d, M, N, false, want_x ? &dr : nullptr, &dc);
-      dw = fp8_product(x, dc, M, dt);
-      if (want_x) dx = fp8_product(dr, w, N, dt);
-    } else {
-      if (want_w) dw = at::zeros({K, N}, dy.options());
-      if (want_x) dx = fp8_product(d, M, w, N, dt);
+    if (want_x) {
+      std::vector<int64_t> shape = dy.sizes().vec();
+      shape.back() = K;
+      dx = at::empty(shape, dy.options());
     }
-    if (want_x) dx = dx.view(shape);
+    if (want_w) dw = M ? at::empty({K, N}, dy.options()) : at::zeros({K, N}, dy.options());
+    if (M > 0) {
+      int64_t end = 0;
+      const Fp8Place dr(both && want_x ? M : 0, N, false, end), dc(both ? N : 0, M, false, end);
+      const size_t nx = want_x ? g_step.fp8_workspace_bytes(M, K, N, dt, !both) : 0;
+      const size_t nw = want_w ? g_step.fp8_workspace_bytes(K, N, M, dt, 0) : 0;
+      const int64_t room = end + (int64_t)std::max(nx, nw);
+      at::Tensor tmp;
+      if (room) tmp = bytes_like(dy, (size_t)room);
+      void* ws = room > end ? static_cast<char*>(tmp.data_ptr()) + end : nullptr;
+      tmoe_fp8_operand r{}, c{};
+      if (both) {
+        c = dc.in(tmp);
+        if (want_x) r = dr.in(tmp);
+        fp8_quantize_into(d, M, N, want_x ? &r : nullptr, &c);
+        const tmoe_fp8_operand x = k.x.in(s[0]);
+        fp8_gemm_into(&x, nullptr, K, c, M, dw, ws, nw);
+      }
+      if (want_x) fp8_gemm_into(both ? &r : nullptr, &d, M, k.w.in(s[0]), N, dx, ws, nx);
+    }
     return once({dx, dw, at::Tensor()}, kFp8Matmul);
   }
 };
@@ -439,8 +491,7 @@ PyObject* fp8_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
       out = Fp8Matmul::apply(x, w, c)[0];
     } else {
       const at::NoGradGuard no_grad;
-      Fp8Kept k;
-      out = fp8_matmul_forward(c, k);
+      out = fp8_matmul_forward(c, nullptr);
     }
   }
   return THPVariable_Wrap(std::move(out));
