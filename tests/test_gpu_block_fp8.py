@@ -196,6 +196,22 @@ def test_matmul_and_gradients(pkg, dev, M, K, N, dtype):
     near(y4, o["y"], o["y_mag"], steps(K, dtype), "y without gradients")
 
 
+@dtypes
+def test_one_gradient_of_two(pkg, dev, dtype):
+    """What is asked of a product that kept both operands, one at a time and again: the same bits."""
+    x, w = (values(s, dtype, sum(s)).to(dev).requires_grad_() for s in ((150, 200), (200, 70)))
+    dy = values((150, 70), dtype, 3).to(dev)
+    y = pkg.fp8_matmul(x, w)
+    both = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    for leaf, want in zip((x, w), both):
+        got, = torch.autograd.grad(y, leaf, dy, retain_graph=True)
+        assert torch.equal(got, want)
+    (y * dy).sum().backward()
+    assert torch.equal(x.grad, both[0]) and torch.equal(w.grad, both[1])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, x, dy)
+
+
 def test_matmul_views(pkg, dev):
     """Leading axes, strided and expanded operands and gradients, no tokens."""
     x, w = values((6, 11, 200), torch.float32, 1).to(dev).requires_grad_(), values((300, 200), torch.float32, 2).to(dev)
