@@ -105,8 +105,10 @@ hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_a
   for (int64_t i = 0; i < count;) {
     const Group g = group_from(t, i, count);
     uint16_t* plane = reinterpret_cast<uint16_t*>(static_cast<char*>(ws) + g.planes_at());
-    // Tiles of 128 x 128 where those fill the chip: one of 2048 x 2048, 136 of them in half of A: 773 us a
-    // step against 938 with 64 x 64; 64 of 256 x 512, 192: 283 against 341
+    // Tiles of 128 x 128 where X has one for each compute unit and half of A some for every fourth. us a
+    // step, 128 against 64: 2048 x 2048 (136 of A, 256 of X) 762 and 987, 6144 x 1536 (78, 576) 1151 and 1333, 32
+    // of 256 x 512 (96, 256) 208 and 218; 1536 x 1536 (78, 144) 590 and 499, 1024 x 4096 (36, 256) 450 and
+    // 434, 16 of 256 x 512 (48, 128) 181 and 152
     int64_t pairs128 = 0, square = 0;
     for (int64_t k = i; k < g.end; ++k) {
       const Shape q = shape_of(t[k]);
@@ -115,7 +117,7 @@ hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_a
       pairs128 += t[k].batch * side * (side + 1) / 2;
       square += t[k].batch * ceil_div(q.rp, 128) * ceil_div(q.cp, 128);
     }
-    const int64_t bt = pairs128 >= 128 && square >= 256 ? 128 : 64;
+    const int64_t bt = pairs128 >= 72 && square >= 256 ? 128 : 64;
     // the Gram products' summed axes are cut into slices of about what each work-group that the
     // chip holds has to do in the mean: a long one alone would keep the rest waiting
     int64_t work = 0;

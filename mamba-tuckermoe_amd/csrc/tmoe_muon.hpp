@@ -18,9 +18,9 @@
 //
 // Small groups are bound by launches: a step of three matrices of up to 256 x 1024 is 22 of them, of
 // 4 to 6 us. Large ones by memory and matrix units together: 66 layers (2112 matrices of 256 x 512
-// and 139 M elements of wider ones, in float32) take 14.7 ms, of it the third products 6.5 (the bytes
+// and 139 M elements of wider ones, in float32) take 14.3 ms, of it the third products 6.6 (the bytes
 // of X, X' and the parameters alone 3.5 at a copy's rate, three fp16 products at the library's rate 3.2), the Gram
-// products 4.0, B 2.3, and the two passes before them 1.8.
+// products 3.6, B 2.1, and the two passes before them 1.8.
 #pragma once
 
 #include "tmoe_mma.hpp"
