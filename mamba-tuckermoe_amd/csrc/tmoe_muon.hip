@@ -53,7 +53,7 @@ Group group_from(const tmoe_muon_tensor* t, int64_t i, int64_t count) {
 }
 
 // 64 x 64: 16 KB stages, two work-groups of four waves to a compute unit. Three stages, and three
-// work-groups, took 129 us a step against 124 (three small matrices of 128 to 256) and 406 against 389 (34 of 256 x 1024 and wider).
+// work-groups, took 129 us a step against 124 (six small matrices) and 406 against 389 (up to 1024 x 2304).
 using Small = dev::MuonTile<64, 64, 2, 2, 4>;
 // 128 x 128, for the symmetric products eight waves in two groups, for the third product two
 // work-groups of four waves, one of which has its products while the other starts or stores: of 96 of
