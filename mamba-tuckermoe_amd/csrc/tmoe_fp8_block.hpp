@@ -404,7 +404,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_gemm(Fp8GemmArgs a) {
   }
 }
 
-// out = the sum of the planes, in their order; 4.2 us for 15 of 256 x 1536, 8 for two of 768 x 4608
+// out = the sum of the planes, in their order; 4.2 us for ten of 1536 x 256, 8 for two of 768 x 4608
 template <class T>
 __global__ __launch_bounds__(256) void k_fp8_sum(const float* __restrict__ planes, int n, int64_t count,
                                                  T* __restrict__ out) {

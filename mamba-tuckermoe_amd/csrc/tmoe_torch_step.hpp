@@ -69,11 +69,12 @@ struct ExpertRouter : torch::autograd::Function<ExpertRouter> {
     variable_list o = expert_router_forward(c);
     ctx->mark_non_differentiable({o[0], o[2]});
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({raw.is_same(c.raw) ? raw : c.raw, c.mask.value_or(at::Tensor()), o[0], o[1]});
-    ctx->saved_data["k"] = c.k;
-    ctx->saved_data["score"] = c.score;
-    ctx->saved_data["scale"] = c.scale;
-    ctx->saved_data["renormalize"] = c.renormalize;
+    variable_list kept{raw.is_same(c.raw) ? raw : c.raw, o[0].detach(), o[1].detach()};
+    if (c.mask) kept.push_back(*c.mask);
+    ctx->save_for_backward(std::move(kept));
+    // (one number: each entry of saved_data costs a string and a node)
+    ctx->saved_data["form"] = (int64_t)(c.k << 34 | c.score << 33 | (int64_t)c.renormalize << 32 |
+                                        (int64_t)c10::bit_cast<uint32_t>((float)c.scale));
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -81,16 +82,17 @@ struct ExpertRouter : torch::autograd::Function<ExpertRouter> {
     const variable_list s = ctx->get_saved_variables();
     ExpertRouterCall c;
     c.raw = s[0];
-    if (s[1].defined()) c.mask = s[1];
-    c.k = ctx->saved_data["k"].toInt();
-    c.score = ctx->saved_data["score"].toInt();
-    c.scale = ctx->saved_data["scale"].toDouble();
-    c.renormalize = ctx->saved_data["renormalize"].toBool();
+    if (s.size() > 3) c.mask = s[3];
+    const int64_t form = ctx->saved_data["form"].toInt();
+    c.k = form >> 34;
+    c.score = form >> 33 & 1;
+    c.renormalize = form >> 32 & 1;
+    c.scale = c10::bit_cast<float>((uint32_t)form);
     const c10::DeviceGuard guard(c.raw.device());
     const tmoe_expert_router r = c.args();
     const at::Tensor dw = g[1].contiguous();
     at::Tensor draw = at::empty({r.B, r.E}, c.raw.options());
-    check_rc(g_step.expert_router_backward(&r, s[2].const_data_ptr<int64_t>(), s[3].const_data_ptr<float>(),
+    check_rc(g_step.expert_router_backward(&r, s[1].const_data_ptr<int64_t>(), s[2].const_data_ptr<float>(),
                                            dw.const_data_ptr<float>(), draw.data_ptr(),
                                            current_stream(c.raw)));
     return once({draw, at::Tensor()}, kExpertRouter);
