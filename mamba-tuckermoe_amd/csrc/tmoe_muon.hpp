@@ -60,20 +60,23 @@ __device__ __forceinline__ void join8f(u32x4 hi, u32x4 lo, float (&v)[8]) {
   for (int j = 0; j < 8; ++j) v[j] = (float)h[j] + (float)l[j];
 }
 
-// The last tensor whose first tile (of the kind that `first` gives) is no later than `tile`: 64
-// entries at a time, by ballots. A whole wave's call.
+// The last tensor whose first work-group (of the kind that `first` gives) is no later than `tile`. A
+// whole wave's call: each lane loads one tensor's entry, and the one that a ballot finds is
+// broadcast, so that no load waits for which it is.
 template <class F>
-__device__ __forceinline__ int muon_find(int count, uint32_t tile, F first) {
-  int lo = 0, n = count;
+__device__ __forceinline__ MuonDesc muon_take(const MuonDesc* t, int count, uint32_t tile, F first) {
+  constexpr int W = sizeof(MuonDesc) / 4;
+  static_assert(kMuonTensors <= 64 && sizeof(MuonDesc) % 4 == 0, "a lane a tensor");
+  struct Words {
+    uint32_t w[W];
+  };
   const int lane = threadIdx.x & 63;
-  while (n > 1) {
-    const int step = (n + 63) / 64, at = lo + lane * step;
-    const bool before = lane * step < n && first(at) <= tile;
-    const int k = 63 - __clzll(__ballot(before));     // (lane 0's always is)
-    lo += k * step;
-    n = n - k * step < step ? n - k * step : step;
-  }
-  return __builtin_amdgcn_readfirstlane(lo);
+  const MuonDesc mine = t[cmin_dev(lane, count - 1)];
+  const int k = 63 - __clzll(__ballot(lane < count && first(mine) <= tile));     // (lane 0's always is)
+  Words u = __builtin_bit_cast(Words, mine);
+#pragma unroll
+  for (int i = 0; i < W; ++i) u.w[i] = __builtin_amdgcn_readlane(u.w[i], k);
+  return __builtin_bit_cast(MuonDesc, u);
 }
 
 __device__ __forceinline__ float muon_u(float g, float m, float mu, bool nesterov) {
@@ -143,7 +146,7 @@ __global__ __launch_bounds__(kMuonThreads) void k_muon_momentum(MuonFirstArgs fi
   if (blockIdx.x == 0)
     for (int i = tid; i < a.count * (int)(sizeof(MuonDesc) / 4); i += kMuonThreads)
       reinterpret_cast<uint32_t*>(a.t)[i] = reinterpret_cast<const uint32_t*>(first.t)[i];
-  const MuonDesc& d = first.t[muon_find(a.count, blockIdx.x, [&](int k) { return first.t[k].chunk0; })];
+  const MuonDesc d = muon_take(first.t, a.count, blockIdx.x, [](const MuonDesc& t) { return t.chunk0; });
   const uint32_t c = blockIdx.x - d.chunk0;
   const int64_t n = (int64_t)d.rows * d.cols, mat = c / d.chunks, e0 = (int64_t)(c % d.chunks) * kMuonChunk;
   const T* g = static_cast<const T*>(d.g) + mat * n;
@@ -180,7 +183,7 @@ template <class T>
 __global__ __launch_bounds__(kMuonThreads) void k_muon_start(MuonArgs a) {
   __shared__ float s_part[kMuonThreads / 64];
   const int tid = threadIdx.x;
-  const MuonDesc d = a.t[muon_find(a.count, blockIdx.x, [&](int k) { return a.t[k].tile0; })];
+  const MuonDesc d = muon_take(a.t, a.count, blockIdx.x, [](const MuonDesc& t) { return t.tile0; });
   const int64_t padded = (int64_t)((d.rows + 63) & ~63) * ((d.cols + 63) & ~63);
   const uint32_t per = (uint32_t)((padded + kMuonChunk - 1) / kMuonChunk), t = blockIdx.x - d.tile0;
   const int64_t mat = t / per;
@@ -615,15 +618,14 @@ __global__ __launch_bounds__(TL::kThreads) void k_muon_gemm(MuonArgs a) {
   char* smem = reinterpret_cast<char*>(s_mem);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / TL::WN, wn = wave % TL::WN;
-  auto first = [&](int k) {
-    return PHASE == kMuonGram ? a.t[k].gram0 : PHASE == kMuonPoly ? a.t[k].sym0 : a.t[k].app0;
+  auto first = [](const MuonDesc& t) {
+    return PHASE == kMuonGram ? t.gram0 : PHASE == kMuonPoly ? t.sym0 : t.app0;
   };
   // work-groups go round the eight XCDs: each gets a run of neighbours, which share X in its L2
   const uint32_t each = gridDim.x / 8, place = blockIdx.x < each * 8 ? blockIdx.x % 8 * each + blockIdx.x / 8 : blockIdx.x;
-  const int which = muon_find(a.count, place, first);
-  const MuonDesc d = a.t[which];
+  const MuonDesc d = muon_take(a.t, a.count, place, first);
   const bool tall = d.rows > d.cols;
-  uint32_t t = place - first(which);
+  uint32_t t = place - first(d);
   int64_t mat;
   int tm, tn, slice = 0;
   {
@@ -775,8 +777,7 @@ __global__ __launch_bounds__(64) void k_muon_sum(MuonArgs a) {
   constexpr int BT = TL::BM, kBlocks = TL::W * TL::FM * TL::FN;      // of 32 x 32 in a tile
   __shared__ float s_res[32][33];
   const int lane = threadIdx.x;
-  const int which = muon_find(a.count, blockIdx.x, [&](int k) { return a.t[k].sum0; });
-  const MuonDesc d = a.t[which];
+  const MuonDesc d = muon_take(a.t, a.count, blockIdx.x, [](const MuonDesc& t) { return t.sum0; });
   uint32_t t = blockIdx.x - d.sum0;
   const int blk = t % kBlocks;
   t /= kBlocks;
