@@ -10,8 +10,8 @@
 // second one out of fp16's smallest numbers), and a product is three matrix instructions: high
 // high, high low and low high, fp32 sums. One bf16 number instead puts the update 1e-2 off.
 //
-// A launch takes all matrices of a group of tensors: a work-group finds its tile's tensor in the
-// launch's arguments. A and B, symmetric, are computed by half and stored twice. X lies as its
+// A launch takes all matrices of a group of tensors: a work-group finds its tile's tensor in a
+// table in the workspace. A and B, symmetric, are computed by half and stored twice. X lies as its
 // parameter does, its symmetric products along either axis: what is summed over rows (a tall
 // matrix's X^T X, a wide one's B X) is read transposed from LDS. B holds a on its diagonal as well,
 // so that X' = B X and nothing else is read.
