@@ -118,8 +118,9 @@ hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_a
       square += t[k].batch * ceil_div(q.rp, 128) * ceil_div(q.cp, 128);
     }
     const int64_t bt = pairs128 >= 72 && square >= 256 ? 128 : 64;
-    // the Gram products' summed axes are cut into slices of about what each work-group that the
-    // chip holds has to do in the mean: a long one alone would keep the rest waiting
+    // The Gram products' summed axes are cut into slices of about what each work-group that the
+    // chip holds has to do in the mean: a long one alone would keep the rest waiting. Not under 14 K
+    // tiles of 64 x 64 a slice, for what the sum costs: 135 us a step of nine small matrices, 140 with 8 or 16.
     int64_t work = 0;
     for (int64_t k = i; k < g.end; ++k) {
       if (empty(t[k])) continue;
@@ -127,7 +128,7 @@ hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_a
       const int64_t side = ceil_div(q.m, bt);
       work += t[k].batch * side * (side + 1) / 2 * (std::max(q.rp, q.cp) / dev::kMuonK);
     }
-    const int64_t mean = std::max(ceil_div(work, bt == 128 ? 256 : 512), bt == 128 ? (int64_t)16 : (int64_t)8);
+    const int64_t mean = std::max(ceil_div(work, bt == 128 ? 256 : 512), bt == 128 ? (int64_t)16 : (int64_t)14);
     uint32_t chunk0 = 0, tile0 = 0, gram0 = 0, sum0 = 0, sym0 = 0, app0 = 0;
     a.count = a.cur = 0;
     for (; i < g.end; ++i) {
