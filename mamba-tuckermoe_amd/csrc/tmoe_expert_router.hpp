@@ -5,12 +5,15 @@
 //   idx = the k largest b of the open groups;  w_j = scale s_j / (sum_i s_i + 1e-20), or scale s_j
 // all of them compared as in float64, the lowest index first on ties. With neither bias nor
 // groups b has the logits' own order, and those are compared. A masked token has idx -1, w 0
-// and no gradient. With t_j = dw_j - sum_i dw_i w_i / scale (renormalised; else dw_j):
+// and no gradient. Renormalised, with u = w / scale, r = 1 - sum u = 1e-20 / (sum s + 1e-20) in closed form
+// and D = sum_i u_i (dw_i - dw_0), differences to dw_0 since one weight may be next to all:
+//   t_j = dw_j - sum_i dw_i u_i = (dw_j - dw_0) - D + dw_0 r;  sum_j u_j t_j = r (D + (1 - r) dw_0)
 //   sigmoid  draw_j = w_j t_j (1 - s_j) where selected, else 0
-//   softmax  draw_e = s_e (scale t_e - sum_j w_j t_j), which renormalised is w_j t_j where selected,
-//            else 0: the logits are not needed there
-// t_j is taken from differences to dw_0 (one weight may be next to all), with
-// 1 - sum w / scale = 1e-20 / (sum s + 1e-20) in closed form.
+//   softmax  draw_e = w_e t_e (where selected) - scale s_e sum_j u_j t_j
+// A softmax's r is next to nothing unless a bias selects scores of 1e-14 and less in all. There the row's
+// logits are read for it; elsewhere sum w tells that it is below 2^-20, it is left out (16 roundings of
+// what it stands beside), and the logits are not needed. Not renormalised t_j = dw_j, and
+//   sigmoid  draw_j = w_j t_j (1 - s_j);  softmax  draw_e = scale s_e (t_e - sum_j s_j t_j)
 //
 // Ranks. A token's experts lie in L lanes, eight to a lane. Scores become whole numbers of 24
 // bits over the range that the biases leave them ([-bm, 1 + bm]; softmax before its division,
@@ -361,8 +364,9 @@ __global__ __launch_bounds__(1024) void k_expert_router_counts(ExpertRouterArgs 
   a.counts[e] = n;
 }
 
-// The gradient of a token from its k selected experts alone (but a softmax that is not
-// renormalised, whose every expert has one): the row is put together in LDS and stored whole.
+// The gradient of a token from its k selected experts alone (but for a softmax that is not
+// renormalised or whose r counts, where every expert has one): the row is put together in LDS and
+// stored whole.
 // Bound by those bytes where there are many tokens: (131072, 64) in float32 17 us, 2.3 TB/s with what it
 // reads; (4096, 256) 4.6 us.
 template <class T, int L>
@@ -389,12 +393,38 @@ __global__ __launch_bounds__(kErThreads) void k_expert_router_bwd(ExpertRouterAr
         const int64_t e = a.idx[b * k + i];
         const float w = a.w[b * k + i];
         D = fmaf(w * inv_c, a.renormalize ? a.dw[b * k + i] - top : a.dw[b * k + i], D);
-        if (!softmax && e >= 0 && e < E) S += sigmoid_close(load_as_f32(row + e));
+        if (softmax) S = fmaf(w, inv_c, S);
+        else if (e >= 0 && e < E) S += sigmoid_close(load_as_f32(row + e));
       }
       D = lanes_sum<L>(D);
       S = lanes_sum<L>(S);
-      // what 1e-20 leaves of one
-      const float rest = softmax ? 0.f : top * (1e-20f / (S + 1e-20f));
+      const bool small = softmax && a.renormalize && !(S >= 1.f - 0x1p-20f);
+      float v[V], m = 0.f, unit = 1.f;           // of a row whose every expert has a gradient
+      if (dense || small) {
+        float sum = 0.f;
+        router_load<T, V>(row, e0, E, v);
+        m = v[0];
+#pragma unroll
+        for (int j = 1; j < V; ++j) m = __builtin_elementwise_maximum(m, v[j]);
+        m = lanes_top<L>(m);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          v[j] = e0 + j < E ? exp_close(v[j] - m) : 0.f;
+          sum += v[j];
+        }
+        unit = lanes_sum<L>(sum);
+      }
+      if (small) {
+        S = 0.f;
+        for (int i = l; i < k; i += L) {
+          const int64_t e = a.idx[b * k + i];
+          if (e >= 0 && e < E) S += exp_close(load_as_f32(row + e) - m);
+        }
+        S = lanes_sum<L>(S) / unit;
+      }
+      const float f = a.scale / unit;
+      // r, what 1e-20 leaves of one, and its part of t
+      const float r = softmax && !small ? 0.f : 1e-20f / (S + 1e-20f), rest = top * r;
       for (int i = l; i < k; i += L) {
         const int64_t e = a.idx[b * k + i];
         if (e < 0 || e >= E) continue;
@@ -410,20 +440,12 @@ __global__ __launch_bounds__(kErThreads) void k_expert_router_bwd(ExpertRouterAr
 #pragma unroll
       for (int j = 0; j < V; ++j) sel[e0 + j] = 0.f;
       if (dense) {
-        float v[V], m, sum = 0.f;
-        router_load<T, V>(row, e0, E, v);
-        m = v[0];
-#pragma unroll
-        for (int j = 1; j < V; ++j) m = __builtin_elementwise_maximum(m, v[j]);
-        m = lanes_top<L>(m);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          v[j] = e0 + j < E ? exp_close(v[j] - m) : 0.f;
-          sum += v[j];
-        }
-        const float f = a.scale / lanes_sum<L>(sum);
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = v[j] * f * (o[j] - D);
+      } else if (small) {
+        const float all = r * fmaf(S / (S + 1e-20f), top, D);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = fmaf(-v[j] * f, all, o[j]);
       }
       er_order();
     }

@@ -197,3 +197,42 @@ def test_captured_and_streams(pkg, dev):
     side.synchronize()
     for p, q in zip(other, want):
         assert torch.equal(p, q)
+
+
+@dtypes
+@pytest.mark.parametrize("E,k,groups,top", [(4, 2, 1, 1), (8, 1, 1, 1), (64, 6, 8, 3), (256, 16, 1, 1)])
+def test_small_selected_scores(pkg, dev, E, k, groups, top, dtype):
+    """A bias that selects experts whose softmax scores lie 20 to 80 below another's: 1e-20 is a part,
+    or all, of what a weight is divided by, and the other expert has a gradient too.
+
+    Logits T apart have a difference that float32 rounds by 2^-24 T, and an exponential takes that as it
+    is: T steps for a score and for a sum of them, 2 T for a weight (beside its 48). A selected gradient is
+    w (g - top - D + top r): 2 T of w, 2 T of D's weights and T of r, another's s r (D + ...) less than that:
+    5 T beside the 128. The kernel leaves r out below 2^-20: 16 steps, and as many of its sum's. A score
+    below float32's normal numbers may be lost: 2^-126 over the 1e-20 in a weight."""
+    g = torch.Generator().manual_seed(E)
+    B = 200
+    raw = torch.randn(B, E, generator=g)
+    raw[:, E - 1] += torch.linspace(20, 80, B)
+    bias = torch.zeros(E)
+    bias[:E - E // groups] = 3.0            # (never the last group)
+    if groups == 1:
+        bias[:E - 1] = 3.0
+    bias += 0.1 * torch.randn(E, generator=g)
+    raw = raw.to(dtype).to(dev)
+    T = float((raw.amax(-1) - raw.amin(-1)).max())
+    dw = torch.randn(B, k, generator=g)
+    some = (torch.rand(B, generator=g) < 0.7).to(dev)
+    for mask, scale, renorm in ((None, 1.0, True), (None, 2.5, True), (some, 2.5, True), (some, 1.0, False)):
+        kw = dict(groups=groups, top_groups=top, scale=scale, renormalize=renorm)
+        leaf = raw.clone().requires_grad_()
+        r = pkg.fused_expert_router(leaf, k, bias=bias.to(dev), mask=mask, **kw)
+        o = er.route(f64(raw), k, bias=f64(bias), mask=None if mask is None else mask.cpu().numpy(),
+                     dw=dw.numpy(), **kw)
+        assert np.array_equal(r.idx.cpu().numpy(), o["idx"]) and not (r.idx == E - 1).any()
+        lost = scale * 2.0 ** -126 / (1e-20 if renorm else 1.0)
+        n, m = 48 + 2 * T, 128 + 5 * T + 32
+        near(r.weights, o["w"], o["w"] + lost / (n * 2.0 ** -24), n, "w")
+        draw, = torch.autograd.grad(r.weights, leaf, dw.to(dev))
+        far = 4 * float(dw.abs().max())
+        near(draw, o["draw"], o["draw_mag"] + far * lost / (m * 2.0 ** -24), m, "draw")
