@@ -530,8 +530,8 @@ int tmoe_fp8_gemm_values(const void* x, int64_t M, int64_t row_stride, int x_dty
  *   p = p (1 - lr weight_decay) - lr update_rms sqrt(max(rows, cols)) X
  * p and g of dtype TMOE_BF16 or TMOE_F32, m fp32; X is held in 22 bits, sums in fp32, p is rounded
  * once. With m null in a tensor u = g. With write_only p is X instead, and need not hold
- * anything. A matrix whose u is not finite, or the sum of whose squares is not in fp32, gets no
- * finite p. The coefficients have to keep x in [-2, 2] and b x^2 + c x^4 in [-16, 16] over the
+ * anything. |u| is taken in 64 bits; a matrix whose u is not finite (in fp32) gets no finite p. The
+ * coefficients have to keep x in [-2, 2] and b x^2 + c x^4 in [-16, 16] over the
  * steps from [0, 1] on (what X, A and B are stored in has no room for more). steps 1 to 16;
  * rows, cols <= 2^22, the smaller of them <= 2^16, a tensor's elements <= 2^36; tensors without
  * elements are passed over. Workspace of at least tmoe_muon_workspace_bytes(tensors, count) bytes,

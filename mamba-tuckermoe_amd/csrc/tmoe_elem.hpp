@@ -56,6 +56,12 @@ __device__ __forceinline__ float lanes_sum(float v) {
   }));
 }
 template <int L>
+__device__ __forceinline__ double lanes_sum64(double v) {
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) v += __shfl_xor(v, o);
+  return v;
+}
+template <int L>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
   return lanes_reduce<L>(v, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
 }

@@ -67,12 +67,6 @@ __device__ __forceinline__ uint64_t lanes_max64(uint64_t v) {
   const uint32_t hi = lanes_max<L>((uint32_t)(v >> 32));
   return (uint64_t)hi << 32 | lanes_max<L>((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
 }
-template <int L>
-__device__ __forceinline__ double lanes_sum64(double v) {
-#pragma unroll
-  for (int o = 1; o < L; o <<= 1) v += __shfl_xor(v, o);
-  return v;
-}
 
 // the largest of L lanes' floats, NaN if one of them is
 template <int L>

@@ -35,7 +35,7 @@ constexpr int64_t kTableBytes = (kMuonTensors * (int64_t)sizeof(MuonDesc) + 255)
 // the tensors from i on that are a group: their end, and what they need
 struct Group {
   int64_t end, chunks, halves;
-  int64_t planes_at() const { return up(kTableBytes + chunks * 4, 256); }
+  int64_t planes_at() const { return up(kTableBytes + chunks * 8, 256); }
   int64_t bytes() const { return planes_at() + 2 * halves; }
 };
 Group group_from(const tmoe_muon_tensor* t, int64_t i, int64_t count) {
@@ -98,7 +98,7 @@ hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_a
   MuonFirstArgs first{};
   MuonArgs& a = first.a;
   a.t = static_cast<MuonDesc*>(ws);
-  a.sums = reinterpret_cast<float*>(static_cast<char*>(ws) + kTableBytes);
+  a.sums = reinterpret_cast<double*>(static_cast<char*>(ws) + kTableBytes);
   a.mu = (float)s.momentum; a.eps = (float)s.eps; a.nesterov = s.nesterov; a.write_only = s.write_only;
   a.a = (float)s.coefficients[0]; a.b = (float)s.coefficients[1]; a.c = (float)s.coefficients[2];
   a.keep = (float)(1.0 - s.lr * s.weight_decay);

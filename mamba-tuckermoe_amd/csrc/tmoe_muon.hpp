@@ -137,7 +137,8 @@ struct MuonPlanes {
   __device__ __forceinline__ uint16_t* x(int which) const { return x0 + which * 2 * xs; }
 };
 
-// m = mu m + g, and each chunk's sum of u^2; the first work-group leaves the tensors' table. Bound by
+// m = mu m + g, and each chunk's sum of u^2, in 64 bits: a finite u's squares may be past fp32 at either
+// end (1e20, or 1e-25 with an eps as small), and as many conversions are nothing beside the bytes; the first work-group leaves the tensors' table. Bound by
 // memory, 5.5 TB/s (83 M elements in fp32: 170 us)
 template <class T>
 __global__ __launch_bounds__(kMuonThreads) void k_muon_momentum(MuonFirstArgs first) {
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(kMuonThreads) void k_muon_momentum(MuonFirstArgs fi
   const int64_t n = (int64_t)d.rows * d.cols, mat = c / d.chunks, e0 = (int64_t)(c % d.chunks) * kMuonChunk;
   const T* g = static_cast<const T*>(d.g) + mat * n;
   float* m = d.m ? d.m + mat * n : nullptr;
-  float sum = 0.f;
+  double sum = 0.0;
   const int64_t e1 = e0 + kMuonChunk < n ? e0 + kMuonChunk : n;
 #pragma unroll 2
   for (int64_t e = e0 + tid * 8; e < e1; e += kMuonThreads * 8) {
@@ -167,10 +168,10 @@ __global__ __launch_bounds__(kMuonThreads) void k_muon_momentum(MuonFirstArgs fi
       muon_store8(m + e, e1 - e, q);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fmaf(v[j], v[j], sum);
+    for (int j = 0; j < 8; ++j) sum = fma((double)v[j], (double)v[j], sum);
   }
-  sum = lanes_sum<64>(sum);
-  __shared__ float s[kMuonThreads / 64];
+  sum = lanes_sum64<64>(sum);
+  __shared__ double s[kMuonThreads / 64];
   if ((tid & 63) == 0) s[tid >> 6] = sum;
   __syncthreads();
   if (tid == 0) a.sums[blockIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
@@ -181,19 +182,22 @@ __global__ __launch_bounds__(kMuonThreads) void k_muon_momentum(MuonFirstArgs fi
 // 4 written and 4 read
 template <class T>
 __global__ __launch_bounds__(kMuonThreads) void k_muon_start(MuonArgs a) {
-  __shared__ float s_part[kMuonThreads / 64];
+  __shared__ double s_part[kMuonThreads / 64];
   const int tid = threadIdx.x;
   const MuonDesc d = muon_take(a.t, a.count, blockIdx.x, [](const MuonDesc& t) { return t.tile0; });
   const int64_t padded = (int64_t)((d.rows + 63) & ~63) * ((d.cols + 63) & ~63);
   const uint32_t per = (uint32_t)((padded + kMuonChunk - 1) / kMuonChunk), t = blockIdx.x - d.tile0;
   const int64_t mat = t / per;
   const MuonPlanes w(d, mat);
-  float sum = 0.f;
+  double sum = 0.0;
   for (uint32_t c = tid; c < d.chunks; c += kMuonThreads) sum += a.sums[d.chunk0 + mat * d.chunks + c];
-  sum = lanes_sum<64>(sum);
+  sum = lanes_sum64<64>(sum);
   if ((tid & 63) == 0) s_part[tid >> 6] = sum;
   __syncthreads();
-  const float f = kMuonOne / (sqrtf((s_part[0] + s_part[1]) + (s_part[2] + s_part[3])) + a.eps);
+  // 1 / (|u| + eps) as 2^-ex and a number in (1, 2], which fp32 holds whatever |u| is
+  const double norm = sqrt((s_part[0] + s_part[1]) + (s_part[2] + s_part[3])) + (double)a.eps;
+  int ex = 0;
+  const float f = norm < INFINITY ? (float)(kMuonOne / frexp(norm, &ex)) : NAN;
   const int64_t n = (int64_t)d.rows * d.cols;
   const T* g = static_cast<const T*>(d.g) + mat * n;
   const float* m = d.m ? d.m + mat * n : nullptr;
@@ -215,7 +219,7 @@ __global__ __launch_bounds__(kMuonThreads) void k_muon_start(MuonArgs a) {
       }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= f;
+    for (int j = 0; j < 8; ++j) v[j] = ldexpf(v[j], -ex) * f;
     u32x4 hi, lo;
     split8(v, hi, lo);
     *reinterpret_cast<u32x4*>(w.x0 + q * 8) = hi;

@@ -81,7 +81,7 @@ struct MuonDesc {
 constexpr int kMuonTensors = 48;     // of a group
 struct MuonArgs {
   MuonDesc* t;             // the group's tensors, in the workspace
-  float* sums;
+  double* sums;            // of a chunk's squares
   int count, cur, nesterov, write_only;
   float mu, eps, a, b, c, keep;
 };

@@ -11,7 +11,7 @@ and the update's is lr update_rms: with update_rms 0.2 that of an AdamW step of 
 
 A step is one launch for each product of all tensors (tmoe_muon_step), and two before them:
 bfloat16 or float32 parameters (..., rows, cols) on a HIP device, each of whose last two axes is a
-matrix; float32 momenta, sums in float32, X held in 22 bits.
+matrix; float32 momenta, sums in float32 (|u|'s in float64), X held in 22 bits.
 """
 from __future__ import annotations
 

@@ -221,3 +221,22 @@ def test_optimizer(pkg, dev):
         with torch.cuda.graph(graph):
             first.step()
     assert fresh not in first.state or not first.state[fresh]
+
+
+@dtypes
+@pytest.mark.parametrize("scale", [1e15, 1e20, 3e30, 1e-18, 1e-25, 3e-36])
+def test_squares_past_float32(pkg, dev, scale, dtype):
+    """Finite matrices the sum of whose squares leaves float32 at either end are orthogonalised as any
+    others are, and matrices of zeros beside them stay zeros with the smallest eps."""
+    us = [(matrices(s, 9) * scale).to(dtype) for s in ((40, 70), (130, 64), (3, 20, 33))]
+    us[2][1] = 0
+    eps = 1e-37 if scale < 1 else 1e-7
+    for u, got in zip(us, pkg.orthogonalize([u.to(dev) for u in us], eps=eps)):
+        X, off = mn.orthogonalize(f64(u), eps=eps)
+        near(got, X, off, scale)
+    assert (got[1] == 0).all()
+    p, _, m = _lists([(40, 70)], dtype, dev)
+    o = mn.muon(f64(p[0]), f64(us[0]), f64(m[0]) * scale, 0.02, eps=eps)
+    q = [m[0] * scale]
+    pkg.muon_step(p, [us[0].to(dev)], q, lr=0.02, eps=eps)
+    near(p[0], o["p"], o["off"], scale)
