@@ -240,3 +240,23 @@ def test_squares_past_float32(pkg, dev, scale, dtype):
     q = [m[0] * scale]
     pkg.muon_step(p, [us[0].to(dev)], q, lr=0.02, eps=eps)
     near(p[0], o["p"], o["off"], scale)
+
+
+def test_wide_tiles_element_by_element(pkg, dev):
+    """test_single_elements_of_a_step's bound in the kernels of 128 x 128 tiles: many matrices at once,
+    wide and tall, with ragged edges and with Gram products cut into slices."""
+    a, b, c = 3.4445, -4.7750, 2.0315
+    shapes = [(40, 256, 512), (512, 128), (300, 200), (129, 4097), (257, 33), (4097, 130), (1001, 77)]
+    us = [matrices(s, i).to(dev) for i, s in enumerate(shapes)]
+    for u, got in zip(us, pkg.orthogonalize(us, steps=1)):
+        x = u.double()
+        x = x / (x.flatten(-2).norm(dim=-1)[..., None, None] + 1e-7)
+        t = x if u.shape[-2] <= u.shape[-1] else x.mT
+        m = t.abs()
+        A, M = t @ t.mT.contiguous(), m @ m.mT.contiguous()
+        want, mag = a * t + (b * A + c * (A @ A)) @ t, a * m + (abs(b) * M + c * (M @ M)) @ m
+        if t is not x:
+            want, mag = want.mT, mag.mT
+        off = (got.double() - want).abs()
+        n = 2 * max(u.shape[-2:]) + 2 * min(u.shape[-2:]) + 40
+        assert (off <= n * 2.0 ** -24 * mag + 1e-9).all(), (u.shape, float((off / mag).max()))
