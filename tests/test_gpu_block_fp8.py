@@ -276,3 +276,21 @@ def test_captured_and_streams(pkg, dev):
         side.synchronize()
         for p, q in zip(other, want):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("M,K,N", [(2040, 1100, 8100), (4096, 1024, 4096), (2049, 129, 8200)])
+def test_wide_tiles_in_the_whole(pkg, dev, M, K, N):
+    """bfloat16 results of tiles of 256 x 256 are no more than their own rounding off in each row's and
+    each column's norm. What the 8-bit instruction cuts is, for terms without an order, 2^-18 of their
+    magnitudes' sum, which is sqrt(K) at most times their own root of squares: 2^-18 sqrt(K) < 2^-12."""
+    x, w = values((M, K), torch.bfloat16, 3).to(dev), values((N, K), torch.bfloat16, 4).to(dev)
+    a, b = pkg.fp8_quantize(x), pkg.fp8_quantize(w, True)
+    assert pkg._lib.lib().tmoe_fp8_gemm_workspace_bytes(M, N, K, pkg._lib.TMOE_BF16, 0) == 0
+    want = pkg.fp8_dequantize(a).double() @ pkg.fp8_dequantize(b).double().t().contiguous()
+    got = pkg.fp8_block_matmul(a, b)
+    off = got.double() - want
+    exact = pkg.fp8_block_matmul(a, b, torch.float32).double()
+    for axis in (0, 1):
+        size = want.norm(dim=axis)
+        assert (off.norm(dim=axis) <= (2.0 ** -8 + 2.0 ** -12) * size).all()
+        assert ((exact - want).norm(dim=axis) <= 2.0 ** -20 * size).all()
