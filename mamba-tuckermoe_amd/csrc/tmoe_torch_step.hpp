@@ -503,10 +503,11 @@ PyObject* fp8_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // ---- Muon ----------------------------------------------------------------------
 
 // muon(params, grads, momenta or None, lr, momentum, weight_decay, update_rms, eps, coefficients (a,
-// b, c), steps, nesterov, write only): params None: a list of new tensors like grads
+// b, c), steps, nesterov, write only, check only): params None: a list of new tensors like grads. Check
+// only: refuses what the call would refuse, and does nothing
 PyObject* muon(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (bad_args(nargs, 12, "muon")) return nullptr;
+  if (bad_args(nargs, 13, "muon")) return nullptr;
   const bool write_only = a[0] == Py_None;
   const char* const who = write_only ? "orthogonalize" : "muon_step";
   auto list = [&](PyObject* o, const char* what, size_t want) {
@@ -540,6 +541,9 @@ PyObject* muon(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   s.steps = (int32_t)steps;
   s.nesterov = PyObject_IsTrue(a[10]);
   s.write_only = write_only;
+  const bool check_only = PyObject_IsTrue(a[12]);
+  s.dtype = TMOE_F32;
+  if (n == 0 || check_only) check_rc(g_step.muon_step(nullptr, 0, &s, nullptr, 0, nullptr));   // the numbers alone
   if (n == 0) return PyList_New(0);
   const at::Device dev = g[0].device();
   const auto dt = g[0].scalar_type();
@@ -595,6 +599,7 @@ PyObject* muon(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
                 std::any_of(g.begin(), g.end(), [](const at::Tensor& x) { return x.requires_grad(); })),
               who, " has no gradient: give the matrices detached");
   check_hip(g[0], who);
+  if (check_only) return none();
   {
     pybind11::gil_scoped_release nogil;
     const c10::DeviceGuard guard(dev);

@@ -32,6 +32,21 @@ def _coefficients(c):
     return c
 
 
+def _check_numbers(who: str, o) -> None:
+    if not 0.0 <= o["momentum"] < 1.0:
+        raise ValueError(f"{who}: momentum {o['momentum']}")
+    if not o["lr"] >= 0.0 or not o["weight_decay"] >= 0.0 or not o["update_rms"] >= 0.0 or not o["eps"] > 0.0:
+        raise ValueError(f"{who}: lr {o['lr']}, weight_decay {o['weight_decay']}, update_rms "
+                         f"{o['update_rms']}, eps {o['eps']}")
+
+
+def _step(params, grads, momenta, o, check: bool = False) -> None:
+    """muon_step with the options o, or (check) its refusals alone."""
+    _lib.native().muon(params, grads, momenta, float(o["lr"]), float(o["momentum"]), float(o["weight_decay"]),
+                       float(o["update_rms"]), float(o["eps"]), _coefficients(o["coefficients"]),
+                       int(o["steps"]), bool(o["nesterov"]), False, check)
+
+
 def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
               momenta: Sequence[torch.Tensor], *, lr: float, momentum: float = 0.95,
               nesterov: bool = True, weight_decay: float = 0.1, update_rms: float = 0.2, steps: int = 5,
@@ -39,13 +54,10 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     """One step on lists of tensors of one dtype on one device, in place. Parameters and momenta
     (float32) are contiguous. What is written may share no memory, nor with a gradient. The
     coefficients have to keep singular values within [-2, 2]."""
-    if not 0.0 <= momentum < 1.0:
-        raise ValueError(f"muon_step: momentum {momentum}")
-    if not lr >= 0.0 or not weight_decay >= 0.0 or not update_rms >= 0.0 or not eps > 0.0:
-        raise ValueError(f"muon_step: lr {lr}, weight_decay {weight_decay}, update_rms {update_rms}, eps {eps}")
-    _lib.native().muon(params, grads, momenta, float(lr), float(momentum), float(weight_decay),
-                       float(update_rms), float(eps), _coefficients(coefficients), int(steps),
-                       bool(nesterov), False)
+    o = dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, update_rms=update_rms,
+             steps=steps, coefficients=coefficients, eps=eps)
+    _check_numbers("muon_step", o)
+    _step(params, grads, momenta, o)
 
 
 def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = 5,
@@ -56,7 +68,7 @@ def orthogonalize(matrices: Union[torch.Tensor, Sequence[torch.Tensor]], steps: 
     if not eps > 0.0:
         raise ValueError(f"orthogonalize: eps {eps}")
     out = _lib.native().muon(None, [matrices] if one else matrices, None, 0.0, 0.0, 0.0, 0.0, float(eps),
-                             _coefficients(coefficients), int(steps), False, True)
+                             _coefficients(coefficients), int(steps), False, True, False)
     return out[0] if one else out
 
 
@@ -77,14 +89,13 @@ class FusedMuon(torch.optim.Optimizer):
 
     @staticmethod
     def _check_options(o) -> None:
-        if not 0.0 <= o["momentum"] < 1.0:
-            raise ValueError(f"FusedMuon: momentum {o['momentum']}")
-        if not o["lr"] >= 0.0 or not o["weight_decay"] >= 0.0 or not o["update_rms"] >= 0.0 or not o["eps"] > 0.0:
-            raise ValueError(f"FusedMuon: lr {o['lr']}, weight_decay {o['weight_decay']}, update_rms "
-                             f"{o['update_rms']}, eps {o['eps']}")
+        _check_numbers("FusedMuon", o)
         if not 1 <= o["steps"] <= 16:
             raise ValueError(f"FusedMuon: steps {o['steps']} (1 to 16)")
-        _coefficients(o["coefficients"])
+        try:
+            _step([], [], [], o, True)      # whether the coefficients stay in range
+        except RuntimeError as e:
+            raise ValueError(f"FusedMuon: {e}") from None
 
     def add_param_group(self, param_group) -> None:
         self._check_options({**self.defaults, **param_group})
@@ -98,13 +109,15 @@ class FusedMuon(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
-        """One step over every parameter that has a gradient; closure as in torch.optim."""
+        """One step over every parameter that has a gradient; closure as in torch.optim. What is
+        refused is refused before anything changes."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = []
-        for group in self.param_groups:      # what is refused is refused before anything changes
+        work = []       # (group, parameters, gradients, momenta) of each group, device and dtype
+        for group in self.param_groups:
+            _check_numbers("FusedMuon", group)
             runs = {}
             for p in group["params"]:
                 if p.grad is None:
@@ -115,17 +128,18 @@ class FusedMuon(torch.optim.Optimizer):
                     raise RuntimeError("FusedMuon: a parameter's first step inside a graph capture: make "
                                        "one step with these gradients before the capture")
                 runs.setdefault((p.device, p.dtype), []).append(p)
-            work.append((group, runs))
-        for group, runs in work:
             for ps in runs.values():
-                for p in ps:
-                    if not self.state[p]:
-                        self.state[p]["momentum_buffer"] = torch.zeros_like(
-                            p, dtype=torch.float32, memory_format=torch.contiguous_format)
-                muon_step(ps, [p.grad for p in ps], [self.state[p]["momentum_buffer"] for p in ps],
-                          lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
-                          weight_decay=group["weight_decay"], update_rms=group["update_rms"],
-                          steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])
+                ms = [self.state[p]["momentum_buffer"] if self.state.get(p) else torch.zeros_like(
+                    p, dtype=torch.float32, memory_format=torch.contiguous_format) for p in ps]
+                work.append((group, ps, [p.grad for p in ps], ms))
+        if len(work) > 1:                   # (a call by itself refuses before it launches)
+            for group, ps, gs, ms in work:
+                _step(ps, gs, ms, group, True)
+        for group, ps, gs, ms in work:
+            _step(ps, gs, ms, group)
+            for p, m in zip(ps, ms):
+                if not self.state[p]:
+                    self.state[p]["momentum_buffer"] = m
         return loss
 
     def load_state_dict(self, state_dict) -> None:

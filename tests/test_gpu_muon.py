@@ -260,3 +260,57 @@ def test_wide_tiles_element_by_element(pkg, dev):
         off = (got.double() - want).abs()
         n = 2 * max(u.shape[-2:]) + 2 * min(u.shape[-2:]) + 40
         assert (off <= n * 2.0 ** -24 * mag + 1e-9).all(), (u.shape, float((off / mag).max()))
+
+
+def test_a_refused_step_changes_nothing(pkg, dev):
+    """Of two groups the second is refused: parameters, momenta and states are as they were."""
+    def build(extra, **kw):
+        a = torch.nn.Parameter(matrices((40, 70), 1).to(dev))
+        b = torch.nn.Parameter(matrices((20, 30), 2).bfloat16().to(dev))
+        return [a, b, extra], pkg.FusedMuon([{"params": [a, b]}, {"params": [extra], **kw}], lr=0.1)
+
+    def grads(ps):
+        for i, p in enumerate(ps):
+            p.grad = torch.ones_like(p) * (i + 1)
+    good = lambda: torch.nn.Parameter(matrices((6, 9), 3).to(dev))  # noqa: E731
+    base = torch.zeros(200, device=dev)
+    cases = [(torch.nn.Parameter(matrices((9, 6), 3).to(dev).t()), "contiguous"),
+             (torch.nn.Parameter(matrices((6, 9), 3).half().to(dev)), "dtype"),
+             (torch.nn.Parameter(matrices((6, 9), 3)), "HIP devices only")]
+    for extra, text in cases:
+        ps, opt = build(extra)
+        grads(ps)
+        before = [p.detach().clone() for p in ps]
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match=text):
+                opt.step()
+            assert all(torch.equal(p.detach(), q) for p, q in zip(ps, before))
+            assert not any(opt.state.get(p) for p in ps)
+    for key, bad in (("lr", -1.0), ("momentum", 1.0), ("lr", float("inf")), ("steps", 99), ("coefficients", (5.0, 0.0, 0.0))):
+        ps, opt = build(good())
+        grads(ps)
+        opt.step()
+        before = [t.clone() for p in ps for t in (p.detach(), opt.state[p]["momentum_buffer"])]
+        keep = opt.param_groups[1][key]
+        opt.param_groups[1][key] = bad
+        with pytest.raises((ValueError, RuntimeError)):
+            opt.step()
+        after = [t for p in ps for t in (p.detach(), opt.state[p]["momentum_buffer"])]
+        assert all(torch.equal(x, y) for x, y in zip(before, after))
+        opt.param_groups[1][key] = keep
+        opt.step()
+        assert not any(torch.equal(x, y) for x, y in zip(before, after))
+    # a run by itself whose tensors share memory, and a state that is not float32
+    one, two = (torch.nn.Parameter(base[i:i + 100].view(10, 10)) for i in (0, 50))
+    opt = pkg.FusedMuon([one, two])
+    grads([one, two])
+    with pytest.raises(RuntimeError, match="share"):
+        opt.step()
+    assert (base == 0).all() and not opt.state.get(one) and not opt.state.get(two)
+    ps, opt = build(good())
+    grads(ps)
+    opt.state[ps[2]]["momentum_buffer"] = torch.zeros(6, 9, device=dev, dtype=torch.bfloat16)
+    before = [p.detach().clone() for p in ps]
+    with pytest.raises(RuntimeError, match="momentum of float32"):
+        opt.step()
+    assert all(torch.equal(p.detach(), q) for p, q in zip(ps, before)) and not opt.state.get(ps[0])

@@ -154,3 +154,20 @@ def test_optimizer_options_and_states(pkg):
             {**sd, "state": {0: {"exp_avg": torch.zeros(4, 6)}}})
     with pytest.raises(ValueError, match="steps"):
         new.load_state_dict({**sd, "param_groups": [{**sd["param_groups"][0], "steps": 0}]})
+
+
+def test_coefficients_are_refused_with_the_group(pkg):
+    w = torch.nn.Parameter(torch.zeros(4, 6))
+    for c in ((5.0, 0.0, 0.0), (1.0, -40.0, 39.5), (math.nan, 0.0, 0.0)):
+        with pytest.raises(ValueError, match="do not stay in range"):
+            pkg.FusedMuon([w], coefficients=c)
+        opt = pkg.FusedMuon([w])
+        with pytest.raises(ValueError, match="do not stay in range"):
+            opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2, 2))], "coefficients": c})
+        sd = opt.state_dict()
+        with pytest.raises(ValueError, match="do not stay in range"):
+            opt.load_state_dict({**sd, "param_groups": [{**sd["param_groups"][0], "coefficients": c}]})
+        with pytest.raises(RuntimeError, match="do not stay in range"):
+            pkg.muon_step([], [], [], lr=0.1, coefficients=c)
+    with pytest.raises(ValueError):
+        pkg.FusedMuon([w], lr=math.inf)
