@@ -139,7 +139,8 @@ class TuckerMoETrain(torch.nn.Module):
     instead, without a temperature and without losses (0.0 each): what keeps the experts even is
     `balance_bias` (E; a buffer, float32 whatever the module is cast to), which update_balance()
     moves after a step. `fp8_products` makes the products with U_in and U_out, forward and
-    backward, in 8-bit blocks (block_fp8.fp8_matmul)."""
+    backward, in 8-bit blocks (block_fp8.fp8_matmul), of operands cast as torch.matmul's are
+    under autocast (to bfloat16: float16 is refused)."""
 
     _ROUTING = ("score", "groups", "top_groups", "renormalize", "scale")
 
@@ -188,7 +189,12 @@ class TuckerMoETrain(torch.nn.Module):
         self.balance_bias.add_(torch.sign(c.mean() - c), alpha=rate)
 
     def _product(self, x, u):
-        return fp8_matmul(x, u) if self.fp8_products else torch.matmul(x, u)
+        if not self.fp8_products:
+            return torch.matmul(x, u)
+        if torch.is_autocast_enabled(x.device.type):        # as it casts torch.matmul's operands
+            dtype = torch.get_autocast_dtype(x.device.type)
+            x, u = (t if t.dtype == torch.float64 else t.to(dtype) for t in (x, u))
+        return fp8_matmul(x, u)
 
     def _route(self, xf, step, mask):
         """(idx, top_p, lb_loss, z_loss)."""

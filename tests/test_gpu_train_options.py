@@ -193,3 +193,36 @@ def test_a_captured_step(pkg, dev):
         torch.cuda.synchronize()
         for u, v in zip(pe, pc):
             assert torch.equal(u, v)
+
+
+@dtypes
+@pytest.mark.parametrize("options", [dict(routing={}), dict(fused_router=True)], ids=["routing", "capped"])
+def test_autocast(pkg, dev, dtype, options):
+    """A layer of float32 parameters under autocast with fp8_products: the same expressions with both of
+    each product's operands cast, bit for bit, and gradients of the leaves' types. Without
+    fp8_products the layer runs there as well, and the two are an fp8 rounding apart (2^-4 for each of two
+    operands in two products: 4 2^-4, random)."""
+    torch.manual_seed(7)
+    sizes = dict(num_experts=8, r2=64, r3=64)
+    m = pkg.TuckerMoETrain(128, 96, fp8_products=True, **sizes, **options).to(dev)
+    full = pkg.TuckerMoETrain(128, 96, **sizes, **options).to(dev)
+    full.load_state_dict(m.state_dict())
+    x = torch.randn(3, 67, 128, device=dev).to(dtype).requires_grad_()
+    g = torch.randn(3, 67, 96, device=dev)
+    with torch.autocast("cuda", torch.bfloat16):
+        out, _, _ = m(x)
+        other, _, _ = full(x)
+        xf = x.reshape(-1, 128)
+        idx, top_p, _, _ = m._route(xf, None, None)
+        xs = m.inner_norm(pkg.fp8_matmul(xf.bfloat16(), m.U_in.bfloat16()))
+        core = pkg.FusedLatentMoE.apply(xs, torch.einsum("er,rst->est", m.U_expert, m.core), idx, top_p).to(dtype)
+        want = pkg.fp8_matmul(core.bfloat16(), m.U_out.bfloat16()).reshape(3, 67, 96) + m.bias
+    assert torch.equal(out, want) and out.dtype == other.dtype
+    leaves = [x, *m.parameters()]
+    got = torch.autograd.grad(out, leaves, g.to(out.dtype))
+    for u, v, leaf in zip(got, torch.autograd.grad(want, leaves, g.to(out.dtype)), leaves):
+        assert torch.equal(u, v) and u.dtype == leaf.dtype
+    assert onp.rel_l2(f64(out), f64(other)) <= 4 * 2.0 ** -4
+    with torch.autocast("cuda", torch.float16):
+        with pytest.raises(RuntimeError, match="Half"):
+            m(x)

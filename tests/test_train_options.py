@@ -52,3 +52,31 @@ def test_refusals(pkg):
     for kw in (dict(routing={}), dict(fp8_products=True, fused_router=True)):
         with pytest.raises(RuntimeError, match="HIP"):
             _layer(pkg, **kw)(torch.randn(3, 64))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_products_are_cast_under_autocast(pkg, monkeypatch, dtype):
+    """Float32 parameters, a hidden state of either type: both products' operands are autocast's, as
+    torch.matmul's in their place, and outside it they are what they are."""
+    import mamba_tuckermoe_amd.latent as lat
+    seen = []
+
+    def product(x, w):
+        seen.append((x.dtype, w.dtype))
+        return x @ w
+    monkeypatch.setattr(lat, "fp8_matmul", product)
+    monkeypatch.setattr(lat.FusedLatentMoE, "apply", staticmethod(
+        lambda xs, G, idx, p: torch.einsum("br,bkrs,bk->bs", xs, G[idx], p.to(xs.dtype))))
+    monkeypatch.setattr(lat, "fused_router", lambda raw, k, *a: (
+        *reversed(torch.softmax(raw.float(), -1).topk(k)), 0.0, 0.0, None))
+    x = torch.randn(5, 64).to(dtype).requires_grad_()
+    m = _layer(pkg, fused_router=True, fp8_products=True)
+    with torch.autocast("cpu", torch.bfloat16):
+        out, _, _ = m(x)
+    out.float().square().sum().backward()
+    assert seen == [(torch.bfloat16, torch.bfloat16)] * 2
+    assert x.grad.dtype == dtype and all(p.grad.dtype == torch.float32 for p in m.parameters())
+    if dtype == torch.float32:
+        del seen[:]
+        m(x)
+        assert seen == [(torch.float32, torch.float32)] * 2
