@@ -503,7 +503,11 @@ int tmoe_expert_router_backward(const tmoe_expert_router* router, const int64_t*
  *
  * tmoe_fp8_gemm: out (M, N) of dtype, contiguous, from a (M, K) and b (N, K):
  *   out[m, n] = sum_b sa[m, b] sb[n, b] sum_{k in b} a[m, k] b[n, k]
- * in fp32. tmoe_fp8_gemm_values: the same with a the operand that quantising x (M, K) by rows
+ * Blocks are summed in fp32. Within a block a TMOE_F32 out has fp32 sums too; a TMOE_BF16 one has
+ * the 8-bit matrix instruction's, which cuts each product at 2^-13 of the largest of up to 16 that
+ * it adds together: at most 2^-9 of sum |terms| off, some 2^-18 of it where they have no order,
+ * beside the result's own 2^-9 (for bf16 of fp32 sums: out in TMOE_F32, rounded by the caller).
+ * tmoe_fp8_gemm_values: the same with a the operand that quantising x (M, K) by rows
  * would make. The order of its sums depends on the sizes alone. K, N and the rows of an operand
  * <= 2^23, M of out <= 2^23. Workspaces of at least tmoe_fp8_gemm_workspace_bytes(M, N, K,
  * dtype, values) bytes (0: none), 16-byte aligned. M == 0 is a no-op. Stream-ordered, no allocation. */
