@@ -108,7 +108,7 @@ hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_a
     // Tiles of 128 x 128 where X has one for each compute unit and half of A some for every fourth. us a
     // step, 128 against 64: 2048 x 2048 (136 of A, 256 of X) 762 and 987, 6144 x 1536 (78, 576) 1151 and 1333, 32
     // of 256 x 512 (96, 256) 208 and 218; 1536 x 1536 (78, 144) 590 and 499, 1024 x 4096 (36, 256) 450 and
-    // 434, 16 of 256 x 512 (48, 128) 181 and 152
+    // 434, 16 of 256 x 512 (48, 128) 181 and 152. Between 36 and 78 of A, and 144 and 256 of X, nothing was.
     int64_t pairs128 = 0, square = 0;
     for (int64_t k = i; k < g.end; ++k) {
       const Shape q = shape_of(t[k]);
@@ -119,8 +119,10 @@ hipError_t muon(const tmoe_muon_tensor* t, int64_t count, const tmoe_muon_step_a
     }
     const int64_t bt = pairs128 >= 72 && square >= 256 ? 128 : 64;
     // The Gram products' summed axes are cut into slices of about what each work-group that the
-    // chip holds has to do in the mean: a long one alone would keep the rest waiting. Not under 14 K
-    // tiles of 64 x 64 a slice, for what the sum costs: 135 us a step of nine small matrices, 140 with 8 or 16.
+    // chip holds has to do in the mean: a long one alone would keep the rest waiting. For what the sum
+    // costs that mean is taken as 14 K tiles at least (16 of 128 x 128), and an axis cut evenly into the
+    // fewest slices of no more: 16 K tiles are two of 8, 32 three of 11, 11 and 10. A step of nine small
+    // matrices takes 135 us so and 140 with 8 or with 16 as the least; between those only 14 was measured.
     int64_t work = 0;
     for (int64_t k = i; k < g.end; ++k) {
       if (empty(t[k])) continue;
