@@ -143,6 +143,7 @@ class TuckerMoETrain(torch.nn.Module):
     under autocast (to bfloat16: float16 is refused)."""
 
     _ROUTING = ("score", "groups", "top_groups", "renormalize", "scale")
+    routing, fp8_products = None, False     # (of modules that were pickled without them)
 
     def __init__(self, dim_in, dim_out, num_experts=8, top_k=2, r1=4, r2=1024, r3=256,
                  fused_router=False, routing: Optional[dict] = None, fp8_products=False):

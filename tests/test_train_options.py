@@ -80,3 +80,17 @@ def test_products_are_cast_under_autocast(pkg, monkeypatch, dtype):
         del seen[:]
         m(x)
         assert seen == [(torch.float32, torch.float32)] * 2
+
+
+def test_a_layer_of_an_older_pickle(pkg, monkeypatch):
+    """A whole module saved before the options existed has neither attribute: it is the layer it was."""
+    import mamba_tuckermoe_amd.latent as lat
+    monkeypatch.setattr(lat.FusedLatentMoE, "apply", staticmethod(
+        lambda xs, G, idx, p: torch.einsum("br,bkrs,bk->bs", xs, G[idx], p)))
+    m = _layer(pkg)
+    x = torch.randn(5, 64)
+    want, lb, z = m(x)
+    for name in ("routing", "fp8_products"):
+        del m.__dict__[name]
+    out, lb2, z2 = m(x)
+    assert torch.equal(out, want) and torch.equal(lb, lb2) and torch.equal(z, z2)
