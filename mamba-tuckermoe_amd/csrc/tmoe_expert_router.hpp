@@ -365,7 +365,7 @@ __global__ __launch_bounds__(1024) void k_expert_router_counts(ExpertRouterArgs 
 // renormalised or whose r counts, where every expert has one): the row is put together in LDS and
 // stored whole.
 // Bound by those bytes where there are many tokens: (131072, 64) in float32 17 us, 2.3 TB/s with what it
-// reads; (4096, 256) 4.6 us.
+// reads; (4096, 256) 4.7 us.
 template <class T, int L>
 __global__ __launch_bounds__(kErThreads) void k_expert_router_bwd(ExpertRouterArgs a) {
   constexpr int V = kErV, G = kErThreads / L;
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(kErThreads) void k_expert_router_bwd(ExpertRouterAr
       D = lanes_sum<L>(D);
       S = lanes_sum<L>(S);
       const bool small = softmax && a.renormalize && !(S >= 1.f - 0x1p-20f);
-      float v[V], m = 0.f, unit = 1.f;           // of a row whose every expert has a gradient
+      float v[V], m = 0.f, unit = 1.f, f = 0.f;  // of a row whose every expert has a gradient
       if (dense || small) {
         float sum = 0.f;
         router_load<T, V>(row, e0, E, v);
@@ -410,6 +410,7 @@ __global__ __launch_bounds__(kErThreads) void k_expert_router_bwd(ExpertRouterAr
           sum += v[j];
         }
         unit = lanes_sum<L>(sum);
+        f = a.scale / unit;
       }
       if (small) {
         S = 0.f;
@@ -419,7 +420,6 @@ __global__ __launch_bounds__(kErThreads) void k_expert_router_bwd(ExpertRouterAr
         }
         S = lanes_sum<L>(S) / unit;
       }
-      const float f = a.scale / unit;
       // r, what 1e-20 leaves of one, and its part of t
       const float r = softmax && !small ? 0.f : 1e-20f / (S + 1e-20f), rest = top * r;
       for (int i = l; i < k; i += L) {

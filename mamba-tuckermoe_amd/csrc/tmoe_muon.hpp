@@ -139,7 +139,7 @@ struct MuonPlanes {
 
 // m = mu m + g, and each chunk's sum of u^2, in 64 bits: a finite u's squares may be past fp32 at either
 // end (1e20, or 1e-25 with an eps as small), and as many conversions are nothing beside the bytes; the first work-group leaves the tensors' table. Bound by
-// memory, 5.5 TB/s (83 M elements in fp32: 170 us)
+// memory, 5.5 TB/s (83 M elements in fp32: 172 us)
 template <class T>
 __global__ __launch_bounds__(kMuonThreads) void k_muon_momentum(MuonFirstArgs first) {
   const int tid = threadIdx.x;
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kMuonThreads) void k_muon_momentum(MuonFirstArgs fi
 }
 
 // X = u / (|u| + eps) in its padded planes, zeros past the matrix; a work-group takes 8192 elements.
-// Bound by memory, 5.1 TB/s (197 us): u is formed again from g and m, 8 bytes, where a plane of it would be
+// Bound by memory, 5.1 TB/s (199 us): u is formed again from g and m, 8 bytes, where a plane of it would be
 // 4 written and 4 read
 template <class T>
 __global__ __launch_bounds__(kMuonThreads) void k_muon_start(MuonArgs a) {

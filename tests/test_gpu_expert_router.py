@@ -236,3 +236,13 @@ def test_small_selected_scores(pkg, dev, E, k, groups, top, dtype):
         draw, = torch.autograd.grad(r.weights, leaf, dw.to(dev))
         far = 4 * float(dw.abs().max())
         near(draw, o["draw"], o["draw_mag"] + far * lost / (m * 2.0 ** -24), m, "draw")
+
+
+@dtypes
+@pytest.mark.parametrize("E,k,groups,top", [(4, 2, 1, 1), (8, 1, 1, 1), (64, 6, 8, 3)])
+def test_small_sigmoids(pkg, dev, E, k, groups, top, dtype):
+    """Sigmoids of 20 to 80 below zero: 1e-20 is a part, or all, of what a weight is divided by."""
+    raw = torch.randn(200, E, generator=torch.Generator().manual_seed(E)) - torch.linspace(20, 80, 200)[:, None]
+    raw = raw.to(dtype).to(dev)
+    for bias in (None, biases(E, "sigmoid", 1)):
+        check(pkg, raw, k, 3, bias=bias, score="sigmoid", groups=groups, top_groups=top, scale=2.5)
