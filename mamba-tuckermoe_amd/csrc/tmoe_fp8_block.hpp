@@ -185,9 +185,9 @@ __device__ __forceinline__ bf16x8 bf16_of(int lo, int hi) {
 // while 2^-23 counts between groups and to the accumulator. Random rows of 128 come out 4e-6 of
 // their magnitudes' sum off, a five-hundredth of the rounding of a bf16 result, which take it: with
 // fp32 sums they are as far from the float64 product (1.662e-3 in the norm at M = N = K = 4096, 1.657e-3 at
-// 16384 x 4608 x 768, either way) and take 159 us instead of 79 there, 144 instead of 85 here. fp32
-// results (kExact) are summed in fp32: the codes as bf16, whose instruction keeps all 24 bits, at
-// half the rate.
+// 16384 x 4608 x 768, either way) and take 159 us instead of 79 there, 144 instead of 85 here (one
+// row of 1536 to 6144: 5.2 and 4.9). fp32 results (kExact) are summed in fp32: the codes as bf16, whose
+// instruction keeps all 24 bits, at half the rate.
 template <bool kExact>
 __device__ __forceinline__ f32x16 mma_fp8(i32x8 a, i32x8 b, f32x16 c) {
   if constexpr (kExact) {
